@@ -44,7 +44,7 @@ extern "C" {
  * 102: dim_head 256 (its kernels keep no forward partials: the sa2_saved_*_bytes queries return 0 and a non-NULL
  * `saved` is refused)
  * The number stands for what existing calls do.  Functions added beside them (sa2_fwd_ws, sa2_bwd_split, sa2_bwd_split_padded,
- * sa2_convert, sa2_wgrad and their size queries) leave it as it is: look them up by name. */
+ * sa2_convert, sa2_wgrad, the serving functions and their size queries) leave it as it is: look them up by name. */
 #define SA2_VERSION 102
 
 typedef enum sa2_status {
@@ -288,6 +288,82 @@ int sa2_qkv_norm_bwd(const sa2_problem *prob, const void *qkv, int64_t row_strid
 int64_t sa2_wgrad_workspace_bytes(int64_t rows, int32_t out_features, int32_t in_features);
 int sa2_wgrad(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, int64_t rows, int32_t out_features, int32_t in_features,
               void *dw, void *workspace, int64_t workspace_bytes, void *hip_stream);
+
+/* ---- serving: paged caches, attention over them, sampling ----
+ *
+ * A pool holds the rows of one key or value set of one layer: `pages` pages of `page_size` rows of kv_heads x pool_dim elements (bf16 or
+ * fp16, innermost stride 1, 16-byte aligned rows; strides in elements).  Position x of sequence s is row x % page_size of page
+ * tables[s][x / page_size].  lengths[s] tokens of a sequence are in the cache, the rows of the call included; counts[s] (NULL: all) of the
+ * call's `rows` rows per sequence are there, the others are padding.  Row t is at position lengths[s] - counts[s] + t.  tables, lengths and counts are device
+ * memory and are not checked on the host: counts are taken into 0 .. rows, lengths below 0 as 0, and a table entry outside 0 .. pages - 1, like a position beyond the
+ * table or below 0, is a place that is not there: nothing of it is attended to or written.  Rows that attend to nothing (padding included) are zero. */
+typedef struct sa2_pool {
+    void   *ptr;
+    int64_t stride_page, stride_row, stride_head;
+} sa2_pool;
+typedef struct sa2_paged_index {
+    const int32_t *tables;        /* [batch] rows of table_width entries */
+    int64_t table_stride;         /* entries between rows */
+    const int32_t *lengths;       /* [batch] */
+    const int32_t *counts;        /* [batch], or NULL */
+} sa2_paged_index;
+typedef struct sa2_paged_problem {
+    int32_t batch, rows;          /* sequences, new rows of each */
+    int32_t heads, kv_heads;
+    int32_t dim_head;             /* channels of q and out; channels of the pools beyond it have to hold zeros */
+    int32_t pool_dim;             /* channels of a pool's row: a multiple of 8 up to 256, at least dim_head */
+    int32_t page_size, pages, table_width;
+    int32_t w1, w2;               /* windows (2-simplicial form only) */
+    int32_t max_length;           /* no sequence is longer; 0: not known (a wrong value costs time, not correctness) */
+    float   scale;
+    int32_t dtype;                /* sa2_element of q, out and the pools: SA2_ELEMENT_BF16 or SA2_ELEMENT_F16 */
+} sa2_paged_problem;
+
+/* Dense causal attention of the new rows: out[s,t,h] = sum over 0 <= j <= p of softmax_j(scale q . k[j]) v[j], p the row's position, query
+ * head h on key/value head h / (heads / kv_heads).  The workspace (16-byte aligned, needs no clearing) holds the fp32 results of key shares; 0 bytes where the
+ * keys are not shared out.  No counterpart in the reference, whose models recompute every token. */
+int64_t sa2_paged_attn_workspace_bytes(const sa2_paged_problem *prob);   /* -1 if the problem is invalid */
+int sa2_paged_attn(const sa2_paged_problem *prob, const sa2_tensor *q, const sa2_pool *k, const sa2_pool *v, const sa2_paged_index *at, const sa2_tensor *out,
+                   void *workspace, int64_t workspace_bytes, void *hip_stream);
+
+/* The 2-simplicial form: the attended set of sa2_fwd (p - w1 < j <= p, p - w2 < k <= p, neither below 0) for the new rows alone. */
+int64_t sa2_paged_simplicial_attn_workspace_bytes(const sa2_paged_problem *prob);
+int sa2_paged_simplicial_attn(const sa2_paged_problem *prob, const sa2_tensor *q, const sa2_pool *k1, const sa2_pool *k2, const sa2_pool *v1, const sa2_pool *v2,
+                              const sa2_paged_index *at, const sa2_tensor *out, void *workspace, int64_t workspace_bytes, void *hip_stream);
+
+/* New rows into the pages, for up to SA2_APPEND_MOST pools that share one geometry.  rows: (batch, rows, kv_heads, dim_head) of src_type, rounded to
+ * the pools' type; channels dim_head .. pool_dim - 1 of the written rows are zero. */
+typedef struct sa2_append_item {
+    sa2_pool pool;
+    sa2_tensor rows;
+} sa2_append_item;
+#define SA2_APPEND_MOST 4
+int sa2_paged_append(const sa2_paged_problem *prob, const sa2_append_item *items, int32_t count, int32_t src_type, const sa2_paged_index *at, void *hip_stream);
+
+/* Pages to other pages of the same pool, for every pool: page pairs[2 i] to page pairs[2 i + 1] (host memory, read before the call returns).
+ * A page is `bytes` consecutive bytes.  Refused: pages outside the pools, a page written twice or written and read. */
+typedef struct sa2_page_pool {
+    void   *ptr;
+    int64_t stride;               /* bytes between pages */
+    int64_t bytes;                /* of a page */
+    int64_t pages;
+} sa2_page_pool;
+int sa2_copy_pages(const sa2_page_pool *pools, int32_t count, const int32_t *pairs, int64_t n_pairs, void *hip_stream);
+
+/* One token per row of logits[rows][vocab] (sa2_element, innermost stride 1).  With the tokens ordered by (logit descending, index ascending) and
+ * p = softmax(logits / temperature), a token is kept if its rank is below top_k (top_k <= 0: any), the mass in front of it below top_p (top_p >= 1: any) and
+ * p >= min_p * max p; the first always is.  tokens[r] is the kept one with the largest logit / temperature - log(-log u), u = noise[r][token] in [0, 1) (fp32), ties to the
+ * lowest index; temperature <= 0: the first in the order.  logprobs[r] is its logarithm under softmax(logits).  A logit that is not a number counts as
+ * -infinity; a row without any other logit gives token -1 and -infinity.  The four parameters are fp32 / int32 device arrays [rows], or NULL: the number beside them. */
+typedef struct sa2_sample_params {
+    const float *temperature, *top_p, *min_p;
+    const int32_t *top_k;
+    float temperature_all, top_p_all, min_p_all;
+    int32_t top_k_all;
+} sa2_sample_params;
+int64_t sa2_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int sa2_sample(const void *logits, int32_t type, int64_t rows, int64_t vocab, int64_t stride, const float *noise, int64_t noise_stride,
+               const sa2_sample_params *params, int64_t *tokens, float *logprobs, void *workspace, int64_t workspace_bytes, void *hip_stream);
 
 #ifdef __cplusplus
 }

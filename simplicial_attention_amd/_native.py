@@ -32,7 +32,9 @@ EXPORTS = ('sa2_version', 'sa2_last_error', 'sa2_supported', 'sa2_saved_t_bytes'
            'sa2_bwd_split', 'sa2_bwd_split_padded', 'sa2_bwd_split_workspace_bytes', 'sa2_bwd_dq_dkv2', 'sa2_bwd_dkv1', 'sa2_bwd',
            'sa2_bwd_noalloc_scratch_bytes', 'sa2_bwd_noalloc',
            'sa2_convert', 'sa2_qkv_norm_fwd', 'sa2_qkv_norm_bwd_workspace_bytes', 'sa2_qkv_norm_bwd',
-           'sa2_wgrad_workspace_bytes', 'sa2_wgrad')
+           'sa2_wgrad_workspace_bytes', 'sa2_wgrad',
+           'sa2_paged_attn_workspace_bytes', 'sa2_paged_attn', 'sa2_paged_simplicial_attn_workspace_bytes', 'sa2_paged_simplicial_attn',
+           'sa2_paged_append', 'sa2_copy_pages', 'sa2_sample_workspace_bytes', 'sa2_sample')
 
 
 class Sa2Error(RuntimeError):
@@ -56,6 +58,33 @@ class TensorArg(ctypes.Structure):
 class Saved(ctypes.Structure):
     """sa2_saved: optional forward by-products (per-offset T and its reference)."""
     _fields_ = [('t', ctypes.c_void_p), ('m', ctypes.c_void_p)]
+
+
+class Pool(ctypes.Structure):
+    """sa2_pool: the pages of one key or value set."""
+    _fields_ = [('ptr', ctypes.c_void_p), ('stride_page', ctypes.c_int64), ('stride_row', ctypes.c_int64), ('stride_head', ctypes.c_int64)]
+
+
+class PagedIndex(ctypes.Structure):
+    _fields_ = [('tables', ctypes.c_void_p), ('table_stride', ctypes.c_int64), ('lengths', ctypes.c_void_p), ('counts', ctypes.c_void_p)]
+
+
+class PagedProblem(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ('batch', 'rows', 'heads', 'kv_heads', 'dim_head', 'pool_dim', 'page_size', 'pages', 'table_width',
+                                                    'w1', 'w2', 'max_length')] + [('scale', ctypes.c_float), ('dtype', ctypes.c_int32)]
+
+
+class AppendItem(ctypes.Structure):
+    _fields_ = [('pool', Pool), ('rows', TensorArg)]
+
+
+class PagePool(ctypes.Structure):
+    _fields_ = [('ptr', ctypes.c_void_p), ('stride', ctypes.c_int64), ('bytes', ctypes.c_int64), ('pages', ctypes.c_int64)]
+
+
+class SampleParams(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ('temperature', 'top_p', 'min_p', 'top_k')] + [
+        ('temperature_all', ctypes.c_float), ('top_p_all', ctypes.c_float), ('min_p_all', ctypes.c_float), ('top_k_all', ctypes.c_int32)]
 
 
 _lib = None
@@ -113,6 +142,22 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.sa2_wgrad_workspace_bytes.argtypes = [I64, ctypes.c_int32, ctypes.c_int32]
     lib.sa2_wgrad.restype = ctypes.c_int
     lib.sa2_wgrad.argtypes = [V, I64, V, I64, I64, ctypes.c_int32, ctypes.c_int32, V, V, I64, V]
+    G, L, X = ctypes.POINTER(PagedProblem), ctypes.POINTER(Pool), ctypes.POINTER(PagedIndex)
+    for name in ('sa2_paged_attn_workspace_bytes', 'sa2_paged_simplicial_attn_workspace_bytes'):
+        getattr(lib, name).restype = I64
+        getattr(lib, name).argtypes = [G]
+    lib.sa2_paged_attn.restype = ctypes.c_int
+    lib.sa2_paged_attn.argtypes = [G, T, L, L, X, T, V, I64, V]
+    lib.sa2_paged_simplicial_attn.restype = ctypes.c_int
+    lib.sa2_paged_simplicial_attn.argtypes = [G, T, L, L, L, L, X, T, V, I64, V]
+    lib.sa2_paged_append.restype = ctypes.c_int
+    lib.sa2_paged_append.argtypes = [G, ctypes.POINTER(AppendItem), ctypes.c_int32, ctypes.c_int32, X, V]
+    lib.sa2_copy_pages.restype = ctypes.c_int
+    lib.sa2_copy_pages.argtypes = [ctypes.POINTER(PagePool), ctypes.c_int32, V, I64, V]
+    lib.sa2_sample_workspace_bytes.restype = I64
+    lib.sa2_sample_workspace_bytes.argtypes = [I64, I64]
+    lib.sa2_sample.restype = ctypes.c_int
+    lib.sa2_sample.argtypes = [V, ctypes.c_int32, I64, I64, I64, V, I64, ctypes.POINTER(SampleParams), V, V, V, I64, V]
     return lib
 
 

@@ -20,6 +20,7 @@
 #include "sa2_wgrad.hpp"
 #include "sa2_fwd.hpp"
 #include "sa2_launch.hpp"
+#include "sa2_status.hpp"
 #ifdef SA2_PROFILING
 #include "sa2_prof_mix.hpp"
 #endif
@@ -35,6 +36,23 @@ int fail(int code, const char *fmt, ...) {
     va_end(ap);
     return code;
 }
+
+}  // namespace
+
+int sa2::fail_with(int code, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+int sa2::launched(const char *what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? SA2_OK : fail(SA2_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+}
+
+namespace {
 
 int check_problem(const sa2_problem *p) {
     if (!p) return fail(SA2_ERR_NULL_POINTER, "problem is NULL");

@@ -1,0 +1,205 @@
+// C entry points of the attention over paged caches (kernels: sa2_paged.hpp).
+#include "sa2_paged.hpp"
+
+#include <cmath>
+#include <cstdlib>
+
+#include "sa2.h"
+#include "sa2_status.hpp"
+
+namespace {
+
+using namespace sa2;
+
+#define SA2_TRY(expr)                  \
+    do {                               \
+        int rc_ = (expr);              \
+        if (rc_ != SA2_OK) return rc_; \
+    } while (0)
+
+int kernel_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+PageDiv page_div(int ps) {
+    // floor(x / ps) = (x * mul) >> 31 + s with mul = floor(2^(31 + s) / ps) + 1, s = ceil(log2 ps): exact for x < 2^31
+    uint32_t s = 0;
+    while ((1ll << s) < ps) ++s;
+    return {(uint32_t)ps, (uint32_t)((1ull << (31 + s)) / ps + 1), s ? s - 1 : 0};
+}
+
+int check_problem(const sa2_paged_problem *p, bool simplicial) {
+    if (!p) return fail_with(SA2_ERR_NULL_POINTER, "problem is NULL");
+    if (p->batch < 1 || p->rows < 1 || p->heads < 1 || p->kv_heads < 1 || p->page_size < 1 || p->pages < 1 || p->table_width < 1)
+        return fail_with(SA2_ERR_BAD_SHAPE, "batch=%d rows=%d heads=%d kv_heads=%d page_size=%d pages=%d table_width=%d must all be >= 1", p->batch, p->rows,
+                         p->heads, p->kv_heads, p->page_size, p->pages, p->table_width);
+    if (p->heads % p->kv_heads != 0) return fail_with(SA2_ERR_BAD_SHAPE, "heads=%d is not a multiple of kv_heads=%d", p->heads, p->kv_heads);
+    if (p->dim_head < 1 || p->pool_dim < p->dim_head || p->pool_dim > 256 || p->pool_dim % 8 != 0)
+        return fail_with(SA2_ERR_UNSUPPORTED, "dim_head=%d in pools of %d channels: a multiple of 8 up to 256 that holds the head is supported", p->dim_head,
+                         p->pool_dim);
+    if (p->dtype != SA2_ELEMENT_BF16 && p->dtype != SA2_ELEMENT_F16) return fail_with(SA2_ERR_UNSUPPORTED, "dtype %d is not supported (bf16 or fp16)", p->dtype);
+    if (simplicial && (p->w1 < 1 || p->w2 < 1)) return fail_with(SA2_ERR_BAD_SHAPE, "windows w1=%d w2=%d must be >= 1", p->w1, p->w2);
+    if (!(p->scale > 0.f) || !std::isfinite(p->scale)) return fail_with(SA2_ERR_BAD_SHAPE, "scale must be positive and finite");
+    if (p->max_length < 0) return fail_with(SA2_ERR_BAD_SHAPE, "max_length=%d must be >= 0 (0: what the tables can name)", p->max_length);
+    if ((int64_t)p->batch * p->rows * p->heads > 0x1fffffffll) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
+    return SA2_OK;
+}
+
+// How the work is laid out: a function of the problem alone.
+struct Plan {
+    bool many;
+    int dim, row_tiles, splits, dblocks;
+    int64_t grid, rows;
+    int64_t bytes() const { return splits * dblocks > 1 ? splits * dblocks * rows * (dim * 4 + 8) : 0; }
+};
+
+Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
+    Plan x{};
+    x.dim = kernel_dim(p->pool_dim);
+    x.rows = (int64_t)p->batch * p->rows * p->heads;
+    const int G = p->heads / p->kv_heads;
+    const int64_t per = (int64_t)p->rows * G, seqs = (int64_t)p->batch * p->kv_heads;
+    const int64_t reach = (int64_t)p->table_width * p->page_size;
+    const int64_t most = p->max_length > 0 && p->max_length < reach ? p->max_length : reach;
+    const int64_t keys = simplicial && p->w1 < most ? p->w1 : most;
+    const int64_t tiles = (keys + 31) / 32;
+    x.dblocks = simplicial ? (p->w2 + 31) / 32 : 1;
+    const int waves = x.dim == 256 ? 4 : 8;
+    x.many = simplicial ? per >= 8 : per > 32;
+    const int64_t per_wg = x.many ? (simplicial ? waves : waves * 32) : (simplicial ? 1 : 32);
+    x.row_tiles = (int)((per + per_wg - 1) / per_wg);
+    const int64_t items = seqs * x.row_tiles * x.dblocks;
+    // two workgroups per CU; a share has at least `least` tiles (a wave of the few-row form then has two)
+    const int64_t few_waves = x.dim == 256 ? 2 : x.dim == 128 ? 4 : 8;
+    const int64_t least = x.many ? 32 : 4 * few_waves;
+    int64_t splits = (512 + items - 1) / items;
+    if (splits > tiles / least) splits = tiles / least;
+    x.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
+    x.grid = items * x.splits;
+    return x;
+}
+
+int check_pool(const sa2_paged_problem *p, const sa2_pool *t, const char *name) {
+    if (!t || !t->ptr) return fail_with(SA2_ERR_NULL_POINTER, "pool %s is NULL", name);
+    if ((reinterpret_cast<uintptr_t>(t->ptr) & 15) != 0 || (t->stride_page & 7) != 0 || (t->stride_row & 7) != 0 || (t->stride_head & 7) != 0)
+        return fail_with(SA2_ERR_ALIGNMENT, "pool %s: base pointer must be 16-byte aligned and strides multiples of 8 elements", name);
+    (void)p;
+    return SA2_OK;
+}
+
+PagedPool pool_of(const sa2_pool *t) {
+    PagedPool x{};
+    if (t) x = {static_cast<const char *>(t->ptr), t->stride_page * 2, t->stride_row * 2, t->stride_head * 2};
+    return x;
+}
+
+bool whole_pieces(const sa2_tensor *t, int channels) {
+    return channels % 8 == 0 && (reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && t->stride_b % 8 == 0 && t->stride_n % 8 == 0 && t->stride_h % 8 == 0;
+}
+
+template <class E, int D, bool SIMP>
+void launch(const Plan &x, const PagedParams &k, hipStream_t stream) {
+    if (x.many) hipLaunchKernelGGL((paged_many_kernel<E, D, SIMP>), dim3((unsigned)x.grid), dim3(ManyCfg<D>::NW * 64), 0, stream, k);
+    else hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP>), dim3((unsigned)x.grid), dim3(FewCfg<D>::NW * 64), 0, stream, k);
+    if (x.splits * x.dblocks > 1) {
+        const int per = 256 / (D / 8);
+        hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)((x.rows + per - 1) / per)), dim3(256), 0, stream, k);
+    }
+}
+
+template <class E, bool SIMP>
+void launch_dim(const Plan &x, const PagedParams &k, hipStream_t stream) {
+    switch (x.dim) {
+        case 32: launch<E, 32, SIMP>(x, k, stream); break;
+        case 64: launch<E, 64, SIMP>(x, k, stream); break;
+        case 128: launch<E, 128, SIMP>(x, k, stream); break;
+        default: launch<E, 256, SIMP>(x, k, stream); break;
+    }
+}
+
+int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, const sa2_pool *k1, const sa2_pool *k2, const sa2_pool *v1, const sa2_pool *v2,
+           const sa2_paged_index *at, const sa2_tensor *out, void *workspace, int64_t workspace_bytes, void *stream) {
+    SA2_TRY(check_problem(p, simplicial));
+    SA2_TRY(check_pool(p, k1, simplicial ? "k1" : "k"));
+    SA2_TRY(check_pool(p, v1, simplicial ? "v1" : "v"));
+    if (simplicial) {
+        SA2_TRY(check_pool(p, k2, "k2"));
+        SA2_TRY(check_pool(p, v2, "v2"));
+    }
+    if (!q || !q->ptr) return fail_with(SA2_ERR_NULL_POINTER, "tensor q is NULL");
+    if (!out || !out->ptr) return fail_with(SA2_ERR_NULL_POINTER, "tensor out is NULL");
+    if (!at || !at->tables || !at->lengths) return fail_with(SA2_ERR_NULL_POINTER, "tables and lengths are required");
+    const Plan x = plan_of(p, simplicial);
+    if (x.grid > 0x7fffffffll) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
+    if (x.bytes() > 0 && (!workspace || workspace_bytes < x.bytes()))
+        return fail_with(SA2_ERR_BAD_SHAPE, "workspace of %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0), (long long)x.bytes());
+    if (x.bytes() > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return fail_with(SA2_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
+    PagedParams k{};
+    k.q = static_cast<const char *>(q->ptr);
+    k.q_sb = q->stride_b * 2;
+    k.q_sn = q->stride_n * 2;
+    k.q_sh = q->stride_h * 2;
+    k.o = static_cast<char *>(out->ptr);
+    k.o_sb = out->stride_b * 2;
+    k.o_sn = out->stride_n * 2;
+    k.o_sh = out->stride_h * 2;
+    k.k1 = pool_of(k1);
+    k.v1 = pool_of(v1);
+    k.k2 = pool_of(k2);
+    k.v2 = pool_of(v2);
+    k.tables = at->tables;
+    k.lengths = at->lengths;
+    k.counts = at->counts;
+    k.t_sb = at->table_stride;
+    k.div = page_div(p->page_size);
+    k.pages = p->pages;
+    k.width = p->table_width;
+    k.B = p->batch;
+    k.n = p->rows;
+    k.H = p->heads;
+    k.HK = p->kv_heads;
+    k.G = p->heads / p->kv_heads;
+    k.dq = p->dim_head;
+    k.dp = p->pool_dim;
+    k.q_vec = whole_pieces(q, p->dim_head);
+    k.o_vec = whole_pieces(out, p->dim_head);
+    k.w1 = p->w1;
+    k.w2 = p->w2;
+    k.scale_log2e = p->scale * kLog2e;
+    k.row_tiles = x.row_tiles;
+    k.splits = x.splits;
+    k.dblocks = x.dblocks;
+    if (x.bytes() > 0) {
+        k.part_o = static_cast<float *>(workspace);
+        k.part_ml = reinterpret_cast<float2 *>(k.part_o + (int64_t)x.splits * x.dblocks * x.rows * x.dim);
+    }
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (p->dtype == SA2_ELEMENT_F16) {
+        if (simplicial) launch_dim<ElemF16, true>(x, k, s);
+        else launch_dim<ElemF16, false>(x, k, s);
+    } else {
+        if (simplicial) launch_dim<ElemBf16, true>(x, k, s);
+        else launch_dim<ElemBf16, false>(x, k, s);
+    }
+    return launched(simplicial ? "paged 2-simplicial attention" : "paged attention");
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t sa2_paged_attn_workspace_bytes(const sa2_paged_problem *prob) { return check_problem(prob, false) == SA2_OK ? plan_of(prob, false).bytes() : -1; }
+
+int sa2_paged_attn(const sa2_paged_problem *prob, const sa2_tensor *q, const sa2_pool *k, const sa2_pool *v, const sa2_paged_index *at, const sa2_tensor *out,
+                   void *workspace, int64_t workspace_bytes, void *hip_stream) {
+    return attend(false, prob, q, k, nullptr, v, nullptr, at, out, workspace, workspace_bytes, hip_stream);
+}
+
+int64_t sa2_paged_simplicial_attn_workspace_bytes(const sa2_paged_problem *prob) {
+    return check_problem(prob, true) == SA2_OK ? plan_of(prob, true).bytes() : -1;
+}
+
+int sa2_paged_simplicial_attn(const sa2_paged_problem *prob, const sa2_tensor *q, const sa2_pool *k1, const sa2_pool *k2, const sa2_pool *v1, const sa2_pool *v2,
+                              const sa2_paged_index *at, const sa2_tensor *out, void *workspace, int64_t workspace_bytes, void *hip_stream) {
+    return attend(true, prob, q, k1, k2, v1, v2, at, out, workspace, workspace_bytes, hip_stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,810 @@
+// Attention of new tokens over a paged cache: dense causal attention and its sliding-window 2-simplicial form.
+//
+// A pool holds pages of `ps` rows; position x of a sequence is row x % ps of page table[x / ps].  Row t of a sequence's chunk sits at
+// position p = length - count + t.  Both operators are one product pair over 32-row key tiles and 32 columns,
+//     S^T = K A^T      P^T = exp2(c S^T - M)      O^T += V^T P^T        (c = scale log2(e), M the column's reference)
+// and differ in what a column is:
+//   dense        column = (token, query head of the group):  A = q, keys 0 .. p, the column's O is an output row
+//   2-simplicial column = offset d = p - k of ONE (token, query head):  A = q * k2[p - d], keys (p - w1, p] of the first set,
+//                o = sum over columns of v2[p - d] * O, so the 32 offsets of a token share its window and one product does them all
+// Softmax: the reference M of a column moves only when a tile's weights outgrow 2^60 (fp16: 2^14) on it, the first tile included
+// (M starts far below every logit), so the ordinary tile has no maximum and no rescale.  Sums and accumulators are fp32; the weights
+// are rounded to the element type for the second product, and so is q * k2 for the first.
+//
+// Keys that are not there (beyond the walked range, missing pages) are fetched from a row of zeros and masked; a value row that a
+// column does not attend never reaches it, whatever it holds (0 * NaN is not 0: see value_products).
+#pragma once
+
+#include "sa2_common.hpp"
+#include "sa2_lds.hpp"
+
+namespace sa2 {
+
+struct ElemBf16 {
+    static constexpr float kBig = 1.152921504606846976e18f;      // 2^60
+    static constexpr uint32_t kExp = 0x7f80u;
+    static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
+    static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+    static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) { return mfma32(a, b, c); }
+};
+
+struct ElemF16 {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    static constexpr float kBig = 16384.f;                       // 2^14: weights stay below the largest fp16 number
+    static constexpr uint32_t kExp = 0x7c00u;
+    static __device__ __forceinline__ float lo(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
+    static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        f16x2 v = {(_Float16)a, (_Float16)b};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+    static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+
+struct PagedPool {
+    const char *ptr;
+    int64_t sp, sr, sh;       // bytes between pages, rows of a page, heads
+};
+
+// division by the page size as a multiplication (dividends below 2^31)
+struct PageDiv {
+    uint32_t ps, mul, shift;
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return ps == 1 ? x : __umulhi(x, mul) >> shift; }
+};
+
+struct PagedParams {
+    const char *q;
+    int64_t q_sb, q_sn, q_sh;
+    char *o;
+    int64_t o_sb, o_sn, o_sh;
+    PagedPool k1, v1, k2, v2;                 // (k2, v2: 2-simplicial form only)
+    const int32_t *tables, *lengths, *counts; // (counts nullptr: n for every sequence)
+    int64_t t_sb;
+    PageDiv div;
+    int pages, width;                         // pages of a pool, entries of a table
+    int B, n, H, HK, G;
+    int dq, dp;                               // channels of q and the output, and of a pool's row (a multiple of 8)
+    int q_vec, o_vec;                         // rows of q / the output are 16-byte aligned and whole pieces
+    int w1, w2;
+    float scale_log2e;
+    int row_tiles;                            // workgroups (per sequence and key/value head) that the rows take
+    int splits, dblocks;                      // shares of the keys; blocks of 32 offsets
+    // partial results where splits * dblocks > 1: fp32 [part][B n H][D] and [part][B n H] (reference, sum)
+    float *part_o;
+    float2 *part_ml;
+};
+
+constexpr float kNoRef = -1e30f;              // reference of a column that has met no key yet
+__device__ __attribute__((aligned(16))) uint32_t g_paged_zero_row[4];
+
+// One direct-to-LDS load of 16 bytes per lane from addresses of its own (load_to_lds16 with 64-bit lane addresses)
+__device__ __forceinline__ void load_to_lds16_from(const char *addr, uint32_t lds_addr) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(addr), "s"(lds_addr) : "memory");
+}
+// LDS reads issued before have left the memory (a direct load may overwrite what they read)
+__device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// ---- what a workgroup knows about its sequence
+struct PagedSeq {
+    const int32_t *table;
+    int first, count;        // position of row 0 of the chunk (negative: rows before the sequence attend to nothing), rows that are there
+    int reach;               // positions that the table can name
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedParams &p, int b) {
+    PagedSeq s;
+    s.table = p.tables + b * p.t_sb;
+    const int length = p.lengths[b];
+    int count = p.counts ? p.counts[b] : p.n;
+    count = count < 0 ? 0 : (count > p.n ? p.n : count);
+    s.first = (length < 0 ? 0 : length) - count;
+    s.count = count;
+    const int64_t reach = (int64_t)p.width * p.div.ps;
+    s.reach = reach > 0x7fffffff ? 0x7fffffff : (int)reach;
+    return s;
+}
+// page of a position, -1 where there is none
+__device__ __forceinline__ int paged_page(const PagedParams &p, const PagedSeq &s, int x) {
+    if (x < 0 || x >= s.reach) return -1;
+    const int id = s.table[p.div((uint32_t)x)];
+    return (unsigned)id < (unsigned)p.pages ? id : -1;
+}
+__device__ __forceinline__ const char *paged_row(const PagedPool &pool, int page, int row) {
+    return pool.ptr + (int64_t)page * pool.sp + (int64_t)row * pool.sr;
+}
+
+// channels d0 .. d0 + 7 of a row of q as a packed piece (zeros beyond its channels)
+template <class E>
+__device__ __forceinline__ u32x4 paged_q_piece(const PagedParams &p, const char *row, int d0) {
+    if (p.q_vec) return d0 < p.dq ? ld_global16(row + d0 * 2) : (u32x4){0u, 0u, 0u, 0u};
+    u32x4 r;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t a = d0 + 2 * w < p.dq ? *reinterpret_cast<const uint16_t *>(row + (d0 + 2 * w) * 2) : 0u;
+        const uint32_t b = d0 + 2 * w + 1 < p.dq ? *reinterpret_cast<const uint16_t *>(row + (d0 + 2 * w + 1) * 2) : 0u;
+        r[w] = a | (b << 16);
+    }
+    return r;
+}
+template <class E>
+__device__ __forceinline__ void paged_store8(const PagedParams &p, char *row, int d0, const float (&x)[8]) {
+    const u32x4 v = {E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(x[4], x[5]), E::pack(x[6], x[7])};
+    if (p.o_vec) {
+        if (d0 < p.dq) st_global16(row + d0 * 2, v);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (d0 + e < p.dq) *reinterpret_cast<uint16_t *>(row + (d0 + e) * 2) = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+}
+
+// ---- one wave's 32 columns
+template <class E, int D>
+struct PagedWave {
+    using RT = DmaTile<D>;
+    static constexpr int KS = D / 16, DT = D / 32;
+    u32x4 A[KS];
+    f32x16 O[DT];
+    float M, l;              // reference (log2 units) and this half's sum of the column's weights
+    int lo, hi;              // keys the column attends (empty: lo > hi)
+    int most_lo, least_hi;   // over the columns that attend to anything: keys between them need no mask
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) O[dt] = zero16();
+        M = kNoRef;
+        l = 0.f;
+    }
+    __device__ __forceinline__ void limits(int lo_, int hi_, bool on) {
+        lo = on ? lo_ : 1;
+        hi = on ? hi_ : 0;
+        int a = on ? lo_ : -0x7fffffff, z = on ? hi_ : 0x7fffffff;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            a = max(a, __shfl_xor(a, m));
+            z = min(z, __shfl_xor(z, m));
+        }
+        most_lo = uniform(a);
+        least_hi = uniform(z);
+    }
+
+    __device__ __forceinline__ static float both_halves_max(float x) {
+        auto sw = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);
+        return fmaxf(as_f32(sw[0]), as_f32(sw[1]));
+    }
+
+    __device__ __forceinline__ f32x16 logits(const char *k_lane) const {
+        f32x16 S = zero16();
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) S = E::mfma(RT::row_frag(k_lane, kk), A[kk], S);
+        return S;
+    }
+
+    // keys of the tile at `tile` that are there: bit j; masks S accordingly
+    __device__ __forceinline__ void mask(f32x16 &S, int tile, uint32_t there, int hf) const {
+        const int a = lo - tile - 4 * hf, z = hi - tile - 4 * hf;
+        const uint32_t bits = there >> (4 * hf);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int j = 8 * (r >> 2) + (r & 3);
+            S[r] = j >= a && j <= z && ((bits >> j) & 1u) ? S[r] : -INFINITY;
+        }
+    }
+
+    // weights of a tile, packed; moves the column's reference where they outgrow it
+    __device__ __forceinline__ void weights(const f32x16 &S, float c, u32x4 (&pb)[2]) {
+        float sum = 0.f;
+        auto take = [&] {
+            sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const float e0 = fast_exp2(S[r] * c - M), e1 = fast_exp2(S[r + 1] * c - M);
+                sum += e0 + e1;
+                pb[r >> 3][(r & 7) >> 1] = E::pack(e0, e1);
+            }
+        };
+        take();
+        if (__builtin_expect(wave_any(!(sum < E::kBig)), 0)) {
+            float top = S[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, S[r]);
+            const float ref = fmaxf(M, both_halves_max(top) * c);
+            const float f = fast_exp2(M - ref);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) O[dt][r] *= f;
+            l *= f;
+            M = ref;
+            take();
+        }
+        l += sum;
+    }
+
+    // O^T += V^T P^T.  `guard`: some column does not attend some key of the tile, so a value that is not finite must be kept from it.
+    // `ONE` (all columns attend to the same keys): those the columns do not attend are cleared in the operand.  Otherwise, where the tile
+    // holds such a value, every group of columns with its own last key gets a product of its own.
+    template <bool ONE>
+    __device__ __forceinline__ void values(const char *v_lane, const u32x4 (&pb)[2], bool guard, int tile, uint32_t there, int hf) {
+        if (!guard) {
+#pragma unroll
+            for (int k2s = 0; k2s < 2; ++k2s)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) O[dt] = E::mfma(RT::tr_frag(v_lane, k2s, dt), pb[k2s], O[dt]);
+            return;
+        }
+        auto key_masks = [&](uint32_t keys, u32x4 (&m)[2]) {
+            const uint32_t bits = keys >> (4 * hf);
+#pragma unroll
+            for (int k2s = 0; k2s < 2; ++k2s)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int j = 16 * k2s + 8 * (w >> 1) + 2 * (w & 1);
+                    m[k2s][w] = ((bits >> j) & 1u ? 0xffffu : 0u) | ((bits >> (j + 1)) & 1u ? 0xffff0000u : 0u);
+                }
+        };
+        auto keys_up_to = [&](int a, int z) {       // keys a .. z of the tile
+            a = a - tile < 0 ? 0 : a - tile;
+            z = z - tile > 31 ? 31 : z - tile;
+            return a > z ? 0u : (0xffffffffu >> (31 - z)) & (0xffffffffu << a);
+        };
+        if (ONE) {
+            u32x4 m[2];
+            key_masks(there & keys_up_to(most_lo, least_hi), m);
+#pragma unroll
+            for (int k2s = 0; k2s < 2; ++k2s)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) O[dt] = E::mfma(RT::tr_frag(v_lane, k2s, dt) & m[k2s], pb[k2s], O[dt]);
+            return;
+        }
+        uint32_t odd = 0u;
+#pragma unroll
+        for (int k2s = 0; k2s < 2; ++k2s)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const u32x4 v = RT::tr_frag(v_lane, k2s, dt);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) odd |= (uint32_t)((v[w] & E::kExp) == E::kExp) | (uint32_t)(((v[w] >> 16) & E::kExp) == E::kExp);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        asm volatile("" ::: "memory");         // (the products read the tile again: held, it would take all registers)
+        if (__builtin_expect(!wave_any(odd != 0u), 1)) {
+#pragma unroll
+            for (int k2s = 0; k2s < 2; ++k2s)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) O[dt] = E::mfma(RT::tr_frag(v_lane, k2s, dt), pb[k2s], O[dt]);
+            return;
+        }
+        // last keys inside the tile, then the columns that attend to all of it
+        for (int z = max(0, min(31, least_hi - tile)); z < 32; ++z) {
+            const bool mine = lo <= hi && (z < 31 ? hi - tile == z : hi - tile >= 31);
+            if (!wave_any(mine)) continue;
+            u32x4 m[2];
+            key_masks(there & keys_up_to(0, tile + z), m);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                f32x16 x = zero16();
+#pragma unroll
+                for (int k2s = 0; k2s < 2; ++k2s) x = E::mfma(RT::tr_frag(v_lane, k2s, dt) & m[k2s], pb[k2s], x);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) O[dt][r] = mine ? O[dt][r] + x[r] : O[dt][r];
+                asm volatile("" ::: "memory");
+            }
+        }
+    }
+
+    __device__ __forceinline__ bool needs_mask(int tile, uint32_t there) const { return tile < most_lo || tile + 31 > least_hi || there != 0xffffffffu; }
+
+    // the sum of the column's weights, in both halves
+    __device__ __forceinline__ float whole_sum() const {
+        auto sw = __builtin_amdgcn_permlane32_swap(as_u32(l), as_u32(l), false, false);
+        return as_f32(sw[0]) + as_f32(sw[1]);
+    }
+};
+
+// ---- 2-simplicial form: from the columns (offsets) of one (token, head) to its output row
+//
+// y[v] of a lane: channel 32 (v / 16) + 16 hf + v % 16 of its column.  Adds the columns and leaves NV / 32 (at least one) sums per
+// lane: y[i] of lane c is the sum for v = base(c) + i.
+template <int NV>
+struct ColumnSum {
+    static constexpr int LEFT = NV > 32 ? NV / 32 : 1;
+    static __device__ __forceinline__ int base(int c) {
+        int b = 0, n = NV;
+#pragma unroll
+        for (int bit = 16; bit >= 1; bit >>= 1)
+            if (n > 1) {
+                n /= 2;
+                b += c & bit ? n : 0;
+            }
+        return b;
+    }
+    template <int N, int BIT>
+    static __device__ __forceinline__ void step(float (&y)[NV], int c) {
+        if constexpr (BIT >= 1) {
+            if constexpr (N > 1) {
+                const bool up = c & BIT;
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) {
+                    const float keep = up ? y[i + N / 2] : y[i], send = up ? y[i] : y[i + N / 2];
+                    y[i] = keep + __shfl_xor(send, BIT);
+                }
+                step<N / 2, BIT / 2>(y, c);
+            } else {
+                y[0] += __shfl_xor(y[0], BIT);
+                step<1, BIT / 2>(y, c);
+            }
+        }
+    }
+    static __device__ __forceinline__ void add(float (&y)[NV], int c) { step<NV, 16>(y, c); }
+};
+
+template <class E, int D>
+struct SimplicialColumns {
+    static constexpr int KS = D / 16, DT = D / 32;
+    int page2, row2;          // place of the column's second row (page2 < 0: there is none)
+
+    // A = q * k2 of the column's offset
+    __device__ __forceinline__ void build(const PagedParams &p, const PagedSeq &s, PagedWave<E, D> &w, const char *q_row, int pos, int d, int hk, int hf, bool on) {
+        const int x = pos - d;
+        page2 = on && d < p.w2 ? paged_page(p, s, x) : -1;
+        row2 = page2 >= 0 ? x - (int)p.div((uint32_t)x) * (int)p.div.ps : 0;
+        const char *k2 = paged_row(p.k2, page2, row2) + hk * p.k2.sh;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            const int d0 = 16 * kk + 8 * hf;
+            u32x4 a = {0u, 0u, 0u, 0u};
+            if (page2 >= 0 && d0 < p.dp) {
+                const u32x4 f = paged_q_piece<E>(p, q_row, d0), k = ld_global16(k2 + d0 * 2);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = E::pack(E::lo(f[i]) * E::lo(k[i]), E::hi(f[i]) * E::hi(k[i]));
+            }
+            w.A[kk] = a;
+        }
+    }
+
+    // the wave's columns as one row relative to one reference: o[v] (see ColumnSum), ref, sum
+    __device__ __forceinline__ void finish(const PagedParams &p, const PagedWave<E, D> &w, int hk, int c, int hf, float (&y)[16 * DT], float &ref, float &sum) const {
+        // (columns without a second row, and those that met no key, hold nothing that counts)
+        const float column = w.whole_sum();
+        const bool live = page2 >= 0 && column != 0.f;
+        ref = live ? w.M : kNoRef;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) ref = fmaxf(ref, __shfl_xor(ref, m));
+        const float f = live ? fast_exp2(w.M - ref) : 0.f;
+        sum = live ? column * f : 0.f;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) sum += __shfl_xor(sum, m);
+        const char *v2 = paged_row(p.v2, page2, row2) + hk * p.v2.sh;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int d0 = 32 * dt + 16 * hf + 8 * half;
+                const bool there = live && d0 < p.dp;
+                const u32x4 v = there ? ld_global16(v2 + d0 * 2) : (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = 16 * dt + 8 * half + 2 * i;
+                    y[at] = there ? w.O[dt][8 * half + 2 * i] * f * E::lo(v[i]) : 0.f;
+                    y[at + 1] = there ? w.O[dt][8 * half + 2 * i + 1] * f * E::hi(v[i]) : 0.f;
+                }
+            }
+        ColumnSum<16 * DT>::add(y, c);
+    }
+};
+
+// ---- few rows: every wave walks key tiles of its own
+//
+// A workgroup has 32 columns (dense: up to 32 rows of one sequence and key/value head; 2-simplicial: one token and head) and a share
+// of their keys; its waves take the tiles in turn, each with a K and a V tile of its own in LDS, and merge at the end.  No barrier in the walk: the
+// next K tile is requested when the logits of a tile are formed, the next V tile behind its second product, so a wave always has
+// a tile in flight and a CU sixteen waves of them.
+template <int D>
+struct FewCfg {
+    using RT = DmaTile<D>;
+    static constexpr int NW = D == 256 ? 2 : D == 128 ? 4 : 8;
+    static constexpr int SEG = 2048;                                // positions whose pages are kept in LDS at a time
+    static constexpr int RING = NW * 2 * RT::BYTES;
+    static_assert(RING - RT::CP < 65536, "the LDS address of a direct load travels in 16 bits of M0");
+    static constexpr int OP = D + 4;                                // floats per row of the merge
+    static constexpr int MERGE = NW * 32 * OP * 4;
+    static constexpr int WALK = RING + SEG * 4;
+    static constexpr int XCH = MERGE > WALK ? MERGE : WALK;         // references and sums of the waves
+    static constexpr int LDS = XCH + 2 * NW * 32 * 4;
+};
+
+template <class E, int D, bool SIMP>
+__global__ __launch_bounds__(FewCfg<D>::NW * 64) void paged_few_kernel(PagedParams p) {
+    using C = FewCfg<D>;
+    using RT = DmaTile<D>;
+    constexpr int NW = C::NW, DT = D / 32;
+    __shared__ __attribute__((aligned(16))) char lds[C::LDS];
+    int *seg = reinterpret_cast<int *>(lds + C::RING);
+    const int tid = threadIdx.x, wave = wave_index(), lane = tid & 63, c = lane & 31, hf = lane >> 5;
+
+    // item = ((b, hk), row tile, part)
+    const int parts = p.splits * p.dblocks;
+    int item = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int part = uniform(item % parts);
+    item = uniform(item / parts);
+    const int tile_r = uniform(item % p.row_tiles);
+    item = uniform(item / p.row_tiles);
+    const int hk = uniform(item % p.HK), b = uniform(item / p.HK);
+    const int split = uniform(part % p.splits), db = uniform(part / p.splits);
+    const PagedSeq s = paged_seq(p, b);
+
+    // the columns: token t, head of the group g
+    const int R = SIMP ? tile_r : tile_r * 32 + c;
+    const int t = R / p.G, g = R - t * p.G, h = hk * p.G + g;
+    const int pos = s.first + t;
+    const bool row_there = R < p.n * p.G;
+    const bool on = row_there && t < s.count && pos >= 0;
+    const int t_last = SIMP ? t : min((tile_r * 32 + 31) / p.G, s.count - 1);
+    const int last = min(s.first + t_last, s.reach - 1);              // last key of any column
+    const int first_key = SIMP ? max(0, s.first + t - p.w1 + 1) : 0;
+    const bool any = SIMP ? on : tile_r * 32 / p.G < s.count && last >= 0;
+    const int tiles = any && last >= first_key ? (last - first_key) / 32 + 1 : 0;
+    const int tile_a = (int)((int64_t)tiles * split / p.splits), tile_z = (int)((int64_t)tiles * (split + 1) / p.splits);
+
+    const char *q_row = p.q + b * p.q_sb + (int64_t)(row_there ? t : 0) * p.q_sn + (int64_t)(row_there ? h : 0) * p.q_sh;
+    PagedWave<E, D> w;
+    SimplicialColumns<E, D> cols;
+    w.clear();
+    if (tile_a < tile_z) {
+        if constexpr (SIMP) {
+            cols.build(p, s, w, q_row, pos, 32 * db + c, hk, hf, on);
+            w.limits(first_key, pos, on && cols.page2 >= 0);
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) w.A[kk] = on ? paged_q_piece<E>(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
+            w.limits(0, pos, on);
+        }
+    } else if constexpr (SIMP) {
+        cols.page2 = -1;
+        cols.row2 = 0;
+    }
+
+    const char *const kg = p.k1.ptr + hk * p.k1.sh, *const vg = p.v1.ptr + hk * p.v1.sh;
+    char *const kt = lds + wave * 2 * RT::BYTES, *const vt = kt + RT::BYTES;
+    const uint32_t kt_at = (uint32_t)(uintptr_t)kt, vt_at = (uint32_t)(uintptr_t)vt;
+    const char *const zero = reinterpret_cast<const char *>(g_paged_zero_row);
+    const int st_col = RT::st_col(lane);
+    const bool col_there = st_col < p.dp * 2;
+    constexpr int SEG_TILES = C::SEG / 32;
+    for (int seg_a = tile_a; seg_a < tile_z; seg_a += SEG_TILES) {
+        const int seg_z = min(tile_z, seg_a + SEG_TILES);
+        __syncthreads();
+        for (int x = tid; x < (seg_z - seg_a) * 32; x += NW * 64) {
+            const int at = first_key + seg_a * 32 + x;
+            seg[x] = at <= last ? paged_page(p, s, at) : -1;
+        }
+        __syncthreads();
+        auto request = [&](const PagedPool &pool, const char *base, uint32_t lds_at, int tile) {
+#pragma unroll
+            for (int ch = 0; ch < RT::NCH; ++ch) {
+                const int x = 32 * (tile - seg_a) + RT::st_row(ch, lane);
+                const int at = first_key + 32 * seg_a + x, page = seg[x];
+                const int row = at - (int)p.div((uint32_t)at) * (int)p.div.ps;
+                const char *from = base + (int64_t)page * pool.sp + (int64_t)row * pool.sr + st_col;
+                load_to_lds16_from(page >= 0 && col_there ? from : zero, lds_at + ch * RT::CP);
+            }
+        };
+        int u = seg_a + wave;
+        if (u < seg_z) {
+            request(p.k1, kg, kt_at, u);
+            request(p.v1, vg, vt_at, u);
+        }
+        for (; u < seg_z; u += NW) {
+            const int tile = first_key + 32 * u, next = u + NW;
+            const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(seg[32 * (u - seg_a) + c] >= 0);
+            wait_loads<RT::NCH>();
+            f32x16 S = w.logits(kt + RT::row_lane(lane));
+            wait_lds_reads();
+            if (next < seg_z) request(p.k1, kg, kt_at, next);
+            const bool masked = w.needs_mask(tile, there);
+            if (masked) w.mask(S, tile, there, hf);
+            u32x4 pb[2];
+            w.weights(S, p.scale_log2e, pb);
+            if (next < seg_z) wait_loads<RT::NCH>();
+            else wait_loads<0>();
+            // (a workgroup with one token has no key that some of its columns attend and others do not)
+            w.template values<SIMP>(vt + RT::tr_lane(lane), pb, !SIMP && p.n > 1 && masked, tile, there, hf);
+            wait_lds_reads();
+            if (next < seg_z) request(p.v1, vg, vt_at, next);
+        }
+    }
+
+    // ---- merge of the waves
+    __syncthreads();
+    float *xm = reinterpret_cast<float *>(lds + C::XCH), *xl = xm + NW * 32;
+    float *mo = reinterpret_cast<float *>(lds);
+    const int64_t rows = (int64_t)p.B * p.n * p.H;
+    if constexpr (SIMP) {
+        float y[16 * DT], ref, sum;
+        cols.finish(p, w, hk, c, hf, y, ref, sum);
+        if (lane == 0) {
+            xm[wave] = ref;
+            xl[wave] = sum;
+        }
+        const int base = ColumnSum<16 * DT>::base(c);
+#pragma unroll
+        for (int i = 0; i < ColumnSum<16 * DT>::LEFT; ++i) {
+            const int v = base + i;
+            mo[wave * D + 32 * (v >> 4) + 16 * hf + (v & 15)] = y[i];
+        }
+        __syncthreads();
+        float top = xm[0], total = 0.f;
+#pragma unroll
+        for (int x = 1; x < NW; ++x) top = fmaxf(top, xm[x]);
+#pragma unroll
+        for (int x = 0; x < NW; ++x) total += xl[x] * fast_exp2(xm[x] - top);
+        const int64_t row = ((int64_t)b * p.n + t) * p.H + h;
+        for (int d0 = tid * 8; d0 < D; d0 += NW * 64 * 8) {
+            float z[8] = {};
+#pragma unroll
+            for (int x = 0; x < NW; ++x) {
+                const float f = fast_exp2(xm[x] - top);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] += f * mo[x * D + d0 + e];
+            }
+            if (parts == 1) {
+                const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] *= inv;
+                paged_store8<E>(p, p.o + b * p.o_sb + t * p.o_sn + h * p.o_sh, d0, z);
+            } else {
+                float *dst = p.part_o + ((int64_t)part * rows + row) * D + d0;
+                *reinterpret_cast<float4 *>(dst) = make_float4(z[0], z[1], z[2], z[3]);
+                *reinterpret_cast<float4 *>(dst + 4) = make_float4(z[4], z[5], z[6], z[7]);
+            }
+        }
+        if (parts > 1 && tid == 0) p.part_ml[part * rows + row] = make_float2(top, total);
+    } else {
+        if (!on) w.clear();
+        const float sum = w.whole_sum();
+        if (hf == 0) {
+            xm[wave * 32 + c] = w.M;
+            xl[wave * 32 + c] = sum;
+        }
+        if (row_there) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    *reinterpret_cast<float4 *>(mo + (wave * 32 + c) * C::OP + 32 * dt + 16 * hf + r) =
+                        make_float4(w.O[dt][r], w.O[dt][r + 1], w.O[dt][r + 2], w.O[dt][r + 3]);
+        }
+        __syncthreads();
+        const int rows_here = min(32, p.n * p.G - tile_r * 32);
+        for (int x = tid; x < rows_here * (D / 8); x += NW * 64) {
+            const int rr = x / (D / 8), d0 = 8 * (x % (D / 8));
+            float top = xm[rr], total = 0.f, z[8] = {};
+#pragma unroll
+            for (int y = 1; y < NW; ++y) top = fmaxf(top, xm[y * 32 + rr]);
+#pragma unroll
+            for (int y = 0; y < NW; ++y) {
+                const float f = fast_exp2(xm[y * 32 + rr] - top);
+                total += f * xl[y * 32 + rr];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] += f * mo[(y * 32 + rr) * C::OP + d0 + e];
+            }
+            const int R2 = tile_r * 32 + rr, t2 = R2 / p.G, h2 = hk * p.G + R2 - t2 * p.G;
+            if (parts == 1) {
+                const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] *= inv;
+                paged_store8<E>(p, p.o + b * p.o_sb + t2 * p.o_sn + h2 * p.o_sh, d0, z);
+            } else {
+                const int64_t row = ((int64_t)b * p.n + t2) * p.H + h2;
+                float *dst = p.part_o + ((int64_t)part * rows + row) * D + d0;
+                *reinterpret_cast<float4 *>(dst) = make_float4(z[0], z[1], z[2], z[3]);
+                *reinterpret_cast<float4 *>(dst + 4) = make_float4(z[4], z[5], z[6], z[7]);
+                if (d0 == 0) p.part_ml[part * rows + row] = make_float2(top, total);
+            }
+        }
+    }
+}
+
+// ---- many rows: the waves of a workgroup walk the same key tiles
+//
+// A workgroup has NW x 32 columns (dense: rows of one sequence and key/value head; 2-simplicial: NW (token, head) units) and walks the
+// union of their keys; K and V tiles stream through an LDS ring that all waves read, one tile and one barrier per step.
+template <int D>
+struct ManyCfg {
+    using RT = DmaTile<D>;
+    static constexpr int NW = D == 256 ? 4 : 8;
+    static constexpr int BUF = 2 * RT::BYTES;                       // a K tile and a V tile
+    static constexpr int NBUF = D == 256 ? 2 : 4;
+    static constexpr int RING = NBUF * BUF;
+    static_assert(RING - RT::CP < 65536, "the LDS address of a direct load travels in 16 bits of M0");
+    static constexpr int SEG = 2048;                                // circular: pages of 64 tiles, refilled by halves
+    static constexpr int LDS = RING + SEG * 4;
+    static constexpr int LOADS = 2 * RT::NCH > NW ? 2 * RT::NCH / NW : 1;    // per wave and tile
+};
+
+template <class E, int D, bool SIMP>
+__global__ __launch_bounds__(ManyCfg<D>::NW * 64) void paged_many_kernel(PagedParams p) {
+    using C = ManyCfg<D>;
+    using RT = DmaTile<D>;
+    constexpr int NW = C::NW, DT = D / 32, NBUF = C::NBUF;
+    __shared__ __attribute__((aligned(16))) char lds[C::LDS];
+    int *seg = reinterpret_cast<int *>(lds + C::RING);
+    const int tid = threadIdx.x, wave = wave_index(), lane = tid & 63, c = lane & 31, hf = lane >> 5;
+    constexpr int PER_WG = SIMP ? NW : NW * 32;        // rows (t, g) of a workgroup
+
+    const int parts = p.splits * p.dblocks;
+    int item = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int part = uniform(item % parts);
+    item = uniform(item / parts);
+    const int tile_r = p.row_tiles - 1 - uniform(item % p.row_tiles);     // (the longest first)
+    item = uniform(item / p.row_tiles);
+    const int hk = uniform(item % p.HK), b = uniform(item / p.HK);
+    const int split = uniform(part % p.splits), db = uniform(part / p.splits);
+    const PagedSeq s = paged_seq(p, b);
+
+    const int R0 = tile_r * PER_WG, R = SIMP ? R0 + wave : R0 + wave * 32 + c;
+    const int t = R / p.G, g = R - t * p.G, h = hk * p.G + g;
+    const int pos = s.first + t;
+    const bool row_there = R < p.n * p.G;
+    const bool on = row_there && t < s.count && pos >= 0;
+    const int t_first = R0 / p.G, t_last = min((R0 + PER_WG - 1) / p.G, s.count - 1);
+    const int last = min(s.first + t_last, s.reach - 1);
+    const int first_key = SIMP ? max(0, s.first + t_first - p.w1 + 1) : 0;
+    const int tiles = t_first < s.count && last >= first_key ? (last - first_key) / 32 + 1 : 0;
+    const int tile_a = (int)((int64_t)tiles * split / p.splits), tile_z = (int)((int64_t)tiles * (split + 1) / p.splits);
+    const int NT = tile_z - tile_a;
+
+    const char *q_row = p.q + b * p.q_sb + (int64_t)(row_there ? t : 0) * p.q_sn + (int64_t)(row_there ? h : 0) * p.q_sh;
+    PagedWave<E, D> w;
+    SimplicialColumns<E, D> cols;
+    w.clear();
+    if constexpr (SIMP) {
+        cols.build(p, s, w, q_row, pos, 32 * db + c, hk, hf, on);
+        w.limits(max(0, pos - p.w1 + 1), pos, on && cols.page2 >= 0);
+    } else {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) w.A[kk] = on ? paged_q_piece<E>(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
+        w.limits(0, pos, on);
+    }
+    // keys that any column of the wave attends
+    int wave_lo = w.lo <= w.hi ? w.lo : 0x7fffffff, wave_hi = w.lo <= w.hi ? w.hi : -1;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        wave_lo = min(wave_lo, __shfl_xor(wave_lo, m));
+        wave_hi = max(wave_hi, __shfl_xor(wave_hi, m));
+    }
+    wave_lo = uniform(wave_lo);
+    wave_hi = uniform(wave_hi);
+
+    const char *const kg = p.k1.ptr + hk * p.k1.sh, *const vg = p.v1.ptr + hk * p.v1.sh;
+    const char *const zero = reinterpret_cast<const char *>(g_paged_zero_row);
+    const int st_col = RT::st_col(lane);
+    const bool col_there = st_col < p.dp * 2;
+    const int start = first_key + 32 * tile_a;          // position of step 0
+    auto fill = [&](int from, int count) {              // pages of the positions start + from ..
+        for (int x = from + tid; x < from + count; x += NW * 64) {
+            const int at = start + x;
+            seg[x & (C::SEG - 1)] = at <= last && at >= 0 ? paged_page(p, s, at) : -1;
+        }
+    };
+    auto request = [&](int u) {                          // this wave's share of the transfers of step u
+        const uint32_t buf = (uint32_t)(uintptr_t)lds + (u % NBUF) * C::BUF;
+#pragma unroll
+        for (int i = 0; i < C::LOADS; ++i) {
+            const int x = wave + i * NW;                 // chunk x % NCH of K (x < NCH) or V
+            if (x >= 2 * RT::NCH) break;
+            const bool is_v = x >= RT::NCH;
+            const int ch = is_v ? x - RT::NCH : x;
+            const PagedPool &pool = is_v ? p.v1 : p.k1;
+            const int y = 32 * u + RT::st_row(ch, lane);
+            const int at = start + y, page = seg[y & (C::SEG - 1)];
+            const int row = at - (int)p.div((uint32_t)at) * (int)p.div.ps;
+            const char *from = (is_v ? vg : kg) + (int64_t)page * pool.sp + (int64_t)row * pool.sr + st_col;
+            load_to_lds16_from(page >= 0 && col_there ? from : zero, buf + (is_v ? RT::BYTES : 0) + ch * RT::CP);
+        }
+    };
+    if (NT > 0) {
+        fill(0, C::SEG);
+        __syncthreads();
+        for (int u = 0; u < NBUF - 1; ++u) request(u);
+        for (int u = 0; u < NT; ++u) {
+            // the transfers of step u have landed (this wave's; the barrier says so for the others'), and every wave is done with step u - 1
+            wait_lds_reads();
+            wait_loads<(NBUF - 2) * C::LOADS>();
+            __syncthreads();
+            request(u + NBUF - 1);
+            if ((u & 31) == 0 && u > 0) fill(32 * u + C::SEG / 2, C::SEG / 2);
+            const int tile = start + 32 * u;
+            if (tile + 31 < wave_lo || tile > wave_hi) continue;
+            const char *buf = lds + (u % NBUF) * C::BUF;
+            const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(seg[(32 * u + c) & (C::SEG - 1)] >= 0);
+            f32x16 S = w.logits(buf + RT::row_lane(lane));
+            const bool masked = w.needs_mask(tile, there);
+            if (masked) w.mask(S, tile, there, hf);
+            u32x4 pb[2];
+            w.weights(S, p.scale_log2e, pb);
+            w.template values<SIMP>(buf + RT::BYTES + RT::tr_lane(lane), pb, masked, tile, there, hf);
+        }
+        wait_loads<0>();
+    }
+
+    const int64_t rows = (int64_t)p.B * p.n * p.H, row = ((int64_t)b * p.n + t) * p.H + h;
+    if constexpr (SIMP) {
+        float y[16 * DT], ref, sum;
+        cols.finish(p, w, hk, c, hf, y, ref, sum);
+        if (!row_there) return;
+        const int base = ColumnSum<16 * DT>::base(c);
+        if (parts == 1) {
+            const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+            char *orow = p.o + b * p.o_sb + t * p.o_sn + h * p.o_sh;
+#pragma unroll
+            for (int i = 0; i < ColumnSum<16 * DT>::LEFT; ++i) {
+                const int d = 32 * ((base + i) >> 4) + 16 * hf + ((base + i) & 15);
+                if (d < p.dq && (16 * DT >= 32 || (c & 1) == 0)) *reinterpret_cast<uint16_t *>(orow + d * 2) = (uint16_t)E::pack(y[i] * inv, 0.f);
+            }
+        } else {
+            float *dst = p.part_o + ((int64_t)part * rows + row) * D;
+#pragma unroll
+            for (int i = 0; i < ColumnSum<16 * DT>::LEFT; ++i)
+                if (16 * DT >= 32 || (c & 1) == 0) dst[32 * ((base + i) >> 4) + 16 * hf + ((base + i) & 15)] = y[i];
+            if (lane == 0) p.part_ml[part * rows + row] = make_float2(ref, sum);
+        }
+    } else {
+        if (!on) w.clear();
+        const float sum = w.whole_sum();
+        if (!row_there) return;
+        if (parts == 1) {
+            const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+            char *orow = p.o + b * p.o_sb + t * p.o_sn + h * p.o_sh;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float z[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[e] = w.O[dt][8 * half + e] * inv;
+                    paged_store8<E>(p, orow, 32 * dt + 16 * hf + 8 * half, z);
+                }
+        } else {
+            store_row_f32<DT>(p.part_o + ((int64_t)part * rows + row) * D + 16 * hf, w.O, 1.f);
+            if (hf == 0) p.part_ml[part * rows + row] = make_float2(w.M, sum);
+        }
+    }
+}
+
+// ---- partial results of a row merged: D / 8 threads per row
+template <class E, int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
+    constexpr int TPR = D / 8;
+    const int64_t rows = (int64_t)p.B * p.n * p.H, row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    if (row >= rows) return;
+    const int d0 = 8 * (threadIdx.x % TPR), parts = p.splits * p.dblocks;
+    float top = kNoRef;
+    for (int x = 0; x < parts; ++x) {
+        const float2 ml = p.part_ml[x * rows + row];
+        top = ml.y == 0.f ? top : fmaxf(top, ml.x);
+    }
+    float total = 0.f, z[8] = {};
+    for (int x = 0; x < parts; ++x) {
+        const float2 ml = p.part_ml[x * rows + row];
+        if (ml.y == 0.f) continue;                   // (nothing attended: its row is not read)
+        const float f = fast_exp2(ml.x - top);
+        const float *src = p.part_o + ((int64_t)x * rows + row) * D + d0;
+        const float4 a = *reinterpret_cast<const float4 *>(src), c = *reinterpret_cast<const float4 *>(src + 4);
+        total += f * ml.y;
+        z[0] += f * a.x; z[1] += f * a.y; z[2] += f * a.z; z[3] += f * a.w;
+        z[4] += f * c.x; z[5] += f * c.y; z[6] += f * c.z; z[7] += f * c.w;
+    }
+    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] *= inv;
+    const int64_t bt = row / p.H;
+    const int h = (int)(row - bt * p.H), b = (int)(bt / p.n), t = (int)(bt - (int64_t)b * p.n);
+    paged_store8<E>(p, p.o + b * p.o_sb + t * p.o_sn + h * p.o_sh, d0, z);
+}
+
+}  // namespace sa2

@@ -2,7 +2,7 @@
 // nodes, in one native call per direction.  (From Python through ctypes the same work took 25 us for a forward and 150 us
 // for a forward and backward, which is what small calls then cost whatever the kernels do.)
 //
-// Bound to Python as the module _sa2_torch; two_simplicial_attention.py and qkv_norm.py are its callers.
+// Bound to Python as the module _sa2_torch; two_simplicial_attention.py, qkv_norm.py, linear.py, paged.py and sampling.py are its callers.
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -490,6 +490,199 @@ Tensor linear(const Tensor &x, const Tensor &w, const std::optional<Tensor> &bia
     return plain ? at::linear(x, w, bias) : Linear::apply(x, w, bias);
 }
 
+// ---- serving: paged caches and sampling (no gradients: a call that autograd would have to see is refused)
+void refuse_autograd(const char *what, std::initializer_list<const Tensor *> inputs) {
+    for (const Tensor *t : inputs)
+        if (in_autograd({t}) || foreign(*t)) raise(PyExc_RuntimeError, std::string(what) + " has no derivative and takes plain tensors: call it under torch.no_grad()");
+}
+
+std::string shape_text(const Tensor &t) { return std::string(py::str(py::cast(t.sizes().vec()))); }
+
+// int32 vectors and tables that the kernels read
+void check_index(const Tensor &t, const Tensor &q, const char *name, int64_t dims, int64_t rows) {
+    if (t.scalar_type() != at::kInt) raise(PyExc_TypeError, std::string(name) + " must be int32");
+    if (t.dim() != dims || t.size(0) != rows || t.device() != q.device())
+        raise(PyExc_ValueError, std::string(name) + " " + shape_text(t) + " does not match " + std::to_string(rows) + " sequences on " + q.device().str());
+}
+
+struct PagedCall {
+    sa2_paged_problem prob{};
+    sa2_paged_index at{};
+    Tensor tables, lengths, counts;
+    bool empty = false;              // no rows, or no place that any row could be at
+};
+
+sa2_pool pool_arg(const Tensor &t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+
+// `x`: (b, n, heads, d) rows of the call
+PagedCall paged_call(const Tensor &x, const std::vector<Tensor> &pools, const Tensor &tables, const Tensor &lengths, const std::optional<Tensor> &counts) {
+    if (x.dim() != 4) raise(PyExc_ValueError, "expected (batch, rows, heads, dim_head) rows");
+    const Tensor &first = pools[0];
+    for (const Tensor &t : pools) {
+        if (!t.is_cuda() || !x.is_cuda()) raise(PyExc_AssertionError, "paged caches live on the GPU only");
+        if ((t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kHalf) || t.scalar_type() != first.scalar_type())
+            raise(PyExc_TypeError, "pages must share one dtype out of bfloat16 and float16");
+        if (t.dim() != 4 || t.sizes() != first.sizes() || t.device() != x.device())
+            raise(PyExc_ValueError, "pages must be (pages, page_size, kv_heads, dim) tensors of one shape on the rows' device, got " + shape_text(t));
+        if (t.numel() > 0 && ((t.size(3) > 1 && t.stride(3) != 1) || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || t.stride(0) % 8 || t.stride(1) % 8 || t.stride(2) % 8))
+            raise(PyExc_ValueError, "rows of pages must be contiguous and 16-byte aligned");
+    }
+    const int64_t dim = first.size(3);
+    if (dim < 1 || dim > 256 || dim % 8 != 0 || x.size(3) < 1 || x.size(3) > dim)
+        raise(PyExc_NotImplementedError, "rows of " + std::to_string(x.size(3)) + " channels in pages of " + std::to_string(dim) +
+                                             ": pages need a multiple of 8 channels up to 256, at least those of the rows");
+    const int64_t b = x.size(0), n = x.size(1);
+    check_index(tables, x, "tables", 2, b);
+    check_index(lengths, x, "lengths", 1, b);
+    if (counts) check_index(*counts, x, "counts", 1, b);
+    PagedCall c;
+    c.tables = tables.stride(1) == 1 || tables.size(1) <= 1 ? tables : tables.contiguous();
+    c.lengths = lengths.contiguous();
+    if (counts) c.counts = counts->contiguous();
+    c.empty = x.numel() == 0 || first.numel() == 0 || tables.size(1) == 0;
+    if (std::max({b, n, x.size(2), first.size(0), first.size(1), first.size(2), tables.size(1)}) > INT32_MAX) raise(PyExc_ValueError, "sizes beyond 32 bits");
+    sa2_paged_problem &p = c.prob;
+    p.batch = (int32_t)b;
+    p.rows = (int32_t)n;
+    p.kv_heads = (int32_t)first.size(2);
+    p.heads = (int32_t)x.size(2);
+    p.dim_head = (int32_t)x.size(3);
+    p.pool_dim = (int32_t)dim;
+    p.page_size = (int32_t)first.size(1);
+    p.pages = (int32_t)first.size(0);
+    p.table_width = (int32_t)tables.size(1);
+    p.dtype = element_of(first);
+    p.w1 = p.w2 = 1;
+    p.scale = 1.f;
+    c.at = {static_cast<const int32_t *>(c.tables.data_ptr()), c.tables.stride(0), static_cast<const int32_t *>(c.lengths.data_ptr()),
+            c.counts.defined() ? static_cast<const int32_t *>(c.counts.data_ptr()) : nullptr};
+    return c;
+}
+
+Tensor paged_attend(const Tensor &q_in, const std::vector<Tensor> &keys, const std::vector<Tensor> &values, const Tensor &tables, const Tensor &lengths,
+                    const std::optional<Tensor> &counts, int64_t w1, int64_t w2, std::optional<double> scale, std::optional<int64_t> max_length) {
+    std::vector<Tensor> pools(keys);
+    pools.insert(pools.end(), values.begin(), values.end());
+    for (const Tensor &t : pools) refuse_autograd("attention over a paged cache", {&t});
+    refuse_autograd("attention over a paged cache", {&q_in});
+    const Tensor q = q_in.dim() == 4 && q_in.stride(3) != 1 ? q_in.contiguous() : q_in;
+    PagedCall c = paged_call(q, pools, tables, lengths, counts);
+    if (q.scalar_type() != pools[0].scalar_type()) raise(PyExc_TypeError, "q and the pages must share one dtype");
+    const int64_t kv = pools[0].size(2);
+    if (kv < 1 || q.size(2) % kv != 0) raise(PyExc_ValueError, "query heads " + std::to_string(q.size(2)) + " not divisible by key/value heads " + std::to_string(kv));
+    const bool simplicial = keys.size() == 2;
+    if (w1 < 1 || w2 < 1) raise(PyExc_ValueError, "window sizes must be at least 1");
+    if (max_length && *max_length < 0) raise(PyExc_ValueError, "max_length must not be negative");
+    c.prob.w1 = (int32_t)std::min<int64_t>(w1, INT32_MAX);
+    c.prob.w2 = (int32_t)std::min<int64_t>(w2, INT32_MAX);
+    c.prob.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)q.size(3)));
+    c.prob.max_length = max_length ? (int32_t)std::min<int64_t>(*max_length, INT32_MAX) : 0;
+    const c10::DeviceGuard guard(q.device());
+    if (c.empty) return at::zeros(q.sizes(), q.options());
+    const Tensor out = at::empty(q.sizes(), q.options());
+    const int64_t bytes = simplicial ? sa2_paged_simplicial_attn_workspace_bytes(&c.prob) : sa2_paged_attn_workspace_bytes(&c.prob);
+    Tensor ws;
+    if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
+    void *const wsp = bytes > 0 ? ws.data_ptr() : nullptr;
+    const sa2_tensor aq = arg(q), ao = arg(out);
+    sa2_pool a[4];
+    for (size_t i = 0; i < pools.size(); ++i) a[i] = pool_arg(pools[i]);
+    if (simplicial) check(sa2_paged_simplicial_attn(&c.prob, &aq, &a[0], &a[1], &a[2], &a[3], &c.at, &ao, wsp, std::max<int64_t>(bytes, 0), stream_of(q)));
+    else check(sa2_paged_attn(&c.prob, &aq, &a[0], &a[1], &c.at, &ao, wsp, std::max<int64_t>(bytes, 0), stream_of(q)));
+    return out;
+}
+
+void paged_append(const std::vector<Tensor> &pools, const std::vector<Tensor> &rows_in, const Tensor &tables, const Tensor &lengths, const std::optional<Tensor> &counts) {
+    if (pools.empty() || pools.size() != rows_in.size() || pools.size() > SA2_APPEND_MOST)
+        raise(PyExc_ValueError, "as many rows as pages are required, 1 to " + std::to_string(SA2_APPEND_MOST));
+    for (const Tensor &t : pools) refuse_autograd("paged_append", {&t});
+    std::vector<Tensor> rows;
+    for (const Tensor &t : rows_in) {
+        refuse_autograd("paged_append", {&t});
+        if (element_of(t) < 0 || t.scalar_type() != rows_in[0].scalar_type()) raise(PyExc_TypeError, "rows must share one dtype out of bfloat16, float16, float32");
+        rows.push_back(t.dim() == 4 && t.stride(3) != 1 ? t.contiguous() : t);
+    }
+    const PagedCall c = paged_call(rows[0], pools, tables, lengths, counts);
+    for (const Tensor &t : rows)
+        if (t.sizes() != rows[0].sizes() || t.size(2) != pools[0].size(2) || t.device() != rows[0].device())
+            raise(PyExc_ValueError, "rows " + shape_text(t) + " do not match the pages' " + shape_text(pools[0]));
+    if (c.empty) return;
+    const c10::DeviceGuard guard(rows[0].device());
+    sa2_append_item items[SA2_APPEND_MOST];
+    for (size_t i = 0; i < pools.size(); ++i) items[i] = {pool_arg(pools[i]), arg(rows[i])};
+    check(sa2_paged_append(&c.prob, items, (int32_t)pools.size(), element_of(rows[0]), &c.at, stream_of(rows[0])));
+}
+
+void copy_pages(const std::vector<Tensor> &pools, const Tensor &pairs_in) {
+    if (pools.empty()) raise(PyExc_ValueError, "no pages to copy in");
+    if (pairs_in.is_cuda() || pairs_in.dim() != 2 || pairs_in.size(1) != 2) raise(PyExc_ValueError, "pairs must be a (count, 2) tensor in host memory");
+    if (!at::isIntegralType(pairs_in.scalar_type(), false)) raise(PyExc_TypeError, "pairs must be integers");
+    std::vector<sa2_page_pool> items;
+    for (const Tensor &t : pools) {
+        refuse_autograd("copy_pages", {&t});
+        if (!t.is_cuda()) raise(PyExc_AssertionError, "paged caches live on the GPU only");
+        if (t.device() != pools[0].device()) raise(PyExc_ValueError, "pages must be on one device");
+        if (t.dim() < 2 || t.numel() == 0 || !t[0].is_contiguous()) raise(PyExc_ValueError, "a page must be contiguous: " + shape_text(t));
+        const int64_t size = (int64_t)t.element_size(), bytes = t[0].numel() * size;
+        items.push_back({t.data_ptr(), t.size(0) > 1 ? t.stride(0) * size : bytes, bytes, t.size(0)});
+    }
+    if (pairs_in.scalar_type() == at::kLong && pairs_in.numel() > 0 && (pairs_in.max().item<int64_t>() > INT32_MAX || pairs_in.min().item<int64_t>() < 0))
+        raise(PyExc_ValueError, "pairs name pages that do not exist");
+    const Tensor pairs = pairs_in.to(at::kInt).contiguous();
+    const c10::DeviceGuard guard(pools[0].device());
+    check(sa2_copy_pages(items.data(), (int32_t)items.size(), static_cast<const int32_t *>(pairs.data_ptr()), pairs.size(0), stream_of(pools[0])));
+}
+
+// a parameter of sampling: a number for all rows, or one per row
+template <typename T>
+const T *per_row(const std::optional<Tensor> &t, const Tensor &logits, int64_t rows, at::ScalarType type, const char *name, Tensor &keep) {
+    if (!t) return nullptr;
+    if (t->scalar_type() != type) raise(PyExc_TypeError, std::string(name) + " must be " + (type == at::kInt ? "int32" : "float32"));
+    if (t->numel() != rows || t->device() != logits.device()) raise(PyExc_ValueError, std::string(name) + " " + shape_text(*t) + " does not match " + std::to_string(rows) + " rows");
+    keep = t->contiguous();
+    return static_cast<const T *>(keep.data_ptr());
+}
+
+std::tuple<Tensor, Tensor> sample_tokens(const Tensor &logits_in, const Tensor &noise_in, const std::optional<Tensor> &temperature, const std::optional<Tensor> &top_k,
+                                         const std::optional<Tensor> &top_p, const std::optional<Tensor> &min_p, double temperature_all, int64_t top_k_all,
+                                         double top_p_all, double min_p_all) {
+    refuse_autograd("sample_tokens", {&logits_in, &noise_in});
+    if (!logits_in.is_cuda() || !noise_in.is_cuda()) raise(PyExc_AssertionError, "sample_tokens runs on the GPU only");
+    if (element_of(logits_in) < 0) raise(PyExc_TypeError, "logits must be bfloat16, float16 or float32");
+    if (noise_in.scalar_type() != at::kFloat) raise(PyExc_TypeError, "noise must be float32");
+    if (logits_in.dim() < 1 || noise_in.sizes() != logits_in.sizes() || noise_in.device() != logits_in.device())
+        raise(PyExc_ValueError, "noise " + shape_text(noise_in) + " does not match the logits' " + shape_text(logits_in));
+    const int64_t vocab = logits_in.size(-1);
+    if (vocab < 1) raise(PyExc_ValueError, "an empty vocabulary");
+    const auto shape = logits_in.sizes().slice(0, logits_in.dim() - 1);
+    const c10::DeviceGuard guard(logits_in.device());
+    const Tensor tokens = at::empty(shape, logits_in.options().dtype(at::kLong)), logprobs = at::empty(shape, logits_in.options().dtype(at::kFloat));
+    if (tokens.numel() == 0) return {tokens, logprobs};
+    auto rows_of_2d = [&](const Tensor &t) {
+        const Tensor x = t.dim() == 2 ? t : t.reshape({-1, vocab});
+        return x.stride(1) == 1 || vocab == 1 ? x : x.contiguous();
+    };
+    const Tensor logits = rows_of_2d(logits_in), noise = rows_of_2d(noise_in);
+    const int64_t rows = logits.size(0);
+    Tensor keep[4];
+    sa2_sample_params p{};
+    p.temperature = per_row<float>(temperature, logits, rows, at::kFloat, "temperature", keep[0]);
+    p.top_k = per_row<int32_t>(top_k, logits, rows, at::kInt, "top_k", keep[1]);
+    p.top_p = per_row<float>(top_p, logits, rows, at::kFloat, "top_p", keep[2]);
+    p.min_p = per_row<float>(min_p, logits, rows, at::kFloat, "min_p", keep[3]);
+    p.temperature_all = (float)temperature_all;
+    p.top_k_all = (int32_t)std::max<int64_t>(0, std::min<int64_t>(top_k_all, INT32_MAX));
+    p.top_p_all = (float)top_p_all;
+    p.min_p_all = (float)min_p_all;
+    const int64_t bytes = sa2_sample_workspace_bytes(rows, vocab);
+    Tensor ws;
+    if (bytes > 0) ws = at::empty({bytes}, logits.options().dtype(at::kByte));
+    check(sa2_sample(logits.data_ptr(), element_of(logits), rows, vocab, logits.stride(0), static_cast<const float *>(noise.data_ptr()), noise.stride(0), &p,
+                     static_cast<int64_t *>(tokens.data_ptr()), static_cast<float *>(logprobs.data_ptr()), bytes > 0 ? ws.data_ptr() : nullptr, std::max<int64_t>(bytes, 0),
+                     stream_of(logits)));
+    return {tokens, logprobs};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_sa2_torch, m) {
@@ -500,5 +693,9 @@ PYBIND11_MODULE(_sa2_torch, m) {
     m.def("qkv_norm_forward", &qkv_norm_forward);
     m.def("qkv_norm_backward", &qkv_norm_backward);
     m.def("linear", &linear);
+    m.def("paged_attend", &paged_attend);
+    m.def("paged_append", &paged_append);
+    m.def("copy_pages", &copy_pages);
+    m.def("sample_tokens", &sample_tokens);
     m.def("released_bytes", [](int device) { return device >= 0 && device < kMostDevices ? g_released[device].load() : int64_t(0); });
 }
