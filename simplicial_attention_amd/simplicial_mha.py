@@ -84,13 +84,16 @@ class HigherOrderAttention(nn.Module):
                 and all(n.eps == self.q_norm.eps for n in (*self.k_norms, *self.v_norms)))
 
     def forward(self, tokens):
+        return self.attend_with(tokens, self.attend)
+
+    def attend_with(self, tokens, attend):
         tokens = self.prenorm(tokens)
         qkv = apply_linear(self.to_qkv, tokens)
         if qkv.dim() == 3 and self._can_fuse(qkv):
             from .qkv_norm import fused_qkv_norm
             norms = (self.q_norm, *self.k_norms, *self.v_norms)
             q, k1, k2, v1, v2 = fused_qkv_norm(qkv, norms, self.heads, self.key_value_heads, self.split_dims[0] // self.heads)
-            out = self.attend(q, (k1, k2), (v1, v2))
+            out = attend(q, (k1, k2), (v1, v2))
             return self.postnorm(apply_linear(self.combine_heads, out.flatten(-2)))
         q, k, v = qkv.split(self.split_dims, dim=-1)
         queries = self._split(q, self.heads)
@@ -100,7 +103,7 @@ class HigherOrderAttention(nn.Module):
             queries = self.q_norm(queries)
             keys = tuple(norm(t) for norm, t in zip(self.k_norms, keys))
             values = tuple(norm(t) for norm, t in zip(self.v_norms, values))
-        out = self.attend(queries, keys, values)
+        out = attend(queries, keys, values)
         if self.head_first_dim:
             out = out.transpose(1, 2)
         out = apply_linear(self.combine_heads, out.flatten(-2))

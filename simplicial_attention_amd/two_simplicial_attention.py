@@ -177,3 +177,24 @@ class SlidingWindowTwoSimplicialMHA(HigherOrderAttention):
         assert 'head_first_dim' not in kwargs
         attend = partial(sliding_two_simplicial_attn, w1=w1, w2=w2, causal=True)
         super().__init__(*args, number_key_value_sets=2, head_first_dim=False, attend=attend, **kwargs)
+        self.w1, self.w2 = w1, w2
+
+    @torch.no_grad()
+    def forward_cached(self, tokens, keys, values, batch):
+        """``forward`` for new tokens (b, n, dim) behind those in a paged cache: ``keys`` and ``values`` are the layer's two pools each, ``batch`` says
+        where the rows go (:meth:`PagedCache.extend`).  Rows beyond ``batch.counts`` are padding."""
+        from .paged import paged_append, paged_two_simplicial_attn
+
+        def attend(q, k, v):
+            at = (batch.tables, batch.lengths, batch.counts)
+            pool, dim = keys[0], q.shape[-1]
+            if k[0].shape[-1] == v[0].shape[-1]:
+                paged_append((*keys, *values), (*k, *v), *at)
+            else:
+                paged_append(keys, k, *at)
+                paged_append(values, v, *at)
+                q = F.pad(q, (0, pool.shape[-1] - dim))
+            out = paged_two_simplicial_attn(q.to(pool.dtype), keys, values, *at, w1=self.w1, w2=self.w2, scale=dim ** -0.5, max_length=batch.max_length)
+            return out[..., :v[0].shape[-1]].to(tokens.dtype)
+
+        return self.attend_with(tokens, attend)
