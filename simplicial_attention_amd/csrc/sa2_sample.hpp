@@ -3,14 +3,30 @@
 // Order the tokens of a row by (logit descending, index ascending) and let p = softmax(logit / T).  A token is kept if its rank is below
 // top_k, the mass in front of it below top_p, and p at least min_p times the largest; every one of these keeps a prefix of the order, so
 // the kept tokens are a prefix too.  The token is the kept one with the largest  logit / T - log(-log u),  which draws from p restricted to the
-// prefix.  No sort: the best of ALL tokens is the answer if it is kept, and otherwise nothing behind it is, so the race is run again among the tokens
+// prefix (compared as  p / -log u,  one logarithm and a reciprocal).  No sort: the best of ALL tokens is the answer if it is kept, and otherwise nothing behind it is, so the race is run again among the tokens
 // in front of it.  Whether a token is kept takes two sums over the tokens in front of it, formed in the pass that runs the next race.
 // Each race that fails leaves a uniformly drawn share of the mass, so their number grows with the logarithm of the vocabulary at most.
+//
+// Rows of up to 4096 tokens stay in the registers of one workgroup.  Longer ones are read once, 4096 tokens per workgroup, which leaves the chunk's sums, the best token
+// of an unfiltered row, and the largest logit of every 16 tokens.  A second kernel merges them, one workgroup per row; the largest logits
+// of the sixteens bound the kept prefix so closely that the races of a filtered row, and its random numbers, are looked up for few tokens.
+// Weights are exp2 of log2 units: exp2, log2 and reciprocals are single instructions, exact to an ulp.
 #pragma once
 
 #include "sa2_common.hpp"
 
 namespace sa2 {
+
+constexpr int kSampleEach = 16;            // tokens of a thread
+constexpr int kSampleThreads = 256;
+constexpr int kSampleChunk = kSampleEach * kSampleThreads;
+
+struct SampleRecord {                      // what a workgroup leaves of a chunk
+    float top, mass1, massT, score;        // largest logit; sums of exp(x - top) and exp((x - top) / T); the best token's score, relative to `top`
+    int top_at, best_at;                   // (-1: no token)
+    float best;                            // logit of the best
+    int pad;
+};
 
 struct SampleParams {
     const char *logits;
@@ -21,26 +37,50 @@ struct SampleParams {
     const int32_t *top_k;
     float temperature_all, top_p_all, min_p_all;
     int top_k_all;
-    int vocab;
+    int vocab, chunks;
     int64_t *tokens;
     float *logprobs;
+    SampleRecord *records;        // [rows][chunks]
+    float *tops;                  // [rows][chunks][kSampleThreads]: largest logit of a thread's tokens
 };
 
 constexpr float kMostFloat = 3.402823466e38f;
-template <int TYPE>
-__device__ __forceinline__ float logit_at(const char *row, int i) {
-    float x;
-    if constexpr (TYPE == 2) x = reinterpret_cast<const float *>(row)[i];
-    else {
-        const uint16_t w = reinterpret_cast<const uint16_t *>(row)[i];
-        x = TYPE == 1 ? (float)__builtin_bit_cast(_Float16, w) : as_f32((uint32_t)w << 16);
-    }
-    // (not a number: never drawn; infinity: the largest number)
-    return x != x ? -INFINITY : fminf(x, kMostFloat);
-}
+// (not a number: never drawn; infinity: the largest number)
+__device__ __forceinline__ float clean_logit(float x) { return fminf(fmaxf(x, -INFINITY), kMostFloat); }
 
-// -log(-log u), u held inside (0, 1)
-__device__ __forceinline__ float gumbel(float u) { return -logf(-logf(fminf(fmaxf(u, 1.17549435e-38f), 0.99999994f))); }
+template <int TYPE>
+struct Logits {
+    static constexpr int SIZE = TYPE == 2 ? 4 : 2, PIECE = 16 / SIZE, PIECES = kSampleEach / PIECE;
+    static __device__ __forceinline__ float one(uint16_t w) { return TYPE == 1 ? (float)__builtin_bit_cast(_Float16, w) : as_f32((uint32_t)w << 16); }
+    static __device__ __forceinline__ float at(const char *row, int i) {
+        if constexpr (TYPE == 2) return clean_logit(reinterpret_cast<const float *>(row)[i]);
+        else return clean_logit(one(reinterpret_cast<const uint16_t *>(row)[i]));
+    }
+    // token of element e of thread t of a chunk: pieces of 16 bytes, neighbours in neighbouring threads
+    static __device__ __forceinline__ int index(int chunk, int threads, int t, int e) {
+        return chunk * threads * kSampleEach + ((e / PIECE) * threads + t) * PIECE + e % PIECE;
+    }
+    // a piece at any alignment; tokens beyond the vocabulary are -inf
+    static __device__ __forceinline__ void piece(const char *row, int i, int vocab, float (&x)[PIECE]) {
+        if (i + PIECE <= vocab) {
+            u32x4 w;
+            __builtin_memcpy(&w, row + (int64_t)i * SIZE, 16);
+#pragma unroll
+            for (int e = 0; e < PIECE; ++e) {
+                if constexpr (TYPE == 2) x[e] = clean_logit(as_f32(w[e]));
+                else x[e] = clean_logit(one((uint16_t)(w[e >> 1] >> (16 * (e & 1)))));
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < PIECE; ++e) x[e] = i + e < vocab ? at(row, i + e) : -INFINITY;
+        }
+    }
+};
+
+// 1 / -log2 u, u held inside (0, 1): a token's score is its weight times this
+__device__ __forceinline__ float race_factor(float u) {
+    return __builtin_amdgcn_rcpf(-__builtin_amdgcn_logf(fminf(fmaxf(u, 1.17549435e-38f), 0.99999994f)));
+}
 
 struct Best {
     float score, x;
@@ -51,110 +91,323 @@ __device__ __forceinline__ bool beats(const Best &a, const Best &b) {
     return a.score > b.score || (a.score == b.score && a.index < b.index);
 }
 
+// ---- reductions of a wave in the vector unit (lane 63 collects), then of the workgroup through LDS; orders are fixed
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t identity, uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)identity, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <typename OP>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t x, uint32_t identity, OP op) {
+    x = op(x, dpp<0x111, 0xf>(identity, x));          // the row's lanes 1, 2, 4 and 8 before this one
+    x = op(x, dpp<0x112, 0xf>(identity, x));
+    x = op(x, dpp<0x114, 0xf>(identity, x));
+    x = op(x, dpp<0x118, 0xf>(identity, x));
+    x = op(x, dpp<0x142, 0xa>(identity, x));          // lane 15 of a row into the next row
+    x = op(x, dpp<0x143, 0xc>(identity, x));          // lane 31 into the upper half
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    return as_f32(wave_reduce(as_u32(x), 0u, [](uint32_t a, uint32_t b) { return as_u32(as_f32(a) + as_f32(b)); }));
+}
+__device__ __forceinline__ float wave_max(float x) {
+    return as_f32(wave_reduce(as_u32(x), 0xff800000u, [](uint32_t a, uint32_t b) { return as_u32(fmaxf(as_f32(a), as_f32(b))); }));
+}
+__device__ __forceinline__ uint32_t wave_min(uint32_t x) {
+    return wave_reduce(x, 0xffffffffu, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+// the lane's bests' first (scores are numbers; index -1, as the largest unsigned number, loses)
+__device__ __forceinline__ Best wave_first(const Best &v) {
+    const float s = wave_max(v.index < 0 ? -INFINITY : v.score);
+    const uint32_t i = wave_min(v.score == s ? (uint32_t)v.index : 0xffffffffu);
+    const uint64_t owner = __builtin_amdgcn_ballot_w64((uint32_t)v.index == i);
+    const int lane = (int)__builtin_ctzll(owner | (1ull << 63));
+    return {s, as_f32((uint32_t)__builtin_amdgcn_readlane((int)as_u32(v.x), lane)), (int)i};
+}
+
 template <int THREADS>
 struct RowReduce {
     static constexpr int NW = THREADS / 64;
-    float f[NW];
-    Best best[NW];
-    template <typename OP>
-    __device__ float all(float v, OP op) {
-#pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) v = op(v, __shfl_xor(v, m));
-        if (NW == 1) return v;
+    float a[NW], b[NW], x[NW];
+    int i[NW];
+    // sums of two numbers
+    __device__ __forceinline__ void add(float &p, float &q) {
+        p = wave_sum(p);
+        q = wave_sum(q);
+        if (NW == 1) return;
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) f[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = f[0];
-        for (int w = 1; w < NW; ++w) v = op(v, f[w]);
-        return v;
-    }
-    __device__ Best all(Best v) {
-#pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) {
-            const Best o = {__shfl_xor(v.score, m), __shfl_xor(v.x, m), __shfl_xor(v.index, m)};
-            if (beats(o, v)) v = o;
+        if (lane == 0) {
+            a[w] = p;
+            b[w] = q;
         }
+        __syncthreads();
+        p = wave_sum(lane < NW ? a[lane % NW] : 0.f);
+        q = wave_sum(lane < NW ? b[lane % NW] : 0.f);
+    }
+    __device__ __forceinline__ Best first(Best v) {
+        v = wave_first(v);
         if (NW == 1) return v;
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = v;
+        if (lane == 0) {
+            a[w] = v.score;
+            x[w] = v.x;
+            i[w] = v.index;
+        }
         __syncthreads();
-        v = best[0];
-        for (int w = 1; w < NW; ++w)
-            if (beats(best[w], v)) v = best[w];
-        return v;
+        return wave_first(lane < NW ? Best{a[lane % NW], x[lane % NW], i[lane % NW]} : Best{-INFINITY, 0.f, -1});
     }
 };
 
-template <int TYPE, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
-    __shared__ RowReduce<THREADS> red;
-    const int64_t r = blockIdx.x;
-    const int V = p.vocab;
-    const char *row = p.logits + r * p.stride * (TYPE == 2 ? 4 : 2);
-    const float *noise = p.noise + r * p.noise_stride;
-    const float T = p.temperature ? p.temperature[r] : p.temperature_all;
-    const float top_p = p.top_p ? p.top_p[r] : p.top_p_all, min_p = p.min_p ? p.min_p[r] : p.min_p_all;
-    const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
-    const auto add = [](float a, float b) { return a + b; };
-
-    // the largest logit, in front of all others in the order
-    Best top = {-INFINITY, 0.f, -1};
-    for (int i = threadIdx.x; i < V; i += THREADS) {
-        const float x = logit_at<TYPE>(row, i);
-        const Best o = {x, x, i};
-        if (x > -INFINITY && beats(o, top)) top = o;
+struct RowRules {
+    float inv, top_p, min_p;      // inv: log2(e) / T, 0 for a greedy row
+    int top_k;
+    bool greedy;
+    __device__ RowRules(const SampleParams &p, int64_t r) {
+        const float T = p.temperature ? p.temperature[r] : p.temperature_all;
+        greedy = !(T > 0.f);
+        inv = greedy ? 0.f : fminf(kLog2e / T, kMostFloat);
+        top_p = p.top_p ? p.top_p[r] : p.top_p_all;
+        min_p = p.min_p ? p.min_p[r] : p.min_p_all;
+        top_k = p.top_k ? p.top_k[r] : p.top_k_all;
     }
-    top = red.all(top);
-    if (top.index < 0) {                      // nothing to draw from
-        if (threadIdx.x == 0) {
-            p.tokens[r] = -1;
-            p.logprobs[r] = -INFINITY;
+    __device__ bool filters() const { return top_k > 0 || top_p < 1.f || !(min_p <= 0.f); }
+    // a token with `count` tokens and the mass `front` in front of it
+    __device__ bool keeps(float count, float front, float mass, float weight) const {
+        return (top_k <= 0 || count < (float)top_k) && (top_p >= 1.f || front < top_p * mass) && weight >= min_p;
+    }
+};
+
+__device__ __forceinline__ void write_token(const SampleParams &p, int64_t r, const Best &best, float top, float mass1) {
+    p.tokens[r] = best.index;
+    p.logprobs[r] = best.index < 0 ? -INFINITY : best.x - top - kLn2 * __builtin_amdgcn_logf(mass1);
+}
+
+// a token in a race (tokens enter in ascending order: ties stay with the first)
+__device__ __forceinline__ void enter(Best &mine, float x, int i, float score) {
+    if (score > mine.score) mine = {score, x, i};
+}
+constexpr Best kNobody = {0.f, 0.f, -1};      // (a weight too small for fp32 loses to any other)
+
+// EACH: tokens of a thread.  ONE: the row is one chunk, and this kernel finishes it; else a row with top_k runs no race here
+template <int TYPE, int THREADS, int EACH, bool ONE>
+__global__ __launch_bounds__(THREADS) void sample_chunk_kernel(SampleParams p) {
+    using L = Logits<TYPE>;
+    constexpr int PIECES = EACH / L::PIECE;
+    __shared__ RowReduce<THREADS> red;
+    const int64_t r = ONE ? blockIdx.x : blockIdx.x / p.chunks;
+    const int chunk = ONE ? 0 : blockIdx.x - (int)r * p.chunks;
+    const int tid = threadIdx.x, V = p.vocab;
+    const char *row = p.logits + r * p.stride * L::SIZE;
+    const float *noise = p.noise + r * p.noise_stride;
+    const RowRules rules(p, r);
+    const bool races = !rules.greedy && (ONE || rules.top_k <= 0);
+    auto first_of = [&](int q) { return chunk * THREADS * EACH + (q * THREADS + tid) * L::PIECE; };
+    float x[EACH], u[EACH];
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+        const int i = first_of(q);
+        float y[L::PIECE];
+        L::piece(row, i, V, y);
+#pragma unroll
+        for (int e = 0; e < L::PIECE; ++e) x[q * L::PIECE + e] = y[e];
+    }
+    if (races) {
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q) {
+            const int i = first_of(q);
+            if (i + L::PIECE <= V) {
+                __builtin_memcpy(&u[q * L::PIECE], noise + i, 4 * L::PIECE);
+            } else {
+#pragma unroll
+                for (int e = 0; e < L::PIECE; ++e) u[q * L::PIECE + e] = i + e < V ? noise[i + e] : 0.f;
+            }
         }
+    }
+    auto index = [&](int e) { return first_of(e / L::PIECE) + e % L::PIECE; };
+    float most = x[0];
+#pragma unroll
+    for (int e = 1; e < EACH; ++e) most = fmaxf(most, x[e]);
+    if (!ONE) p.tops[(r * p.chunks + chunk) * THREADS + tid] = most;
+    Best top = {most, most, -1};
+    if (most > -INFINITY) {
+#pragma unroll
+        for (int e = EACH - 1; e >= 0; --e)    // (a thread's tokens ascend: the first that equals)
+            top.index = x[e] == most ? index(e) : top.index;
+    }
+    top = red.first(top);
+    if (ONE && top.index < 0) {                // nothing to draw from
+        if (tid == 0) write_token(p, r, top, 0.f, 1.f);
         return;
     }
-    const bool greedy = !(T > 0.f);
-    const float inv = greedy ? 0.f : fminf(1.f / T, kMostFloat);
-    Best best = top;
-    float sum = 0.f, mass = 0.f;
-    Best mine = {0.f, 0.f, -1};
-    for (int i = threadIdx.x; i < V; i += THREADS) {
-        const float x = logit_at<TYPE>(row, i);
-        if (!(x > -INFINITY)) continue;
-        sum += expf(x - top.x);
-        if (greedy) continue;
-        const float y = (x - top.x) * inv, e = expf(y);
-        mass += e;
-        if (e >= min_p || i == top.index) {
-            const Best o = {y + gumbel(noise[i]), x, i};
-            if (beats(o, mine)) mine = o;
-        }
-    }
-    sum = red.all(sum, add);
-    if (!greedy) {
-        mass = red.all(mass, add);
-        best = red.all(mine);
-        while (best.index != top.index && (top_k > 0 || top_p < 1.f)) {
-            float front = 0.f, count = 0.f;   // (counts up to 2^24 are exact)
-            mine = {0.f, 0.f, -1};
-            for (int i = threadIdx.x; i < V; i += THREADS) {
-                const float x = logit_at<TYPE>(row, i);
-                if (!(x > best.x || (x == best.x && i < best.index))) continue;
-                const float y = (x - top.x) * inv, e = expf(y);
-                front += e;
-                count += 1.f;
-                const Best o = {y + gumbel(noise[i]), x, i};
-                if (beats(o, mine)) mine = o;
+    float mass1 = 0.f, mass = 0.f;
+    Best mine = kNobody;
+    float w[EACH];                             // weights; then u: scores
+    if (top.index >= 0) {
+        // (-inf: a weight of zero; inv is finite, so 0 stays 0)
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) mass1 += fast_exp2((x[e] - top.x) * kLog2e);
+        if (!rules.greedy && (races || rules.top_p < 1.f)) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                w[e] = fast_exp2((x[e] - top.x) * rules.inv);
+                mass += w[e];
             }
-            front = red.all(front, add);
-            count = red.all(count, add);
-            if ((top_k <= 0 || count < (float)top_k) && (top_p >= 1.f || front < top_p * mass)) break;
-            best = red.all(mine);
+        }
+        if (races) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                u[e] = w[e] * race_factor(u[e]);
+                enter(mine, x[e], index(e), u[e]);
+            }
         }
     }
-    if (threadIdx.x == 0) {
-        p.tokens[r] = best.index;
-        p.logprobs[r] = best.x - top.x - logf(sum);
+    red.add(mass1, mass);
+    Best best = rules.greedy ? top : red.first(mine);
+    if constexpr (!ONE) {
+        if (tid == 0) p.records[r * p.chunks + chunk] = {top.x, mass1, mass, best.score, top.index, best.index, best.x, 0};
+        return;
     }
+    while (!rules.greedy && best.index != top.index && rules.filters()) {
+        float front = 0.f, count = 0.f;
+        mine = kNobody;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const bool in = x[e] > best.x || (x[e] == best.x && index(e) < best.index);
+            front += in ? w[e] : 0.f;
+            count += in ? 1.f : 0.f;
+            enter(mine, x[e], index(e), in ? u[e] : 0.f);
+        }
+        red.add(front, count);
+        if (rules.keeps(count, front, mass, fast_exp2((best.x - top.x) * rules.inv))) break;
+        best = red.first(mine);
+    }
+    if (tid == 0) write_token(p, r, best, top.x, mass1);
+}
+
+// The chunks of a row merged; rows with filters: their races (the first one is the chunks' where there is no top_k).  The threads' largest logits bound the kept prefix from behind: if k of
+// them are at least v, no token below v has a rank below k, and if they alone hold top_p of the mass, no token below v is inside it.  The largest such v
+// (to 16 bits) is found by bisection in registers; races then look at the sixteens alone whose largest logit is in front.
+constexpr int kRowThreads = 1024, kRowBatch = 8;       // sixteens per thread that a pass looks at together
+template <int TYPE>
+__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleParams p) {
+    using L = Logits<TYPE>;
+    constexpr int THREADS = kRowThreads;
+    __shared__ RowReduce<THREADS> red;
+    __shared__ uint16_t list[THREADS / 64][kRowBatch * 64];
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), V = p.vocab;
+    const char *row = p.logits + r * p.stride * L::SIZE;
+    const float *noise = p.noise + r * p.noise_stride;
+    const RowRules rules(p, r);
+    const SampleRecord *records = p.records + r * p.chunks;
+    Best top = {-INFINITY, -INFINITY, -1};
+    for (int c = tid; c < p.chunks; c += THREADS) {
+        const Best o = {records[c].top, records[c].top, records[c].top_at};
+        if (beats(o, top)) top = o;
+    }
+    top = red.first(top);
+    if (top.index < 0) {
+        if (tid == 0) write_token(p, r, top, 0.f, 1.f);
+        return;
+    }
+    const bool races = !rules.greedy && rules.filters();
+    float mass1 = 0.f, mass = 0.f;
+    Best best = kNobody;
+    for (int c = tid; c < p.chunks; c += THREADS) {
+        const SampleRecord o = records[c];
+        if (o.top_at < 0) continue;
+        const float d = o.top - top.x, y = d * rules.inv;
+        mass1 += o.mass1 * fast_exp2(d * kLog2e);
+        mass += o.massT * fast_exp2(y);
+        enter(best, o.best, o.best_at, o.score * fast_exp2(y));
+    }
+    red.add(mass1, mass);
+    best = rules.greedy ? top : red.first(best);
+    if (!races) {
+        if (tid == 0) write_token(p, r, best, top.x, mass1);
+        return;
+    }
+    const float *tops = p.tops + r * p.chunks * kSampleThreads;
+    const int groups = p.chunks * kSampleThreads;
+    float g[kRowBatch];
+#pragma unroll
+    for (int k = 0; k < kRowBatch; ++k) g[k] = k * THREADS + tid < groups ? tops[k * THREADS + tid] : -INFINITY;
+
+    // keys: unsigned numbers in the order of the floats
+    float cut = -INFINITY;
+    if (rules.top_k > 0) {
+        auto key = [](float x) { return as_u32(x) & 0x80000000u ? ~as_u32(x) : as_u32(x) | 0x80000000u; };
+        const float enough = rules.top_p < 1.f ? rules.top_p * mass * 1.0001f : INFINITY;       // (sums in another order)
+        const float many = rules.top_k > 0 ? (float)rules.top_k : INFINITY;
+        uint32_t v = 0u;
+        for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+            float count = 0.f, held = 0.f;
+#pragma unroll
+            for (int k = 0; k < kRowBatch; ++k)
+                if (key(g[k]) >= (v | bit) && g[k] > -INFINITY) {
+                    count += 1.f;
+                    held += fast_exp2((g[k] - top.x) * rules.inv);
+                }
+            red.add(count, held);
+            if (count >= many || held >= enough) v |= bit;
+        }
+        if (v) cut = as_f32(v & 0x80000000u ? v & 0x7fffffffu : ~v);
+    }
+    // tokens in front of (x, i): a race among them, their number and mass
+    auto race = [&](float cut_x, int cut_i, float &count, float &front) {
+        Best mine = kNobody;
+        count = front = 0.f;
+        for (int base = 0; base < groups; base += kRowBatch * THREADS) {
+            int listed = 0;
+#pragma unroll
+            for (int k = 0; k < kRowBatch; ++k) {
+                const int at = base + k * THREADS + tid;
+                const float t = base == 0 ? g[k] : at < groups ? tops[at] : -INFINITY;
+                const bool in = t >= cut_x && t > -INFINITY && fast_exp2((t - top.x) * rules.inv) >= rules.min_p;
+                const uint64_t who = __builtin_amdgcn_ballot_w64(in);
+                if (in) list[wave][listed + __builtin_popcountll(who & ((1ull << lane) - 1))] = (uint16_t)(k * THREADS + tid);
+                listed += __builtin_popcountll(who);
+            }
+            // (a wave reads what it wrote) one lane per piece of 16 bytes of a listed sixteen
+            constexpr int AT_ONCE = 64 / L::PIECES;
+            for (int k = 0; k < listed; k += AT_ONCE) {
+                const int which = k + lane / L::PIECES;
+                if (which >= listed) continue;
+                const int at = base + list[wave][which];
+                const int i = L::index(at / kSampleThreads, kSampleThreads, at % kSampleThreads, lane % L::PIECES * L::PIECE);
+                float x[L::PIECE], u[L::PIECE];
+                L::piece(row, i, V, x);
+                if (i + L::PIECE <= V) {
+                    __builtin_memcpy(u, noise + i, 4 * L::PIECE);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < L::PIECE; ++e) u[e] = i + e < V ? noise[i + e] : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < L::PIECE; ++e) {
+                    const float w = fast_exp2((x[e] - top.x) * rules.inv);
+                    const bool in = (x[e] > cut_x || (x[e] == cut_x && i + e < cut_i)) && w >= rules.min_p && x[e] > -INFINITY;
+                    front += in ? w : 0.f;
+                    count += in ? 1.f : 0.f;
+                    const float score = in ? w * race_factor(u[e]) : 0.f;
+                    // (the list is not in the order of the tokens)
+                    if (score > mine.score || (score == mine.score && in && (unsigned)(i + e) < (unsigned)mine.index)) mine = {score, x[e], i + e};
+                }
+            }
+        }
+        red.add(front, count);
+        return red.first(mine);
+    };
+    float count, front;
+    if (rules.top_k > 0) best = race(cut, 0x7fffffff, count, front);
+    while (best.index != top.index && best.index >= 0) {
+        const Best next = race(best.x, best.index, count, front);
+        if (rules.keeps(count, front, mass, fast_exp2((best.x - top.x) * rules.inv))) break;
+        best = next;
+    }
+    if (best.index < 0) best = top;            // (a min_p that nothing reaches)
+    if (tid == 0) write_token(p, r, best, top.x, mass1);
 }
 
 }  // namespace sa2

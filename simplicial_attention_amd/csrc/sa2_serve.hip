@@ -16,8 +16,16 @@ bool pieces16(const void *ptr, int64_t a, int64_t b, int64_t c) { return (reinte
 
 template <int TYPE>
 void launch_sample(int64_t rows, const SampleParams &k, hipStream_t s) {
-    if (k.vocab <= 2048) hipLaunchKernelGGL((sample_kernel<TYPE, 256>), dim3((unsigned)rows), dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((sample_kernel<TYPE, 1024>), dim3((unsigned)rows), dim3(1024), 0, s, k);
+    const dim3 grid((unsigned)(rows * k.chunks));
+    constexpr int N = kSampleThreads, E = kSampleEach;
+    // one wave up to 1024 tokens (no barriers), a piece per thread where that is enough
+    if (k.vocab <= 64 * Logits<TYPE>::PIECE) hipLaunchKernelGGL((sample_chunk_kernel<TYPE, 64, Logits<TYPE>::PIECE, true>), grid, dim3(64), 0, s, k);
+    else if (k.vocab <= 64 * E) hipLaunchKernelGGL((sample_chunk_kernel<TYPE, 64, E, true>), grid, dim3(64), 0, s, k);
+    else if (k.chunks == 1) hipLaunchKernelGGL((sample_chunk_kernel<TYPE, N, E, true>), grid, dim3(N), 0, s, k);
+    else {
+        hipLaunchKernelGGL((sample_chunk_kernel<TYPE, N, E, false>), grid, dim3(N), 0, s, k);
+        hipLaunchKernelGGL(sample_row_kernel<TYPE>, dim3((unsigned)rows), dim3(kRowThreads), 0, s, k);
+    }
 }
 
 }  // namespace
@@ -127,7 +135,11 @@ int sa2_copy_pages(const sa2_page_pool *pools, int32_t count, const int32_t *pai
     return SA2_OK;
 }
 
-int64_t sa2_sample_workspace_bytes(int64_t rows, int64_t vocab) { return rows < 1 || vocab < 1 ? -1 : 0; }
+int64_t sa2_sample_workspace_bytes(int64_t rows, int64_t vocab) {
+    if (rows < 1 || vocab < 1 || vocab > (1 << 24)) return -1;
+    const int64_t chunks = (vocab + kSampleChunk - 1) / kSampleChunk;
+    return chunks == 1 ? 0 : rows * chunks * (int64_t)(sizeof(SampleRecord) + 4 * kSampleThreads);
+}
 
 int sa2_sample(const void *logits, int32_t type, int64_t rows, int64_t vocab, int64_t stride, const float *noise, int64_t noise_stride,
                const sa2_sample_params *params, int64_t *tokens, float *logprobs, void *workspace, int64_t workspace_bytes, void *hip_stream) {
@@ -136,8 +148,11 @@ int sa2_sample(const void *logits, int32_t type, int64_t rows, int64_t vocab, in
     if (type < 0 || type > 2) return fail_with(SA2_ERR_UNSUPPORTED, "logits of type %d", type);
     if ((reinterpret_cast<uintptr_t>(logits) & (type == SA2_ELEMENT_F32 ? 3 : 1)) != 0 || (reinterpret_cast<uintptr_t>(noise) & 3) != 0)
         return fail_with(SA2_ERR_ALIGNMENT, "logits and noise must be aligned to their elements");
-    (void)workspace;
-    (void)workspace_bytes;
+    const int64_t bytes = sa2_sample_workspace_bytes(rows, vocab), chunks = (vocab + kSampleChunk - 1) / kSampleChunk;
+    if (rows * chunks > 0x7fffffff) return fail_with(SA2_ERR_BAD_SHAPE, "rows=%lld vocab=%lld: too large for a 1-D grid", (long long)rows, (long long)vocab);
+    if (bytes > 0 && (!workspace || workspace_bytes < bytes))
+        return fail_with(SA2_ERR_BAD_SHAPE, "workspace of %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0), (long long)bytes);
+    if (bytes > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return fail_with(SA2_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
     SampleParams k{};
     k.logits = static_cast<const char *>(logits);
     k.stride = stride;
@@ -152,6 +167,11 @@ int sa2_sample(const void *logits, int32_t type, int64_t rows, int64_t vocab, in
     k.min_p_all = params->min_p_all;
     k.top_k_all = params->top_k_all;
     k.vocab = (int)vocab;
+    k.chunks = (int)chunks;
+    if (bytes > 0) {
+        k.records = static_cast<SampleRecord *>(workspace);
+        k.tops = reinterpret_cast<float *>(k.records + rows * chunks);
+    }
     k.tokens = tokens;
     k.logprobs = logprobs;
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);

@@ -622,9 +622,14 @@ void copy_pages(const std::vector<Tensor> &pools, const Tensor &pairs_in) {
         refuse_autograd("copy_pages", {&t});
         if (!t.is_cuda()) raise(PyExc_AssertionError, "paged caches live on the GPU only");
         if (t.device() != pools[0].device()) raise(PyExc_ValueError, "pages must be on one device");
-        if (t.dim() < 2 || t.numel() == 0 || !t[0].is_contiguous()) raise(PyExc_ValueError, "a page must be contiguous: " + shape_text(t));
-        const int64_t size = (int64_t)t.element_size(), bytes = t[0].numel() * size;
-        items.push_back({t.data_ptr(), t.size(0) > 1 ? t.stride(0) * size : bytes, bytes, t.size(0)});
+        bool contiguous = t.dim() >= 2 && t.numel() > 0;
+        int64_t bytes = (int64_t)t.element_size();
+        for (int64_t x = t.dim() - 1; contiguous && x >= 1; --x) {
+            contiguous = t.size(x) == 1 || t.stride(x) * (int64_t)t.element_size() == bytes;
+            bytes *= t.size(x);
+        }
+        if (!contiguous) raise(PyExc_ValueError, "a page must be contiguous: " + shape_text(t));
+        items.push_back({t.data_ptr(), t.size(0) > 1 ? t.stride(0) * (int64_t)t.element_size() : bytes, bytes, t.size(0)});
     }
     if (pairs_in.scalar_type() == at::kLong && pairs_in.numel() > 0 && (pairs_in.max().item<int64_t>() > INT32_MAX || pairs_in.min().item<int64_t>() < 0))
         raise(PyExc_ValueError, "pairs name pages that do not exist");
