@@ -20,10 +20,10 @@ using namespace sa2;
 int kernel_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 PageDiv page_div(int ps) {
-    // floor(x / ps) = (x * mul) >> 31 + s with mul = floor(2^(31 + s) / ps) + 1, s = ceil(log2 ps): exact for x < 2^31
+    // floor(x / ps) = (x * mul) >> (31 + s) with mul = floor(2^(31 + s) / ps) + 1, s = ceil(log2 ps): exact for x < 2^31
     uint32_t s = 0;
     while ((1ll << s) < ps) ++s;
-    return {(uint32_t)ps, (uint32_t)((1ull << (31 + s)) / ps + 1), s ? s - 1 : 0};
+    return {(uint32_t)ps, (uint32_t)((1ull << (31 + s)) / ps + 1), 31 + s};
 }
 
 int check_problem(const sa2_paged_problem *p, bool simplicial) {
@@ -62,7 +62,7 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
     const int64_t keys = simplicial && p->w1 < most ? p->w1 : most;
     const int64_t tiles = (keys + 31) / 32;
     x.dblocks = simplicial ? (p->w2 + 31) / 32 : 1;
-    const int waves = x.dim == 256 ? 4 : 8;
+    const int waves = x.dim == 256 || simplicial ? 4 : 8;
     x.many = simplicial ? per >= 8 : per > 32;
     const int64_t per_wg = x.many ? (simplicial ? waves : waves * 32) : (simplicial ? 1 : 32);
     x.row_tiles = (int)((per + per_wg - 1) / per_wg);
@@ -97,8 +97,9 @@ bool whole_pieces(const sa2_tensor *t, int channels) {
 
 template <class E, int D, bool SIMP>
 void launch(const Plan &x, const PagedParams &k, hipStream_t stream) {
-    if (x.many) hipLaunchKernelGGL((paged_many_kernel<E, D, SIMP>), dim3((unsigned)x.grid), dim3(ManyCfg<D>::NW * 64), 0, stream, k);
-    else hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP>), dim3((unsigned)x.grid), dim3(FewCfg<D>::NW * 64), 0, stream, k);
+    if (x.many) hipLaunchKernelGGL((paged_many_kernel<E, D, SIMP>), dim3((unsigned)x.grid), dim3(ManyCfg<D, SIMP>::NW * 64), 0, stream, k);
+    else if (!SIMP && k.n > 1) hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, !SIMP>), dim3((unsigned)x.grid), dim3(FewCfg<D>::NW * 64), 0, stream, k);
+    else hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, false>), dim3((unsigned)x.grid), dim3(FewCfg<D>::NW * 64), 0, stream, k);
     if (x.splits * x.dblocks > 1) {
         const int per = 256 / (D / 8);
         hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)((x.rows + per - 1) / per)), dim3(256), 0, stream, k);

@@ -27,6 +27,9 @@ struct ElemBf16 {
     static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
     static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) { return mfma32(a, b, c); }
+    static __device__ __forceinline__ void mfma_in_place(f32x16 &acc, u32x4 a, u32x4 b) {
+        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(a), "v"(b));
+    }
 };
 
 struct ElemF16 {
@@ -43,7 +46,16 @@ struct ElemF16 {
     static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ void mfma_in_place(f32x16 &acc, u32x4 a, u32x4 b) {
+        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(acc) : "v"(a), "v"(b));
+    }
 };
+// mfma_in_place: the accumulator's registers are the result's.  (Left to itself the compiler gives a product of the loop below other registers than its
+// addend, and copies 16 of them per product and step.)  Written as assembly, so the wait states it needs are this code's business: two
+// behind a VALU write of an operand are in it, and products_done stands in front of whatever else reads the accumulators (18 wait
+// states behind an MFMA of 16 passes).  The compiler must not move an accumulator between two of them: kernels that use it are held to ordinary registers
+// (-amdgpu-mfma-vgpr-form, two waves per SIMD or more, no spills).
+__device__ __forceinline__ void products_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 struct PagedPool {
     const char *ptr;
@@ -53,7 +65,7 @@ struct PagedPool {
 // division by the page size as a multiplication (dividends below 2^31)
 struct PageDiv {
     uint32_t ps, mul, shift;
-    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return ps == 1 ? x : __umulhi(x, mul) >> shift; }
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)(((uint64_t)x * mul) >> shift); }
 };
 
 struct PagedParams {
@@ -79,7 +91,7 @@ struct PagedParams {
 };
 
 constexpr float kNoRef = -1e30f;              // reference of a column that has met no key yet
-__device__ __attribute__((aligned(16))) uint32_t g_paged_zero_row[4];
+__device__ __attribute__((aligned(16))) uint32_t g_paged_zero_row[128];
 
 // One direct-to-LDS load of 16 bytes per lane from addresses of its own (load_to_lds16 with 64-bit lane addresses)
 __device__ __forceinline__ void load_to_lds16_from(const char *addr, uint32_t lds_addr) {
@@ -159,6 +171,7 @@ struct PagedWave {
         l = 0.f;
     }
     __device__ __forceinline__ void limits(int lo_, int hi_, bool on) {
+        on = on && lo_ <= hi_;
         lo = on ? lo_ : 1;
         hi = on ? hi_ : 0;
         int a = on ? lo_ : -0x7fffffff, z = on ? hi_ : 0x7fffffff;
@@ -194,34 +207,44 @@ struct PagedWave {
         }
     }
 
-    // weights of a tile, packed; moves the column's reference where they outgrow it
-    __device__ __forceinline__ void weights(const f32x16 &S, float c, u32x4 (&pb)[2]) {
-        float sum = 0.f;
-        auto take = [&] {
-            sum = 0.f;
+    // weights of a tile, packed, and their sum; false (in every lane) if some column's outgrow its reference
+    __device__ __forceinline__ bool weights(const f32x16 &S, float c, u32x4 (&pb)[2], float &sum) const {
+        sum = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                const float e0 = fast_exp2(S[r] * c - M), e1 = fast_exp2(S[r + 1] * c - M);
-                sum += e0 + e1;
-                pb[r >> 3][(r & 7) >> 1] = E::pack(e0, e1);
-            }
-        };
-        take();
-        if (__builtin_expect(wave_any(!(sum < E::kBig)), 0)) {
-            float top = S[0];
+        for (int r = 0; r < 16; r += 2) {
+            const float e0 = fast_exp2(S[r] * c - M), e1 = fast_exp2(S[r + 1] * c - M);
+            sum += e0 + e1;
+            pb[r >> 3][(r & 7) >> 1] = E::pack(e0, e1);
+        }
+        return !wave_any(!(sum < E::kBig));
+    }
+    // moves the reference of every column up to the tile's largest logit
+    __device__ __forceinline__ void move_reference(const f32x16 &S, float c) {
+        float top = S[0];
 #pragma unroll
-            for (int r = 1; r < 16; ++r) top = fmaxf(top, S[r]);
-            const float ref = fmaxf(M, both_halves_max(top) * c);
-            const float f = fast_exp2(M - ref);
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, S[r]);
+        const float ref = fmaxf(M, both_halves_max(top) * c);
+        const float f = fast_exp2(M - ref);
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) O[dt][r] *= f;
-            l *= f;
-            M = ref;
-            take();
+            for (int r = 0; r < 16; ++r) O[dt][r] *= f;
+        l *= f;
+        M = ref;
+    }
+    // the plain form of a step
+    template <bool ONE>
+    __device__ __forceinline__ void step(const char *k_lane, const char *v_lane, float c, bool masked, bool guard, int tile, uint32_t there, int hf) {
+        f32x16 S = logits(k_lane);
+        if (masked) mask(S, tile, there, hf);
+        u32x4 pb[2];
+        float sum;
+        if (__builtin_expect(!weights(S, c, pb, sum), 0)) {
+            move_reference(S, c);
+            weights(S, c, pb, sum);
         }
         l += sum;
+        values<ONE>(v_lane, pb, guard, tile, there, hf);
     }
 
     // O^T += V^T P^T.  `guard`: some column does not attend some key of the tile, so a value that is not finite must be kept from it.
@@ -407,6 +430,7 @@ template <int D>
 struct FewCfg {
     using RT = DmaTile<D>;
     static constexpr int NW = D == 256 ? 2 : D == 128 ? 4 : 8;
+    static constexpr int WPE = D == 256 ? 1 : D == 128 ? 2 : 4;     // two workgroups per CU
     static constexpr int SEG = 2048;                                // positions whose pages are kept in LDS at a time
     static constexpr int RING = NW * 2 * RT::BYTES;
     static_assert(RING - RT::CP < 65536, "the LDS address of a direct load travels in 16 bits of M0");
@@ -417,8 +441,9 @@ struct FewCfg {
     static constexpr int LDS = XCH + 2 * NW * 32 * 4;
 };
 
-template <class E, int D, bool SIMP>
-__global__ __launch_bounds__(FewCfg<D>::NW * 64) void paged_few_kernel(PagedParams p) {
+// MIXED: the columns are rows at different positions (dense, more than one token)
+template <class E, int D, bool SIMP, bool MIXED>
+__global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per_eu(FewCfg<D>::WPE, FewCfg<D>::WPE))) void paged_few_kernel(PagedParams p) {
     using C = FewCfg<D>;
     using RT = DmaTile<D>;
     constexpr int NW = C::NW, DT = D / 32;
@@ -457,11 +482,11 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) void paged_few_kernel(PagedPara
     if (tile_a < tile_z) {
         if constexpr (SIMP) {
             cols.build(p, s, w, q_row, pos, 32 * db + c, hk, hf, on);
-            w.limits(first_key, pos, on && cols.page2 >= 0);
+            w.limits(first_key, min(pos, last), on && cols.page2 >= 0);
         } else {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) w.A[kk] = on ? paged_q_piece<E>(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
-            w.limits(0, pos, on);
+            w.limits(0, min(pos, last), on);
         }
     } else if constexpr (SIMP) {
         cols.page2 = -1;
@@ -508,11 +533,16 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) void paged_few_kernel(PagedPara
             const bool masked = w.needs_mask(tile, there);
             if (masked) w.mask(S, tile, there, hf);
             u32x4 pb[2];
-            w.weights(S, p.scale_log2e, pb);
+            float sum;
+            if (__builtin_expect(!w.weights(S, p.scale_log2e, pb, sum), 0)) {
+                w.move_reference(S, p.scale_log2e);
+                w.weights(S, p.scale_log2e, pb, sum);
+            }
+            w.l += sum;
             if (next < seg_z) wait_loads<RT::NCH>();
             else wait_loads<0>();
             // (a workgroup with one token has no key that some of its columns attend and others do not)
-            w.template values<SIMP>(vt + RT::tr_lane(lane), pb, !SIMP && p.n > 1 && masked, tile, there, hf);
+            w.template values<!MIXED>(vt + RT::tr_lane(lane), pb, MIXED && masked, tile, there, hf);
             wait_lds_reads();
             if (next < seg_z) request(p.v1, vg, vt_at, next);
         }
@@ -612,27 +642,37 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) void paged_few_kernel(PagedPara
 // ---- many rows: the waves of a workgroup walk the same key tiles
 //
 // A workgroup has NW x 32 columns (dense: rows of one sequence and key/value head; 2-simplicial: NW (token, head) units) and walks the
-// union of their keys; K and V tiles stream through an LDS ring that all waves read, one tile and one barrier per step.
-template <int D>
+// union of their keys; K and V tiles stream through an LDS ring of four buffers that all waves read, one tile and one barrier per step.  A step's
+// fragments travel through windows of FW registers sets, requested FW products before their use: V's along the logit chain, the next
+// tile's K along the value chain (a scheduling fence behind every product keeps them there).  Steps that need a mask, two or three of a
+// walk, take the plain form of PagedWave.
+template <int D, bool SIMP>
 struct ManyCfg {
     using RT = DmaTile<D>;
-    static constexpr int NW = D == 256 ? 4 : 8;
+    static constexpr int NW = D == 256 || SIMP ? 4 : 8;
     static constexpr int BUF = 2 * RT::BYTES;                       // a K tile and a V tile
     static constexpr int NBUF = D == 256 ? 2 : 4;
+    static constexpr bool AHEAD = NBUF == 4;                        // the next tile has landed while a tile is used
+    static constexpr int WPE = D == 256 ? 1 : D == 128 ? 2 : D == 64 && !SIMP ? 3 : 4;     // waves per SIMD
+    static constexpr int FW = D == 128 ? 4 : 2;
     static constexpr int RING = NBUF * BUF;
     static_assert(RING - RT::CP < 65536, "the LDS address of a direct load travels in 16 bits of M0");
-    static constexpr int SEG = 2048;                                // circular: pages of 64 tiles, refilled by halves
-    static constexpr int LDS = RING + SEG * 4;
+    static constexpr int SEG = SIMP ? 512 : 1024;                   // circular: places of 16 (32) tiles, refilled by halves
+    static constexpr int HALF = SEG / 64;                           // tiles of a half
+    static constexpr int LDS = RING + 2 * SEG * 8 + 16;
     static constexpr int LOADS = 2 * RT::NCH > NW ? 2 * RT::NCH / NW : 1;    // per wave and tile
 };
 
 template <class E, int D, bool SIMP>
-__global__ __launch_bounds__(ManyCfg<D>::NW * 64) void paged_many_kernel(PagedParams p) {
-    using C = ManyCfg<D>;
+__global__ __launch_bounds__((ManyCfg<D, SIMP>::NW * 64)) __attribute__((amdgpu_waves_per_eu(ManyCfg<D, SIMP>::WPE, ManyCfg<D, SIMP>::WPE))) void
+paged_many_kernel(PagedParams p) {
+    using C = ManyCfg<D, SIMP>;
     using RT = DmaTile<D>;
-    constexpr int NW = C::NW, DT = D / 32, NBUF = C::NBUF;
+    constexpr int NW = C::NW, DT = D / 32, KS = D / 16, NBUF = C::NBUF, FW = C::FW;
     __shared__ __attribute__((aligned(16))) char lds[C::LDS];
-    int *seg = reinterpret_cast<int *>(lds + C::RING);
+    // addresses of the walked positions' rows in the K and the V pool; a row of zeros where there is none
+    const char **seg_k = reinterpret_cast<const char **>(lds + C::RING), **seg_v = seg_k + C::SEG;
+    int *gaps = reinterpret_cast<int *>(lds + C::RING + 2 * C::SEG * 8);     // per half: keys are missing in front of the last one
     const int tid = threadIdx.x, wave = wave_index(), lane = tid & 63, c = lane & 31, hf = lane >> 5;
     constexpr int PER_WG = SIMP ? NW : NW * 32;        // rows (t, g) of a workgroup
 
@@ -658,76 +698,165 @@ __global__ __launch_bounds__(ManyCfg<D>::NW * 64) void paged_many_kernel(PagedPa
     const int tile_a = (int)((int64_t)tiles * split / p.splits), tile_z = (int)((int64_t)tiles * (split + 1) / p.splits);
     const int NT = tile_z - tile_a;
 
-    const char *q_row = p.q + b * p.q_sb + (int64_t)(row_there ? t : 0) * p.q_sn + (int64_t)(row_there ? h : 0) * p.q_sh;
-    PagedWave<E, D> w;
-    SimplicialColumns<E, D> cols;
-    w.clear();
-    if constexpr (SIMP) {
-        cols.build(p, s, w, q_row, pos, 32 * db + c, hk, hf, on);
-        w.limits(max(0, pos - p.w1 + 1), pos, on && cols.page2 >= 0);
-    } else {
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) w.A[kk] = on ? paged_q_piece<E>(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
-        w.limits(0, pos, on);
-    }
-    // keys that any column of the wave attends
-    int wave_lo = w.lo <= w.hi ? w.lo : 0x7fffffff, wave_hi = w.lo <= w.hi ? w.hi : -1;
-#pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-        wave_lo = min(wave_lo, __shfl_xor(wave_lo, m));
-        wave_hi = max(wave_hi, __shfl_xor(wave_hi, m));
-    }
-    wave_lo = uniform(wave_lo);
-    wave_hi = uniform(wave_hi);
-
-    const char *const kg = p.k1.ptr + hk * p.k1.sh, *const vg = p.v1.ptr + hk * p.v1.sh;
-    const char *const zero = reinterpret_cast<const char *>(g_paged_zero_row);
+    const char *const k_head = p.k1.ptr + hk * p.k1.sh, *const v_head = p.v1.ptr + hk * p.v1.sh;
+    const char *zero = reinterpret_cast<const char *>(g_paged_zero_row);
+    asm volatile("" : "+s"(zero));                       // (formed once)
     const int st_col = RT::st_col(lane);
     const bool col_there = st_col < p.dp * 2;
     const int start = first_key + 32 * tile_a;          // position of step 0
-    auto fill = [&](int from, int count) {              // pages of the positions start + from ..
-        for (int x = from + tid; x < from + count; x += NW * 64) {
+    auto fill = [&](int half) {                          // places of the tiles half * HALF ..
+        const int from = half * (C::SEG / 2);
+        int missing = 0;
+        for (int x = from + tid; x < from + C::SEG / 2; x += NW * 64) {
             const int at = start + x;
-            seg[x & (C::SEG - 1)] = at <= last && at >= 0 ? paged_page(p, s, at) : -1;
+            const int page = at <= last && at >= 0 ? paged_page(p, s, at) : -1;
+            const int row = at - (int)p.div((uint32_t)at) * (int)p.div.ps;
+            seg_k[x & (C::SEG - 1)] = page < 0 ? zero : k_head + (int64_t)page * p.k1.sp + (int64_t)row * p.k1.sr;
+            seg_v[x & (C::SEG - 1)] = page < 0 ? zero : v_head + (int64_t)page * p.v1.sp + (int64_t)row * p.v1.sr;
+            missing |= page < 0 && at <= last;
         }
+        if (missing) gaps[half & 1] = 1;
+    };
+    // keys of a tile that are there (keys beyond the last one are masked as the columns' future)
+    auto there_of = [&](int u, int any_gap) {
+        return any_gap ? (uint32_t)__builtin_amdgcn_ballot_w64(seg_k[(32 * u + c) & (C::SEG - 1)] != zero || start + 32 * u + c > last) : 0xffffffffu;
     };
     auto request = [&](int u) {                          // this wave's share of the transfers of step u
-        const uint32_t buf = (uint32_t)(uintptr_t)lds + (u % NBUF) * C::BUF;
+        const uint32_t buf = (uint32_t)(uintptr_t)lds + (u & (NBUF - 1)) * C::BUF;
 #pragma unroll
         for (int i = 0; i < C::LOADS; ++i) {
             const int x = wave + i * NW;                 // chunk x % NCH of K (x < NCH) or V
-            if (x >= 2 * RT::NCH) break;
-            const bool is_v = x >= RT::NCH;
+            if (2 * RT::NCH < NW && x >= 2 * RT::NCH) break;
+            const bool is_v = RT::NCH >= NW ? i >= RT::NCH / NW : x >= RT::NCH;
             const int ch = is_v ? x - RT::NCH : x;
-            const PagedPool &pool = is_v ? p.v1 : p.k1;
-            const int y = 32 * u + RT::st_row(ch, lane);
-            const int at = start + y, page = seg[y & (C::SEG - 1)];
-            const int row = at - (int)p.div((uint32_t)at) * (int)p.div.ps;
-            const char *from = (is_v ? vg : kg) + (int64_t)page * pool.sp + (int64_t)row * pool.sr + st_col;
-            load_to_lds16_from(page >= 0 && col_there ? from : zero, buf + (is_v ? RT::BYTES : 0) + ch * RT::CP);
+            const char *from = (is_v ? seg_v : seg_k)[(32 * u + RT::st_row(ch, lane)) & (C::SEG - 1)];
+            asm volatile("" : "+v"(from));
+            load_to_lds16_from(col_there ? from + st_col : zero, buf + (is_v ? RT::BYTES : 0) + ch * RT::CP);
         }
     };
+
+    PagedWave<E, D> w;
+    SimplicialColumns<E, D> cols;
     if (NT > 0) {
-        fill(0, C::SEG);
+        if (tid < 2) gaps[tid] = 0;
+        __syncthreads();
+        fill(0);
+        fill(1);
         __syncthreads();
         for (int u = 0; u < NBUF - 1; ++u) request(u);
-        for (int u = 0; u < NT; ++u) {
-            // the transfers of step u have landed (this wave's; the barrier says so for the others'), and every wave is done with step u - 1
-            wait_lds_reads();
-            wait_loads<(NBUF - 2) * C::LOADS>();
+    }
+    // (the columns are read behind the first transfers)
+    const char *q_row = p.q + b * p.q_sb + (int64_t)(row_there ? t : 0) * p.q_sn + (int64_t)(row_there ? h : 0) * p.q_sh;
+    w.clear();
+    if constexpr (SIMP) {
+        cols.build(p, s, w, q_row, pos, 32 * db + c, hk, hf, on);
+        w.limits(max(0, pos - p.w1 + 1), min(pos, last), on && cols.page2 >= 0);
+    } else {
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) w.A[kk] = on ? paged_q_piece<E>(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
+        w.limits(0, min(pos, last), on);
+    }
+    // (in registers from here on: a wait for them inside the walk would wait for the transfers too)
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) asm volatile("" : "+v"(w.A[kk]));
+    if (NT > 0) {
+        // steps that any column of the wave attends
+        int lo = w.lo <= w.hi ? w.lo : 0x7fffffff, hi = w.lo <= w.hi ? w.hi : -1;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            lo = min(lo, __shfl_xor(lo, m));
+            hi = max(hi, __shfl_xor(hi, m));
+        }
+        lo = uniform(lo);
+        hi = uniform(hi);
+        const int u_a = lo > hi || hi < start ? NT : min(NT, max(0, lo - start) >> 5), u_z = lo > hi || hi < start ? NT : min(NT, ((hi - start) >> 5) + 1);
+        const int k_lane = RT::row_lane(lane), v_lane = RT::BYTES + RT::tr_lane(lane);
+        u32x4 kf[FW];
+        u32x2 vf[FW][2];
+        // start of step u: the tile of step u + 1 (of step u, where there are two buffers) has landed and every wave is done with step u - 1
+        auto open_step = [&]() {
+            wait_loads<C::AHEAD ? C::LOADS : 0>();
             __syncthreads();
-            request(u + NBUF - 1);
-            if ((u & 31) == 0 && u > 0) fill(32 * u + C::SEG / 2, C::SEG / 2);
-            const int tile = start + 32 * u;
-            if (tile + 31 < wave_lo || tile > wave_hi) continue;
-            const char *buf = lds + (u % NBUF) * C::BUF;
-            const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(seg[(32 * u + c) & (C::SEG - 1)] >= 0);
-            f32x16 S = w.logits(buf + RT::row_lane(lane));
-            const bool masked = w.needs_mask(tile, there);
-            if (masked) w.mask(S, tile, there, hf);
-            u32x4 pb[2];
-            w.weights(S, p.scale_log2e, pb);
-            w.template values<SIMP>(buf + RT::BYTES + RT::tr_lane(lane), pb, masked, tile, there, hf);
+        };
+        if (C::AHEAD) wait_loads<0>();
+        for (int u = 0; u < NT;) {
+            // sixteen steps at a time: the places of the sixteen that follow go where those of the sixteen before were
+            __syncthreads();
+            const int half = u / C::HALF, any_gap = uniform(gaps[half & 1]);
+            if (half > 0) {
+                __syncthreads();
+                if (tid == 0) gaps[(half + 1) & 1] = 0;
+                __syncthreads();
+                fill(half + 1);
+            }
+            const int end = min(NT, u + C::HALF), z = min(end, u_z);
+            // steps in front of it need no mask
+            const int m_z = any_gap ? u : min(z, ((w.least_hi - start - 31) >> 5) + 1);
+            for (; u < min(end, u_a); ++u) {
+                open_step();
+                request(u + NBUF - 1);
+            }
+            while (u < z) {
+                bool opened = false;      // the step is open already (its weights outgrew a reference)
+                if (C::AHEAD && u < m_z && start + 32 * u >= w.most_lo) {
+                    const char *first = lds + (u & (NBUF - 1)) * C::BUF + k_lane;
+#pragma unroll
+                    for (int kk = 0; kk < FW; ++kk) kf[kk] = ld_lds16(first + RT::row_imm(kk));
+                    do {
+                        open_step();
+                        const char *buf = lds + (u & (NBUF - 1)) * C::BUF;
+                        f32x16 S = zero16();
+                        auto read_vf = [&](int f) {
+                            vf[f % FW][0] = lds_read_tr<D, 0>(buf + v_lane + RT::tr_imm(16 * (f / DT), 32 * (f % DT)), 0, 0);
+                            vf[f % FW][1] = lds_read_tr<D, 0>(buf + v_lane + RT::tr_imm(16 * (f / DT) + 8, 32 * (f % DT)), 0, 0);
+                        };
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int kk = 0; kk < KS; ++kk) {
+                            S = E::mfma(kf[kk % FW], w.A[kk], S);
+                            if (kk == 0) request(u + NBUF - 1);
+                            if (kk + FW < KS) kf[kk % FW] = ld_lds16(buf + k_lane + RT::row_imm(kk + FW));
+                            if (kk >= KS - FW) read_vf(kk - (KS - FW));
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                        u32x4 pb[2];
+                        float sum;
+                        if (__builtin_expect(!w.weights(S, p.scale_log2e, pb, sum), 0)) {
+                            opened = true;
+                            break;
+                        }
+                        w.l += sum;
+                        const char *next = lds + ((u + 1) & (NBUF - 1)) * C::BUF + k_lane;
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int m = 0; m < 2 * DT; ++m) {
+                            const u32x4 v = {vf[m % FW][0][0], vf[m % FW][0][1], vf[m % FW][1][0], vf[m % FW][1][1]};
+                            E::mfma_in_place(w.O[m % DT], v, pb[m / DT]);
+                            if (m + FW < 2 * DT) read_vf(m + FW);
+                            if (m >= 2 * DT - FW) kf[m - (2 * DT - FW)] = ld_lds16(next + RT::row_imm(m - (2 * DT - FW)));
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                        ++u;
+                    } while (u < m_z);
+                    products_done();
+                    if (!opened) continue;
+                }
+                // steps with a mask, and those that move a reference
+                if (!opened) {
+                    open_step();
+                    request(u + NBUF - 1);
+                }
+                const char *buf = lds + (u & (NBUF - 1)) * C::BUF;
+                const int tile = start + 32 * u;
+                const uint32_t there = there_of(u, any_gap);
+                const bool masked = w.needs_mask(tile, there);
+                w.template step<SIMP>(buf + k_lane, buf + v_lane, p.scale_log2e, masked, masked, tile, there, hf);
+                ++u;
+            }
+            for (; u < end; ++u) {
+                open_step();
+                request(u + NBUF - 1);
+            }
         }
         wait_loads<0>();
     }
