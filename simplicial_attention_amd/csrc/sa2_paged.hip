@@ -63,16 +63,38 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
     const int64_t tiles = (keys + 31) / 32;
     x.dblocks = simplicial ? (p->w2 + 31) / 32 : 1;
     const int waves = x.dim == 256 || simplicial ? 4 : 8;
-    x.many = simplicial ? per >= 8 : per > 32;
+    // 2-simplicial: a workgroup per (token, head) while all of them run at once, else units that share their keys (one sequence, 8 heads of 64 channels, w1 512,
+    // w2 32: 64 tokens 14.5 and 16.6 us, 128 tokens 26.3 and 16.7; four sequences of 128 channels: 16 tokens 20.3 and 22.7, 64 tokens 75 and 30)
+    x.many = simplicial ? seqs * per * x.dblocks > 512 : per > 32;
     const int64_t per_wg = x.many ? (simplicial ? waves : waves * 32) : (simplicial ? 1 : 32);
     x.row_tiles = (int)((per + per_wg - 1) / per_wg);
     const int64_t items = seqs * x.row_tiles * x.dblocks;
-    // two workgroups per CU; a share has at least `least` tiles (a wave of the few-row form then has two)
-    const int64_t few_waves = x.dim == 256 ? 2 : x.dim == 128 ? 4 : 8;
-    const int64_t least = x.many ? 32 : 4 * few_waves;
-    int64_t splits = (512 + items - 1) / items;
-    if (splits > tiles / least) splits = tiles / least;
-    x.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
+    int64_t splits = 1;
+    if (x.many) {
+        // The shares k of an item run on 256 CUs, one workgroup each (the 2-simplicial form two), in whole rounds; starting and ending a workgroup costs
+        // about six tiles (sixteen), the merge six.  Measured and estimated agree in order: 128 items of 1008 tiles in 1, 2, 3, 4, 8 shares 797, 503, 600, 519, 573 us;
+        // 2-simplicial, 256 items of 16 tiles in 1, 2, 4 shares 16.7, 18.4, 25.4
+        const int64_t slots = simplicial && x.dim < 256 ? 512 : 256, around = simplicial ? 16 : 6;
+        int64_t least = 0;
+        for (int64_t k = 1; k <= 64 && (k == 1 || k * 8 <= tiles); ++k) {
+            const int64_t cost = (items * k + slots - 1) / slots * (tiles / k + around) + (k > 1 ? 6 : 0);
+            if (k == 1 || cost < least) {
+                least = cost;
+                splits = k;
+            }
+        }
+    } else {
+        // 2048 waves fill the chip, and twice as many balance sequences of different lengths where a wave keeps eight tiles (one token of 16
+        // sequences of up to 32768 in 8, 16, 32 shares: 139, 131, 137 us; of 8 up to 8192: 17.6, 18.5, 23.3).  A wave has a tile at least, and short walks are not worth a
+        // merge (one sequence of 1024 in 1, 4 shares: 11.0, 10.6; of 2048 in 1, 8: 17.1, 11.2)
+        const int64_t waves = x.dim == 256 ? 2 : x.dim == 128 ? 4 : 8;
+        if (tiles >= 4 * waves) {
+            splits = (2048 + items * waves - 1) / (items * waves);
+            if (2 * splits * waves * 8 <= tiles) splits *= 2;
+            if (splits > tiles / waves) splits = tiles / waves;
+        }
+    }
+    x.splits = (int)(splits > 256 ? 256 : splits);
     x.grid = items * x.splits;
     return x;
 }
@@ -101,8 +123,10 @@ void launch(const Plan &x, const PagedParams &k, hipStream_t stream) {
     else if (!SIMP && k.n > 1) hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, !SIMP>), dim3((unsigned)x.grid), dim3(FewCfg<D>::NW * 64), 0, stream, k);
     else hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, false>), dim3((unsigned)x.grid), dim3(FewCfg<D>::NW * 64), 0, stream, k);
     if (x.splits * x.dblocks > 1) {
-        const int per = 256 / (D / 8);
-        hipLaunchKernelGGL((paged_merge_kernel<E, D>), dim3((unsigned)((x.rows + per - 1) / per)), dim3(256), 0, stream, k);
+        const int pg = x.splits * x.dblocks >= 8 ? 8 : 1, per = 256 / (D / 8) / pg;
+        const dim3 grid((unsigned)((x.rows + per - 1) / per));
+        if (pg > 1) hipLaunchKernelGGL((paged_merge_kernel<E, D, 8>), grid, dim3(256), 0, stream, k);
+        else hipLaunchKernelGGL((paged_merge_kernel<E, D, 1>), grid, dim3(256), 0, stream, k);
     }
 }
 

@@ -905,29 +905,54 @@ paged_many_kernel(PagedParams p) {
     }
 }
 
-// ---- partial results of a row merged: D / 8 threads per row
-template <class E, int D>
+// ---- partial results of a row merged: D / 8 threads per part, PG parts at a time (few rows with many parts are a chain of
+// dependent loads otherwise), the groups' sums added in order
+template <class E, int D, int PG>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
-    constexpr int TPR = D / 8;
-    const int64_t rows = (int64_t)p.B * p.n * p.H, row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    constexpr int TPR = D / 8, RPW = 256 / (TPR * PG);
+    __shared__ float sums[PG > 1 ? 256 : 1][PG > 1 ? 11 : 1];
+    const int64_t rows = (int64_t)p.B * p.n * p.H, row = (int64_t)blockIdx.x * RPW + threadIdx.x / (TPR * PG);
+    const int d0 = 8 * (threadIdx.x % TPR), group = threadIdx.x / TPR % PG, parts = p.splits * p.dblocks;
+    float top = kNoRef, total = 0.f, z[8] = {};
+    if (row < rows) {
+        // (a part that attended to nothing has left no row)
+#pragma unroll 4
+        for (int x = group; x < parts; x += PG) {
+            const float2 ml = p.part_ml[x * rows + row];
+            if (ml.y == 0.f) continue;
+            const float *src = p.part_o + ((int64_t)x * rows + row) * D + d0;
+            const float4 a = *reinterpret_cast<const float4 *>(src), c = *reinterpret_cast<const float4 *>(src + 4);
+            const float ref = fmaxf(top, ml.x), f = fast_exp2(ml.x - ref), old = fast_exp2(top - ref);
+            top = ref;
+            total = total * old + f * ml.y;
+            z[0] = z[0] * old + f * a.x; z[1] = z[1] * old + f * a.y; z[2] = z[2] * old + f * a.z; z[3] = z[3] * old + f * a.w;
+            z[4] = z[4] * old + f * c.x; z[5] = z[5] * old + f * c.y; z[6] = z[6] * old + f * c.z; z[7] = z[7] * old + f * c.w;
+        }
+    }
+    if constexpr (PG > 1) {
+        float *mine = sums[threadIdx.x];
+        mine[8] = top;
+        mine[9] = total;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mine[e] = z[e];
+        __syncthreads();
+        if (group) return;
+#pragma unroll
+        for (int y = 1; y < PG; ++y) top = fmaxf(top, mine[y * TPR * 11 + 8]);
+        const float own = fast_exp2(mine[8] - top);
+        total *= own;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] *= own;
+#pragma unroll
+        for (int y = 1; y < PG; ++y) {
+            const float *other = mine + y * TPR * 11;
+            const float f = fast_exp2(other[8] - top);
+            total += f * other[9];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] += f * other[e];
+        }
+    }
     if (row >= rows) return;
-    const int d0 = 8 * (threadIdx.x % TPR), parts = p.splits * p.dblocks;
-    float top = kNoRef;
-    for (int x = 0; x < parts; ++x) {
-        const float2 ml = p.part_ml[x * rows + row];
-        top = ml.y == 0.f ? top : fmaxf(top, ml.x);
-    }
-    float total = 0.f, z[8] = {};
-    for (int x = 0; x < parts; ++x) {
-        const float2 ml = p.part_ml[x * rows + row];
-        if (ml.y == 0.f) continue;                   // (nothing attended: its row is not read)
-        const float f = fast_exp2(ml.x - top);
-        const float *src = p.part_o + ((int64_t)x * rows + row) * D + d0;
-        const float4 a = *reinterpret_cast<const float4 *>(src), c = *reinterpret_cast<const float4 *>(src + 4);
-        total += f * ml.y;
-        z[0] += f * a.x; z[1] += f * a.y; z[2] += f * a.z; z[3] += f * a.w;
-        z[4] += f * c.x; z[5] += f * c.y; z[6] += f * c.z; z[7] += f * c.w;
-    }
     const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] *= inv;
