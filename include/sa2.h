@@ -310,7 +310,8 @@ typedef struct sa2_paged_index {
 typedef struct sa2_paged_problem {
     int32_t batch, rows;          /* sequences, new rows of each */
     int32_t heads, kv_heads;
-    int32_t dim_head;             /* channels of q and out; channels of the pools beyond it have to hold zeros */
+    int32_t dim_head;             /* channels of q and out (attention: a multiple of 8, 16-byte aligned rows; appended rows: any); channels
+                                     of the pools beyond it have to hold zeros */
     int32_t pool_dim;             /* channels of a pool's row: a multiple of 8 up to 256, at least dim_head */
     int32_t page_size, pages, table_width;
     int32_t w1, w2;               /* windows (2-simplicial form only) */

@@ -19,11 +19,11 @@ using namespace sa2;
 
 int kernel_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-PageDiv page_div(int ps) {
-    // floor(x / ps) = (x * mul) >> (31 + s) with mul = floor(2^(31 + s) / ps) + 1, s = ceil(log2 ps): exact for x < 2^31
+Divisor divisor(int by) {
+    // floor(x / by) = (x * mul) >> (31 + s) with mul = floor(2^(31 + s) / by) + 1, s = ceil(log2 by): exact for x < 2^31
     uint32_t s = 0;
-    while ((1ll << s) < ps) ++s;
-    return {(uint32_t)ps, (uint32_t)((1ull << (31 + s)) / ps + 1), 31 + s};
+    while ((1ll << s) < by) ++s;
+    return {(uint32_t)by, (uint32_t)((1ull << (31 + s)) / by + 1), 31 + s};
 }
 
 int check_problem(const sa2_paged_problem *p, bool simplicial) {
@@ -32,9 +32,9 @@ int check_problem(const sa2_paged_problem *p, bool simplicial) {
         return fail_with(SA2_ERR_BAD_SHAPE, "batch=%d rows=%d heads=%d kv_heads=%d page_size=%d pages=%d table_width=%d must all be >= 1", p->batch, p->rows,
                          p->heads, p->kv_heads, p->page_size, p->pages, p->table_width);
     if (p->heads % p->kv_heads != 0) return fail_with(SA2_ERR_BAD_SHAPE, "heads=%d is not a multiple of kv_heads=%d", p->heads, p->kv_heads);
-    if (p->dim_head < 1 || p->pool_dim < p->dim_head || p->pool_dim > 256 || p->pool_dim % 8 != 0)
-        return fail_with(SA2_ERR_UNSUPPORTED, "dim_head=%d in pools of %d channels: a multiple of 8 up to 256 that holds the head is supported", p->dim_head,
-                         p->pool_dim);
+    if (p->dim_head < 8 || p->dim_head % 8 != 0 || p->pool_dim < p->dim_head || p->pool_dim > 256 || p->pool_dim % 8 != 0)
+        return fail_with(SA2_ERR_UNSUPPORTED, "dim_head=%d in pools of %d channels: multiples of 8 up to 256, pools at least as wide as the head, are supported",
+                         p->dim_head, p->pool_dim);
     if (p->dtype != SA2_ELEMENT_BF16 && p->dtype != SA2_ELEMENT_F16) return fail_with(SA2_ERR_UNSUPPORTED, "dtype %d is not supported (bf16 or fp16)", p->dtype);
     if (simplicial && (p->w1 < 1 || p->w2 < 1)) return fail_with(SA2_ERR_BAD_SHAPE, "windows w1=%d w2=%d must be >= 1", p->w1, p->w2);
     if (!(p->scale > 0.f) || !std::isfinite(p->scale)) return fail_with(SA2_ERR_BAD_SHAPE, "scale must be positive and finite");
@@ -99,11 +99,17 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
     return x;
 }
 
-int check_pool(const sa2_paged_problem *p, const sa2_pool *t, const char *name) {
+int check_rows(const sa2_tensor *t, const char *name) {
+    if (!t || !t->ptr) return fail_with(SA2_ERR_NULL_POINTER, "tensor %s is NULL", name);
+    if ((reinterpret_cast<uintptr_t>(t->ptr) & 15) != 0 || (t->stride_b & 7) != 0 || (t->stride_n & 7) != 0 || (t->stride_h & 7) != 0)
+        return fail_with(SA2_ERR_ALIGNMENT, "tensor %s: base pointer must be 16-byte aligned and strides multiples of 8 elements", name);
+    return SA2_OK;
+}
+
+int check_pool(const sa2_pool *t, const char *name) {
     if (!t || !t->ptr) return fail_with(SA2_ERR_NULL_POINTER, "pool %s is NULL", name);
     if ((reinterpret_cast<uintptr_t>(t->ptr) & 15) != 0 || (t->stride_page & 7) != 0 || (t->stride_row & 7) != 0 || (t->stride_head & 7) != 0)
         return fail_with(SA2_ERR_ALIGNMENT, "pool %s: base pointer must be 16-byte aligned and strides multiples of 8 elements", name);
-    (void)p;
     return SA2_OK;
 }
 
@@ -113,15 +119,14 @@ PagedPool pool_of(const sa2_pool *t) {
     return x;
 }
 
-bool whole_pieces(const sa2_tensor *t, int channels) {
-    return channels % 8 == 0 && (reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && t->stride_b % 8 == 0 && t->stride_n % 8 == 0 && t->stride_h % 8 == 0;
-}
-
 template <class E, int D, bool SIMP>
 void launch(const Plan &x, const PagedParams &k, hipStream_t stream) {
     if (x.many) hipLaunchKernelGGL((paged_many_kernel<E, D, SIMP>), dim3((unsigned)x.grid), dim3(ManyCfg<D, SIMP>::NW * 64), 0, stream, k);
-    else if (!SIMP && k.n > 1) hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, !SIMP>), dim3((unsigned)x.grid), dim3(FewCfg<D>::NW * 64), 0, stream, k);
-    else hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, false>), dim3((unsigned)x.grid), dim3(FewCfg<D>::NW * 64), 0, stream, k);
+    else {
+        const dim3 grid((unsigned)(k.B * k.HK), (unsigned)x.row_tiles, (unsigned)(x.splits * x.dblocks));
+        if (!SIMP && k.n > 1) hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, !SIMP>), grid, dim3(FewCfg<D>::NW * 64), 0, stream, k);
+        else hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, false>), grid, dim3(FewCfg<D>::NW * 64), 0, stream, k);
+    }
     if (x.splits * x.dblocks > 1) {
         const int pg = x.splits * x.dblocks >= 8 ? 8 : 1, per = 256 / (D / 8) / pg;
         const dim3 grid((unsigned)((x.rows + per - 1) / per));
@@ -143,14 +148,14 @@ void launch_dim(const Plan &x, const PagedParams &k, hipStream_t stream) {
 int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, const sa2_pool *k1, const sa2_pool *k2, const sa2_pool *v1, const sa2_pool *v2,
            const sa2_paged_index *at, const sa2_tensor *out, void *workspace, int64_t workspace_bytes, void *stream) {
     SA2_TRY(check_problem(p, simplicial));
-    SA2_TRY(check_pool(p, k1, simplicial ? "k1" : "k"));
-    SA2_TRY(check_pool(p, v1, simplicial ? "v1" : "v"));
+    SA2_TRY(check_pool(k1, simplicial ? "k1" : "k"));
+    SA2_TRY(check_pool(v1, simplicial ? "v1" : "v"));
     if (simplicial) {
-        SA2_TRY(check_pool(p, k2, "k2"));
-        SA2_TRY(check_pool(p, v2, "v2"));
+        SA2_TRY(check_pool(k2, "k2"));
+        SA2_TRY(check_pool(v2, "v2"));
     }
-    if (!q || !q->ptr) return fail_with(SA2_ERR_NULL_POINTER, "tensor q is NULL");
-    if (!out || !out->ptr) return fail_with(SA2_ERR_NULL_POINTER, "tensor out is NULL");
+    SA2_TRY(check_rows(q, "q"));
+    SA2_TRY(check_rows(out, "out"));
     if (!at || !at->tables || !at->lengths) return fail_with(SA2_ERR_NULL_POINTER, "tables and lengths are required");
     const Plan x = plan_of(p, simplicial);
     if (x.grid > 0x7fffffffll) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
@@ -174,7 +179,8 @@ int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, con
     k.lengths = at->lengths;
     k.counts = at->counts;
     k.t_sb = at->table_stride;
-    k.div = page_div(p->page_size);
+    k.div = divisor(p->page_size);
+    k.group = divisor(p->heads / p->kv_heads);
     k.pages = p->pages;
     k.width = p->table_width;
     k.B = p->batch;
@@ -184,8 +190,6 @@ int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, con
     k.G = p->heads / p->kv_heads;
     k.dq = p->dim_head;
     k.dp = p->pool_dim;
-    k.q_vec = whole_pieces(q, p->dim_head);
-    k.o_vec = whole_pieces(out, p->dim_head);
     k.w1 = p->w1;
     k.w2 = p->w2;
     k.scale_log2e = p->scale * kLog2e;

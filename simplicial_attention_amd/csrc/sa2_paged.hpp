@@ -62,9 +62,9 @@ struct PagedPool {
     int64_t sp, sr, sh;       // bytes between pages, rows of a page, heads
 };
 
-// division by the page size as a multiplication (dividends below 2^31)
-struct PageDiv {
-    uint32_t ps, mul, shift;
+// division by a number that the host knows as a multiplication (dividends below 2^31)
+struct Divisor {
+    uint32_t by, mul, shift;
     __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)(((uint64_t)x * mul) >> shift); }
 };
 
@@ -76,11 +76,10 @@ struct PagedParams {
     PagedPool k1, v1, k2, v2;                 // (k2, v2: 2-simplicial form only)
     const int32_t *tables, *lengths, *counts; // (counts nullptr: n for every sequence)
     int64_t t_sb;
-    PageDiv div;
+    Divisor div, group;                       // by the page size, by G
     int pages, width;                         // pages of a pool, entries of a table
     int B, n, H, HK, G;
-    int dq, dp;                               // channels of q and the output, and of a pool's row (a multiple of 8)
-    int q_vec, o_vec;                         // rows of q / the output are 16-byte aligned and whole pieces
+    int dq, dp;                               // channels of q and the output, and of a pool's row (multiples of 8)
     int w1, w2;
     float scale_log2e;
     int row_tiles;                            // workgroups (per sequence and key/value head) that the rows take
@@ -114,7 +113,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams &p, int b) {
     count = count < 0 ? 0 : (count > p.n ? p.n : count);
     s.first = (length < 0 ? 0 : length) - count;
     s.count = count;
-    const int64_t reach = (int64_t)p.width * p.div.ps;
+    const int64_t reach = (int64_t)p.width * p.div.by;
     s.reach = reach > 0x7fffffff ? 0x7fffffff : (int)reach;
     return s;
 }
@@ -128,29 +127,13 @@ __device__ __forceinline__ const char *paged_row(const PagedPool &pool, int page
     return pool.ptr + (int64_t)page * pool.sp + (int64_t)row * pool.sr;
 }
 
-// channels d0 .. d0 + 7 of a row of q as a packed piece (zeros beyond its channels)
-template <class E>
+// channels d0 .. d0 + 7 of a row of q (zeros beyond its channels); the same of the output
 __device__ __forceinline__ u32x4 paged_q_piece(const PagedParams &p, const char *row, int d0) {
-    if (p.q_vec) return d0 < p.dq ? ld_global16(row + d0 * 2) : (u32x4){0u, 0u, 0u, 0u};
-    u32x4 r;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const uint32_t a = d0 + 2 * w < p.dq ? *reinterpret_cast<const uint16_t *>(row + (d0 + 2 * w) * 2) : 0u;
-        const uint32_t b = d0 + 2 * w + 1 < p.dq ? *reinterpret_cast<const uint16_t *>(row + (d0 + 2 * w + 1) * 2) : 0u;
-        r[w] = a | (b << 16);
-    }
-    return r;
+    return d0 < p.dq ? ld_global16(row + d0 * 2) : (u32x4){0u, 0u, 0u, 0u};
 }
 template <class E>
 __device__ __forceinline__ void paged_store8(const PagedParams &p, char *row, int d0, const float (&x)[8]) {
-    const u32x4 v = {E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(x[4], x[5]), E::pack(x[6], x[7])};
-    if (p.o_vec) {
-        if (d0 < p.dq) st_global16(row + d0 * 2, v);
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (d0 + e < p.dq) *reinterpret_cast<uint16_t *>(row + (d0 + e) * 2) = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+    if (d0 < p.dq) st_global16(row + d0 * 2, (u32x4){E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(x[4], x[5]), E::pack(x[6], x[7])});
 }
 
 // ---- one wave's 32 columns
@@ -170,18 +153,13 @@ struct PagedWave {
         M = kNoRef;
         l = 0.f;
     }
-    __device__ __forceinline__ void limits(int lo_, int hi_, bool on) {
+    // this column's keys, and the bounds over all columns (`any`: there is one that attends to something)
+    __device__ __forceinline__ void limits(int lo_, int hi_, bool on, bool any, int most_lo_, int least_hi_) {
         on = on && lo_ <= hi_;
         lo = on ? lo_ : 1;
         hi = on ? hi_ : 0;
-        int a = on ? lo_ : -0x7fffffff, z = on ? hi_ : 0x7fffffff;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            a = max(a, __shfl_xor(a, m));
-            z = min(z, __shfl_xor(z, m));
-        }
-        most_lo = uniform(a);
-        least_hi = uniform(z);
+        most_lo = any ? most_lo_ : -0x7fffffff;
+        least_hi = any ? least_hi_ : 0x7fffffff;
     }
 
     __device__ __forceinline__ static float both_halves_max(float x) {
@@ -330,8 +308,9 @@ struct PagedWave {
 
 // ---- 2-simplicial form: from the columns (offsets) of one (token, head) to its output row
 //
-// y[v] of a lane: channel 32 (v / 16) + 16 hf + v % 16 of its column.  Adds the columns and leaves NV / 32 (at least one) sums per
-// lane: y[i] of lane c is the sum for v = base(c) + i.
+// y[v] of a lane: channel 32 (v / 16) + 16 hf + v % 16 of its column.  Adds the columns of a half and leaves NV / 32 (at least one) sums per
+// lane: y[i] of lane c is the sum for v = base(c) + i.  Every step halves what a lane holds: it gives one half away and adds the other lane's
+// share of the half it keeps.  Rows of 16 lanes trade by a swap, lanes of a row with their mirror image in 16, 8, 4 and 2.
 template <int NV>
 struct ColumnSum {
     static constexpr int LEFT = NV > 32 ? NV / 32 : 1;
@@ -345,24 +324,44 @@ struct ColumnSum {
             }
         return b;
     }
+    template <int CTRL>
+    static __device__ __forceinline__ float other(float x) {
+        return as_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)as_u32(x), CTRL, 0xf, 0xf, false));
+    }
     template <int N, int BIT>
     static __device__ __forceinline__ void step(float (&y)[NV], int c) {
         if constexpr (BIT >= 1) {
+            constexpr int CTRL = BIT == 8 ? 0x140 : BIT == 4 ? 0x141 : BIT == 2 ? 0x1b : 0xb1;      // row_mirror, row_half_mirror, quad_perm 3210, 1032
             if constexpr (N > 1) {
                 const bool up = c & BIT;
 #pragma unroll
                 for (int i = 0; i < N / 2; ++i) {
-                    const float keep = up ? y[i + N / 2] : y[i], send = up ? y[i] : y[i + N / 2];
-                    y[i] = keep + __shfl_xor(send, BIT);
+                    if constexpr (BIT == 16) {
+                        auto sw = __builtin_amdgcn_permlane16_swap(as_u32(y[i]), as_u32(y[i + N / 2]), false, false);
+                        y[i] = as_f32(sw[0]) + as_f32(sw[1]);
+                    } else {
+                        const float keep = up ? y[i + N / 2] : y[i], send = up ? y[i] : y[i + N / 2];
+                        y[i] = keep + other<CTRL>(send);
+                    }
                 }
                 step<N / 2, BIT / 2>(y, c);
             } else {
-                y[0] += __shfl_xor(y[0], BIT);
+                y[0] += other<CTRL>(y[0]);
                 step<1, BIT / 2>(y, c);
             }
         }
     }
     static __device__ __forceinline__ void add(float (&y)[NV], int c) { step<NV, 16>(y, c); }
+    // sum and maximum over the 32 lanes of a half, in all of them
+    template <typename OP>
+    static __device__ __forceinline__ float all(float x, OP op) {
+        x = op(x, other<0xb1>(x));
+        x = op(x, other<0x1b>(x));
+        x = op(x, other<0x141>(x));
+        x = op(x, other<0x140>(x));
+        auto sw = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
+        return op(as_f32(sw[0]), as_f32(sw[1]));
+    }
 };
 
 template <class E, int D>
@@ -374,14 +373,14 @@ struct SimplicialColumns {
     __device__ __forceinline__ void build(const PagedParams &p, const PagedSeq &s, PagedWave<E, D> &w, const char *q_row, int pos, int d, int hk, int hf, bool on) {
         const int x = pos - d;
         page2 = on && d < p.w2 ? paged_page(p, s, x) : -1;
-        row2 = page2 >= 0 ? x - (int)p.div((uint32_t)x) * (int)p.div.ps : 0;
+        row2 = page2 >= 0 ? x - (int)p.div((uint32_t)x) * (int)p.div.by : 0;
         const char *k2 = paged_row(p.k2, page2, row2) + hk * p.k2.sh;
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
             const int d0 = 16 * kk + 8 * hf;
             u32x4 a = {0u, 0u, 0u, 0u};
             if (page2 >= 0 && d0 < p.dp) {
-                const u32x4 f = paged_q_piece<E>(p, q_row, d0), k = ld_global16(k2 + d0 * 2);
+                const u32x4 f = paged_q_piece(p, q_row, d0), k = ld_global16(k2 + d0 * 2);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) a[i] = E::pack(E::lo(f[i]) * E::lo(k[i]), E::hi(f[i]) * E::hi(k[i]));
             }
@@ -391,30 +390,26 @@ struct SimplicialColumns {
 
     // the wave's columns as one row relative to one reference: o[v] (see ColumnSum), ref, sum
     __device__ __forceinline__ void finish(const PagedParams &p, const PagedWave<E, D> &w, int hk, int c, int hf, float (&y)[16 * DT], float &ref, float &sum) const {
+        const char *v2 = paged_row(p.v2, page2, row2) + hk * p.v2.sh;
+        u32x4 v[2 * DT];
+#pragma unroll
+        for (int x = 0; x < 2 * DT; ++x) {
+            const int d0 = 32 * (x >> 1) + 16 * hf + 8 * (x & 1);
+            v[x] = page2 >= 0 && d0 < p.dp ? ld_global16(v2 + d0 * 2) : (u32x4){0u, 0u, 0u, 0u};
+        }
         // (columns without a second row, and those that met no key, hold nothing that counts)
         const float column = w.whole_sum();
         const bool live = page2 >= 0 && column != 0.f;
-        ref = live ? w.M : kNoRef;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) ref = fmaxf(ref, __shfl_xor(ref, m));
+        ref = ColumnSum<16 * DT>::all(live ? w.M : kNoRef, [](float a, float b) { return fmaxf(a, b); });
         const float f = live ? fast_exp2(w.M - ref) : 0.f;
-        sum = live ? column * f : 0.f;
+        sum = ColumnSum<16 * DT>::all(live ? column * f : 0.f, [](float a, float b) { return a + b; });
 #pragma unroll
-        for (int m = 1; m < 32; m <<= 1) sum += __shfl_xor(sum, m);
-        const char *v2 = paged_row(p.v2, page2, row2) + hk * p.v2.sh;
+        for (int x = 0; x < 2 * DT; ++x)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int d0 = 32 * dt + 16 * hf + 8 * half;
-                const bool there = live && d0 < p.dp;
-                const u32x4 v = there ? ld_global16(v2 + d0 * 2) : (u32x4){0u, 0u, 0u, 0u};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int at = 16 * dt + 8 * half + 2 * i;
-                    y[at] = there ? w.O[dt][8 * half + 2 * i] * f * E::lo(v[i]) : 0.f;
-                    y[at + 1] = there ? w.O[dt][8 * half + 2 * i + 1] * f * E::hi(v[i]) : 0.f;
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int at = 8 * x + 2 * i;
+                y[at] = live ? w.O[x >> 1][at & 15] * f * E::lo(v[x][i]) : 0.f;
+                y[at + 1] = live ? w.O[x >> 1][(at & 15) + 1] * f * E::hi(v[x][i]) : 0.f;
             }
         ColumnSum<16 * DT>::add(y, c);
     }
@@ -451,100 +446,109 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
     int *seg = reinterpret_cast<int *>(lds + C::RING);
     const int tid = threadIdx.x, wave = wave_index(), lane = tid & 63, c = lane & 31, hf = lane >> 5;
 
-    // item = ((b, hk), row tile, part)
-    const int parts = p.splits * p.dblocks;
-    int item = xcd_contiguous(blockIdx.x, gridDim.x);
-    const int part = uniform(item % parts);
-    item = uniform(item / parts);
-    const int tile_r = uniform(item % p.row_tiles);
-    item = uniform(item / p.row_tiles);
-    const int hk = uniform(item % p.HK), b = uniform(item / p.HK);
-    const int split = uniform(part % p.splits), db = uniform(part / p.splits);
+    // grid: (sequence and key/value head, row tile, part)
+    const int parts = p.splits * p.dblocks, part = blockIdx.z, tile_r = blockIdx.y;
+    const int b = uniform(blockIdx.x / p.HK), hk = blockIdx.x - b * p.HK;
+    const int db = p.dblocks == 1 ? 0 : uniform(part / p.splits), split = part - db * p.splits;
     const PagedSeq s = paged_seq(p, b);
 
     // the columns: token t, head of the group g
     const int R = SIMP ? tile_r : tile_r * 32 + c;
-    const int t = R / p.G, g = R - t * p.G, h = hk * p.G + g;
+    const int t = (int)p.group((uint32_t)R), g = R - t * p.G, h = hk * p.G + g;
     const int pos = s.first + t;
     const bool row_there = R < p.n * p.G;
     const bool on = row_there && t < s.count && pos >= 0;
-    const int t_last = SIMP ? t : min((tile_r * 32 + 31) / p.G, s.count - 1);
+    // (first and last token of the columns)
+    const int t_first = MIXED ? max((int)p.group((uint32_t)(tile_r * 32)), -s.first) : (SIMP ? t : 0);
+    const int t_last = MIXED ? min((int)p.group((uint32_t)(tile_r * 32 + 31)), s.count - 1) : t_first;
     const int last = min(s.first + t_last, s.reach - 1);              // last key of any column
     const int first_key = SIMP ? max(0, s.first + t - p.w1 + 1) : 0;
-    const bool any = SIMP ? on : tile_r * 32 / p.G < s.count && last >= 0;
-    const int tiles = any && last >= first_key ? (last - first_key) / 32 + 1 : 0;
-    const int tile_a = (int)((int64_t)tiles * split / p.splits), tile_z = (int)((int64_t)tiles * (split + 1) / p.splits);
+    const bool any = t_first < s.count && t_first <= t_last && last >= first_key;
+    const int tiles = any ? (last - first_key) / 32 + 1 : 0;
+    const int tile_a = p.splits == 1 ? 0 : (int)((int64_t)tiles * split / p.splits), tile_z = p.splits == 1 ? tiles : (int)((int64_t)tiles * (split + 1) / p.splits);
 
     const char *q_row = p.q + b * p.q_sb + (int64_t)(row_there ? t : 0) * p.q_sn + (int64_t)(row_there ? h : 0) * p.q_sh;
     PagedWave<E, D> w;
     SimplicialColumns<E, D> cols;
     w.clear();
-    if (tile_a < tile_z) {
-        if constexpr (SIMP) {
-            cols.build(p, s, w, q_row, pos, 32 * db + c, hk, hf, on);
-            w.limits(first_key, min(pos, last), on && cols.page2 >= 0);
-        } else {
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) w.A[kk] = on ? paged_q_piece<E>(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
-            w.limits(0, min(pos, last), on);
-        }
-    } else if constexpr (SIMP) {
-        cols.page2 = -1;
-        cols.row2 = 0;
-    }
-
-    const char *const kg = p.k1.ptr + hk * p.k1.sh, *const vg = p.v1.ptr + hk * p.v1.sh;
+    cols.page2 = -1;
+    cols.row2 = 0;
     char *const kt = lds + wave * 2 * RT::BYTES, *const vt = kt + RT::BYTES;
-    const uint32_t kt_at = (uint32_t)(uintptr_t)kt, vt_at = (uint32_t)(uintptr_t)vt;
+    const uint32_t kt_at = (uint32_t)(uintptr_t)kt;
     const char *const zero = reinterpret_cast<const char *>(g_paged_zero_row);
     const int st_col = RT::st_col(lane);
     const bool col_there = st_col < p.dp * 2;
     constexpr int SEG_TILES = C::SEG / 32;
-    for (int seg_a = tile_a; seg_a < tile_z; seg_a += SEG_TILES) {
-        const int seg_z = min(tile_z, seg_a + SEG_TILES);
-        __syncthreads();
+    int seg_a = tile_a, seg_z = tile_a, u = tile_a;
+    // requests a tile's rows of K or V (a rolled loop: a call of few rows runs through its code once, and fetching code is what it waits for)
+    auto request = [&](int is_v, int tile) {
+        const char *const base = (is_v ? p.v1.ptr : p.k1.ptr) + hk * (is_v ? p.v1.sh : p.k1.sh) + st_col;
+        const int64_t sp = is_v ? p.v1.sp : p.k1.sp, sr = is_v ? p.v1.sr : p.k1.sr;
+        const uint32_t to = kt_at + is_v * RT::BYTES;
+        int x = 32 * (tile - seg_a) + RT::st_row(0, lane);
+#pragma unroll 1
+        for (int ch = 0; ch < RT::NCH; ++ch, x += RT::RPC) {
+            const int at = first_key + 32 * seg_a + x, page = seg[x];
+            const int row = at - (int)p.div((uint32_t)at) * (int)p.div.by;
+            const char *from = base + (int64_t)page * sp + (int64_t)row * sr;
+            load_to_lds16_from(page >= 0 && col_there ? from : zero, to + ch * RT::CP);
+        }
+    };
+    // pages of the next positions, and the wave's first tile of them
+    auto open_segment = [&](int early) {
+        seg_z = min(tile_z, seg_a + SEG_TILES);
         for (int x = tid; x < (seg_z - seg_a) * 32; x += NW * 64) {
             const int at = first_key + seg_a * 32 + x;
-            seg[x] = at <= last ? paged_page(p, s, at) : -1;
+            seg[x] = at > last ? -1 : early >= -1 && x < NW * 64 ? early : paged_page(p, s, at);
         }
         __syncthreads();
-        auto request = [&](const PagedPool &pool, const char *base, uint32_t lds_at, int tile) {
-#pragma unroll
-            for (int ch = 0; ch < RT::NCH; ++ch) {
-                const int x = 32 * (tile - seg_a) + RT::st_row(ch, lane);
-                const int at = first_key + 32 * seg_a + x, page = seg[x];
-                const int row = at - (int)p.div((uint32_t)at) * (int)p.div.ps;
-                const char *from = base + (int64_t)page * pool.sp + (int64_t)row * pool.sr + st_col;
-                load_to_lds16_from(page >= 0 && col_there ? from : zero, lds_at + ch * RT::CP);
-            }
-        };
-        int u = seg_a + wave;
+        u = seg_a + wave;
         if (u < seg_z) {
-            request(p.k1, kg, kt_at, u);
-            request(p.v1, vg, vt_at, u);
+#pragma unroll 1
+            for (int is_v = 0; is_v < 2; ++is_v) request(is_v, u);
         }
-        for (; u < seg_z; u += NW) {
-            const int tile = first_key + 32 * u, next = u + NW;
-            const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(seg[32 * (u - seg_a) + c] >= 0);
-            wait_loads<RT::NCH>();
-            f32x16 S = w.logits(kt + RT::row_lane(lane));
-            wait_lds_reads();
-            if (next < seg_z) request(p.k1, kg, kt_at, next);
-            const bool masked = w.needs_mask(tile, there);
-            if (masked) w.mask(S, tile, there, hf);
-            u32x4 pb[2];
-            float sum;
-            if (__builtin_expect(!w.weights(S, p.scale_log2e, pb, sum), 0)) {
-                w.move_reference(S, p.scale_log2e);
-                w.weights(S, p.scale_log2e, pb, sum);
+    };
+    // (an undivided walk starts at position 0: its first pages are looked up beside the length)
+    const int early = !SIMP && p.splits == 1 ? paged_page(p, s, tid) : -2;
+    if (tile_a < tile_z) {
+        open_segment(early);
+        // the columns, read behind the first transfers
+        if constexpr (SIMP) {
+            cols.build(p, s, w, q_row, pos, 32 * db + c, hk, hf, on);
+            w.limits(first_key, last, on && cols.page2 >= 0, true, first_key, last);
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) w.A[kk] = on ? paged_q_piece(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
+            w.limits(0, min(pos, last), on, true, 0, min(s.first + t_first, last));
+        }
+        for (;;) {
+            for (; u < seg_z; u += NW) {
+                const int tile = first_key + 32 * u, next = u + NW;
+                const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(seg[32 * (u - seg_a) + c] >= 0);
+                wait_loads<RT::NCH>();
+                f32x16 S = w.logits(kt + RT::row_lane(lane));
+                wait_lds_reads();
+                if (next < seg_z) request(0, next);
+                const bool masked = w.needs_mask(tile, there);
+                if (masked) w.mask(S, tile, there, hf);
+                u32x4 pb[2];
+                float sum;
+                if (__builtin_expect(!w.weights(S, p.scale_log2e, pb, sum), 0)) {
+                    w.move_reference(S, p.scale_log2e);
+                    w.weights(S, p.scale_log2e, pb, sum);
+                }
+                w.l += sum;
+                if (next < seg_z) wait_loads<RT::NCH>();
+                else wait_loads<0>();
+                // (a workgroup with one token has no key that some of its columns attend and others do not)
+                w.template values<!MIXED>(vt + RT::tr_lane(lane), pb, MIXED && masked, tile, there, hf);
+                wait_lds_reads();
+                if (next < seg_z) request(1, next);
             }
-            w.l += sum;
-            if (next < seg_z) wait_loads<RT::NCH>();
-            else wait_loads<0>();
-            // (a workgroup with one token has no key that some of its columns attend and others do not)
-            w.template values<!MIXED>(vt + RT::tr_lane(lane), pb, MIXED && masked, tile, there, hf);
-            wait_lds_reads();
-            if (next < seg_z) request(p.v1, vg, vt_at, next);
+            seg_a += SEG_TILES;
+            if (seg_a >= tile_z) break;
+            __syncthreads();
+            open_segment(-2);
         }
     }
 
@@ -622,7 +626,7 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
 #pragma unroll
                 for (int e = 0; e < 8; ++e) z[e] += f * mo[(y * 32 + rr) * C::OP + d0 + e];
             }
-            const int R2 = tile_r * 32 + rr, t2 = R2 / p.G, h2 = hk * p.G + R2 - t2 * p.G;
+            const int R2 = tile_r * 32 + rr, t2 = (int)p.group((uint32_t)R2), h2 = hk * p.G + R2 - t2 * p.G;
             if (parts == 1) {
                 const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
 #pragma unroll
@@ -687,11 +691,11 @@ paged_many_kernel(PagedParams p) {
     const PagedSeq s = paged_seq(p, b);
 
     const int R0 = tile_r * PER_WG, R = SIMP ? R0 + wave : R0 + wave * 32 + c;
-    const int t = R / p.G, g = R - t * p.G, h = hk * p.G + g;
+    const int t = (int)p.group((uint32_t)R), g = R - t * p.G, h = hk * p.G + g;
     const int pos = s.first + t;
     const bool row_there = R < p.n * p.G;
     const bool on = row_there && t < s.count && pos >= 0;
-    const int t_first = R0 / p.G, t_last = min((R0 + PER_WG - 1) / p.G, s.count - 1);
+    const int t_first = (int)p.group((uint32_t)R0), t_last = min((int)p.group((uint32_t)(R0 + PER_WG - 1)), s.count - 1);
     const int last = min(s.first + t_last, s.reach - 1);
     const int first_key = SIMP ? max(0, s.first + t_first - p.w1 + 1) : 0;
     const int tiles = t_first < s.count && last >= first_key ? (last - first_key) / 32 + 1 : 0;
@@ -710,7 +714,7 @@ paged_many_kernel(PagedParams p) {
         for (int x = from + tid; x < from + C::SEG / 2; x += NW * 64) {
             const int at = start + x;
             const int page = at <= last && at >= 0 ? paged_page(p, s, at) : -1;
-            const int row = at - (int)p.div((uint32_t)at) * (int)p.div.ps;
+            const int row = at - (int)p.div((uint32_t)at) * (int)p.div.by;
             seg_k[x & (C::SEG - 1)] = page < 0 ? zero : k_head + (int64_t)page * p.k1.sp + (int64_t)row * p.k1.sr;
             seg_v[x & (C::SEG - 1)] = page < 0 ? zero : v_head + (int64_t)page * p.v1.sp + (int64_t)row * p.v1.sr;
             missing |= page < 0 && at <= last;
@@ -748,27 +752,32 @@ paged_many_kernel(PagedParams p) {
     // (the columns are read behind the first transfers)
     const char *q_row = p.q + b * p.q_sb + (int64_t)(row_there ? t : 0) * p.q_sn + (int64_t)(row_there ? h : 0) * p.q_sh;
     w.clear();
+    // keys that any column of the wave attends
+    int lo, hi;
     if constexpr (SIMP) {
         cols.build(p, s, w, q_row, pos, 32 * db + c, hk, hf, on);
-        w.limits(max(0, pos - p.w1 + 1), min(pos, last), on && cols.page2 >= 0);
+        const bool any = wave_any(on && cols.page2 >= 0);
+        lo = any ? max(0, pos - p.w1 + 1) : 0x7fffffff;
+        hi = any ? min(pos, last) : -1;
+        w.limits(lo, hi, on && cols.page2 >= 0, any && lo <= hi, lo, hi);
     } else {
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) w.A[kk] = on ? paged_q_piece<E>(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
-        w.limits(0, min(pos, last), on);
+        for (int kk = 0; kk < KS; ++kk) w.A[kk] = on ? paged_q_piece(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
+        const int t0 = max((int)p.group((uint32_t)(R0 + 32 * wave)), -s.first), t1 = min((int)p.group((uint32_t)(R0 + 32 * wave + 31)), s.count - 1);
+        const bool any = t0 <= t1 && last >= 0;
+        lo = any ? 0 : 0x7fffffff;
+        hi = any ? min(s.first + t1, last) : -1;
+        w.limits(0, min(pos, last), on, any, 0, min(s.first + t0, last));
     }
+    lo = uniform(lo);
+    hi = uniform(hi);
+    w.most_lo = uniform(w.most_lo);
+    w.least_hi = uniform(w.least_hi);
     // (in registers from here on: a wait for them inside the walk would wait for the transfers too)
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) asm volatile("" : "+v"(w.A[kk]));
     if (NT > 0) {
-        // steps that any column of the wave attends
-        int lo = w.lo <= w.hi ? w.lo : 0x7fffffff, hi = w.lo <= w.hi ? w.hi : -1;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            lo = min(lo, __shfl_xor(lo, m));
-            hi = max(hi, __shfl_xor(hi, m));
-        }
-        lo = uniform(lo);
-        hi = uniform(hi);
+        // their steps
         const int u_a = lo > hi || hi < start ? NT : min(NT, max(0, lo - start) >> 5), u_z = lo > hi || hi < start ? NT : min(NT, ((hi - start) >> 5) + 1);
         const int k_lane = RT::row_lane(lane), v_lane = RT::BYTES + RT::tr_lane(lane);
         u32x4 kf[FW];

@@ -565,7 +565,15 @@ Tensor paged_attend(const Tensor &q_in, const std::vector<Tensor> &keys, const s
     pools.insert(pools.end(), values.begin(), values.end());
     for (const Tensor &t : pools) refuse_autograd("attention over a paged cache", {&t});
     refuse_autograd("attention over a paged cache", {&q_in});
-    const Tensor q = q_in.dim() == 4 && q_in.stride(3) != 1 ? q_in.contiguous() : q_in;
+    // (rows of whole aligned pieces: others are copied, and channels of zeros appended)
+    Tensor q = q_in;
+    if (q_in.dim() == 4 && q_in.numel() > 0 && q_in.is_cuda()) {
+        const bool whole = q_in.size(3) % 8 == 0;
+        if (!whole || q_in.stride(3) != 1 || reinterpret_cast<uintptr_t>(q_in.data_ptr()) % 16 || q_in.stride(0) % 8 || q_in.stride(1) % 8 || q_in.stride(2) % 8) {
+            const c10::DeviceGuard guard(q_in.device());
+            q = whole ? q_in.clone(at::MemoryFormat::Contiguous) : at::constant_pad_nd(q_in, {0, 8 - q_in.size(3) % 8}).contiguous();
+        }
+    }
     PagedCall c = paged_call(q, pools, tables, lengths, counts);
     if (q.scalar_type() != pools[0].scalar_type()) raise(PyExc_TypeError, "q and the pages must share one dtype");
     const int64_t kv = pools[0].size(2);
@@ -575,10 +583,10 @@ Tensor paged_attend(const Tensor &q_in, const std::vector<Tensor> &keys, const s
     if (max_length && *max_length < 0) raise(PyExc_ValueError, "max_length must not be negative");
     c.prob.w1 = (int32_t)std::min<int64_t>(w1, INT32_MAX);
     c.prob.w2 = (int32_t)std::min<int64_t>(w2, INT32_MAX);
-    c.prob.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)q.size(3)));
+    c.prob.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)q_in.size(3)));
     c.prob.max_length = max_length ? (int32_t)std::min<int64_t>(*max_length, INT32_MAX) : 0;
     const c10::DeviceGuard guard(q.device());
-    if (c.empty) return at::zeros(q.sizes(), q.options());
+    if (c.empty) return at::zeros(q_in.sizes(), q_in.options());
     const Tensor out = at::empty(q.sizes(), q.options());
     const int64_t bytes = simplicial ? sa2_paged_simplicial_attn_workspace_bytes(&c.prob) : sa2_paged_attn_workspace_bytes(&c.prob);
     Tensor ws;
@@ -589,7 +597,7 @@ Tensor paged_attend(const Tensor &q_in, const std::vector<Tensor> &keys, const s
     for (size_t i = 0; i < pools.size(); ++i) a[i] = pool_arg(pools[i]);
     if (simplicial) check(sa2_paged_simplicial_attn(&c.prob, &aq, &a[0], &a[1], &a[2], &a[3], &c.at, &ao, wsp, std::max<int64_t>(bytes, 0), stream_of(q)));
     else check(sa2_paged_attn(&c.prob, &aq, &a[0], &a[1], &c.at, &ao, wsp, std::max<int64_t>(bytes, 0), stream_of(q)));
-    return out;
+    return out.size(3) == q_in.size(3) ? out : out.narrow(3, 0, q_in.size(3)).contiguous();
 }
 
 void paged_append(const std::vector<Tensor> &pools, const std::vector<Tensor> &rows_in, const Tensor &tables, const Tensor &lengths, const std::optional<Tensor> &counts) {
