@@ -52,10 +52,8 @@ struct ElemF16 {
 };
 // mfma_in_place: the accumulator's registers are the result's.  (Left to itself the compiler gives a product of the loop below other registers than its
 // addend, and copies 16 of them per product and step.)  Written as assembly, so the wait states it needs are this code's business: two
-// behind a VALU write of an operand are in it, and products_done stands in front of whatever else reads the accumulators (18 wait
-// states behind an MFMA of 16 passes).  The compiler must not move an accumulator between two of them: kernels that use it are held to ordinary registers
+// behind a VALU write of an operand are in it, and PagedWave::settle stands behind a run of them.  The compiler must not move an accumulator between two of them: kernels that use it are held to ordinary registers
 // (-amdgpu-mfma-vgpr-form, two waves per SIMD or more, no spills).
-__device__ __forceinline__ void products_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 struct PagedPool {
     const char *ptr;
@@ -137,7 +135,8 @@ __device__ __forceinline__ void paged_store8(const PagedParams &p, char *row, in
 }
 
 // ---- one wave's 32 columns
-template <class E, int D>
+// IN_PLACE: value products by mfma_in_place
+template <class E, int D, bool IN_PLACE = false>
 struct PagedWave {
     using RT = DmaTile<D>;
     static constexpr int KS = D / 16, DT = D / 32;
@@ -165,6 +164,18 @@ struct PagedWave {
     __device__ __forceinline__ static float both_halves_max(float x) {
         auto sw = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);
         return fmaxf(as_f32(sw[0]), as_f32(sw[1]));
+    }
+
+    __device__ __forceinline__ void add_product(int dt, u32x4 v, u32x4 w) {
+        if constexpr (IN_PLACE) E::mfma_in_place(O[dt], v, w);
+        else O[dt] = E::mfma(v, w, O[dt]);
+    }
+    // behind in-place products, in front of whatever else reads or copies the accumulators (18 wait states behind an MFMA of 16 passes)
+    __device__ __forceinline__ void settle() {
+        if constexpr (IN_PLACE) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) asm volatile("s_nop 15\n\ts_nop 1" : "+v"(O[dt]));
+        }
     }
 
     __device__ __forceinline__ f32x16 logits(const char *k_lane) const {
@@ -234,7 +245,8 @@ struct PagedWave {
 #pragma unroll
             for (int k2s = 0; k2s < 2; ++k2s)
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) O[dt] = E::mfma(RT::tr_frag(v_lane, k2s, dt), pb[k2s], O[dt]);
+                for (int dt = 0; dt < DT; ++dt) add_product(dt, RT::tr_frag(v_lane, k2s, dt), pb[k2s]);
+            settle();
             return;
         }
         auto key_masks = [&](uint32_t keys, u32x4 (&m)[2]) {
@@ -258,7 +270,8 @@ struct PagedWave {
 #pragma unroll
             for (int k2s = 0; k2s < 2; ++k2s)
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) O[dt] = E::mfma(RT::tr_frag(v_lane, k2s, dt) & m[k2s], pb[k2s], O[dt]);
+                for (int dt = 0; dt < DT; ++dt) add_product(dt, RT::tr_frag(v_lane, k2s, dt) & m[k2s], pb[k2s]);
+            settle();
             return;
         }
         uint32_t odd = 0u;
@@ -276,7 +289,8 @@ struct PagedWave {
 #pragma unroll
             for (int k2s = 0; k2s < 2; ++k2s)
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) O[dt] = E::mfma(RT::tr_frag(v_lane, k2s, dt), pb[k2s], O[dt]);
+                for (int dt = 0; dt < DT; ++dt) add_product(dt, RT::tr_frag(v_lane, k2s, dt), pb[k2s]);
+            settle();
             return;
         }
         // last keys inside the tile, then the columns that attend to all of it
@@ -370,7 +384,8 @@ struct SimplicialColumns {
     int page2, row2;          // place of the column's second row (page2 < 0: there is none)
 
     // A = q * k2 of the column's offset
-    __device__ __forceinline__ void build(const PagedParams &p, const PagedSeq &s, PagedWave<E, D> &w, const char *q_row, int pos, int d, int hk, int hf, bool on) {
+    template <class W>
+    __device__ __forceinline__ void build(const PagedParams &p, const PagedSeq &s, W &w, const char *q_row, int pos, int d, int hk, int hf, bool on) {
         const int x = pos - d;
         page2 = on && d < p.w2 ? paged_page(p, s, x) : -1;
         row2 = page2 >= 0 ? x - (int)p.div((uint32_t)x) * (int)p.div.by : 0;
@@ -389,7 +404,8 @@ struct SimplicialColumns {
     }
 
     // the wave's columns as one row relative to one reference: o[v] (see ColumnSum), ref, sum
-    __device__ __forceinline__ void finish(const PagedParams &p, const PagedWave<E, D> &w, int hk, int c, int hf, float (&y)[16 * DT], float &ref, float &sum) const {
+    template <class W>
+    __device__ __forceinline__ void finish(const PagedParams &p, const W &w, int hk, int c, int hf, float (&y)[16 * DT], float &ref, float &sum) const {
         const char *v2 = paged_row(p.v2, page2, row2) + hk * p.v2.sh;
         u32x4 v[2 * DT];
 #pragma unroll
@@ -676,7 +692,7 @@ paged_many_kernel(PagedParams p) {
     __shared__ __attribute__((aligned(16))) char lds[C::LDS];
     // addresses of the walked positions' rows in the K and the V pool; a row of zeros where there is none
     const char **seg_k = reinterpret_cast<const char **>(lds + C::RING), **seg_v = seg_k + C::SEG;
-    int *gaps = reinterpret_cast<int *>(lds + C::RING + 2 * C::SEG * 8);     // per half: keys are missing in front of the last one
+    int *gaps = reinterpret_cast<int *>(lds + C::RING + 2 * C::SEG * 8);     // per half (of four): keys are missing in front of the last one
     const int tid = threadIdx.x, wave = wave_index(), lane = tid & 63, c = lane & 31, hf = lane >> 5;
     constexpr int PER_WG = SIMP ? NW : NW * 32;        // rows (t, g) of a workgroup
 
@@ -719,7 +735,8 @@ paged_many_kernel(PagedParams p) {
             seg_v[x & (C::SEG - 1)] = page < 0 ? zero : v_head + (int64_t)page * p.v1.sp + (int64_t)row * p.v1.sr;
             missing |= page < 0 && at <= last;
         }
-        if (missing) gaps[half & 1] = 1;
+        if (missing) gaps[half & 3] = 1;
+        if (tid == 0) gaps[(half + 1) & 3] = 0;          // (the next one's, long unused)
     };
     // keys of a tile that are there (keys beyond the last one are masked as the columns' future)
     auto there_of = [&](int u, int any_gap) {
@@ -739,12 +756,13 @@ paged_many_kernel(PagedParams p) {
         }
     };
 
-    PagedWave<E, D> w;
+    PagedWave<E, D, (D == 64 || D == 128)> w;
     SimplicialColumns<E, D> cols;
     if (NT > 0) {
-        if (tid < 2) gaps[tid] = 0;
+        if (tid < 4) gaps[tid] = 0;
         __syncthreads();
         fill(0);
+        __syncthreads();
         fill(1);
         __syncthreads();
         for (int u = 0; u < NBUF - 1; ++u) request(u);
@@ -791,10 +809,8 @@ paged_many_kernel(PagedParams p) {
         for (int u = 0; u < NT;) {
             // sixteen steps at a time: the places of the sixteen that follow go where those of the sixteen before were
             __syncthreads();
-            const int half = u / C::HALF, any_gap = uniform(gaps[half & 1]);
+            const int half = u / C::HALF, any_gap = uniform(gaps[half & 3]);
             if (half > 0) {
-                __syncthreads();
-                if (tid == 0) gaps[(half + 1) & 1] = 0;
                 __syncthreads();
                 fill(half + 1);
             }
@@ -840,14 +856,14 @@ paged_many_kernel(PagedParams p) {
 #pragma unroll
                         for (int m = 0; m < 2 * DT; ++m) {
                             const u32x4 v = {vf[m % FW][0][0], vf[m % FW][0][1], vf[m % FW][1][0], vf[m % FW][1][1]};
-                            E::mfma_in_place(w.O[m % DT], v, pb[m / DT]);
+                            w.add_product(m % DT, v, pb[m / DT]);
                             if (m + FW < 2 * DT) read_vf(m + FW);
                             if (m >= 2 * DT - FW) kf[m - (2 * DT - FW)] = ld_lds16(next + RT::row_imm(m - (2 * DT - FW)));
                             __builtin_amdgcn_sched_barrier(0);
                         }
                         ++u;
                     } while (u < m_z);
-                    products_done();
+                    w.settle();
                     if (!opened) continue;
                 }
                 // steps with a mask, and those that move a reference
@@ -870,6 +886,7 @@ paged_many_kernel(PagedParams p) {
         wait_loads<0>();
     }
 
+    w.settle();
     const int64_t rows = (int64_t)p.B * p.n * p.H, row = ((int64_t)b * p.n + t) * p.H + h;
     if constexpr (SIMP) {
         float y[16 * DT], ref, sum;
