@@ -23,6 +23,7 @@ namespace sa2 {
 struct ElemBf16 {
     static constexpr float kBig = 1.152921504606846976e18f;      // 2^60
     static constexpr uint32_t kExp = 0x7f80u;
+    static constexpr float kDown = 1.f;
     static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
     static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
@@ -37,6 +38,7 @@ struct ElemF16 {
     typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
     static constexpr float kBig = 16384.f;                       // 2^14: weights stay below the largest fp16 number
     static constexpr uint32_t kExp = 0x7c00u;
+    static constexpr float kDown = 1.f / 256;                    // of products of two numbers, so that they stay below the largest one
     static __device__ __forceinline__ float lo(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
     static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -79,7 +81,7 @@ struct PagedParams {
     int B, n, H, HK, G;
     int dq, dp;                               // channels of q and the output, and of a pool's row (multiples of 8)
     int w1, w2;
-    float scale_log2e;
+    float scale_log2e;                        // (2-simplicial: of operands that are E::kDown times theirs)
     int row_tiles;                            // workgroups (per sequence and key/value head) that the rows take
     int splits, dblocks;                      // shares of the keys; blocks of 32 offsets
     // partial results where splits * dblocks > 1: fp32 [part][B n H][D] and [part][B n H] (reference, sum)
@@ -135,12 +137,13 @@ __device__ __forceinline__ void paged_store8(const PagedParams &p, char *row, in
 }
 
 // ---- one wave's 32 columns
-// IN_PLACE: value products by mfma_in_place
-template <class E, int D, bool IN_PLACE = false>
+// TWO: the operand of the logits in two parts (q * k2 has twice the digits of an element: rounded to one part it would double the error of
+// the output, in two it is exact)   IN_PLACE: value products by mfma_in_place
+template <class E, int D, bool TWO, bool IN_PLACE = false>
 struct PagedWave {
     using RT = DmaTile<D>;
     static constexpr int KS = D / 16, DT = D / 32;
-    u32x4 A[KS];
+    u32x4 A[KS], A2[TWO ? KS : 1];
     f32x16 O[DT];
     float M, l;              // reference (log2 units) and this half's sum of the column's weights
     int lo, hi;              // keys the column attends (empty: lo > hi)
@@ -178,10 +181,15 @@ struct PagedWave {
         }
     }
 
+    __device__ __forceinline__ f32x16 logit(u32x4 k, int kk, f32x16 S) const {
+        S = E::mfma(k, A[kk], S);
+        if constexpr (TWO) S = E::mfma(k, A2[kk], S);
+        return S;
+    }
     __device__ __forceinline__ f32x16 logits(const char *k_lane) const {
         f32x16 S = zero16();
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) S = E::mfma(RT::row_frag(k_lane, kk), A[kk], S);
+        for (int kk = 0; kk < KS; ++kk) S = logit(RT::row_frag(k_lane, kk), kk, S);
         return S;
     }
 
@@ -207,6 +215,14 @@ struct PagedWave {
         }
         return !wave_any(!(sum < E::kBig));
     }
+    // columns without a reference take the tile's largest logit (they hold nothing yet)
+    __device__ __forceinline__ void first_reference(const f32x16 &S, float c) {
+        float top = S[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, S[r]);
+        const float ref = fmaxf(kNoRef, both_halves_max(top) * c);
+        M = M == kNoRef ? ref : M;
+    }
     // moves the reference of every column up to the tile's largest logit
     __device__ __forceinline__ void move_reference(const f32x16 &S, float c) {
         float top = S[0];
@@ -226,6 +242,7 @@ struct PagedWave {
     __device__ __forceinline__ void step(const char *k_lane, const char *v_lane, float c, bool masked, bool guard, int tile, uint32_t there, int hf) {
         f32x16 S = logits(k_lane);
         if (masked) mask(S, tile, there, hf);
+        if (wave_any(M == kNoRef)) first_reference(S, c);
         u32x4 pb[2];
         float sum;
         if (__builtin_expect(!weights(S, c, pb, sum), 0)) {
@@ -393,13 +410,18 @@ struct SimplicialColumns {
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
             const int d0 = 16 * kk + 8 * hf;
-            u32x4 a = {0u, 0u, 0u, 0u};
+            u32x4 a = {0u, 0u, 0u, 0u}, a2 = a;
             if (page2 >= 0 && d0 < p.dp) {
                 const u32x4 f = paged_q_piece(p, q_row, d0), k = ld_global16(k2 + d0 * 2);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = E::pack(E::lo(f[i]) * E::lo(k[i]), E::hi(f[i]) * E::hi(k[i]));
+                for (int i = 0; i < 4; ++i) {
+                    const float x = E::lo(f[i]) * E::kDown * E::lo(k[i]), y = E::hi(f[i]) * E::kDown * E::hi(k[i]);
+                    a[i] = E::pack(x, y);
+                    a2[i] = E::pack(x - E::lo(a[i]), y - E::hi(a[i]));
+                }
             }
             w.A[kk] = a;
+            w.A2[kk] = a2;
         }
     }
 
@@ -419,14 +441,21 @@ struct SimplicialColumns {
         ref = ColumnSum<16 * DT>::all(live ? w.M : kNoRef, [](float a, float b) { return fmaxf(a, b); });
         const float f = live ? fast_exp2(w.M - ref) : 0.f;
         sum = ColumnSum<16 * DT>::all(live ? column * f : 0.f, [](float a, float b) { return a + b; });
+        // (a column that does not count has a factor and a second value of zero; what it holds is only set aside where it is no number: it
+        // attends the same values as the others, but its weights are not numbers where a key is infinite)
+        const bool aside = wave_any(!live && !(column < INFINITY));
 #pragma unroll
         for (int x = 0; x < 2 * DT; ++x)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int at = 8 * x + 2 * i;
-                y[at] = live ? w.O[x >> 1][at & 15] * f * E::lo(v[x][i]) : 0.f;
-                y[at + 1] = live ? w.O[x >> 1][(at & 15) + 1] * f * E::hi(v[x][i]) : 0.f;
+                y[at] = w.O[x >> 1][at & 15] * (f * E::lo(v[x][i]));
+                y[at + 1] = w.O[x >> 1][(at & 15) + 1] * (f * E::hi(v[x][i]));
             }
+        if (__builtin_expect(aside, 0)) {
+#pragma unroll
+            for (int at = 0; at < 16 * DT; ++at) y[at] = live ? y[at] : 0.f;
+        }
         ColumnSum<16 * DT>::add(y, c);
     }
 };
@@ -484,7 +513,7 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
     const int tile_a = p.splits == 1 ? 0 : (int)((int64_t)tiles * split / p.splits), tile_z = p.splits == 1 ? tiles : (int)((int64_t)tiles * (split + 1) / p.splits);
 
     const char *q_row = p.q + b * p.q_sb + (int64_t)(row_there ? t : 0) * p.q_sn + (int64_t)(row_there ? h : 0) * p.q_sh;
-    PagedWave<E, D> w;
+    PagedWave<E, D, SIMP> w;
     SimplicialColumns<E, D> cols;
     w.clear();
     cols.page2 = -1;
@@ -496,18 +525,25 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
     const bool col_there = st_col < p.dp * 2;
     constexpr int SEG_TILES = C::SEG / 32;
     int seg_a = tile_a, seg_z = tile_a, u = tile_a;
-    // requests a tile's rows of K or V (a rolled loop: a call of few rows runs through its code once, and fetching code is what it waits for)
+    // requests a tile's rows of K or V (four transfers at a time: their pages are looked up together)
     auto request = [&](int is_v, int tile) {
         const char *const base = (is_v ? p.v1.ptr : p.k1.ptr) + hk * (is_v ? p.v1.sh : p.k1.sh) + st_col;
         const int64_t sp = is_v ? p.v1.sp : p.k1.sp, sr = is_v ? p.v1.sr : p.k1.sr;
         const uint32_t to = kt_at + is_v * RT::BYTES;
         int x = 32 * (tile - seg_a) + RT::st_row(0, lane);
+        constexpr int AT_ONCE = RT::NCH < 4 ? RT::NCH : 4;
 #pragma unroll 1
-        for (int ch = 0; ch < RT::NCH; ++ch, x += RT::RPC) {
-            const int at = first_key + 32 * seg_a + x, page = seg[x];
-            const int row = at - (int)p.div((uint32_t)at) * (int)p.div.by;
-            const char *from = base + (int64_t)page * sp + (int64_t)row * sr;
-            load_to_lds16_from(page >= 0 && col_there ? from : zero, to + ch * RT::CP);
+        for (int ch = 0; ch < RT::NCH; ch += AT_ONCE, x += AT_ONCE * RT::RPC) {
+            int page[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) page[i] = seg[x + i * RT::RPC];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int at = first_key + 32 * seg_a + x + i * RT::RPC;
+                const int row = at - (int)p.div((uint32_t)at) * (int)p.div.by;
+                const char *from = base + (int64_t)page[i] * sp + (int64_t)row * sr;
+                load_to_lds16_from(page[i] >= 0 && col_there ? from : zero, to + (ch + i) * RT::CP);
+            }
         }
     };
     // pages of the next positions, and the wave's first tile of them
@@ -547,6 +583,7 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
                 if (next < seg_z) request(0, next);
                 const bool masked = w.needs_mask(tile, there);
                 if (masked) w.mask(S, tile, there, hf);
+                if (wave_any(w.M == kNoRef)) w.first_reference(S, p.scale_log2e);
                 u32x4 pb[2];
                 float sum;
                 if (__builtin_expect(!w.weights(S, p.scale_log2e, pb, sum), 0)) {
@@ -756,7 +793,7 @@ paged_many_kernel(PagedParams p) {
         }
     };
 
-    PagedWave<E, D, (D == 64 || D == 128)> w;
+    PagedWave<E, D, SIMP, (D == 64 || D == 128)> w;
     SimplicialColumns<E, D> cols;
     if (NT > 0) {
         if (tid < 4) gaps[tid] = 0;
@@ -793,7 +830,10 @@ paged_many_kernel(PagedParams p) {
     w.least_hi = uniform(w.least_hi);
     // (in registers from here on: a wait for them inside the walk would wait for the transfers too)
 #pragma unroll
-    for (int kk = 0; kk < KS; ++kk) asm volatile("" : "+v"(w.A[kk]));
+    for (int kk = 0; kk < KS; ++kk) {
+        asm volatile("" : "+v"(w.A[kk]));
+        if constexpr (SIMP) asm volatile("" : "+v"(w.A2[kk]));
+    }
     if (NT > 0) {
         // their steps
         const int u_a = lo > hi || hi < start ? NT : min(NT, max(0, lo - start) >> 5), u_z = lo > hi || hi < start ? NT : min(NT, ((hi - start) >> 5) + 1);
@@ -838,7 +878,7 @@ paged_many_kernel(PagedParams p) {
                         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                         for (int kk = 0; kk < KS; ++kk) {
-                            S = E::mfma(kf[kk % FW], w.A[kk], S);
+                            S = w.logit(kf[kk % FW], kk, S);
                             if (kk == 0) request(u + NBUF - 1);
                             if (kk + FW < KS) kf[kk % FW] = ld_lds16(buf + k_lane + RT::row_imm(kk + FW));
                             if (kk >= KS - FW) read_vf(kk - (KS - FW));
