@@ -192,7 +192,7 @@ int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, con
     k.dp = p->pool_dim;
     k.w1 = p->w1;
     k.w2 = p->w2;
-    k.scale_log2e = p->scale * kLog2e / (!simplicial ? 1.f : p->dtype == SA2_ELEMENT_F16 ? ElemF16::kDown : ElemBf16::kDown);
+    k.scale_log2e = p->scale * kLog2e;
     k.row_tiles = x.row_tiles;
     k.splits = x.splits;
     k.dblocks = x.dblocks;

@@ -5,7 +5,7 @@
 //     S^T = K A^T      P^T = exp2(c S^T - M)      O^T += V^T P^T        (c = scale log2(e), M the column's reference)
 // and differ in what a column is:
 //   dense        column = (token, query head of the group):  A = q, keys 0 .. p, the column's O is an output row
-//   2-simplicial column = offset d = p - k of ONE (token, query head):  A = q * k2[p - d], keys (p - w1, p] of the first set,
+//   2-simplicial column = offset d = p - k of ONE (token, query head):  A = c q * k2[p - d] (the chain of products starts from -M), keys (p - w1, p] of the first set,
 //                o = sum over columns of v2[p - d] * O, so the 32 offsets of a token share its window and one product does them all
 // Softmax: the reference M of a column moves only when a tile's weights outgrow 2^60 (fp16: 2^14) on it, the first tile included
 // (M starts far below every logit), so the ordinary tile has no maximum and no rescale.  Sums and accumulators are fp32; the weights
@@ -23,7 +23,7 @@ namespace sa2 {
 struct ElemBf16 {
     static constexpr float kBig = 1.152921504606846976e18f;      // 2^60
     static constexpr uint32_t kExp = 0x7f80u;
-    static constexpr float kDown = 1.f;
+    static __device__ __forceinline__ float fit(float x) { return x; }
     static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
     static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
@@ -38,7 +38,7 @@ struct ElemF16 {
     typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
     static constexpr float kBig = 16384.f;                       // 2^14: weights stay below the largest fp16 number
     static constexpr uint32_t kExp = 0x7c00u;
-    static constexpr float kDown = 1.f / 256;                    // of products of two numbers, so that they stay below the largest one
+    static __device__ __forceinline__ float fit(float x) { return fminf(fmaxf(x, -65504.f), 65504.f); }     // (NaN: the lowest)
     static __device__ __forceinline__ float lo(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
     static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -81,7 +81,7 @@ struct PagedParams {
     int B, n, H, HK, G;
     int dq, dp;                               // channels of q and the output, and of a pool's row (multiples of 8)
     int w1, w2;
-    float scale_log2e;                        // (2-simplicial: of operands that are E::kDown times theirs)
+    float scale_log2e;
     int row_tiles;                            // workgroups (per sequence and key/value head) that the rows take
     int splits, dblocks;                      // shares of the keys; blocks of 32 offsets
     // partial results where splits * dblocks > 1: fp32 [part][B n H][D] and [part][B n H] (reference, sum)
@@ -186,12 +186,14 @@ struct PagedWave {
         if constexpr (TWO) S = E::mfma(k, A2[kk], S);
         return S;
     }
-    __device__ __forceinline__ f32x16 logits(const char *k_lane) const {
-        f32x16 S = zero16();
+    // TWO: relative to `from` (c is in the operand); else the plain products
+    __device__ __forceinline__ f32x16 logits(const char *k_lane, float from) const {
+        f32x16 S = TWO ? splat16(-from) : zero16();
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) S = logit(RT::row_frag(k_lane, kk), kk, S);
         return S;
     }
+    __device__ __forceinline__ bool no_reference() const { return wave_any(M == kNoRef); }
 
     // keys of the tile at `tile` that are there: bit j; masks S accordingly
     __device__ __forceinline__ void mask(f32x16 &S, int tile, uint32_t there, int hf) const {
@@ -209,46 +211,55 @@ struct PagedWave {
         sum = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-            const float e0 = fast_exp2(S[r] * c - M), e1 = fast_exp2(S[r + 1] * c - M);
+            const float e0 = fast_exp2(TWO ? S[r] : S[r] * c - M), e1 = fast_exp2(TWO ? S[r + 1] : S[r + 1] * c - M);
             sum += e0 + e1;
             pb[r >> 3][(r & 7) >> 1] = E::pack(e0, e1);
         }
         return !wave_any(!(sum < E::kBig));
     }
-    // columns without a reference take the tile's largest logit (they hold nothing yet)
-    __device__ __forceinline__ void first_reference(const f32x16 &S, float c) {
+    // the column's largest logit of a tile (TWO: relative to what S is relative to)
+    __device__ __forceinline__ float top_of(const f32x16 &S, float c) const {
         float top = S[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, S[r]);
-        const float ref = fmaxf(kNoRef, both_halves_max(top) * c);
-        M = M == kNoRef ? ref : M;
+        top = both_halves_max(top);
+        return TWO ? top : top * c;
     }
-    // moves the reference of every column up to the tile's largest logit
-    __device__ __forceinline__ void move_reference(const f32x16 &S, float c) {
-        float top = S[0];
+    // Weights of a masked tile whatever the references are.  Columns without one take the tile's largest logit (they hold nothing yet; S of TWO is then
+    // relative to 0); where weights outgrow a reference, all move up to the tile's largest logits
+    __device__ __forceinline__ void any_weights(f32x16 &S, float c, bool fresh, u32x4 (&pb)[2], float &sum) {
+        if (fresh) {
+            const float top = fmaxf(kNoRef, top_of(S, c));
+            M = M == kNoRef ? top : M;
+            if constexpr (TWO) {
 #pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(top, S[r]);
-        const float ref = fmaxf(M, both_halves_max(top) * c);
-        const float f = fast_exp2(M - ref);
+                for (int r = 0; r < 16; ++r) S[r] -= M;
+            }
+        }
+        if (__builtin_expect(!weights(S, c, pb, sum), 0)) {
+            const float top = top_of(S, c), up = TWO ? fmaxf(top, 0.f) : fmaxf(top, M) - M, f = fast_exp2(-up);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) O[dt][r] *= f;
-        l *= f;
-        M = ref;
+                for (int r = 0; r < 16; ++r) O[dt][r] *= f;
+            l *= f;
+            M += up;
+            if constexpr (TWO) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[r] -= up;
+            }
+            weights(S, c, pb, sum);
+        }
     }
     // the plain form of a step
     template <bool ONE>
     __device__ __forceinline__ void step(const char *k_lane, const char *v_lane, float c, bool masked, bool guard, int tile, uint32_t there, int hf) {
-        f32x16 S = logits(k_lane);
+        const bool fresh = no_reference();
+        f32x16 S = logits(k_lane, fresh ? 0.f : M);
         if (masked) mask(S, tile, there, hf);
-        if (wave_any(M == kNoRef)) first_reference(S, c);
         u32x4 pb[2];
         float sum;
-        if (__builtin_expect(!weights(S, c, pb, sum), 0)) {
-            move_reference(S, c);
-            weights(S, c, pb, sum);
-        }
+        any_weights(S, c, fresh, pb, sum);
         l += sum;
         values<ONE>(v_lane, pb, guard, tile, there, hf);
     }
@@ -415,9 +426,9 @@ struct SimplicialColumns {
                 const u32x4 f = paged_q_piece(p, q_row, d0), k = ld_global16(k2 + d0 * 2);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x = E::lo(f[i]) * E::kDown * E::lo(k[i]), y = E::hi(f[i]) * E::kDown * E::hi(k[i]);
-                    a[i] = E::pack(x, y);
-                    a2[i] = E::pack(x - E::lo(a[i]), y - E::hi(a[i]));
+                    const float x = E::lo(f[i]) * p.scale_log2e * E::lo(k[i]), y = E::hi(f[i]) * p.scale_log2e * E::hi(k[i]);
+                    a[i] = E::pack(E::fit(x), E::fit(y));
+                    a2[i] = E::pack(E::fit(x - E::lo(a[i])), E::fit(y - E::hi(a[i])));
                 }
             }
             w.A[kk] = a;
@@ -578,18 +589,15 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
                 const int tile = first_key + 32 * u, next = u + NW;
                 const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(seg[32 * (u - seg_a) + c] >= 0);
                 wait_loads<RT::NCH>();
-                f32x16 S = w.logits(kt + RT::row_lane(lane));
+                const bool fresh = w.no_reference();
+                f32x16 S = w.logits(kt + RT::row_lane(lane), fresh ? 0.f : w.M);
                 wait_lds_reads();
                 if (next < seg_z) request(0, next);
                 const bool masked = w.needs_mask(tile, there);
                 if (masked) w.mask(S, tile, there, hf);
-                if (wave_any(w.M == kNoRef)) w.first_reference(S, p.scale_log2e);
                 u32x4 pb[2];
                 float sum;
-                if (__builtin_expect(!w.weights(S, p.scale_log2e, pb, sum), 0)) {
-                    w.move_reference(S, p.scale_log2e);
-                    w.weights(S, p.scale_log2e, pb, sum);
-                }
+                w.any_weights(S, p.scale_log2e, fresh, pb, sum);
                 w.l += sum;
                 if (next < seg_z) wait_loads<RT::NCH>();
                 else wait_loads<0>();
@@ -863,14 +871,15 @@ paged_many_kernel(PagedParams p) {
             }
             while (u < z) {
                 bool opened = false;      // the step is open already (its weights outgrew a reference)
-                if (C::AHEAD && u < m_z && start + 32 * u >= w.most_lo) {
+                if (C::AHEAD && u < m_z && start + 32 * u >= w.most_lo && !w.no_reference()) {
+                    const f32x16 from = splat16(-w.M);      // (2-simplicial: where the chains of products start)
                     const char *first = lds + (u & (NBUF - 1)) * C::BUF + k_lane;
 #pragma unroll
                     for (int kk = 0; kk < FW; ++kk) kf[kk] = ld_lds16(first + RT::row_imm(kk));
                     do {
                         open_step();
                         const char *buf = lds + (u & (NBUF - 1)) * C::BUF;
-                        f32x16 S = zero16();
+                        f32x16 S = SIMP ? from : zero16();
                         auto read_vf = [&](int f) {
                             vf[f % FW][0] = lds_read_tr<D, 0>(buf + v_lane + RT::tr_imm(16 * (f / DT), 32 * (f % DT)), 0, 0);
                             vf[f % FW][1] = lds_read_tr<D, 0>(buf + v_lane + RT::tr_imm(16 * (f / DT) + 8, 32 * (f % DT)), 0, 0);
