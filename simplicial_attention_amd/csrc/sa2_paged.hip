@@ -121,7 +121,7 @@ PagedPool pool_of(const sa2_pool *t) {
 
 template <class E, int D, bool SIMP>
 void launch(const Plan &x, const PagedParams &k, hipStream_t stream) {
-    if (x.many) hipLaunchKernelGGL((paged_many_kernel<E, D, SIMP>), dim3((unsigned)x.grid), dim3(ManyCfg<D, SIMP>::NW * 64), 0, stream, k);
+    if (x.many) hipLaunchKernelGGL((paged_many_kernel<E, D, SIMP>), dim3((unsigned)((int64_t)k.B * k.HK * x.row_tiles), (unsigned)(x.splits * x.dblocks)), dim3(ManyCfg<D, SIMP>::NW * 64), 0, stream, k);
     else {
         const dim3 grid((unsigned)(k.B * k.HK), (unsigned)x.row_tiles, (unsigned)(x.splits * x.dblocks));
         if (!SIMP && k.n > 1) hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, !SIMP>), grid, dim3(FewCfg<D>::NW * 64), 0, stream, k);
@@ -181,6 +181,8 @@ int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, con
     k.t_sb = at->table_stride;
     k.div = divisor(p->page_size);
     k.group = divisor(p->heads / p->kv_heads);
+    k.heads = divisor(p->kv_heads);
+    k.seqs = divisor(p->batch * p->kv_heads);
     k.pages = p->pages;
     k.width = p->table_width;
     k.B = p->batch;

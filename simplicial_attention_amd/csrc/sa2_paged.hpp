@@ -76,7 +76,7 @@ struct PagedParams {
     PagedPool k1, v1, k2, v2;                 // (k2, v2: 2-simplicial form only)
     const int32_t *tables, *lengths, *counts; // (counts nullptr: n for every sequence)
     int64_t t_sb;
-    Divisor div, group;                       // by the page size, by G
+    Divisor div, group, heads, seqs;          // by the page size, G, HK, B HK
     int pages, width;                         // pages of a pool, entries of a table
     int B, n, H, HK, G;
     int dq, dp;                               // channels of q and the output, and of a pool's row (multiples of 8)
@@ -127,9 +127,12 @@ __device__ __forceinline__ const char *paged_row(const PagedPool &pool, int page
     return pool.ptr + (int64_t)page * pool.sp + (int64_t)row * pool.sr;
 }
 
-// channels d0 .. d0 + 7 of a row of q (zeros beyond its channels); the same of the output
-__device__ __forceinline__ u32x4 paged_q_piece(const PagedParams &p, const char *row, int d0) {
-    return d0 < p.dq ? ld_global16(row + d0 * 2) : (u32x4){0u, 0u, 0u, 0u};
+// channels d0 .. d0 + 7 of a row of `channels`; zeros beyond them, and of a row that is not there.  (An address is chosen, not a branch taken: the
+// pieces of a row are then in flight together)
+__device__ __forceinline__ u32x4 paged_piece(const char *row, int d0, int channels, bool there) {
+    const char *zero = reinterpret_cast<const char *>(g_paged_zero_row), *at = row + d0 * 2;
+    asm volatile("" : "+v"(at));
+    return ld_global16(there && d0 < channels ? at : zero);
 }
 template <class E>
 __device__ __forceinline__ void paged_store8(const PagedParams &p, char *row, int d0, const float (&x)[8]) {
@@ -195,14 +198,33 @@ struct PagedWave {
     }
     __device__ __forceinline__ bool no_reference() const { return wave_any(M == kNoRef); }
 
-    // keys of the tile at `tile` that are there: bit j; masks S accordingly
+    // keys a .. z of the tile at `tile`, bit j for key tile + j
+    __device__ __forceinline__ static uint32_t keys_of(int tile, int a, int z) {
+        a = a - tile < 0 ? 0 : a - tile;
+        z = z - tile > 31 ? 31 : z - tile;
+        return a > z ? 0u : (0xffffffffu >> (31 - z)) & (0xffffffffu << a);
+    }
+    // S of the keys that a column does not attend; `there`: bit j of the keys that are there.  ONE: all columns attend to the same keys, so the masks of
+    // the registers are formed by the scalar unit (row 8 (r / 4) + 4 hf + r % 4 of register r: a bit for either half of the lanes)
+    template <bool ONE>
     __device__ __forceinline__ void mask(f32x16 &S, int tile, uint32_t there, int hf) const {
-        const int a = lo - tile - 4 * hf, z = hi - tile - 4 * hf;
-        const uint32_t bits = there >> (4 * hf);
+        if constexpr (ONE) {
+            const uint32_t keys = there & keys_of(tile, most_lo, least_hi);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int j = 8 * (r >> 2) + (r & 3);
-            S[r] = j >= a && j <= z && ((bits >> j) & 1u) ? S[r] : -INFINITY;
+            for (int r = 0; r < 16; ++r) {
+                const int j = 8 * (r >> 2) + (r & 3);
+                const uint32_t low = (uint32_t)((int)(keys << (31 - j)) >> 31), high = (uint32_t)((int)(keys << (27 - j)) >> 31);
+                const uint64_t lanes = ((uint64_t)high << 32) | low;
+                asm("v_cndmask_b32 %0, %1, %0, %2" : "+v"(S[r]) : "v"(-INFINITY), "s"(lanes));
+            }
+        } else {
+            const int a = lo - tile - 4 * hf, z = hi - tile - 4 * hf;
+            const uint32_t bits = there >> (4 * hf);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = 8 * (r >> 2) + (r & 3);
+                S[r] = j >= a && j <= z && ((bits >> j) & 1u) ? S[r] : -INFINITY;
+            }
         }
     }
 
@@ -256,7 +278,7 @@ struct PagedWave {
     __device__ __forceinline__ void step(const char *k_lane, const char *v_lane, float c, bool masked, bool guard, int tile, uint32_t there, int hf) {
         const bool fresh = no_reference();
         f32x16 S = logits(k_lane, fresh ? 0.f : M);
-        if (masked) mask(S, tile, there, hf);
+        if (masked) mask<ONE>(S, tile, there, hf);
         u32x4 pb[2];
         float sum;
         any_weights(S, c, fresh, pb, sum);
@@ -287,14 +309,9 @@ struct PagedWave {
                     m[k2s][w] = ((bits >> j) & 1u ? 0xffffu : 0u) | ((bits >> (j + 1)) & 1u ? 0xffff0000u : 0u);
                 }
         };
-        auto keys_up_to = [&](int a, int z) {       // keys a .. z of the tile
-            a = a - tile < 0 ? 0 : a - tile;
-            z = z - tile > 31 ? 31 : z - tile;
-            return a > z ? 0u : (0xffffffffu >> (31 - z)) & (0xffffffffu << a);
-        };
         if (ONE) {
             u32x4 m[2];
-            key_masks(there & keys_up_to(most_lo, least_hi), m);
+            key_masks(there & keys_of(tile, most_lo, least_hi), m);
 #pragma unroll
             for (int k2s = 0; k2s < 2; ++k2s)
 #pragma unroll
@@ -326,7 +343,7 @@ struct PagedWave {
             const bool mine = lo <= hi && (z < 31 ? hi - tile == z : hi - tile >= 31);
             if (!wave_any(mine)) continue;
             u32x4 m[2];
-            key_masks(there & keys_up_to(0, tile + z), m);
+            key_masks(there & keys_of(tile, 0, tile + z), m);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 f32x16 x = zero16();
@@ -418,21 +435,24 @@ struct SimplicialColumns {
         page2 = on && d < p.w2 ? paged_page(p, s, x) : -1;
         row2 = page2 >= 0 ? x - (int)p.div((uint32_t)x) * (int)p.div.by : 0;
         const char *k2 = paged_row(p.k2, page2, row2) + hk * p.k2.sh;
+        constexpr int AT_ONCE = KS < 8 ? KS : 8;
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-            const int d0 = 16 * kk + 8 * hf;
-            u32x4 a = {0u, 0u, 0u, 0u}, a2 = a;
-            if (page2 >= 0 && d0 < p.dp) {
-                const u32x4 f = paged_q_piece(p, q_row, d0), k = ld_global16(k2 + d0 * 2);
+        for (int k0 = 0; k0 < KS; k0 += AT_ONCE) {
+            u32x4 f[AT_ONCE], k[AT_ONCE];
+#pragma unroll
+            for (int x = 0; x < AT_ONCE; ++x) {
+                f[x] = paged_piece(q_row, 16 * (k0 + x) + 8 * hf, p.dq, true);
+                k[x] = paged_piece(k2, 16 * (k0 + x) + 8 * hf, p.dp, page2 >= 0);
+            }
+#pragma unroll
+            for (int x = 0; x < AT_ONCE; ++x)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x = E::lo(f[i]) * p.scale_log2e * E::lo(k[i]), y = E::hi(f[i]) * p.scale_log2e * E::hi(k[i]);
-                    a[i] = E::pack(E::fit(x), E::fit(y));
-                    a2[i] = E::pack(E::fit(x - E::lo(a[i])), E::fit(y - E::hi(a[i])));
+                    const float a = E::lo(f[x][i]) * p.scale_log2e * E::lo(k[x][i]), b = E::hi(f[x][i]) * p.scale_log2e * E::hi(k[x][i]);
+                    const uint32_t high = E::pack(E::fit(a), E::fit(b));
+                    w.A[k0 + x][i] = high;
+                    w.A2[k0 + x][i] = E::pack(E::fit(a - E::lo(high)), E::fit(b - E::hi(high)));
                 }
-            }
-            w.A[kk] = a;
-            w.A2[kk] = a2;
         }
     }
 
@@ -444,7 +464,7 @@ struct SimplicialColumns {
 #pragma unroll
         for (int x = 0; x < 2 * DT; ++x) {
             const int d0 = 32 * (x >> 1) + 16 * hf + 8 * (x & 1);
-            v[x] = page2 >= 0 && d0 < p.dp ? ld_global16(v2 + d0 * 2) : (u32x4){0u, 0u, 0u, 0u};
+            v[x] = paged_piece(v2, d0, p.dp, page2 >= 0);
         }
         // (columns without a second row, and those that met no key, hold nothing that counts)
         const float column = w.whole_sum();
@@ -504,7 +524,7 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
 
     // grid: (sequence and key/value head, row tile, part)
     const int parts = p.splits * p.dblocks, part = blockIdx.z, tile_r = blockIdx.y;
-    const int b = uniform(blockIdx.x / p.HK), hk = blockIdx.x - b * p.HK;
+    const int b = uniform((int)p.heads(blockIdx.x)), hk = blockIdx.x - b * p.HK;
     const int db = p.dblocks == 1 ? 0 : uniform(part / p.splits), split = part - db * p.splits;
     const PagedSeq s = paged_seq(p, b);
 
@@ -581,7 +601,7 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
             w.limits(first_key, last, on && cols.page2 >= 0, true, first_key, last);
         } else {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) w.A[kk] = on ? paged_q_piece(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
+            for (int kk = 0; kk < D / 16; ++kk) w.A[kk] = paged_piece(q_row, 16 * kk + 8 * hf, p.dq, on);
             w.limits(0, min(pos, last), on, true, 0, min(s.first + t_first, last));
         }
         for (;;) {
@@ -594,7 +614,7 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
                 wait_lds_reads();
                 if (next < seg_z) request(0, next);
                 const bool masked = w.needs_mask(tile, there);
-                if (masked) w.mask(S, tile, there, hf);
+                if (masked) w.template mask<!MIXED>(S, tile, there, hf);
                 u32x4 pb[2];
                 float sum;
                 w.any_weights(S, p.scale_log2e, fresh, pb, sum);
@@ -741,14 +761,12 @@ paged_many_kernel(PagedParams p) {
     const int tid = threadIdx.x, wave = wave_index(), lane = tid & 63, c = lane & 31, hf = lane >> 5;
     constexpr int PER_WG = SIMP ? NW : NW * 32;        // rows (t, g) of a workgroup
 
-    const int parts = p.splits * p.dblocks;
-    int item = xcd_contiguous(blockIdx.x, gridDim.x);
-    const int part = uniform(item % parts);
-    item = uniform(item / parts);
-    const int tile_r = p.row_tiles - 1 - uniform(item % p.row_tiles);     // (the longest first)
-    item = uniform(item / p.row_tiles);
-    const int hk = uniform(item % p.HK), b = uniform(item / p.HK);
-    const int split = uniform(part % p.splits), db = uniform(part / p.splits);
+    // grid: (row tile, sequence and key/value head with the heads next to each other: one XCD has all workgroups of a head where their number is a multiple
+    // of eight), part; the longest rows first
+    const int parts = p.splits * p.dblocks, part = blockIdx.y;
+    const int row = uniform((int)p.seqs(blockIdx.x)), seq = blockIdx.x - row * (int)p.seqs.by, tile_r = p.row_tiles - 1 - row;
+    const int b = uniform((int)p.heads(seq)), hk = seq - b * p.HK;
+    const int db = p.dblocks == 1 ? 0 : uniform(part / p.splits), split = part - db * p.splits;
     const PagedSeq s = paged_seq(p, b);
 
     const int R0 = tile_r * PER_WG, R = SIMP ? R0 + wave : R0 + wave * 32 + c;
@@ -760,7 +778,7 @@ paged_many_kernel(PagedParams p) {
     const int last = min(s.first + t_last, s.reach - 1);
     const int first_key = SIMP ? max(0, s.first + t_first - p.w1 + 1) : 0;
     const int tiles = t_first < s.count && last >= first_key ? (last - first_key) / 32 + 1 : 0;
-    const int tile_a = (int)((int64_t)tiles * split / p.splits), tile_z = (int)((int64_t)tiles * (split + 1) / p.splits);
+    const int tile_a = p.splits == 1 ? 0 : (int)((int64_t)tiles * split / p.splits), tile_z = p.splits == 1 ? tiles : (int)((int64_t)tiles * (split + 1) / p.splits);
     const int NT = tile_z - tile_a;
 
     const char *const k_head = p.k1.ptr + hk * p.k1.sh, *const v_head = p.v1.ptr + hk * p.v1.sh;
@@ -825,7 +843,7 @@ paged_many_kernel(PagedParams p) {
         w.limits(lo, hi, on && cols.page2 >= 0, any && lo <= hi, lo, hi);
     } else {
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) w.A[kk] = on ? paged_q_piece(p, q_row, 16 * kk + 8 * hf) : (u32x4){0u, 0u, 0u, 0u};
+        for (int kk = 0; kk < KS; ++kk) w.A[kk] = paged_piece(q_row, 16 * kk + 8 * hf, p.dq, on);
         const int t0 = max((int)p.group((uint32_t)(R0 + 32 * wave)), -s.first), t1 = min((int)p.group((uint32_t)(R0 + 32 * wave + 31)), s.count - 1);
         const bool any = t0 <= t1 && last >= 0;
         lo = any ? 0 : 0x7fffffff;
@@ -936,7 +954,7 @@ paged_many_kernel(PagedParams p) {
     }
 
     w.settle();
-    const int64_t rows = (int64_t)p.B * p.n * p.H, row = ((int64_t)b * p.n + t) * p.H + h;
+    const int64_t rows = (int64_t)p.B * p.n * p.H, out_row = ((int64_t)b * p.n + t) * p.H + h;
     if constexpr (SIMP) {
         float y[16 * DT], ref, sum;
         cols.finish(p, w, hk, c, hf, y, ref, sum);
@@ -951,11 +969,11 @@ paged_many_kernel(PagedParams p) {
                 if (d < p.dq && (16 * DT >= 32 || (c & 1) == 0)) *reinterpret_cast<uint16_t *>(orow + d * 2) = (uint16_t)E::pack(y[i] * inv, 0.f);
             }
         } else {
-            float *dst = p.part_o + ((int64_t)part * rows + row) * D;
+            float *dst = p.part_o + ((int64_t)part * rows + out_row) * D;
 #pragma unroll
             for (int i = 0; i < ColumnSum<16 * DT>::LEFT; ++i)
                 if (16 * DT >= 32 || (c & 1) == 0) dst[32 * ((base + i) >> 4) + 16 * hf + ((base + i) & 15)] = y[i];
-            if (lane == 0) p.part_ml[part * rows + row] = make_float2(ref, sum);
+            if (lane == 0) p.part_ml[part * rows + out_row] = make_float2(ref, sum);
         }
     } else {
         if (!on) w.clear();
@@ -974,8 +992,8 @@ paged_many_kernel(PagedParams p) {
                     paged_store8<E>(p, orow, 32 * dt + 16 * hf + 8 * half, z);
                 }
         } else {
-            store_row_f32<DT>(p.part_o + ((int64_t)part * rows + row) * D + 16 * hf, w.O, 1.f);
-            if (hf == 0) p.part_ml[part * rows + row] = make_float2(w.M, sum);
+            store_row_f32<DT>(p.part_o + ((int64_t)part * rows + out_row) * D + 16 * hf, w.O, 1.f);
+            if (hf == 0) p.part_ml[part * rows + out_row] = make_float2(w.M, sum);
         }
     }
 }
