@@ -123,7 +123,8 @@ template <class E, int D, bool SIMP>
 void launch(const Plan &x, const PagedParams &k, hipStream_t stream) {
     if (x.many) hipLaunchKernelGGL((paged_many_kernel<E, D, SIMP>), dim3((unsigned)((int64_t)k.B * k.HK * x.row_tiles), (unsigned)(x.splits * x.dblocks)), dim3(ManyCfg<D, SIMP>::NW * 64), 0, stream, k);
     else {
-        const dim3 grid((unsigned)(k.B * k.HK), (unsigned)x.row_tiles, (unsigned)(x.splits * x.dblocks));
+        const unsigned seqs = k.B * k.HK, parts = x.splits * x.dblocks;
+        const dim3 grid(SIMP ? seqs : seqs * parts, (unsigned)x.row_tiles, SIMP ? parts : 1);
         if (!SIMP && k.n > 1) hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, !SIMP>), grid, dim3(FewCfg<D>::NW * 64), 0, stream, k);
         else hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, false>), grid, dim3(FewCfg<D>::NW * 64), 0, stream, k);
     }
@@ -183,6 +184,7 @@ int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, con
     k.group = divisor(p->heads / p->kv_heads);
     k.heads = divisor(p->kv_heads);
     k.seqs = divisor(p->batch * p->kv_heads);
+    k.parts = divisor(x.splits * x.dblocks);
     k.pages = p->pages;
     k.width = p->table_width;
     k.B = p->batch;

@@ -76,7 +76,7 @@ struct PagedParams {
     PagedPool k1, v1, k2, v2;                 // (k2, v2: 2-simplicial form only)
     const int32_t *tables, *lengths, *counts; // (counts nullptr: n for every sequence)
     int64_t t_sb;
-    Divisor div, group, heads, seqs;          // by the page size, G, HK, B HK
+    Divisor div, group, heads, seqs, parts;   // by the page size, G, HK, B HK, splits * dblocks
     int pages, width;                         // pages of a pool, entries of a table
     int B, n, H, HK, G;
     int dq, dp;                               // channels of q and the output, and of a pool's row (multiples of 8)
@@ -522,9 +522,11 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
     int *seg = reinterpret_cast<int *>(lds + C::RING);
     const int tid = threadIdx.x, wave = wave_index(), lane = tid & 63, c = lane & 31, hf = lane >> 5;
 
-    // grid: (sequence and key/value head, row tile, part)
-    const int parts = p.splits * p.dblocks, part = blockIdx.z, tile_r = blockIdx.y;
-    const int b = uniform((int)p.heads(blockIdx.x)), hk = blockIdx.x - b * p.HK;
+    // Grid.  Dense: the parts of a sequence and key/value head next to each other (their pages are, as a rule: one token of 16 sequences of up to 32768 131 us, heads
+    // next to each other 143).  2-simplicial: (sequence and key/value head, row tile, part), so that the heads of a group are on one XCD
+    const int parts = p.splits * p.dblocks, tile_r = blockIdx.y;
+    const int seq = SIMP ? (int)blockIdx.x : uniform((int)p.parts(blockIdx.x)), part = SIMP ? (int)blockIdx.z : (int)blockIdx.x - seq * parts;
+    const int b = uniform((int)p.heads(seq)), hk = seq - b * p.HK;
     const int db = p.dblocks == 1 ? 0 : uniform(part / p.splits), split = part - db * p.splits;
     const PagedSeq s = paged_seq(p, b);
 
