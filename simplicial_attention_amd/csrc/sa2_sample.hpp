@@ -127,35 +127,62 @@ __device__ __forceinline__ Best wave_first(const Best &v) {
 template <int THREADS>
 struct RowReduce {
     static constexpr int NW = THREADS / 64;
-    float a[NW], b[NW], x[NW];
+    float a[NW], b[NW], s[NW], x[NW];
     int i[NW];
-    // sums of two numbers
-    __device__ __forceinline__ void add(float &p, float &q) {
+    uint32_t n[2][3][NW];
+    // sums of two numbers and the first of the bests, for the whole workgroup
+    __device__ __forceinline__ void all(float &p, float &q, Best &v) {
         p = wave_sum(p);
         q = wave_sum(q);
+        v = wave_first(v);
         if (NW == 1) return;
         const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
         __syncthreads();
         if (lane == 0) {
             a[w] = p;
             b[w] = q;
-        }
-        __syncthreads();
-        p = wave_sum(lane < NW ? a[lane % NW] : 0.f);
-        q = wave_sum(lane < NW ? b[lane % NW] : 0.f);
-    }
-    __device__ __forceinline__ Best first(Best v) {
-        v = wave_first(v);
-        if (NW == 1) return v;
-        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-        __syncthreads();
-        if (lane == 0) {
-            a[w] = v.score;
+            s[w] = v.score;
             x[w] = v.x;
             i[w] = v.index;
         }
         __syncthreads();
-        return wave_first(lane < NW ? Best{a[lane % NW], x[lane % NW], i[lane % NW]} : Best{-INFINITY, 0.f, -1});
+        p = wave_sum(lane < NW ? a[lane % NW] : 0.f);
+        q = wave_sum(lane < NW ? b[lane % NW] : 0.f);
+        v = wave_first(lane < NW ? Best{s[lane % NW], x[lane % NW], i[lane % NW]} : Best{-INFINITY, 0.f, -1});
+    }
+    __device__ __forceinline__ Best first(Best v) {
+        float p = 0.f, q = 0.f;
+        all(p, q, v);
+        return v;
+    }
+    // The largest number v (to 16 bits of its order) that at least k of the workgroup's numbers reach, -infinity if there are not k of them: two bits at a time,
+    // the counts by ballots
+    template <int N>
+    __device__ __forceinline__ float reached_by(const float (&g)[N], uint32_t k) {
+        uint32_t key[N], v = 0u;
+#pragma unroll
+        for (int e = 0; e < N; ++e) key[e] = as_u32(g[e]) & 0x80000000u ? ~as_u32(g[e]) : as_u32(g[e]) | 0x80000000u;
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        for (int shift = 30; shift >= 16; shift -= 2) {
+            uint32_t count[3] = {0u, 0u, 0u};
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+#pragma unroll
+                for (int j = 0; j < 3; ++j) count[j] += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[e] >= (v | ((uint32_t)(j + 1) << shift))));
+            if (NW > 1) {
+                uint32_t(&at)[3][NW] = n[(shift >> 1) & 1];
+                if (lane < 3) at[lane][w] = lane == 0 ? count[0] : lane == 1 ? count[1] : count[2];
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < 3; ++j) {
+                    count[j] = 0u;
+#pragma unroll
+                    for (int y = 0; y < NW; ++y) count[j] += at[j][y];
+                }
+            }
+            v |= (uint32_t)(count[2] >= k ? 3 : count[1] >= k ? 2 : count[0] >= k ? 1 : 0) << shift;
+        }
+        return v <= 0x007fffffu ? -INFINITY : as_f32(v & 0x80000000u ? v & 0x7fffffffu : ~v);
     }
 };
 
@@ -262,32 +289,37 @@ __global__ __launch_bounds__(THREADS) void sample_chunk_kernel(SampleParams p) {
             }
         }
     }
-    red.add(mass1, mass);
-    Best best = rules.greedy ? top : red.first(mine);
+    red.all(mass1, mass, mine);
+    Best best = rules.greedy ? top : mine;
     if constexpr (!ONE) {
         if (tid == 0) p.records[r * p.chunks + chunk] = {top.x, mass1, mass, best.score, top.index, best.index, best.x, 0};
         return;
     }
-    while (!rules.greedy && best.index != top.index && rules.filters()) {
-        float front = 0.f, count = 0.f;
-        mine = kNobody;
+    if (!rules.greedy && best.index != top.index && rules.filters()) {
+        // (with top_k the race is run again in front of the bound, once the winner of all is behind it)
+        const float cut = rules.top_k > 0 ? red.reached_by(x, (uint32_t)rules.top_k) : -INFINITY;
+        if (best.x < cut) best = {0.f, cut, 0x7fffffff};
+        while (best.index != top.index) {
+            float front = 0.f, count = 0.f;
+            mine = kNobody;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-            const bool in = x[e] > best.x || (x[e] == best.x && index(e) < best.index);
-            front += in ? w[e] : 0.f;
-            count += in ? 1.f : 0.f;
-            enter(mine, x[e], index(e), in ? u[e] : 0.f);
+            for (int e = 0; e < EACH; ++e) {
+                const bool in = x[e] > best.x || (x[e] == best.x && index(e) < best.index);
+                front += in ? w[e] : 0.f;
+                count += in ? 1.f : 0.f;
+                enter(mine, x[e], index(e), in ? u[e] : 0.f);
+            }
+            red.all(front, count, mine);
+            if (best.index != 0x7fffffff && rules.keeps(count, front, mass, fast_exp2((best.x - top.x) * rules.inv))) break;
+            best = mine;
         }
-        red.add(front, count);
-        if (rules.keeps(count, front, mass, fast_exp2((best.x - top.x) * rules.inv))) break;
-        best = red.first(mine);
     }
     if (tid == 0) write_token(p, r, best, top.x, mass1);
 }
 
-// The chunks of a row merged; rows with filters: their races (the first one is the chunks' where there is no top_k).  The threads' largest logits bound the kept prefix from behind: if k of
-// them are at least v, no token below v has a rank below k, and if they alone hold top_p of the mass, no token below v is inside it.  The largest such v
-// (to 16 bits) is found by bisection in registers; races then look at the sixteens alone whose largest logit is in front.
+// The chunks of a row merged; rows with filters: their races (the first one is the chunks' where there is no top_k).  The threads' largest logits bound the
+// kept prefix from behind: if k of them are at least v, no token below v has a rank below k.  Races then look at those sixteens alone whose largest logit is in front;
+// a wave that finds few of them keeps their tokens in registers for the races that follow.
 constexpr int kRowThreads = 1024, kRowBatch = 8;       // sixteens per thread that a pass looks at together
 template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleParams p) {
@@ -301,6 +333,12 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleParams p)
     const float *noise = p.noise + r * p.noise_stride;
     const RowRules rules(p, r);
     const SampleRecord *records = p.records + r * p.chunks;
+    const float *tops = p.tops + r * p.chunks * kSampleThreads;
+    const int groups = p.chunks * kSampleThreads;
+    const bool races = !rules.greedy && rules.filters();
+    float g[kRowBatch];
+#pragma unroll
+    for (int k = 0; k < kRowBatch; ++k) g[k] = races && k * THREADS + tid < groups ? tops[k * THREADS + tid] : -INFINITY;
     Best top = {-INFINITY, -INFINITY, -1};
     for (int c = tid; c < p.chunks; c += THREADS) {
         const Best o = {records[c].top, records[c].top, records[c].top_at};
@@ -311,7 +349,6 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleParams p)
         if (tid == 0) write_token(p, r, top, 0.f, 1.f);
         return;
     }
-    const bool races = !rules.greedy && rules.filters();
     float mass1 = 0.f, mass = 0.f;
     Best best = kNobody;
     for (int c = tid; c < p.chunks; c += THREADS) {
@@ -322,85 +359,80 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleParams p)
         mass += o.massT * fast_exp2(y);
         enter(best, o.best, o.best_at, o.score * fast_exp2(y));
     }
-    red.add(mass1, mass);
-    best = rules.greedy ? top : red.first(best);
+    red.all(mass1, mass, best);
+    if (rules.greedy) best = top;
     if (!races) {
         if (tid == 0) write_token(p, r, best, top.x, mass1);
         return;
     }
-    const float *tops = p.tops + r * p.chunks * kSampleThreads;
-    const int groups = p.chunks * kSampleThreads;
-    float g[kRowBatch];
+    constexpr int AT_ONCE = 64 / L::PIECES;     // sixteens that a wave looks at together: one lane per piece of 16 bytes
+    float x[L::PIECE], w[L::PIECE], score[L::PIECE];
+    int i = 0;
+    bool kept = false;                          // (of the wave) x, w and score hold every token that can still be in front
+    auto load_piece = [&](int at) {
+        i = L::index(at / kSampleThreads, kSampleThreads, at % kSampleThreads, lane % L::PIECES * L::PIECE);
+        float u[L::PIECE];
+        L::piece(row, i, V, x);
+        if (i + L::PIECE <= V) {
+            __builtin_memcpy(u, noise + i, 4 * L::PIECE);
+        } else {
 #pragma unroll
-    for (int k = 0; k < kRowBatch; ++k) g[k] = k * THREADS + tid < groups ? tops[k * THREADS + tid] : -INFINITY;
-
-    // keys: unsigned numbers in the order of the floats
-    float cut = -INFINITY;
-    if (rules.top_k > 0) {
-        auto key = [](float x) { return as_u32(x) & 0x80000000u ? ~as_u32(x) : as_u32(x) | 0x80000000u; };
-        const float enough = rules.top_p < 1.f ? rules.top_p * mass * 1.0001f : INFINITY;       // (sums in another order)
-        const float many = rules.top_k > 0 ? (float)rules.top_k : INFINITY;
-        uint32_t v = 0u;
-        for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
-            float count = 0.f, held = 0.f;
-#pragma unroll
-            for (int k = 0; k < kRowBatch; ++k)
-                if (key(g[k]) >= (v | bit) && g[k] > -INFINITY) {
-                    count += 1.f;
-                    held += fast_exp2((g[k] - top.x) * rules.inv);
-                }
-            red.add(count, held);
-            if (count >= many || held >= enough) v |= bit;
+            for (int e = 0; e < L::PIECE; ++e) u[e] = i + e < V ? noise[i + e] : 0.f;
         }
-        if (v) cut = as_f32(v & 0x80000000u ? v & 0x7fffffffu : ~v);
-    }
+#pragma unroll
+        for (int e = 0; e < L::PIECE; ++e) {
+            w[e] = fast_exp2((x[e] - top.x) * rules.inv);
+            score[e] = w[e] * race_factor(u[e]);
+        }
+    };
     // tokens in front of (x, i): a race among them, their number and mass
     auto race = [&](float cut_x, int cut_i, float &count, float &front) {
         Best mine = kNobody;
         count = front = 0.f;
-        for (int base = 0; base < groups; base += kRowBatch * THREADS) {
-            int listed = 0;
+        auto look = [&] {
 #pragma unroll
-            for (int k = 0; k < kRowBatch; ++k) {
-                const int at = base + k * THREADS + tid;
-                const float t = base == 0 ? g[k] : at < groups ? tops[at] : -INFINITY;
-                const bool in = t >= cut_x && t > -INFINITY && fast_exp2((t - top.x) * rules.inv) >= rules.min_p;
-                const uint64_t who = __builtin_amdgcn_ballot_w64(in);
-                if (in) list[wave][listed + __builtin_popcountll(who & ((1ull << lane) - 1))] = (uint16_t)(k * THREADS + tid);
-                listed += __builtin_popcountll(who);
+            for (int e = 0; e < L::PIECE; ++e) {
+                const bool in = (x[e] > cut_x || (x[e] == cut_x && i + e < cut_i)) && w[e] >= rules.min_p && x[e] > -INFINITY;
+                front += in ? w[e] : 0.f;
+                count += in ? 1.f : 0.f;
+                // (the list is not in the order of the tokens)
+                if (in && (score[e] > mine.score || (score[e] == mine.score && (unsigned)(i + e) < (unsigned)mine.index))) mine = {score[e], x[e], i + e};
             }
-            // (a wave reads what it wrote) one lane per piece of 16 bytes of a listed sixteen
-            constexpr int AT_ONCE = 64 / L::PIECES;
-            for (int k = 0; k < listed; k += AT_ONCE) {
-                const int which = k + lane / L::PIECES;
-                if (which >= listed) continue;
-                const int at = base + list[wave][which];
-                const int i = L::index(at / kSampleThreads, kSampleThreads, at % kSampleThreads, lane % L::PIECES * L::PIECE);
-                float x[L::PIECE], u[L::PIECE];
-                L::piece(row, i, V, x);
-                if (i + L::PIECE <= V) {
-                    __builtin_memcpy(u, noise + i, 4 * L::PIECE);
-                } else {
+        };
+        if (kept) {
+            look();
+        } else {
+            for (int base = 0; base < groups; base += kRowBatch * THREADS) {
+                int listed = 0;
 #pragma unroll
-                    for (int e = 0; e < L::PIECE; ++e) u[e] = i + e < V ? noise[i + e] : 0.f;
+                for (int k = 0; k < kRowBatch; ++k) {
+                    const int at = base + k * THREADS + tid;
+                    const float t = base == 0 ? g[k] : at < groups ? tops[at] : -INFINITY;
+                    const bool in = t >= cut_x && t > -INFINITY;
+                    const uint64_t who = __builtin_amdgcn_ballot_w64(in);
+                    if (in) list[wave][listed + __builtin_popcountll(who & ((1ull << lane) - 1))] = (uint16_t)(k * THREADS + tid);
+                    listed += __builtin_popcountll(who);
                 }
+                // (a wave reads what it wrote)
+                kept = listed <= AT_ONCE && groups <= kRowBatch * THREADS;
+                for (int k = 0; k < listed; k += AT_ONCE) {
+                    const int which = k + lane / L::PIECES;
+                    if (which < listed) {
+                        load_piece(base + list[wave][which]);
+                        look();
+                    }
+                }
+                if (kept && lane / L::PIECES >= listed) {
 #pragma unroll
-                for (int e = 0; e < L::PIECE; ++e) {
-                    const float w = fast_exp2((x[e] - top.x) * rules.inv);
-                    const bool in = (x[e] > cut_x || (x[e] == cut_x && i + e < cut_i)) && w >= rules.min_p && x[e] > -INFINITY;
-                    front += in ? w : 0.f;
-                    count += in ? 1.f : 0.f;
-                    const float score = in ? w * race_factor(u[e]) : 0.f;
-                    // (the list is not in the order of the tokens)
-                    if (score > mine.score || (score == mine.score && in && (unsigned)(i + e) < (unsigned)mine.index)) mine = {score, x[e], i + e};
+                    for (int e = 0; e < L::PIECE; ++e) x[e] = -INFINITY;
                 }
             }
         }
-        red.add(front, count);
-        return red.first(mine);
+        red.all(front, count, mine);
+        return mine;
     };
     float count, front;
-    if (rules.top_k > 0) best = race(cut, 0x7fffffff, count, front);
+    if (rules.top_k > 0) best = race(red.reached_by(g, (uint32_t)rules.top_k), 0x7fffffff, count, front);
     while (best.index != top.index && best.index >= 0) {
         const Best next = race(best.x, best.index, count, front);
         if (rules.keeps(count, front, mass, fast_exp2((best.x - top.x) * rules.inv))) break;
