@@ -61,7 +61,7 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
     const int64_t most = p->max_length > 0 && p->max_length < reach ? p->max_length : reach;
     const int64_t keys = simplicial && p->w1 < most ? p->w1 : most;
     const int64_t tiles = (keys + 31) / 32;
-    x.dblocks = simplicial ? (p->w2 + 31) / 32 : 1;
+    x.dblocks = simplicial ? (int)(((p->w2 < reach ? p->w2 : reach) + 31) / 32) : 1;
     const int waves = x.dim == 256 || simplicial ? 4 : 8;
     // 2-simplicial: a workgroup per (token, head) while all of them run at once, else units that share their keys (one sequence, 8 heads of 64 channels, w1 512,
     // w2 32: 64 tokens 14.5 and 16.6 us, 128 tokens 26.3 and 16.7; four sequences of 128 channels: 16 tokens 20.3 and 22.7, 64 tokens 75 and 30)
@@ -94,7 +94,9 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
             if (splits > tiles / waves) splits = tiles / waves;
         }
     }
-    x.splits = (int)(splits > 256 ? 256 : splits);
+    // (a dimension of the grid)
+    const int64_t most_splits = x.dblocks < 255 ? 256 : x.dblocks < 65536 ? 65535 / x.dblocks : 1;
+    x.splits = (int)(splits > most_splits ? most_splits : splits);
     x.grid = items * x.splits;
     return x;
 }
@@ -159,6 +161,7 @@ int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, con
     SA2_TRY(check_rows(out, "out"));
     if (!at || !at->tables || !at->lengths) return fail_with(SA2_ERR_NULL_POINTER, "tables and lengths are required");
     const Plan x = plan_of(p, simplicial);
+    if (x.dblocks > 65535) return fail_with(SA2_ERR_BAD_SHAPE, "w2=%d: at most %d offsets are supported", p->w2, 65535 * 32);
     if (x.grid > 0x7fffffffll) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
     if (x.bytes() > 0 && (!workspace || workspace_bytes < x.bytes()))
         return fail_with(SA2_ERR_BAD_SHAPE, "workspace of %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0), (long long)x.bytes());

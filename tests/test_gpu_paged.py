@@ -355,3 +355,46 @@ def test_nothing_to_do(sets):
     assert run(queries(2, 0, 4, 64), pools, tables, lengths).shape == (2, 0, 4, 64)
     assert run(queries(0, 1, 4, 64), pools, tables[:0], lengths[:0]).shape == (0, 1, 4, 64)
     assert not run(queries(2, 3, 4, 64), pools, tables[:, :0], lengths).any()
+
+
+def test_a_second_window_beyond_everything():
+    """Windows larger than any sequence: all pairs of keys."""
+    lengths = [40, 3]
+    pools, tables = P.make_cache(2, 1, 64, lengths, 16, 2)
+    for n in (1, 30):
+        q = queries(2, n, 2, 64)
+        out = run(q, pools, tables, ints(*lengths), w1=1 << 40, w2=1 << 30)
+        P.check(out, want(q, pools, tables, lengths, w1=64, w2=64))
+
+
+def test_replays_of_a_graph():
+    """A decode step (rows into pages, both attentions, a token) recorded once and replayed on new inputs, with eager work between the replays."""
+    b, h, hk, d, page = 3, 4, 2, 64, 16
+    lengths = [40, 700, 1300]
+    pools, tables = P.make_cache(b, hk, d, lengths, page, 2)
+    at = ints(*lengths)
+    q, logits, noise = queries(b, 1, h, d), torch.randn(b, 5000, device='cuda'), torch.rand(b, 5000, device='cuda')
+    rows = [torch.randn(b, 1, hk, d, device='cuda', dtype=BF16) for _ in range(4)]
+
+    def step():
+        S.paged_append(pools, rows, tables, at)
+        dense = S.paged_attn(q, *pools[:2], tables, at)
+        pairs = S.paged_two_simplicial_attn(q, pools[:2], pools[2:], tables, at, w1=512, w2=32)
+        return dense, pairs, *S.sample_tokens(logits, noise, top_k=50, top_p=0.9)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = step()
+    for replay in range(4):
+        q.copy_(queries(b, 1, h, d, seed=replay))
+        logits.normal_()
+        noise.uniform_()
+        for r in rows:
+            r.normal_()
+        graph.replay()
+        got = [t.clone() for t in recorded]
+        torch.cuda.synchronize()
+        for g, e in zip(got, step()):
+            assert torch.equal(g, e)
