@@ -45,7 +45,8 @@ int check_problem(const sa2_paged_problem *p, bool simplicial) {
 
 // How the work is laid out: a function of the problem alone.
 struct Plan {
-    bool many;
+    bool many, packed;
+    int unit_columns;
     int dim, row_tiles, splits, dblocks;
     int64_t grid, rows;
     int64_t bytes() const { return splits * dblocks > 1 ? splits * dblocks * rows * (dim * 4 + 8) : 0; }
@@ -65,8 +66,14 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
     const int waves = x.dim == 256 || simplicial ? 4 : 8;
     // 2-simplicial: a workgroup per (token, head) while all of them run at once, else units that share their keys (one sequence, 8 heads of 64 channels, w1 512,
     // w2 32: 64 tokens 14.5 and 16.6 us, 128 tokens 26.3 and 16.7; four sequences of 128 channels: 16 tokens 20.3 and 22.7, 64 tokens 75 and 30)
+    // Second windows up to 16 leave columns of a wave to other units: taken where there are more units than 256 workgroups of a unit per wave hold (8 heads, w1 512,
+    // unit per wave and packed: four sequences of 1024 tokens, 128 channels, w2 16, 8 and 4: 433, 393, 387 and 244, 130, 72 us; one of 128 tokens, 64 channels,
+    // w2 8: 15.7 and 16.5)
+    x.unit_columns = 32;
+    while (simplicial && x.unit_columns > 1 && x.unit_columns / 2 >= p->w2) x.unit_columns /= 2;
     x.many = simplicial ? seqs * per * x.dblocks > 512 : per > 32;
-    const int64_t per_wg = x.many ? (simplicial ? waves : waves * 32) : (simplicial ? 1 : 32);
+    x.packed = simplicial && seqs * per > 1024 && x.unit_columns < 32;
+    const int64_t per_wg = x.many ? (simplicial ? waves * (32 / x.unit_columns) : waves * 32) : (simplicial ? 1 : 32);
     x.row_tiles = (int)((per + per_wg - 1) / per_wg);
     const int64_t items = seqs * x.row_tiles * x.dblocks;
     int64_t splits = 1;
@@ -123,8 +130,11 @@ PagedPool pool_of(const sa2_pool *t) {
 
 template <class E, int D, bool SIMP>
 void launch(const Plan &x, const PagedParams &k, hipStream_t stream) {
-    if (x.many) hipLaunchKernelGGL((paged_many_kernel<E, D, SIMP>), dim3((unsigned)((int64_t)k.B * k.HK * x.row_tiles), (unsigned)(x.splits * x.dblocks)), dim3(ManyCfg<D, SIMP>::NW * 64), 0, stream, k);
-    else {
+    if (x.many) {
+        const dim3 grid((unsigned)((int64_t)k.B * k.HK * x.row_tiles), (unsigned)(x.splits * x.dblocks)), block(ManyCfg<D, SIMP>::NW * 64);
+        if (SIMP && x.packed) hipLaunchKernelGGL((paged_many_kernel<E, D, SIMP, SIMP>), grid, block, 0, stream, k);
+        else hipLaunchKernelGGL((paged_many_kernel<E, D, SIMP, false>), grid, block, 0, stream, k);
+    } else {
         const unsigned seqs = k.B * k.HK, parts = x.splits * x.dblocks;
         const dim3 grid(SIMP ? seqs : seqs * parts, (unsigned)x.row_tiles, SIMP ? parts : 1);
         if (!SIMP && k.n > 1) hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, !SIMP>), grid, dim3(FewCfg<D>::NW * 64), 0, stream, k);
@@ -200,6 +210,7 @@ int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, con
     k.w1 = p->w1;
     k.w2 = p->w2;
     k.scale_log2e = p->scale * kLog2e;
+    k.unit_columns = x.unit_columns;
     k.row_tiles = x.row_tiles;
     k.splits = x.splits;
     k.dblocks = x.dblocks;

@@ -82,6 +82,7 @@ struct PagedParams {
     int dq, dp;                               // channels of q and the output, and of a pool's row (multiples of 8)
     int w1, w2;
     float scale_log2e;
+    int unit_columns;                         // 2-simplicial, packed: columns of a (token, head)
     int row_tiles;                            // workgroups (per sequence and key/value head) that the rows take
     int splits, dblocks;                      // shares of the keys; blocks of 32 offsets
     // partial results where splits * dblocks > 1: fp32 [part][B n H][D] and [part][B n H] (reference, sum)
@@ -163,6 +164,7 @@ struct PagedWave {
         on = on && lo_ <= hi_;
         lo = on ? lo_ : 1;
         hi = on ? hi_ : 0;
+        if (!on) M = 0.f;        // (nothing of it is used: it must not look like a column whose weights outgrow its reference)
         most_lo = any ? most_lo_ : -0x7fffffff;
         least_hi = any ? least_hi_ : 0x7fffffff;
     }
@@ -456,9 +458,23 @@ struct SimplicialColumns {
         }
     }
 
-    // the wave's columns as one row relative to one reference: o[v] (see ColumnSum), ref, sum
-    template <class W>
-    __device__ __forceinline__ void finish(const PagedParams &p, const W &w, int hk, int c, int hf, float (&y)[16 * DT], float &ref, float &sum) const {
+    // the sum or the maximum over the `width` neighbouring lanes of a unit, in all of them (a power of two up to 16)
+    template <typename OP>
+    static __device__ __forceinline__ float over(int width, float x, OP op) {
+        using C = ColumnSum<16 * DT>;
+        if (width > 1) x = op(x, C::template other<0xb1>(x));
+        if (width > 2) x = op(x, C::template other<0x1b>(x));
+        if (width > 4) x = op(x, C::template other<0x141>(x));
+        if (width > 8) x = op(x, C::template other<0x140>(x));
+        return x;
+    }
+
+    // The columns of a unit as one row relative to one reference: y, ref, sum.  PACKED: a unit has `width` columns, and each of them ends with the whole
+    // row, y[v] of channel 32 (v / 16) + 16 hf + v % 16; else all 32, and the row is shared out as ColumnSum says
+    template <bool PACKED, class W>
+    __device__ __forceinline__ void finish(const PagedParams &p, const W &w, int hk, int c, int hf, int width, float (&y)[16 * DT], float &ref, float &sum) const {
+        const auto most = [](float a, float b) { return fmaxf(a, b); };
+        const auto plus = [](float a, float b) { return a + b; };
         const char *v2 = paged_row(p.v2, page2, row2) + hk * p.v2.sh;
         u32x4 v[2 * DT];
 #pragma unroll
@@ -469,9 +485,10 @@ struct SimplicialColumns {
         // (columns without a second row, and those that met no key, hold nothing that counts)
         const float column = w.whole_sum();
         const bool live = page2 >= 0 && column != 0.f;
-        ref = ColumnSum<16 * DT>::all(live ? w.M : kNoRef, [](float a, float b) { return fmaxf(a, b); });
-        const float f = live ? fast_exp2(w.M - ref) : 0.f;
-        sum = ColumnSum<16 * DT>::all(live ? column * f : 0.f, [](float a, float b) { return a + b; });
+        const float own = live ? w.M : kNoRef;
+        ref = PACKED ? over(width, own, most) : ColumnSum<16 * DT>::all(own, most);
+        const float f = live ? fast_exp2(w.M - ref) : 0.f, part = live ? column * f : 0.f;
+        sum = PACKED ? over(width, part, plus) : ColumnSum<16 * DT>::all(part, plus);
         // (a column that does not count has a factor and a second value of zero; what it holds is only set aside where it is no number: it
         // attends the same values as the others, but its weights are not numbers where a key is infinite)
         const bool aside = wave_any(!live && !(column < INFINITY));
@@ -487,7 +504,19 @@ struct SimplicialColumns {
 #pragma unroll
             for (int at = 0; at < 16 * DT; ++at) y[at] = live ? y[at] : 0.f;
         }
-        ColumnSum<16 * DT>::add(y, c);
+        if constexpr (PACKED) {
+            using C = ColumnSum<16 * DT>;
+            auto stage = [&](auto ctrl) {
+#pragma unroll
+                for (int at = 0; at < 16 * DT; ++at) y[at] += C::template other<decltype(ctrl)::value>(y[at]);
+            };
+            if (width > 1) stage(std::integral_constant<int, 0xb1>{});
+            if (width > 2) stage(std::integral_constant<int, 0x1b>{});
+            if (width > 4) stage(std::integral_constant<int, 0x141>{});
+            if (width > 8) stage(std::integral_constant<int, 0x140>{});
+        } else {
+            ColumnSum<16 * DT>::add(y, c);
+        }
     }
 };
 
@@ -642,7 +671,7 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
     const int64_t rows = (int64_t)p.B * p.n * p.H;
     if constexpr (SIMP) {
         float y[16 * DT], ref, sum;
-        cols.finish(p, w, hk, c, hf, y, ref, sum);
+        cols.template finish<false>(p, w, hk, c, hf, 32, y, ref, sum);
         if (lane == 0) {
             xm[wave] = ref;
             xl[wave] = sum;
@@ -750,7 +779,9 @@ struct ManyCfg {
     static constexpr int LOADS = 2 * RT::NCH > NW ? 2 * RT::NCH / NW : 1;    // per wave and tile
 };
 
-template <class E, int D, bool SIMP>
+// PACKED (2-simplicial, second windows up to 16): a wave has 32 / width (token, head) units of `width` columns each, width the power of two that holds
+// the window
+template <class E, int D, bool SIMP, bool PACKED>
 __global__ __launch_bounds__((ManyCfg<D, SIMP>::NW * 64)) __attribute__((amdgpu_waves_per_eu(ManyCfg<D, SIMP>::WPE, ManyCfg<D, SIMP>::WPE))) void
 paged_many_kernel(PagedParams p) {
     using C = ManyCfg<D, SIMP>;
@@ -761,7 +792,9 @@ paged_many_kernel(PagedParams p) {
     const char **seg_k = reinterpret_cast<const char **>(lds + C::RING), **seg_v = seg_k + C::SEG;
     int *gaps = reinterpret_cast<int *>(lds + C::RING + 2 * C::SEG * 8);     // per half (of four): keys are missing in front of the last one
     const int tid = threadIdx.x, wave = wave_index(), lane = tid & 63, c = lane & 31, hf = lane >> 5;
-    constexpr int PER_WG = SIMP ? NW : NW * 32;        // rows (t, g) of a workgroup
+    const int width = PACKED ? p.unit_columns : SIMP ? 32 : 1, units = 32 / width;      // columns of a row (t, g), rows of a wave
+    const int PER_WG = NW * units;                      // ... of a workgroup
+    constexpr bool ONE = SIMP && !PACKED;               // all columns of a wave attend to the same keys
 
     // grid: (row tile, sequence and key/value head with the heads next to each other: one XCD has all workgroups of a head where their number is a multiple
     // of eight), part; the longest rows first
@@ -771,7 +804,7 @@ paged_many_kernel(PagedParams p) {
     const int db = p.dblocks == 1 ? 0 : uniform(part / p.splits), split = part - db * p.splits;
     const PagedSeq s = paged_seq(p, b);
 
-    const int R0 = tile_r * PER_WG, R = SIMP ? R0 + wave : R0 + wave * 32 + c;
+    const int R0 = tile_r * PER_WG, R = R0 + wave * units + (PACKED ? c / width : SIMP ? 0 : c);
     const int t = (int)p.group((uint32_t)R), g = R - t * p.G, h = hk * p.G + g;
     const int pos = s.first + t;
     const bool row_there = R < p.n * p.G;
@@ -837,21 +870,19 @@ paged_many_kernel(PagedParams p) {
     w.clear();
     // keys that any column of the wave attends
     int lo, hi;
+    const int t0 = max((int)p.group((uint32_t)(R0 + wave * units)), -s.first), t1 = min((int)p.group((uint32_t)(R0 + wave * units + units - 1)), s.count - 1);
+    bool any = t0 <= t1 && last >= 0;
     if constexpr (SIMP) {
-        cols.build(p, s, w, q_row, pos, 32 * db + c, hk, hf, on);
-        const bool any = wave_any(on && cols.page2 >= 0);
-        lo = any ? max(0, pos - p.w1 + 1) : 0x7fffffff;
-        hi = any ? min(pos, last) : -1;
-        w.limits(lo, hi, on && cols.page2 >= 0, any && lo <= hi, lo, hi);
+        cols.build(p, s, w, q_row, pos, 32 * db + (PACKED ? c & (width - 1) : c), hk, hf, on);
+        any = any && wave_any(on && cols.page2 >= 0);
     } else {
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) w.A[kk] = paged_piece(q_row, 16 * kk + 8 * hf, p.dq, on);
-        const int t0 = max((int)p.group((uint32_t)(R0 + 32 * wave)), -s.first), t1 = min((int)p.group((uint32_t)(R0 + 32 * wave + 31)), s.count - 1);
-        const bool any = t0 <= t1 && last >= 0;
-        lo = any ? 0 : 0x7fffffff;
-        hi = any ? min(s.first + t1, last) : -1;
-        w.limits(0, min(pos, last), on, any, 0, min(s.first + t0, last));
     }
+    lo = any ? (SIMP ? max(0, s.first + t0 - p.w1 + 1) : 0) : 0x7fffffff;
+    hi = any ? min(s.first + t1, last) : -1;
+    any = any && lo <= hi;
+    w.limits(SIMP ? max(0, pos - p.w1 + 1) : 0, min(pos, last), on && (!SIMP || cols.page2 >= 0), any, SIMP ? max(0, s.first + t1 - p.w1 + 1) : 0, min(s.first + t0, last));
     lo = uniform(lo);
     hi = uniform(hi);
     w.most_lo = uniform(w.most_lo);
@@ -944,7 +975,7 @@ paged_many_kernel(PagedParams p) {
                 const int tile = start + 32 * u;
                 const uint32_t there = there_of(u, any_gap);
                 const bool masked = w.needs_mask(tile, there);
-                w.template step<SIMP>(buf + k_lane, buf + v_lane, p.scale_log2e, masked, masked, tile, there, hf);
+                w.template step<ONE>(buf + k_lane, buf + v_lane, p.scale_log2e, masked, masked, tile, there, hf);
                 ++u;
             }
             for (; u < end; ++u) {
@@ -959,8 +990,29 @@ paged_many_kernel(PagedParams p) {
     const int64_t rows = (int64_t)p.B * p.n * p.H, out_row = ((int64_t)b * p.n + t) * p.H + h;
     if constexpr (SIMP) {
         float y[16 * DT], ref, sum;
-        cols.finish(p, w, hk, c, hf, y, ref, sum);
+        cols.template finish<PACKED>(p, w, hk, c, hf, width, y, ref, sum);
         if (!row_there) return;
+        if constexpr (PACKED) {
+            if ((c & (width - 1)) != 0) return;
+            const bool something = sum > 0.f || sum != sum;
+            const float inv = something ? 1.f / sum : 0.f;
+#pragma unroll
+            for (int x = 0; x < 2 * DT; ++x) {
+                const int d0 = 32 * (x >> 1) + 16 * hf + 8 * (x & 1);
+                float z[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = parts > 1 ? y[8 * x + e] : something ? y[8 * x + e] * inv : 0.f;
+                if (parts == 1) {
+                    paged_store8<E>(p, p.o + b * p.o_sb + t * p.o_sn + h * p.o_sh, d0, z);
+                } else {
+                    float *dst = p.part_o + ((int64_t)part * rows + out_row) * D + d0;
+                    *reinterpret_cast<float4 *>(dst) = make_float4(z[0], z[1], z[2], z[3]);
+                    *reinterpret_cast<float4 *>(dst + 4) = make_float4(z[4], z[5], z[6], z[7]);
+                }
+            }
+            if (parts > 1 && hf == 0) p.part_ml[part * rows + out_row] = make_float2(ref, sum);
+            return;
+        }
         const int base = ColumnSum<16 * DT>::base(c);
         if (parts == 1) {
             const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;

@@ -84,6 +84,26 @@ def test_simplicial(case):
     P.check(run(q, pools, tables, ints(*lengths), w1=w1, w2=w2), want(q, pools, tables, lengths, w1=w1, w2=w2))
 
 
+@pytest.mark.parametrize('w2', [1, 2, 3, 4, 7, 8, 9, 16])
+@pytest.mark.parametrize('d,g', [(32, 4), (64, 3), (104, 2), (256, 2)])
+def test_short_second_windows_of_many_tokens(w2, d, g):
+    """Several (token, head) units of a wave: ends of sequences, rows and tokens that are not there, heads of a group, first windows that differ by unit."""
+    b, n, hk, lengths = 3, 131, 2, [131, 40, 390]
+    counts = [131, 57, 100]
+    pools, tables = P.make_cache(b, hk, d, lengths, 16, 2, BF16)
+    q = queries(b, n, hk * g, d)
+    for w1 in (33, 300):
+        out = run(q, pools, tables, ints(*lengths), ints(*counts), w1=w1, w2=w2)
+        P.check(out, want(q, pools, tables, lengths, counts, w1=w1, w2=w2))
+
+
+def test_short_second_window_in_shares():
+    """... where the keys of few units are split, and joined."""
+    pools, tables = P.make_cache(1, 1, 64, [9000], 64, 2, F16)
+    q = queries(1, 1100, 1, 64, F16)
+    P.check(run(q, pools, tables, ints(9000), w1=8000, w2=5), want(q, pools, tables, [9000], w1=8000, w2=5))
+
+
 @pytest.mark.parametrize('n', [1, 6, 45])
 @pytest.mark.parametrize('sets', [1, 2])
 def test_rows_that_are_not_there(n, sets):
