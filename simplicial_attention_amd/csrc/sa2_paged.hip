@@ -39,7 +39,7 @@ int check_problem(const sa2_paged_problem *p, bool simplicial) {
     if (simplicial && (p->w1 < 1 || p->w2 < 1)) return fail_with(SA2_ERR_BAD_SHAPE, "windows w1=%d w2=%d must be >= 1", p->w1, p->w2);
     if (!(p->scale > 0.f) || !std::isfinite(p->scale)) return fail_with(SA2_ERR_BAD_SHAPE, "scale must be positive and finite");
     if (p->max_length < 0) return fail_with(SA2_ERR_BAD_SHAPE, "max_length=%d must be >= 0 (0: what the tables can name)", p->max_length);
-    if ((int64_t)p->batch * p->rows * p->heads > 0x1fffffffll) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
+    if ((int64_t)p->batch * p->rows * p->heads > 0x3ffffffll) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
     return SA2_OK;
 }
 
@@ -48,7 +48,7 @@ struct Plan {
     bool many, packed;
     int unit_columns;
     int dim, row_tiles, splits, dblocks;
-    int64_t grid, rows;
+    int64_t grid, rows;      // workgroups (of the launch's first dimension); output rows
     int64_t bytes() const { return splits * dblocks > 1 ? splits * dblocks * rows * (dim * 4 + 8) : 0; }
 };
 
@@ -104,7 +104,7 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
     // (a dimension of the grid)
     const int64_t most_splits = x.dblocks < 255 ? 256 : x.dblocks < 65536 ? 65535 / x.dblocks : 1;
     x.splits = (int)(splits > most_splits ? most_splits : splits);
-    x.grid = items * x.splits;
+    x.grid = x.many ? seqs * x.row_tiles : simplicial ? seqs : seqs * x.splits;
     return x;
 }
 
@@ -141,7 +141,7 @@ void launch(const Plan &x, const PagedParams &k, hipStream_t stream) {
         else hipLaunchKernelGGL((paged_few_kernel<E, D, SIMP, false>), grid, dim3(FewCfg<D>::NW * 64), 0, stream, k);
     }
     if (x.splits * x.dblocks > 1) {
-        const int pg = x.splits * x.dblocks >= 8 ? 8 : 1, per = 256 / (D / 8) / pg;
+        const int pg = x.splits * x.dblocks >= 8 && x.rows <= 1 << 20 ? 8 : 1, per = 256 / (D / 8) / pg;
         const dim3 grid((unsigned)((x.rows + per - 1) / per));
         if (pg > 1) hipLaunchKernelGGL((paged_merge_kernel<E, D, 8>), grid, dim3(256), 0, stream, k);
         else hipLaunchKernelGGL((paged_merge_kernel<E, D, 1>), grid, dim3(256), 0, stream, k);
@@ -172,7 +172,8 @@ int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, con
     if (!at || !at->tables || !at->lengths) return fail_with(SA2_ERR_NULL_POINTER, "tables and lengths are required");
     const Plan x = plan_of(p, simplicial);
     if (x.dblocks > 65535) return fail_with(SA2_ERR_BAD_SHAPE, "w2=%d: at most %d offsets are supported", p->w2, 65535 * 32);
-    if (x.grid > 0x7fffffffll) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
+    // (a launch has fewer than 2^32 threads, 512 in a workgroup)
+    if (x.grid > 0x7fffffll) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
     if (x.bytes() > 0 && (!workspace || workspace_bytes < x.bytes()))
         return fail_with(SA2_ERR_BAD_SHAPE, "workspace of %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0), (long long)x.bytes());
     if (x.bytes() > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return fail_with(SA2_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");

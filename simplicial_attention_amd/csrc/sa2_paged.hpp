@@ -9,7 +9,8 @@
 //                o = sum over columns of v2[p - d] * O, so the 32 offsets of a token share its window and one product does them all
 // Softmax: the reference M of a column moves only when a tile's weights outgrow 2^60 (fp16: 2^14) on it, the first tile included
 // (M starts far below every logit), so the ordinary tile has no maximum and no rescale.  Sums and accumulators are fp32; the weights
-// are rounded to the element type for the second product, and so is q * k2 for the first.
+// are rounded to the element type for the second product; c q * k2 enters the first in two parts of that type (rounded to one, its error
+// would be the largest of the output's; the logits' products double).
 //
 // Keys that are not there (beyond the walked range, missing pages) are fetched from a row of zeros and masked; a value row that a
 // column does not attend never reaches it, whatever it holds (0 * NaN is not 0: see value_products).
@@ -55,7 +56,7 @@ struct ElemF16 {
 // mfma_in_place: the accumulator's registers are the result's.  (Left to itself the compiler gives a product of the loop below other registers than its
 // addend, and copies 16 of them per product and step.)  Written as assembly, so the wait states it needs are this code's business: two
 // behind a VALU write of an operand are in it, and PagedWave::settle stands behind a run of them.  The compiler must not move an accumulator between two of them: kernels that use it are held to ordinary registers
-// (-amdgpu-mfma-vgpr-form, two waves per SIMD or more, no spills).
+// (-amdgpu-mfma-vgpr-form, two waves per SIMD or more; tests/test_in_place_products.py reads the assembly).
 
 struct PagedPool {
     const char *ptr;
@@ -526,6 +527,10 @@ struct SimplicialColumns {
 // of their keys; its waves take the tiles in turn, each with a K and a V tile of its own in LDS, and merge at the end.  No barrier in the walk: the
 // next K tile is requested when the logits of a tile are formed, the next V tile behind its second product, so a wave always has
 // a tile in flight and a CU sixteen waves of them.
+//
+// Bound by the cache's bytes: one token of 16 sequences of up to 32768, 16 heads on 4 of 128 channels (602 MB) 131 us with its merge, 4.6 TB/s where a copy of 2 GiB
+// reaches 4.9.  The smallest calls are bound by a chain of dependent loads (length, table, rows): 5.8 us for one token over 300 rows, 10.3 for one 2-simplicial
+// token, whose second rows come in front of its keys; an empty launch takes 3.6.
 template <int D>
 struct FewCfg {
     using RT = DmaTile<D>;
@@ -759,9 +764,15 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
 //
 // A workgroup has NW x 32 columns (dense: rows of one sequence and key/value head; 2-simplicial: NW (token, head) units) and walks the
 // union of their keys; K and V tiles stream through an LDS ring of four buffers that all waves read, one tile and one barrier per step.  A step's
-// fragments travel through windows of FW registers sets, requested FW products before their use: V's along the logit chain, the next
+// fragments travel through windows of FW register sets, requested FW products before their use: V's along the logit chain, the next
 // tile's K along the value chain (a scheduling fence behind every product keeps them there).  Steps that need a mask, two or three of a
 // walk, take the plain form of PagedWave.
+//
+// Bound by instruction issue of two waves per SIMD.  Dense, 128 channels: 2048 tokens of 16 heads over 32768 keys 500 to 520 us (532 GFLOP, 1.04 PFLOP/s where a
+// large product of the library reaches 1.27), the matrix unit busy 54 % of the time; a step issues 16 products, 62 other vector instructions and 16 exponentials, which with
+// their issue times fill nine tenths of it.  2-simplicial: 4 x 1024 tokens, 8 heads, w1 512, w2 32 434 us (276 GFLOP, and half of its logits' 138 again for the second part of
+// the operand); its windows are short, so of a wave's 3400 vector instructions 2000 stand in front of and behind the walk.
+// Tried and taken back: the two waves of a SIMD half a step apart by a second barrier (499 -> 581 us).
 template <int D, bool SIMP>
 struct ManyCfg {
     using RT = DmaTile<D>;
@@ -779,7 +790,7 @@ struct ManyCfg {
     static constexpr int LOADS = 2 * RT::NCH > NW ? 2 * RT::NCH / NW : 1;    // per wave and tile
 };
 
-// PACKED (2-simplicial, second windows up to 16): a wave has 32 / width (token, head) units of `width` columns each, width the power of two that holds
+// PACKED (2-simplicial, many units with second windows up to 16): a wave has 32 / width (token, head) units of `width` columns each, width the power of two that holds
 // the window
 template <class E, int D, bool SIMP, bool PACKED>
 __global__ __launch_bounds__((ManyCfg<D, SIMP>::NW * 64)) __attribute__((amdgpu_waves_per_eu(ManyCfg<D, SIMP>::WPE, ManyCfg<D, SIMP>::WPE))) void
@@ -1053,7 +1064,7 @@ paged_many_kernel(PagedParams p) {
 }
 
 // ---- partial results of a row merged: D / 8 threads per part, PG parts at a time (few rows with many parts are a chain of
-// dependent loads otherwise), the groups' sums added in order
+// dependent loads otherwise), the groups' sums added in order.  Measured: 512 rows of 128 channels in up to 32 parts 5 us, beside 127 of the walk
 template <class E, int D, int PG>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
     constexpr int TPR = D / 8, RPW = 256 / (TPR * PG);

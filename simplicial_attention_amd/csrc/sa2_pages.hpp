@@ -1,4 +1,8 @@
 // Rows into the pages of a cache, and pages to other pages.
+//
+// Both are bound by the bytes they read and write, and where these are few by the launch: 64 tokens into four pools 4.7 us (an empty launch 3.6), 8 x 2048 tokens
+// into two pools of 8 x 64 channels (67 MB) 12 us; 512 pages of every pool (1.2 GB) 253 us, 4.8 TB/s where a copy of 2 GiB reaches 4.9; eight pages of
+// 36 pools 7.5 us.
 #pragma once
 
 #include "sa2_common.hpp"

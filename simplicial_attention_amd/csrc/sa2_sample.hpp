@@ -10,6 +10,9 @@
 // Rows of up to 4096 tokens stay in the registers of one workgroup.  Longer ones are read once, 4096 tokens per workgroup, which leaves the chunk's sums, the best token
 // of an unfiltered row, and the largest logit of every 16 tokens.  A second kernel merges them, one workgroup per row; the largest logits
 // of the sixteens bound the kept prefix so closely that the races of a filtered row, and its random numbers, are looked up for few tokens.
+// Measured: 8 rows of 256 tokens 6.3 us (one launch); 96 rows of 100000, half of them with min-p, all with top-k and top-p, 30 us: 12 for the reading (19 MB: the chip
+// is filled by 600 workgroups that read once) and 18 for a chain of reductions over a workgroup (top, bound, races).  A flat row without top-k holds thousands of kept tokens,
+// which its workgroup reads again in every race: 45 to 50 us.
 // Weights are exp2 of log2 units: exp2, log2 and reciprocals are single instructions, exact to an ulp.
 #pragma once
 

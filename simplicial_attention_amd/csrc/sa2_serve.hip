@@ -28,6 +28,9 @@ void launch_sample(int64_t rows, const SampleParams &k, hipStream_t s) {
     }
 }
 
+// workgroups of a launch: fewer than 2^32 threads of 256 a group
+constexpr int64_t kMostGroups = 0xffffff;
+
 }  // namespace
 
 extern "C" {
@@ -67,7 +70,7 @@ int sa2_paged_append(const sa2_paged_problem *p, const sa2_append_item *items, i
     k.pieces = p->pool_dim / 8;
     k.count = count;
     const int64_t threads = (int64_t)p->batch * p->rows * p->kv_heads * k.pieces;
-    if (p->kv_heads > (1 << 24) || (threads + 255) / 256 > 0x7fffffffll) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
+    if (p->kv_heads > (1 << 24) || (threads + 255) / 256 > kMostGroups) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
     const dim3 grid((unsigned)((threads + 255) / 256));
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);
     if (plain) hipLaunchKernelGGL(paged_append_kernel<true>, grid, dim3(256), 0, s, k, src_type, p->dtype);
@@ -89,6 +92,7 @@ int sa2_copy_pages(const sa2_page_pool *pools, int32_t count, const int32_t *pai
         most_bytes = std::max(most_bytes, t.bytes);
         wide = wide && t.bytes % 16 == 0 && pieces16(t.ptr, t.stride, 0, 0);
     }
+    if (n_pairs > least) return fail_with(SA2_ERR_BAD_SHAPE, "%lld pairs of %lld pages: a page is written twice", (long long)n_pairs, (long long)least);
     // what is written may be neither read nor written again: the pairs run in no order
     try {
         std::vector<std::pair<int32_t, bool>> seen;      // (page, written)
@@ -116,9 +120,8 @@ int sa2_copy_pages(const sa2_page_pool *pools, int32_t count, const int32_t *pai
             k.stride[i] = pools[p0 + i].stride;
             k.bytes[i] = (int32_t)pools[p0 + i].bytes;
         }
-        // (workgroups of one launch stay below 2^31)
         const int64_t per_pair = (int64_t)k.pools * k.chunks;
-        const int most = (int)std::max<int64_t>(1, std::min<int64_t>(kCopyPairs, 0x7fffffff / per_pair));
+        const int most = (int)std::max<int64_t>(1, std::min<int64_t>(kCopyPairs, kMostGroups / per_pair));
         for (int64_t i0 = 0; i0 < n_pairs; i0 += most) {
             k.pairs = (int)std::min<int64_t>(most, n_pairs - i0);
             for (int i = 0; i < k.pairs; ++i) {
@@ -149,7 +152,7 @@ int sa2_sample(const void *logits, int32_t type, int64_t rows, int64_t vocab, in
     if ((reinterpret_cast<uintptr_t>(logits) & (type == SA2_ELEMENT_F32 ? 3 : 1)) != 0 || (reinterpret_cast<uintptr_t>(noise) & 3) != 0)
         return fail_with(SA2_ERR_ALIGNMENT, "logits and noise must be aligned to their elements");
     const int64_t bytes = sa2_sample_workspace_bytes(rows, vocab), chunks = (vocab + kSampleChunk - 1) / kSampleChunk;
-    if (rows * chunks > 0x7fffffff) return fail_with(SA2_ERR_BAD_SHAPE, "rows=%lld vocab=%lld: too large for a 1-D grid", (long long)rows, (long long)vocab);
+    if (rows * chunks > kMostGroups || (chunks > 1 && rows > kMostGroups * 256 / kRowThreads)) return fail_with(SA2_ERR_BAD_SHAPE, "rows=%lld vocab=%lld: too large for a 1-D grid", (long long)rows, (long long)vocab);
     if (bytes > 0 && (!workspace || workspace_bytes < bytes))
         return fail_with(SA2_ERR_BAD_SHAPE, "workspace of %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0), (long long)bytes);
     if (bytes > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return fail_with(SA2_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
