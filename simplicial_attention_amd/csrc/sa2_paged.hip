@@ -45,11 +45,12 @@ int check_problem(const sa2_paged_problem *p, bool simplicial) {
 
 // How the work is laid out: a function of the problem alone.
 struct Plan {
-    bool many, packed;
+    bool many, packed, even;
+    int64_t batch;
     int unit_columns;
     int dim, row_tiles, splits, dblocks;
     int64_t grid, rows;      // workgroups (of the launch's first dimension); output rows
-    int64_t bytes() const { return splits * dblocks > 1 ? splits * dblocks * rows * (dim * 4 + 8) : 0; }
+    int64_t bytes() const { return splits * dblocks > 1 ? splits * dblocks * rows * (dim * 4 + 8) + (even ? 0 : 8 * batch) : 0; }
 };
 
 Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
@@ -104,6 +105,9 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
     // (a dimension of the grid)
     const int64_t most_splits = x.dblocks < 255 ? 256 : x.dblocks < 65536 ? 65535 / x.dblocks : 1;
     x.splits = (int)(splits > most_splits ? most_splits : splits);
+    // (a lane for each sequence, and lengths whose quotients are exact)
+    x.even = simplicial || !x.many || x.splits == 1 || p->batch == 1 || p->batch > 64 || reach >= 1ll << 25;
+    x.batch = p->batch;
     x.grid = x.many ? seqs * x.row_tiles : simplicial ? seqs : seqs * x.splits;
     return x;
 }
@@ -215,9 +219,11 @@ int attend(bool simplicial, const sa2_paged_problem *p, const sa2_tensor *q, con
     k.row_tiles = x.row_tiles;
     k.splits = x.splits;
     k.dblocks = x.dblocks;
+    k.even = x.even;
     if (x.bytes() > 0) {
         k.part_o = static_cast<float *>(workspace);
         k.part_ml = reinterpret_cast<float2 *>(k.part_o + (int64_t)x.splits * x.dblocks * x.rows * x.dim);
+        k.shares = reinterpret_cast<int2 *>(k.part_ml + (int64_t)x.splits * x.dblocks * x.rows);
     }
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (p->dtype == SA2_ELEMENT_F16) {

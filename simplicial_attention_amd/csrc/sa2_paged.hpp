@@ -86,9 +86,11 @@ struct PagedParams {
     int unit_columns;                         // 2-simplicial, packed: columns of a (token, head)
     int row_tiles;                            // workgroups (per sequence and key/value head) that the rows take
     int splits, dblocks;                      // shares of the keys; blocks of 32 offsets
-    // partial results where splits * dblocks > 1: fp32 [part][B n H][D] and [part][B n H] (reference, sum)
+    int even;                                 // every sequence has `splits` shares; else see PagedShares
+    // partial results where splits * dblocks > 1: fp32 [place][n H][D] and [place][n H] (reference, sum), B places per share and block of offsets
     float *part_o;
     float2 *part_ml;
+    int2 *shares;                             // (not even) of a sequence: its first place, their number
 };
 
 constexpr float kNoRef = -1e30f;              // reference of a column that has met no key yet
@@ -128,6 +130,45 @@ __device__ __forceinline__ int paged_page(const PagedParams &p, const PagedSeq &
 __device__ __forceinline__ const char *paged_row(const PagedPool &pool, int page, int row) {
     return pool.ptr + (int64_t)page * pool.sp + (int64_t)row * pool.sr;
 }
+
+// Shares of the keys of sequences of different lengths (up to 64 of them): the B splits places that even shares would take go to the sequences as their lengths
+// ask, so that the longest share is as short as it gets.  Every wave of the walk forms them from the lengths, a lane for each sequence.  Measured, even shares
+// and these: 1131 tokens of four sequences, 4 heads on 2 of 128 channels, up to 17739 rows of different lengths 177 and 119 us, all of 17739 rows 181 and 184; 256 tokens of eight
+// sequences, 8 heads on 2 of 128 channels, up to 8192 rows 71 and 55, all of 8192 rows 83 and 85.
+struct PagedShares {
+    PagedSeq s;
+    int count, behind;       // (of the lane's sequence) shares; places up to its last
+    template <typename OP>
+    static __device__ __forceinline__ int scan(int x, OP op) {
+        x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));          // the row's lanes 1, 2, 4 and 8 before this one
+        x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+        x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+        x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+        x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));          // lane 15 of a row into the next row
+        x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));          // lane 31 into the upper half
+        return x;
+    }
+    static __device__ __forceinline__ int plus(int a, int b) { return a + b; }
+    static __device__ __forceinline__ int of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+    __device__ __forceinline__ PagedShares(const PagedParams &p, int lane) {
+        s = paged_seq(p, lane < p.B ? lane : 0);
+        const int end = min(s.first + s.count, s.reach), tiles = lane < p.B && s.count > 0 && end > 0 ? (end + 31) / 32 : 0;
+        const int most = of(scan(tiles, [](int a, int b) { return max(a, b); }), 63), all = of(scan(tiles, plus), 63);
+        // (fewer than 2^20 tiles: the quotient is exact)
+        auto shares = [&](int size) { return tiles > 0 ? (int)(((float)tiles - .5f) * __builtin_amdgcn_rcpf((float)size)) + 1 : 0; };
+        const int places = p.B * p.splits;
+        int size = max(kLeast, (most + p.splits - 1) / p.splits);      // (even shares of the longest fit)
+        int least = min(size, max(kLeast, (all + places - 1) / places));
+        while (least < size) {
+            const int middle = (least + size) >> 1;
+            if (of(scan(shares(middle), plus), 63) <= places) size = middle;
+            else least = middle + 1;
+        }
+        count = shares(size);
+        behind = scan(count, plus);
+    }
+    static constexpr int kLeast = 8;             // tiles of a share that are worth a place
+};
 
 // channels d0 .. d0 + 7 of a row of `channels`; zeros beyond them, and of a row that is not there.  (An address is chosen, not a branch taken: the
 // pieces of a row are then in flight together)
@@ -811,9 +852,23 @@ paged_many_kernel(PagedParams p) {
     // of eight), part; the longest rows first
     const int parts = p.splits * p.dblocks, part = blockIdx.y;
     const int row = uniform((int)p.seqs(blockIdx.x)), seq = blockIdx.x - row * (int)p.seqs.by, tile_r = p.row_tiles - 1 - row;
-    const int b = uniform((int)p.heads(seq)), hk = seq - b * p.HK;
-    const int db = p.dblocks == 1 ? 0 : uniform(part / p.splits), split = part - db * p.splits;
-    const PagedSeq s = paged_seq(p, b);
+    const int grid_b = uniform((int)p.heads(seq)), hk = seq - grid_b * p.HK, place = SIMP ? 0 : part * p.B + grid_b;
+    const int db = p.dblocks == 1 ? 0 : uniform(part / p.splits);
+    int b = grid_b, split = part - db * p.splits, splits = p.splits;
+    PagedSeq s;
+    if (!SIMP && !p.even) {
+        const PagedShares shares(p, lane);
+        // (for the merge)
+        if (blockIdx.x == 0 && part == 0 && tid < p.B) p.shares[tid] = make_int2(shares.behind - shares.count, shares.count);
+        const uint64_t before = __builtin_amdgcn_ballot_w64(shares.behind <= place);
+        b = __builtin_popcountll(before);                // (lanes beyond the sequences add no place)
+        if (b >= p.B) return;
+        splits = PagedShares::of(shares.count, b);
+        split = place - (PagedShares::of(shares.behind, b) - splits);
+        s = {p.tables + b * p.t_sb, PagedShares::of(shares.s.first, b), PagedShares::of(shares.s.count, b), shares.s.reach};
+    } else {
+        s = paged_seq(p, b);
+    }
 
     const int R0 = tile_r * PER_WG, R = R0 + wave * units + (PACKED ? c / width : SIMP ? 0 : c);
     const int t = (int)p.group((uint32_t)R), g = R - t * p.G, h = hk * p.G + g;
@@ -824,7 +879,7 @@ paged_many_kernel(PagedParams p) {
     const int last = min(s.first + t_last, s.reach - 1);
     const int first_key = SIMP ? max(0, s.first + t_first - p.w1 + 1) : 0;
     const int tiles = t_first < s.count && last >= first_key ? (last - first_key) / 32 + 1 : 0;
-    const int tile_a = p.splits == 1 ? 0 : (int)((int64_t)tiles * split / p.splits), tile_z = p.splits == 1 ? tiles : (int)((int64_t)tiles * (split + 1) / p.splits);
+    const int tile_a = splits == 1 ? 0 : (int)((int64_t)tiles * split / splits), tile_z = splits == 1 ? tiles : (int)((int64_t)tiles * (split + 1) / splits);
     const int NT = tile_z - tile_a;
 
     const char *const k_head = p.k1.ptr + hk * p.k1.sh, *const v_head = p.v1.ptr + hk * p.v1.sh;
@@ -998,7 +1053,7 @@ paged_many_kernel(PagedParams p) {
     }
 
     w.settle();
-    const int64_t rows = (int64_t)p.B * p.n * p.H, out_row = ((int64_t)b * p.n + t) * p.H + h;
+    const int64_t part_row = (SIMP ? (int64_t)part * p.B + grid_b : place) * p.n * p.H + (int64_t)t * p.H + h;
     if constexpr (SIMP) {
         float y[16 * DT], ref, sum;
         cols.template finish<PACKED>(p, w, hk, c, hf, width, y, ref, sum);
@@ -1016,12 +1071,12 @@ paged_many_kernel(PagedParams p) {
                 if (parts == 1) {
                     paged_store8<E>(p, p.o + b * p.o_sb + t * p.o_sn + h * p.o_sh, d0, z);
                 } else {
-                    float *dst = p.part_o + ((int64_t)part * rows + out_row) * D + d0;
+                    float *dst = p.part_o + part_row * D + d0;
                     *reinterpret_cast<float4 *>(dst) = make_float4(z[0], z[1], z[2], z[3]);
                     *reinterpret_cast<float4 *>(dst + 4) = make_float4(z[4], z[5], z[6], z[7]);
                 }
             }
-            if (parts > 1 && hf == 0) p.part_ml[part * rows + out_row] = make_float2(ref, sum);
+            if (parts > 1 && hf == 0) p.part_ml[part_row] = make_float2(ref, sum);
             return;
         }
         const int base = ColumnSum<16 * DT>::base(c);
@@ -1034,11 +1089,11 @@ paged_many_kernel(PagedParams p) {
                 if (d < p.dq && (16 * DT >= 32 || (c & 1) == 0)) *reinterpret_cast<uint16_t *>(orow + d * 2) = (uint16_t)E::pack(y[i] * inv, 0.f);
             }
         } else {
-            float *dst = p.part_o + ((int64_t)part * rows + out_row) * D;
+            float *dst = p.part_o + part_row * D;
 #pragma unroll
             for (int i = 0; i < ColumnSum<16 * DT>::LEFT; ++i)
                 if (16 * DT >= 32 || (c & 1) == 0) dst[32 * ((base + i) >> 4) + 16 * hf + ((base + i) & 15)] = y[i];
-            if (lane == 0) p.part_ml[part * rows + out_row] = make_float2(ref, sum);
+            if (lane == 0) p.part_ml[part_row] = make_float2(ref, sum);
         }
     } else {
         if (!on) w.clear();
@@ -1057,8 +1112,8 @@ paged_many_kernel(PagedParams p) {
                     paged_store8<E>(p, orow, 32 * dt + 16 * hf + 8 * half, z);
                 }
         } else {
-            store_row_f32<DT>(p.part_o + ((int64_t)part * rows + out_row) * D + 16 * hf, w.O, 1.f);
-            if (hf == 0) p.part_ml[part * rows + out_row] = make_float2(w.M, sum);
+            store_row_f32<DT>(p.part_o + part_row * D + 16 * hf, w.O, 1.f);
+            if (hf == 0) p.part_ml[part_row] = make_float2(w.M, sum);
         }
     }
 }
@@ -1070,15 +1125,28 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
     constexpr int TPR = D / 8, RPW = 256 / (TPR * PG);
     __shared__ float sums[PG > 1 ? 256 : 1][PG > 1 ? 11 : 1];
     const int64_t rows = (int64_t)p.B * p.n * p.H, row = (int64_t)blockIdx.x * RPW + threadIdx.x / (TPR * PG);
-    const int d0 = 8 * (threadIdx.x % TPR), group = threadIdx.x / TPR % PG, parts = p.splits * p.dblocks;
+    const int d0 = 8 * (threadIdx.x % TPR), group = threadIdx.x / TPR % PG;
+    // (rows are fewer than 2^26)
+    const uint32_t bt = (uint32_t)row / p.H, b = bt / p.n;
+    const int h = (int)((uint32_t)row - bt * p.H), t = (int)(bt - b * p.n);
+    // the row's places: one in each of the parts, or those of its sequence's shares
+    int parts = p.splits * p.dblocks;
+    int64_t from = row, step = rows;
+    if (!p.even) {
+        const int2 of_b = p.shares[min((int)b, p.B - 1)];
+        parts = of_b.y;
+        step = (int64_t)p.n * p.H;
+        from = of_b.x * step + (row - b * step);
+    }
     float top = kNoRef, total = 0.f, z[8] = {};
     if (row < rows) {
         // (a part that attended to nothing has left no row)
 #pragma unroll 4
         for (int x = group; x < parts; x += PG) {
-            const float2 ml = p.part_ml[x * rows + row];
+            const int64_t at = from + x * step;
+            const float2 ml = p.part_ml[at];
             if (ml.y == 0.f) continue;
-            const float *src = p.part_o + ((int64_t)x * rows + row) * D + d0;
+            const float *src = p.part_o + at * D + d0;
             const float4 a = *reinterpret_cast<const float4 *>(src), c = *reinterpret_cast<const float4 *>(src + 4);
             const float ref = fmaxf(top, ml.x), f = fast_exp2(ml.x - ref), old = fast_exp2(top - ref);
             top = ref;
@@ -1114,8 +1182,6 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
     const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] *= inv;
-    const int64_t bt = row / p.H;
-    const int h = (int)(row - bt * p.H), b = (int)(bt / p.n), t = (int)(bt - (int64_t)b * p.n);
     paged_store8<E>(p, p.o + b * p.o_sb + t * p.o_sn + h * p.o_sh, d0, z);
 }
 

@@ -84,6 +84,33 @@ def test_simplicial(case):
     P.check(run(q, pools, tables, ints(*lengths), w1=w1, w2=w2), want(q, pools, tables, lengths, w1=w1, w2=w2))
 
 
+# batch, new tokens, h, hk, d, page, lengths (a number: drawn up to it), dtype
+UNEVEN = [
+    (4, 70, 4, 2, 64, 16, [3000, 0, 40, 70], BF16),
+    (3, 33, 2, 1, 256, 64, [1, 2500, 900], BF16),
+    (5, 50, 2, 2, 128, 24, [33, 2000, 50, 1999, 700], F16),
+    (64, 40, 1, 1, 32, 16, 1500, BF16),
+    (65, 40, 1, 1, 32, 16, 600, BF16),                  # more sequences than a wave has lanes: even shares
+    (2, 300, 8, 1, 64, 32, [6000, 350], BF16),
+]
+
+
+@pytest.mark.parametrize('case', UNEVEN, ids=lambda c: '-'.join(map(str, c[:5])))
+def test_shares_of_sequences_of_different_lengths(case):
+    b, n, h, hk, d, page, lengths, dtype = case
+    if isinstance(lengths, int):
+        lengths = torch.randint(0, lengths + 1, (b,), generator=torch.Generator().manual_seed(3)).tolist()
+    counts = [min(n, x) if i % 3 else n for i, x in enumerate(lengths)]
+    pools, tables = P.make_cache(b, hk, d, lengths, page, 1, dtype)
+    q = queries(b, n, h, d, dtype)
+    out = run(q, pools, tables, ints(*lengths), ints(*counts))
+    P.check(out, want(q, pools, tables, lengths, counts))
+    # the same bits again, and nothing but rounding where a sequence is alone
+    assert torch.equal(out, run(q, pools, tables, ints(*lengths), ints(*counts)))
+    alone = torch.cat([run(q[i:i + 1], pools, tables[i:i + 1], ints(lengths[i]), ints(counts[i])) for i in range(b)])
+    P.check(alone, want(q, pools, tables, lengths, counts))
+
+
 @pytest.mark.parametrize('w2', [1, 2, 3, 4, 7, 8, 9, 16])
 @pytest.mark.parametrize('d,g', [(32, 4), (64, 3), (104, 2), (256, 2)])
 def test_short_second_windows_of_many_tokens(w2, d, g):
