@@ -70,10 +70,10 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
     // Second windows up to 16 leave columns of a wave to other units: taken where there are more units than 256 workgroups of a unit per wave hold (8 heads, w1 512,
     // unit per wave and packed: four sequences of 1024 tokens, 128 channels, w2 16, 8 and 4: 433, 393, 387 and 244, 130, 72 us; one of 128 tokens, 64 channels,
     // w2 8: 15.7 and 16.5)
-    x.unit_columns = 32;
-    while (simplicial && x.unit_columns > 1 && x.unit_columns / 2 >= p->w2) x.unit_columns /= 2;
     x.many = simplicial ? seqs * per * x.dblocks > 512 : per > 32;
-    x.packed = simplicial && seqs * per > 1024 && x.unit_columns < 32;
+    x.packed = simplicial && seqs * per > 1024 && p->w2 <= 16;
+    x.unit_columns = 32;
+    while (x.packed && x.unit_columns > 1 && x.unit_columns / 2 >= p->w2) x.unit_columns /= 2;
     const int64_t per_wg = x.many ? (simplicial ? waves * (32 / x.unit_columns) : waves * 32) : (simplicial ? 1 : 32);
     x.row_tiles = (int)((per + per_wg - 1) / per_wg);
     const int64_t items = seqs * x.row_tiles * x.dblocks;

@@ -124,6 +124,14 @@ def test_short_second_windows_of_many_tokens(w2, d, g):
         P.check(out, want(q, pools, tables, lengths, counts, w1=w1, w2=w2))
 
 
+@pytest.mark.parametrize('n', [64, 65, 100, 128, 129, 140])
+def test_short_second_windows_on_either_side_of_the_rule(n):
+    """512, 520, 800, 1024, 1032 and 1120 (token, head) units."""
+    pools, tables = P.make_cache(2, 1, 32, [n + 20, n], 16, 2, BF16)
+    q = queries(2, n, 4, 32)
+    P.check(run(q, pools, tables, ints(n + 20, n), w1=40, w2=8), want(q, pools, tables, [n + 20, n], w1=40, w2=8))
+
+
 def test_short_second_window_in_shares():
     """... where the keys of few units are split, and joined."""
     pools, tables = P.make_cache(1, 1, 64, [9000], 64, 2, F16)
