@@ -100,6 +100,10 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
             splits = (2048 + items * waves - 1) / (items * waves);
             if (2 * splits * waves * 8 <= tiles) splits *= 2;
             if (splits > tiles / waves) splits = tiles / waves;
+            // ... and beyond 128 parts a wave's walk has to outweigh the longer merge (one token of 8 heads on one, 128 channels: 32768 rows in 128, 256 parts 15.0
+            // and 16.7 us, 131072 rows 28.3 and 24.6; 256 channels, 32768 rows 26.9 and 22.2)
+            const int64_t pays = tiles * x.dim / (512 * waves);
+            if (splits > 128) splits = pays > 128 ? (splits < pays ? splits : pays) : 128;
         }
     }
     // (a dimension of the grid)
