@@ -332,7 +332,7 @@ struct PagedWave {
 
     // O^T += V^T P^T.  `guard`: some column does not attend some key of the tile, so a value that is not finite must be kept from it.
     // `ONE` (all columns attend to the same keys): those the columns do not attend are cleared in the operand.  Otherwise, where the tile
-    // holds such a value, every group of columns with its own last key gets a product of its own.
+    // holds such a value, every group of columns with keys of its own gets a product of its own.
     template <bool ONE>
     __device__ __forceinline__ void values(const char *v_lane, const u32x4 (&pb)[2], bool guard, int tile, uint32_t there, int hf) {
         if (!guard) {
@@ -382,12 +382,13 @@ struct PagedWave {
             settle();
             return;
         }
-        // last keys inside the tile, then the columns that attend to all of it
-        for (int z = max(0, min(31, least_hi - tile)); z < 32; ++z) {
-            const bool mine = lo <= hi && (z < 31 ? hi - tile == z : hi - tile >= 31);
-            if (!wave_any(mine)) continue;
+        const int first = max(0, lo - tile), end = min(31, hi - tile);
+        for (uint64_t left = __builtin_amdgcn_ballot_w64(lo <= hi && first <= end); left != 0;) {
+            const int one = (int)__builtin_ctzll(left), a = __builtin_amdgcn_readlane(first, one), z = __builtin_amdgcn_readlane(end, one);
+            const bool mine = lo <= hi && first == a && end == z;
+            left &= ~__builtin_amdgcn_ballot_w64(mine);
             u32x4 m[2];
-            key_masks(there & keys_of(tile, 0, tile + z), m);
+            key_masks(there & keys_of(tile, tile + a, tile + z), m);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 f32x16 x = zero16();

@@ -132,6 +132,24 @@ def test_short_second_windows_on_either_side_of_the_rule(n):
     P.check(run(q, pools, tables, ints(n + 20, n), w1=40, w2=8), want(q, pools, tables, [n + 20, n], w1=40, w2=8))
 
 
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), -float('inf')])
+def test_units_of_a_wave_keep_their_windows(bad):
+    """Short second windows: a row that is no number reaches the units whose first or second window holds it, and not their neighbours in the wave."""
+    n, at = 150, 77
+    pools, tables = P.make_cache(2, 1, 64, [n, n], 16, 2, BF16)
+    q = queries(2, n, 4, 64)
+    for pool in pools:
+        for s in range(2):
+            pool[tables[s, (at + s) // 16].long(), (at + s) % 16] = bad
+        out = run(q, pools, tables, ints(n, n), w1=20, w2=4)
+        touched = torch.zeros(2, n, dtype=torch.bool, device='cuda')
+        for s in range(2):
+            touched[s, at + s:at + s + 20] = True
+        clean = P.make_cache(2, 1, 64, [n, n], 16, 2, BF16)[0]
+        expected = want(q, clean, tables, [n, n], w1=20, w2=4)
+        P.check(out[~touched], expected[~touched])
+
+
 def test_short_second_window_in_shares():
     """... where the keys of few units are split, and joined."""
     pools, tables = P.make_cache(1, 1, 64, [9000], 64, 2, F16)
