@@ -10,7 +10,8 @@
 // Softmax: the reference M of a column moves only when a tile's weights outgrow 2^60 (fp16: 2^14) on it, the first tile included
 // (M starts far below every logit), so the ordinary tile has no maximum and no rescale.  Sums and accumulators are fp32; the weights
 // are rounded to the element type for the second product; c q * k2 enters the first in two parts of that type (rounded to one, its error
-// would be the largest of the output's; the logits' products double).
+// would be the largest of the output's; the logits' products double).  Where fp16 does not hold a product, both parts of its column are divided by powers of two and
+// its wave walks by plain steps; what is infinite or no number stays so.
 //
 // Keys that are not there (beyond the walked range, missing pages) are fetched from a row of zeros and masked; a value row that a
 // column does not attend never reaches it, whatever it holds (0 * NaN is not 0: see value_products).
@@ -24,7 +25,8 @@ namespace sa2 {
 struct ElemBf16 {
     static constexpr float kBig = 1.152921504606846976e18f;      // 2^60
     static constexpr uint32_t kExp = 0x7f80u;
-    static __device__ __forceinline__ float fit(float x) { return x; }
+    static constexpr bool kNarrow = false;                       // products of two numbers are in the type's range
+    static constexpr float kMost = 3.3895313892515355e38f;       // the largest number
     static __device__ __forceinline__ float lo(uint32_t w) { return bf16_lo(w); }
     static __device__ __forceinline__ float hi(uint32_t w) { return bf16_hi(w); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
@@ -39,7 +41,8 @@ struct ElemF16 {
     typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
     static constexpr float kBig = 16384.f;                       // 2^14: weights stay below the largest fp16 number
     static constexpr uint32_t kExp = 0x7c00u;
-    static __device__ __forceinline__ float fit(float x) { return fminf(fmaxf(x, -65504.f), 65504.f); }     // (NaN: the lowest)
+    static constexpr bool kNarrow = true;
+    static constexpr float kMost = 65504.f;
     static __device__ __forceinline__ float lo(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
     static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -182,11 +185,23 @@ __device__ __forceinline__ void paged_store8(const PagedParams &p, char *row, in
     if (d0 < p.dq) st_global16(row + d0 * 2, (u32x4){E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(x[4], x[5]), E::pack(x[6], x[7])});
 }
 
+// Products q * k2 beyond a narrow type's range: some column of the wave has them, and its two parts hold them divided by ratio * up and by up (powers of two; 1 for
+// the wave's other columns)
+template <bool THERE>
+struct WideProducts {
+    static constexpr bool wide = false;
+};
+template <>
+struct WideProducts<true> {
+    bool wide = false;
+    float ratio = 1.f, up = 1.f;
+};
+
 // ---- one wave's 32 columns
 // TWO: the operand of the logits in two parts (q * k2 has twice the digits of an element: rounded to one part it would double the error of
 // the output, in two it is exact)   IN_PLACE: value products by mfma_in_place
 template <class E, int D, bool TWO, bool IN_PLACE = false>
-struct PagedWave {
+struct PagedWave : WideProducts<TWO && E::kNarrow> {
     using RT = DmaTile<D>;
     static constexpr int KS = D / 16, DT = D / 32;
     u32x4 A[KS], A2[TWO ? KS : 1];
@@ -235,6 +250,20 @@ struct PagedWave {
     }
     // TWO: relative to `from` (c is in the operand); else the plain products
     __device__ __forceinline__ f32x16 logits(const char *k_lane, float from) const {
+        if constexpr (TWO && E::kNarrow) {
+            if (__builtin_expect(this->wide, 0)) {
+                f32x16 S = zero16();
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) S = E::mfma(RT::row_frag(k_lane, kk), A[kk], S);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[r] *= this->ratio;
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) S = E::mfma(RT::row_frag(k_lane, kk), A2[kk], S);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[r] = S[r] * this->up - from;
+                return S;
+            }
+        }
         f32x16 S = TWO ? splat16(-from) : zero16();
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) S = logit(RT::row_frag(k_lane, kk), kk, S);
@@ -481,6 +510,8 @@ struct SimplicialColumns {
         row2 = page2 >= 0 ? x - (int)p.div((uint32_t)x) * (int)p.div.by : 0;
         const char *k2 = paged_row(p.k2, page2, row2) + hk * p.k2.sh;
         constexpr int AT_ONCE = KS < 8 ? KS : 8;
+        const float c = p.scale_log2e;
+        float most = 0.f;         // the column's largest product (NaN left out)
 #pragma unroll
         for (int k0 = 0; k0 < KS; k0 += AT_ONCE) {
             u32x4 f[AT_ONCE], k[AT_ONCE];
@@ -493,13 +524,44 @@ struct SimplicialColumns {
             for (int x = 0; x < AT_ONCE; ++x)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float a = E::lo(f[x][i]) * p.scale_log2e * E::lo(k[x][i]), b = E::hi(f[x][i]) * p.scale_log2e * E::hi(k[x][i]);
-                    const uint32_t high = E::pack(E::fit(a), E::fit(b));
+                    const float a = E::lo(f[x][i]) * c * E::lo(k[x][i]), b = E::hi(f[x][i]) * c * E::hi(k[x][i]);
+                    most = fmaxf(fmaxf(fabsf(a), fabsf(b)), most);
+                    const uint32_t high = E::pack(a, b);
                     w.A[k0 + x][i] = high;
-                    w.A2[k0 + x][i] = E::pack(E::fit(a - E::lo(high)), E::fit(b - E::hi(high)));
+                    w.A2[k0 + x][i] = E::pack(a - E::lo(high), b - E::hi(high));
                 }
         }
+        most = W::both_halves_max(most);
+        if (__builtin_expect(!wave_any(most > E::kMost), 1)) return;
+        // Products that the type does not hold.  An infinite one has no second part (inf - inf is no number).  Finite ones (fp16) are kept divided by powers of two, the second
+        // parts by one of their own, so that small products beside a large one lose no digits to its range
+        float up1 = 1.f, down1 = 1.f, down2 = 1.f;
+        if constexpr (E::kNarrow) {
+            // (beside an infinite product, what two finite factors can reach)
+            const int exponent = most < INFINITY ? exponent_of(most) : exponent_of(c) + 33, e = most > E::kMost ? max(-100, min(100, exponent - 14)) : 0, e2 = max(0, e - 13);
+            w.wide = true;
+            w.ratio = two_to(e - e2);
+            w.up = two_to(e2);
+            up1 = two_to(e);
+            down1 = two_to(-e);
+            down2 = two_to(-e2);
+        }
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            const u32x4 f = paged_piece(q_row, 16 * kk + 8 * hf, p.dq, true), k = paged_piece(k2, 16 * kk + 8 * hf, p.dp, page2 >= 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = E::lo(f[i]) * c * E::lo(k[i]), b = E::hi(f[i]) * c * E::hi(k[i]);
+                const uint32_t high = E::pack(a * down1, b * down1);
+                const float ah = E::lo(high), bh = E::hi(high);
+                w.A[kk][i] = high;
+                w.A2[kk][i] = E::pack(fabsf(ah) < INFINITY ? (a - ah * up1) * down2 : 0.f, fabsf(bh) < INFINITY ? (b - bh * up1) * down2 : 0.f);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
+    static __device__ __forceinline__ int exponent_of(float x) { return (int)(as_u32(x) >> 23 & 255u) - 127; }
+    static __device__ __forceinline__ float two_to(int e) { return as_f32((uint32_t)(127 + e) << 23); }
 
     // the sum or the maximum over the `width` neighbouring lanes of a unit, in all of them (a power of two up to 16)
     template <typename OP>
@@ -982,7 +1044,7 @@ paged_many_kernel(PagedParams p) {
             }
             const int end = min(NT, u + C::HALF), z = min(end, u_z);
             // steps in front of it need no mask
-            const int m_z = any_gap ? u : min(z, ((w.least_hi - start - 31) >> 5) + 1);
+            const int m_z = any_gap || w.wide ? u : min(z, ((w.least_hi - start - 31) >> 5) + 1);
             for (; u < min(end, u_a); ++u) {
                 open_step();
                 request(u + NBUF - 1);
