@@ -594,9 +594,9 @@ struct SimplicialColumns {
         ref = PACKED ? over(width, own, most) : ColumnSum<16 * DT>::all(own, most);
         const float f = live ? fast_exp2(w.M - ref) : 0.f, part = live ? column * f : 0.f;
         sum = PACKED ? over(width, part, plus) : ColumnSum<16 * DT>::all(part, plus);
-        // (a column that does not count has a factor and a second value of zero; what it holds is only set aside where it is no number: it
-        // attends the same values as the others, but its weights are not numbers where a key is infinite)
-        const bool aside = wave_any(!live && !(column < INFINITY));
+        // (a factor of zero does not set aside what a column holds that does not count: its values, its weights where a key is infinite, or its second
+        // value may be no numbers)
+        const bool aside = wave_any(!live);
 #pragma unroll
         for (int x = 0; x < 2 * DT; ++x)
 #pragma unroll
@@ -605,7 +605,7 @@ struct SimplicialColumns {
                 y[at] = w.O[x >> 1][at & 15] * (f * E::lo(v[x][i]));
                 y[at + 1] = w.O[x >> 1][(at & 15) + 1] * (f * E::hi(v[x][i]));
             }
-        if (__builtin_expect(aside, 0)) {
+        if (aside) {
 #pragma unroll
             for (int at = 0; at < 16 * DT; ++at) y[at] = live ? y[at] : 0.f;
         }
