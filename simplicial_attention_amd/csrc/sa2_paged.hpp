@@ -288,7 +288,7 @@ struct PagedWave : WideProducts<TWO && E::kNarrow> {
                 const int j = 8 * (r >> 2) + (r & 3);
                 const uint32_t low = (uint32_t)((int)(keys << (31 - j)) >> 31), high = (uint32_t)((int)(keys << (27 - j)) >> 31);
                 const uint64_t lanes = ((uint64_t)high << 32) | low;
-                asm("v_cndmask_b32 %0, %1, %0, %2" : "+v"(S[r]) : "v"(-INFINITY), "s"(lanes));
+                S[r] = __builtin_amdgcn_inverse_ballot_w64(lanes) ? S[r] : -INFINITY;
             }
         } else {
             const int a = lo - tile - 4 * hf, z = hi - tile - 4 * hf;
