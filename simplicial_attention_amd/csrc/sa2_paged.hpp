@@ -130,6 +130,8 @@ __device__ __forceinline__ int paged_page(const PagedParams &p, const PagedSeq &
     const int id = s.table[p.div((uint32_t)x)];
     return (unsigned)id < (unsigned)p.pages ? id : -1;
 }
+// 2-simplicial: first key of a position (of position 0, for one in front of the sequence: windows may be as large as an int)
+__device__ __forceinline__ int first_key_of(const PagedParams &p, int pos) { return max(0, max(0, pos) - p.w1 + 1); }
 __device__ __forceinline__ const char *paged_row(const PagedPool &pool, int page, int row) {
     return pool.ptr + (int64_t)page * pool.sp + (int64_t)row * pool.sr;
 }
@@ -678,7 +680,7 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
     const int t_first = MIXED ? max((int)p.group((uint32_t)(tile_r * 32)), -s.first) : (SIMP ? t : 0);
     const int t_last = MIXED ? min((int)p.group((uint32_t)(tile_r * 32 + 31)), s.count - 1) : t_first;
     const int last = min(s.first + t_last, s.reach - 1);              // last key of any column
-    const int first_key = SIMP ? max(0, s.first + t - p.w1 + 1) : 0;
+    const int first_key = SIMP ? first_key_of(p, s.first + t) : 0;
     const bool any = t_first < s.count && t_first <= t_last && last >= first_key;
     const int tiles = any ? (last - first_key) / 32 + 1 : 0;
     const int tile_a = p.splits == 1 ? 0 : (int)((int64_t)tiles * split / p.splits), tile_z = p.splits == 1 ? tiles : (int)((int64_t)tiles * (split + 1) / p.splits);
@@ -940,7 +942,7 @@ paged_many_kernel(PagedParams p) {
     const bool on = row_there && t < s.count && pos >= 0;
     const int t_first = (int)p.group((uint32_t)R0), t_last = min((int)p.group((uint32_t)(R0 + PER_WG - 1)), s.count - 1);
     const int last = min(s.first + t_last, s.reach - 1);
-    const int first_key = SIMP ? max(0, s.first + t_first - p.w1 + 1) : 0;
+    const int first_key = SIMP ? first_key_of(p, s.first + t_first) : 0;
     const int tiles = t_first < s.count && last >= first_key ? (last - first_key) / 32 + 1 : 0;
     const int tile_a = splits == 1 ? 0 : (int)((int64_t)tiles * split / splits), tile_z = splits == 1 ? tiles : (int)((int64_t)tiles * (split + 1) / splits);
     const int NT = tile_z - tile_a;
@@ -1008,10 +1010,10 @@ paged_many_kernel(PagedParams p) {
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) w.A[kk] = paged_piece(q_row, 16 * kk + 8 * hf, p.dq, on);
     }
-    lo = any ? (SIMP ? max(0, s.first + t0 - p.w1 + 1) : 0) : 0x7fffffff;
+    lo = any ? (SIMP ? first_key_of(p, s.first + t0) : 0) : 0x7fffffff;
     hi = any ? min(s.first + t1, last) : -1;
     any = any && lo <= hi;
-    w.limits(SIMP ? max(0, pos - p.w1 + 1) : 0, min(pos, last), on && (!SIMP || cols.page2 >= 0), any, SIMP ? max(0, s.first + t1 - p.w1 + 1) : 0, min(s.first + t0, last));
+    w.limits(SIMP ? first_key_of(p, pos) : 0, min(pos, last), on && (!SIMP || cols.page2 >= 0), any, SIMP ? first_key_of(p, s.first + t1) : 0, min(s.first + t0, last));
     lo = uniform(lo);
     hi = uniform(hi);
     w.most_lo = uniform(w.most_lo);
