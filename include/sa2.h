@@ -355,7 +355,8 @@ int sa2_copy_pages(const sa2_page_pool *pools, int32_t count, const int32_t *pai
  * p = softmax(logits / temperature), a token is kept if its rank is below top_k (top_k <= 0: any), the mass in front of it below top_p (top_p >= 1: any) and
  * p >= min_p * max p; the first always is.  tokens[r] is the kept one with the largest logit / temperature - log(-log u), u = noise[r][token] in [0, 1) (fp32), ties to the
  * lowest index; temperature <= 0: the first in the order.  logprobs[r] is its logarithm under softmax(logits).  A logit that is not a number counts as
- * -infinity; a row without any other logit gives token -1 and -infinity.  The four parameters are fp32 / int32 device arrays [rows], or NULL: the number beside them. */
+ * -infinity; a row without any other logit gives token -1 and -infinity.  An infinite temperature weighs all tokens above -infinity alike; a temperature, top_p or min_p that
+ * is not a number leaves the first token.  The four parameters are fp32 / int32 device arrays [rows], or NULL: the number beside them. */
 typedef struct sa2_sample_params {
     const float *temperature, *top_p, *min_p;
     const int32_t *top_k;

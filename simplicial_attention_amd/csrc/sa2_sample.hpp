@@ -190,18 +190,18 @@ struct RowReduce {
 };
 
 struct RowRules {
-    float inv, top_p, min_p;      // inv: log2(e) / T, 0 for a greedy row
+    float inv, top_p, min_p;      // inv: log2(e) / T, above 0 (a logit of -inf times it has to weigh nothing) but for a greedy row
     int top_k;
     bool greedy;
     __device__ RowRules(const SampleParams &p, int64_t r) {
         const float T = p.temperature ? p.temperature[r] : p.temperature_all;
         greedy = !(T > 0.f);
-        inv = greedy ? 0.f : fminf(kLog2e / T, kMostFloat);
+        inv = greedy ? 0.f : fmaxf(fminf(kLog2e / T, kMostFloat), 1e-44f);
         top_p = p.top_p ? p.top_p[r] : p.top_p_all;
         min_p = p.min_p ? p.min_p[r] : p.min_p_all;
         top_k = p.top_k ? p.top_k[r] : p.top_k_all;
     }
-    __device__ bool filters() const { return top_k > 0 || top_p < 1.f || !(min_p <= 0.f); }
+    __device__ bool filters() const { return top_k > 0 || !(top_p >= 1.f) || !(min_p <= 0.f); }
     // a token with `count` tokens and the mass `front` in front of it
     __device__ bool keeps(float count, float front, float mass, float weight) const {
         return (top_k <= 0 || count < (float)top_k) && (top_p >= 1.f || front < top_p * mass) && weight >= min_p;

@@ -18,7 +18,8 @@ def sample_tokens(logits: Tensor, noise: Tensor, *, temperature=1., top_k=0, top
     where ``noise`` (float32, the shape of ``logits``) is uniform on [0, 1).  ``temperature`` 0 takes the first token of the order.  ``logprobs`` are the tokens'
     logarithms under softmax(logits).  A logit that is not a number counts as -inf; a row without any other gives token -1 and -inf.
 
-    Every parameter is a number, or a tensor with one value per row (float32; ``top_k`` int32).
+    Every parameter is a number, or a tensor with one value per row (float32; ``top_k`` int32).  Numbers have to be finite and not negative.  Tensors are read by the kernels alone: a
+    negative temperature is taken as 0, an infinite one weighs all tokens above -inf alike, and a value that is not a number leaves its row the first token.
     """
     given = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     tensors = {name: value if isinstance(value, Tensor) else None for name, value in given.items()}
