@@ -363,7 +363,7 @@ typedef struct sa2_sample_params {
     float temperature_all, top_p_all, min_p_all;
     int32_t top_k_all;
 } sa2_sample_params;
-int64_t sa2_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int64_t sa2_sample_workspace_bytes(int64_t rows, int64_t vocab);     /* -1 without rows or tokens, beyond 2^31 - 1 rows or 2^24 tokens */
 int sa2_sample(const void *logits, int32_t type, int64_t rows, int64_t vocab, int64_t stride, const float *noise, int64_t noise_stride,
                const sa2_sample_params *params, int64_t *tokens, float *logprobs, void *workspace, int64_t workspace_bytes, void *hip_stream);
 

@@ -39,7 +39,7 @@ int check_problem(const sa2_paged_problem *p, bool simplicial) {
     if (simplicial && (p->w1 < 1 || p->w2 < 1)) return fail_with(SA2_ERR_BAD_SHAPE, "windows w1=%d w2=%d must be >= 1", p->w1, p->w2);
     if (!(p->scale > 0.f) || !std::isfinite(p->scale)) return fail_with(SA2_ERR_BAD_SHAPE, "scale must be positive and finite");
     if (p->max_length < 0) return fail_with(SA2_ERR_BAD_SHAPE, "max_length=%d must be >= 0 (0: what the tables can name)", p->max_length);
-    if ((int64_t)p->batch * p->rows * p->heads > 0x3ffffffll) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
+    if (!product_within(p->batch, p->rows, p->heads, 0x3ffffff)) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
     return SA2_OK;
 }
 

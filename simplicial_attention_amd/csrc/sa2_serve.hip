@@ -69,8 +69,9 @@ int sa2_paged_append(const sa2_paged_problem *p, const sa2_append_item *items, i
     k.dim = p->dim_head;
     k.pieces = p->pool_dim / 8;
     k.count = count;
+    if (p->kv_heads > (1 << 24) || !product_within(p->batch, p->rows, (int64_t)p->kv_heads * k.pieces, kMostGroups * 256))
+        return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
     const int64_t threads = (int64_t)p->batch * p->rows * p->kv_heads * k.pieces;
-    if (p->kv_heads > (1 << 24) || (threads + 255) / 256 > kMostGroups) return fail_with(SA2_ERR_BAD_SHAPE, "problem too large for a 1-D grid");
     const dim3 grid((unsigned)((threads + 255) / 256));
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);
     if (plain) hipLaunchKernelGGL(paged_append_kernel<true>, grid, dim3(256), 0, s, k, src_type, p->dtype);
@@ -139,7 +140,7 @@ int sa2_copy_pages(const sa2_page_pool *pools, int32_t count, const int32_t *pai
 }
 
 int64_t sa2_sample_workspace_bytes(int64_t rows, int64_t vocab) {
-    if (rows < 1 || vocab < 1 || vocab > (1 << 24)) return -1;
+    if (rows < 1 || rows > 0x7fffffff || vocab < 1 || vocab > (1 << 24)) return -1;
     const int64_t chunks = (vocab + kSampleChunk - 1) / kSampleChunk;
     return chunks == 1 ? 0 : rows * chunks * (int64_t)(sizeof(SampleRecord) + 4 * kSampleThreads);
 }
