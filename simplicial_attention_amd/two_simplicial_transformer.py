@@ -159,7 +159,10 @@ class TwoSimplicialLM(nn.Module):
 
     @torch.no_grad()
     def logits_cached(self, x, cache, batch, rows=None):
-        """Logits of new tokens (b, n) whose places ``batch = cache.extend(...)`` has made; ``rows`` (b,): of that row of each sequence alone, (b, num_tokens)."""
+        """Logits of new tokens (b, n) whose places ``batch = cache.extend(...)`` has made; ``rows`` (b,): of that row of each sequence alone, (b, num_tokens).
+        Sequences longer than the table of positions are refused."""
+        if batch.max_length > self.pos_emb.num_embeddings:
+            raise ValueError(f'a sequence of {batch.max_length} tokens, positions reach {self.pos_emb.num_embeddings}')
         at = (batch.lengths - batch.counts)[:, None] + torch.arange(x.shape[1], device=x.device)
         # (padding reads some row of the table)
         hidden = self.transformer.forward_cached(self.token_emb(x) + self.pos_emb(at.clamp(0, self.pos_emb.num_embeddings - 1)), cache, batch)
