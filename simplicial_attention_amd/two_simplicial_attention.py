@@ -182,7 +182,7 @@ class SlidingWindowTwoSimplicialMHA(HigherOrderAttention):
     @torch.no_grad()
     def forward_cached(self, tokens, keys, values, batch):
         """``forward`` for new tokens (b, n, dim) behind those in a paged cache: ``keys`` and ``values`` are the layer's two pools each, ``batch`` says
-        where the rows go (:meth:`PagedCache.extend`).  Rows beyond ``batch.counts`` are padding."""
+        where the rows go (:meth:`PagedCache.extend`).  Rows beyond ``batch.counts`` are padding.  Queries, keys and values are rounded to the pools' dtype."""
         from .paged import paged_append, paged_two_simplicial_attn
 
         def attend(q, k, v):

@@ -55,7 +55,8 @@ class Attention(nn.Module):
     @torch.no_grad()
     @torch.jit.unused
     def forward_cached(self, x, keys, values, batch):
-        """``forward`` for new tokens (b, n, dim) behind those in a paged cache: the layer's key and value pool (tuples of one), and where the rows go."""
+        """``forward`` for new tokens (b, n, dim) behind those in a paged cache: the layer's key and value pool (tuples of one), and where the rows go.  Queries, keys and
+        values are rounded to the pools' dtype."""
         b, n, _ = x.shape
         x = self.prenorm(x)
         q = self.to_q(x).view(b, n, self.heads, self.dim_head)
@@ -125,7 +126,8 @@ class TwoSimplicialTransformer(nn.Module):
 
     @torch.no_grad()
     def forward_cached(self, x, cache, batch):
-        """The stack for new tokens (b, n, dim) whose places ``batch = cache.extend(...)`` has made; rows beyond ``batch.counts`` are padding."""
+        """The stack for new tokens (b, n, dim) whose places ``batch = cache.extend(...)`` has made; rows beyond ``batch.counts`` are padding.  Queries, keys and values are
+        rounded to the cache's dtype."""
         for (attn, ff), keys, values in zip(self.layers, cache.keys, cache.values):
             x = x + attn.forward_cached(x, keys, values, batch)
             x = x + ff(x)
@@ -171,12 +173,15 @@ class TwoSimplicialLM(nn.Module):
         return self.to_logits(hidden)
 
     @torch.no_grad()
-    def generate(self, prompts, steps, *, lengths=None, samples=1, temperature=1., top_k=0, top_p=1., min_p=0., generator=None, chunk=512, page_size=64):
+    def generate(self, prompts, steps, *, lengths=None, samples=1, temperature=1., top_k=0, top_p=1., min_p=0., generator=None, chunk=512, page_size=64, dtype=None):
         """``steps`` tokens behind every prompt: prompts (b, n) -> (b, samples, steps) tokens and their log-probabilities.
 
         ``lengths``: tokens of each prompt (host numbers), the others of its row being padding; by default all are prompt.  Prompts are read in chunks of ``chunk`` tokens into a
         paged cache, once for all of a prompt's ``samples``, which share its pages.  Tokens are drawn by :func:`sample_tokens` with uniform
         numbers from ``generator``.
+
+        ``dtype``: of the cache, bfloat16 or float16 (by default the weights', bfloat16 for float32 ones).  Queries, keys and values are rounded to it, those of float32 weights
+        to 8 or 11 bits, of which ``forward`` rounds the 2-simplicial layers' alone (to bfloat16).
         """
         b, n = prompts.shape
         lengths = [n] * b if lengths is None else [int(length) for length in lengths]
@@ -186,7 +191,7 @@ class TwoSimplicialLM(nn.Module):
             raise ValueError(f'{max(lengths)} + {steps} tokens, positions reach {self.pos_emb.num_embeddings}')
         shared = sum(-(-length // page_size) for length in lengths)
         own = samples * sum(-(-(length + steps) // page_size) - length // page_size for length in lengths)
-        cache = self.transformer.cache(shared + own, page_size)
+        cache = self.transformer.cache(shared + own, page_size, dtype)
         sequences = [cache.new() for _ in range(b)]
         first = None
         for start in range(0, max(lengths), chunk):
