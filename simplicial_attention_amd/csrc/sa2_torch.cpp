@@ -639,9 +639,12 @@ void copy_pages(const std::vector<Tensor> &pools, const Tensor &pairs_in) {
         if (!contiguous) raise(PyExc_ValueError, "a page must be contiguous: " + shape_text(t));
         items.push_back({t.data_ptr(), t.size(0) > 1 ? t.stride(0) * (int64_t)t.element_size() : bytes, bytes, t.size(0)});
     }
-    const Tensor wide = pairs_in.to(at::kLong);      // (unsigned numbers beyond its range become negative ones)
-    if (wide.numel() > 0 && (wide.max().item<int64_t>() > INT32_MAX || wide.min().item<int64_t>() < 0)) raise(PyExc_ValueError, "pairs name pages that do not exist");
-    const Tensor pairs = wide.to(at::kInt).contiguous();
+    Tensor pairs = pairs_in;
+    if (pairs_in.element_size() > 2 && pairs_in.scalar_type() != at::kInt && pairs_in.numel() > 0) {
+        pairs = pairs_in.to(at::kLong);              // (unsigned numbers beyond its range become negative ones)
+        if (pairs.max().item<int64_t>() > INT32_MAX || pairs.min().item<int64_t>() < 0) raise(PyExc_ValueError, "pairs name pages that do not exist");
+    }
+    pairs = pairs.to(at::kInt).contiguous();
     const c10::DeviceGuard guard(pools[0].device());
     check(sa2_copy_pages(items.data(), (int32_t)items.size(), static_cast<const int32_t *>(pairs.data_ptr()), pairs.size(0), stream_of(pools[0])));
 }
