@@ -886,7 +886,8 @@ struct ManyCfg {
     static constexpr int BUF = 2 * RT::BYTES;                       // a K tile and a V tile
     static constexpr int NBUF = D == 256 ? 2 : 4;
     static constexpr bool AHEAD = NBUF == 4;                        // the next tile has landed while a tile is used
-    static constexpr int WPE = D == 256 ? 1 : D == 128 ? 2 : D == 64 && !SIMP ? 3 : 4;     // waves per SIMD
+    static constexpr int WPE = D == 256 ? 1 : D == 128 ? 2 : D == 64 ? 3 : 4;     // waves per SIMD that the registers allow
+    static constexpr int WPE_PACKED = D == 64 ? 2 : WPE;
     static constexpr int FW = D == 128 ? 4 : 2;
     static constexpr int RING = NBUF * BUF;
     static_assert(RING - RT::CP < 65536, "the LDS address of a direct load travels in 16 bits of M0");
@@ -899,7 +900,7 @@ struct ManyCfg {
 // PACKED (2-simplicial, many units with second windows up to 16): a wave has 32 / width (token, head) units of `width` columns each, width the power of two that holds
 // the window
 template <class E, int D, bool SIMP, bool PACKED>
-__global__ __launch_bounds__((ManyCfg<D, SIMP>::NW * 64)) __attribute__((amdgpu_waves_per_eu(ManyCfg<D, SIMP>::WPE, ManyCfg<D, SIMP>::WPE))) void
+__global__ __launch_bounds__((ManyCfg<D, SIMP>::NW * 64)) __attribute__((amdgpu_waves_per_eu(PACKED ? ManyCfg<D, SIMP>::WPE_PACKED : ManyCfg<D, SIMP>::WPE, PACKED ? ManyCfg<D, SIMP>::WPE_PACKED : ManyCfg<D, SIMP>::WPE))) void
 paged_many_kernel(PagedParams p) {
     using C = ManyCfg<D, SIMP>;
     using RT = DmaTile<D>;
