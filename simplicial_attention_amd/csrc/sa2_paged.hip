@@ -66,7 +66,9 @@ Plan plan_of(const sa2_paged_problem *p, bool simplicial) {
     x.dblocks = simplicial ? (int)(((p->w2 < reach ? p->w2 : reach) + 31) / 32) : 1;
     const int waves = x.dim == 256 || simplicial ? 4 : 8;
     // 2-simplicial: a workgroup per (token, head) while all of them run at once, else units that share their keys (one sequence, 8 heads of 64 channels, w1 512,
-    // w2 32: 64 tokens 14.5 and 16.6 us, 128 tokens 26.3 and 16.7; four sequences of 128 channels: 16 tokens 20.3 and 22.7, 64 tokens 75 and 30)
+    // w2 32: 64 tokens 14.5 and 16.6 us, 128 tokens 26.3 and 16.7; four sequences of 128 channels: 16 tokens 20.3 and 22.7, 64 tokens 75 and 30).  One token of many sequences follows the
+    // same rule, though its workgroups have waves without a unit where a group has fewer heads than they have waves (64 sequences, w1 512, w2 32: 16 heads on 8, 64 channels 35.3
+    // and 18.4, 128 channels 51.4 and 31.4; 16 heads on 16, 64 channels 38.7 and 35.1, 128 channels 59.9 and 61.6; 16 on 4, 128 channels 43.3 and 27.7)
     // Second windows up to 16 leave columns of a wave to other units: taken where there are more units than 256 workgroups of a unit per wave hold (8 heads, w1 512,
     // unit per wave and packed: four sequences of 1024 tokens, 128 channels, w2 16, 8 and 4: 433, 393, 387 and 244, 130, 72 us; one of 128 tokens, 64 channels,
     // w2 8: 15.7 and 16.5)

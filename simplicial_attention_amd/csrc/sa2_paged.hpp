@@ -9,12 +9,13 @@
 //                o = sum over columns of v2[p - d] * O, so the 32 offsets of a token share its window and one product does them all
 // Softmax: the reference M of a column moves only when a tile's weights outgrow 2^60 (fp16: 2^14) on it, the first tile included
 // (M starts far below every logit), so the ordinary tile has no maximum and no rescale.  Sums and accumulators are fp32; the weights
-// are rounded to the element type for the second product; c q * k2 enters the first in two parts of that type (rounded to one, its error
+// are rounded to the element type for the second product, as the training kernels round theirs (in two parts they would double its length; with it the error is 2.3e-3 of the
+// result in bf16 and 2.9e-4 in fp16, where rounding nothing but the result gives 1.7e-3 and 2.1e-4); c q * k2 enters the first in two parts of that type (rounded to one, its error
 // would be the largest of the output's; the logits' products double).  Where fp16 does not hold a product, both parts of its column are divided by powers of two and
 // its wave walks by plain steps; what is infinite or no number stays so.
 //
 // Keys that are not there (beyond the walked range, missing pages) are fetched from a row of zeros and masked; a value row that a
-// column does not attend never reaches it, whatever it holds (0 * NaN is not 0: see value_products).
+// column does not attend never reaches it, whatever it holds (0 * NaN is not 0: see PagedWave::values).
 #pragma once
 
 #include "sa2_common.hpp"
@@ -237,7 +238,8 @@ struct PagedWave : WideProducts<TWO && E::kNarrow> {
         if constexpr (IN_PLACE) E::mfma_in_place(O[dt], v, w);
         else O[dt] = E::mfma(v, w, O[dt]);
     }
-    // behind in-place products, in front of whatever else reads or copies the accumulators (18 wait states behind an MFMA of 16 passes)
+    // behind in-place products, in front of whatever else reads or copies the accumulators: 18 wait states (a product of 32 x 32 x 16 takes 8 passes, behind which the
+    // compiler leaves 12 of them; the others are a margin)
     __device__ __forceinline__ void settle() {
         if constexpr (IN_PLACE) {
 #pragma unroll
@@ -636,7 +638,8 @@ struct SimplicialColumns {
 //
 // Bound by the cache's bytes: one token of 16 sequences of up to 32768, 16 heads on 4 of 128 channels (602 MB) 131 us with its merge, 4.6 TB/s where a copy of 2 GiB
 // reaches 4.9.  The smallest calls are bound by a chain of dependent loads (length, table, rows): 5.8 us for one token over 300 rows, 10.3 for one 2-simplicial
-// token, whose second rows come in front of its keys; an empty launch takes 3.6.
+// token, whose second rows come in front of its keys; an empty launch takes 3.6.  Several tokens (MIXED; their masks differ by column) spill registers outside the
+// products, 42 at 64 channels and 19 at 128: 4 tokens of 16 sequences of 8192, 16 heads on 4 of 128 channels 66 us at a floor of 54; 8 heads on 4 of 64 channels 32 at 27.
 template <int D>
 struct FewCfg {
     using RT = DmaTile<D>;
@@ -876,7 +879,7 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
 //
 // Bound by instruction issue of two waves per SIMD.  Dense, 128 channels: 2048 tokens of 16 heads over 32768 keys 495 to 533 us by card (532 GFLOP, 1.0 to 1.07 PFLOP/s where a
 // large product of the library reaches 1.27), the matrix unit busy 54 % of the time; a step issues 16 products, 62 other vector instructions and 16 exponentials, which with
-// their issue times fill nine tenths of it.  2-simplicial: 4 x 1024 tokens, 8 heads, w1 512, w2 32 429 to 449 us (276 GFLOP, and half of its logits' 138 again for the second part of
+// their issue times fill nine tenths of it.  2-simplicial: 4 x 1024 tokens, 8 heads, w1 512, w2 32 424 to 449 us (276 GFLOP, and its logits' 138 again for the second part of
 // the operand); its windows are short, so of a wave's 3400 vector instructions 2000 stand in front of and behind the walk.
 // Tried and taken back: the two waves of a SIMD half a step apart by a second barrier (499 -> 581 us).
 template <int D, bool SIMP>

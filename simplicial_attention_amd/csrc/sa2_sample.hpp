@@ -12,7 +12,8 @@
 // of the sixteens bound the kept prefix so closely that the races of a filtered row, and its random numbers, are looked up for few tokens.
 // Measured: 8 rows of 256 tokens 6.3 us (one launch); 96 rows of 100000, half of them with min-p, all with top-k and top-p, 30 us: 12 for the reading (19 MB: the chip
 // is filled by 600 workgroups that read once) and 18 for a chain of reductions over a workgroup (top, bound, races).  A flat row without top-k holds thousands of kept tokens,
-// which its workgroup reads again in every race: 45 to 50 us.
+// which its workgroup reads again in every race: 45 to 50 us.  Without filters the random numbers are read as well: 96 rows of 100000 in bf16 20 us (floor 12), 8 rows of 131072
+// in fp32 9.
 // Weights are exp2 of log2 units: exp2, log2 and reciprocals are single instructions, exact to an ulp.
 #pragma once
 

@@ -23,8 +23,8 @@ def paged_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, tables: Tensor, leng
     """Dense causal attention of a chunk of new tokens over a paged cache that holds them already: q (b, n, h, d) -> (b, n, h, d).
 
     Query head h reads key/value head ``h // (h_q / h_kv)``.  q and the pools share one dtype, bfloat16 or float16; the pools have d channels, or more if
-    those beyond d are zero.  Rows that attend to nothing, padding among them, are zero.  ``max_length``: no sequence is longer (it saves launching work for what the
-    tables could name; a wrong value costs time, not correctness).
+    those beyond d are zero.  Softmax weights are rounded to that dtype for their product with the values; sums are float32.  Rows that attend to nothing, padding among them,
+    are zero.  ``max_length``: no sequence is longer (it saves launching work for what the tables could name; a wrong value costs time, not correctness).
     """
     return _native.torch_ext().paged_attend(q, [k_pages], [v_pages], tables, lengths, counts, 1, 1, scale, max_length)
 
