@@ -8,7 +8,7 @@
 //   2-simplicial column = offset d = p - k of ONE (token, query head):  A = c q * k2[p - d] (the chain of products starts from -M), keys (p - w1, p] of the first set,
 //                o = sum over columns of v2[p - d] * O, so the 32 offsets of a token share its window and one product does them all
 // Softmax: the reference M of a column moves only when a tile's weights outgrow 2^60 (fp16: 2^14) on it, the first tile included
-// (M starts far below every logit), so the ordinary tile has no maximum and no rescale.  Sums and accumulators are fp32; the weights
+// (M starts at the lowest number), so the ordinary tile has no maximum and no rescale.  Sums and accumulators are fp32; the weights
 // are rounded to the element type for the second product, as the training kernels round theirs (in two parts they would double its length; with it the error is 2.3e-3 of the
 // result in bf16 and 2.9e-4 in fp16, where rounding nothing but the result gives 1.7e-3 and 2.1e-4); c q * k2 enters the first in two parts of that type (rounded to one, its error
 // would be the largest of the output's; the logits' products double).  Where fp16 does not hold a product, both parts of its column are divided by powers of two and
@@ -97,7 +97,15 @@ struct PagedParams {
     int2 *shares;                             // (not even) of a sequence: its first place, their number
 };
 
-constexpr float kNoRef = -1e30f;              // reference of a column that has met no key yet
+constexpr float kNoRef = -3.402823466e38f;    // reference of a column that has met no key yet
+// Beyond it (log2 units) a reference is a logit rounded so far that what is formed relative to it, by a chain of products or a fused multiplication, shows it: logits are
+// formed and rounded as the reference was, and it is subtracted then
+constexpr float kFarRef = 1048576.f;
+// c times a logit, rounded: not fused into what is subtracted from it
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
 __device__ __attribute__((aligned(16))) uint32_t g_paged_zero_row[128];
 
 // One direct-to-LDS load of 16 bytes per lane from addresses of its own (load_to_lds16 with 64-bit lane addresses)
@@ -202,7 +210,7 @@ struct WideProducts<true> {
 
 // ---- one wave's 32 columns
 // TWO: the operand of the logits in two parts (q * k2 has twice the digits of an element: rounded to one part it would double the error of
-// the output, in two it is exact)   IN_PLACE: value products by mfma_in_place
+// the output, in two its error is 2^-17 of it)   IN_PLACE: value products by mfma_in_place
 template <class E, int D, bool TWO, bool IN_PLACE = false>
 struct PagedWave : WideProducts<TWO && E::kNarrow> {
     using RT = DmaTile<D>;
@@ -273,7 +281,8 @@ struct PagedWave : WideProducts<TWO && E::kNarrow> {
         for (int kk = 0; kk < KS; ++kk) S = logit(RT::row_frag(k_lane, kk), kk, S);
         return S;
     }
-    __device__ __forceinline__ bool no_reference() const { return wave_any(M == kNoRef); }
+    // some column has no reference yet, or a far one
+    __device__ __forceinline__ bool no_near_reference() const { return wave_any(fabsf(M) > kFarRef); }
 
     // keys a .. z of the tile at `tile`, bit j for key tile + j
     __device__ __forceinline__ static uint32_t keys_of(int tile, int a, int z) {
@@ -305,38 +314,44 @@ struct PagedWave : WideProducts<TWO && E::kNarrow> {
         }
     }
 
-    // weights of a tile, packed, and their sum; false (in every lane) if some column's outgrow its reference
+    // weights of a tile, packed, and their sum; false (in every lane) if some column's outgrow its reference.  (TWO: logits relative to the reference; else SCALED
+    // ones in log2 units, or products where every reference is near)
+    template <bool SCALED = false>
     __device__ __forceinline__ bool weights(const f32x16 &S, float c, u32x4 (&pb)[2], float &sum) const {
         sum = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-            const float e0 = fast_exp2(TWO ? S[r] : S[r] * c - M), e1 = fast_exp2(TWO ? S[r + 1] : S[r + 1] * c - M);
+            const float e0 = fast_exp2(TWO ? S[r] : SCALED ? S[r] - M : S[r] * c - M), e1 = fast_exp2(TWO ? S[r + 1] : SCALED ? S[r + 1] - M : S[r + 1] * c - M);
             sum += e0 + e1;
             pb[r >> 3][(r & 7) >> 1] = E::pack(e0, e1);
         }
         return !wave_any(!(sum < E::kBig));
     }
     // the column's largest logit of a tile (TWO: relative to what S is relative to)
-    __device__ __forceinline__ float top_of(const f32x16 &S, float c) const {
+    __device__ __forceinline__ float top_of(const f32x16 &S) const {
         float top = S[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, S[r]);
-        top = both_halves_max(top);
-        return TWO ? top : top * c;
+        return both_halves_max(top);
     }
     // Weights of a masked tile whatever the references are.  Columns without one take the tile's largest logit (they hold nothing yet; S of TWO is then
-    // relative to 0); where weights outgrow a reference, all move up to the tile's largest logits
+    // relative to 0, as it is beside a far reference); where weights outgrow a reference, all move up to the tile's largest logits.  (Dense logits are scaled before anything is taken from them: the largest
+    // one's weight is 1 whatever its size)
     __device__ __forceinline__ void any_weights(f32x16 &S, float c, bool fresh, u32x4 (&pb)[2], float &sum) {
+        if constexpr (!TWO) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[r] = rounded_product(S[r], c);
+        }
         if (fresh) {
-            const float top = fmaxf(kNoRef, top_of(S, c));
+            const float top = fmaxf(kNoRef, top_of(S));
             M = M == kNoRef ? top : M;
             if constexpr (TWO) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) S[r] -= M;
             }
         }
-        if (__builtin_expect(!weights(S, c, pb, sum), 0)) {
-            const float top = top_of(S, c), up = TWO ? fmaxf(top, 0.f) : fmaxf(top, M) - M, f = fast_exp2(-up);
+        if (__builtin_expect(!weights<true>(S, c, pb, sum), 0)) {
+            const float top = top_of(S), up = TWO ? fmaxf(top, 0.f) : fmaxf(top, M) - M, f = fast_exp2(-up);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -347,13 +362,13 @@ struct PagedWave : WideProducts<TWO && E::kNarrow> {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) S[r] -= up;
             }
-            weights(S, c, pb, sum);
+            weights<true>(S, c, pb, sum);
         }
     }
     // the plain form of a step
     template <bool ONE>
     __device__ __forceinline__ void step(const char *k_lane, const char *v_lane, float c, bool masked, bool guard, int tile, uint32_t there, int hf) {
-        const bool fresh = no_reference();
+        const bool fresh = no_near_reference();
         f32x16 S = logits(k_lane, fresh ? 0.f : M);
         if (masked) mask<ONE>(S, tile, there, hf);
         u32x4 pb[2];
@@ -639,7 +654,7 @@ struct SimplicialColumns {
 // Bound by the cache's bytes: one token of 16 sequences of up to 32768, 16 heads on 4 of 128 channels (602 MB) 131 us with its merge, 4.6 TB/s where a copy of 2 GiB
 // reaches 4.9.  The smallest calls are bound by a chain of dependent loads (length, table, rows): 5.8 us for one token over 300 rows, 10.3 for one 2-simplicial
 // token, whose second rows come in front of its keys; an empty launch takes 3.6.  Several tokens (MIXED; their masks differ by column) spill registers outside the
-// products, 42 at 64 channels and 19 at 128: 4 tokens of 16 sequences of 8192, 16 heads on 4 of 128 channels 66 us at a floor of 54; 8 heads on 4 of 64 channels 32 at 27.
+// products, 42 at 64 channels and 3 at 128: 4 tokens of 16 sequences of 8192, 16 heads on 4 of 128 channels 63 us at a floor of 54; 8 heads on 4 of 64 channels 32 at 27.
 template <int D>
 struct FewCfg {
     using RT = DmaTile<D>;
@@ -754,7 +769,7 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
                 const int tile = first_key + 32 * u, next = u + NW;
                 const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(seg[32 * (u - seg_a) + c] >= 0);
                 wait_loads<RT::NCH>();
-                const bool fresh = w.no_reference();
+                const bool fresh = w.no_near_reference();
                 f32x16 S = w.logits(kt + RT::row_lane(lane), fresh ? 0.f : w.M);
                 wait_lds_reads();
                 if (next < seg_z) request(0, next);
@@ -1057,7 +1072,7 @@ paged_many_kernel(PagedParams p) {
             }
             while (u < z) {
                 bool opened = false;      // the step is open already (its weights outgrew a reference)
-                if (C::AHEAD && u < m_z && start + 32 * u >= w.most_lo && !w.no_reference()) {
+                if (C::AHEAD && u < m_z && start + 32 * u >= w.most_lo && !w.no_near_reference()) {
                     const f32x16 from = splat16(-w.M);      // (2-simplicial: where the chains of products start)
                     const char *first = lds + (u & (NBUF - 1)) * C::BUF + k_lane;
 #pragma unroll
