@@ -79,7 +79,8 @@ class PagedCache:
             raise ValueError('a cache needs pages, and pages rows')
         if dtype not in (torch.bfloat16, torch.float16):
             raise TypeError(f'unsupported dtype {dtype}')
-        self.page_size, self.pages, self.device = page_size, pages, torch.device(device)
+        # (as a device of its own: 'cuda' alone is whichever is current)
+        self.page_size, self.pages, self.device = page_size, pages, torch.empty(0, device=device).device
         self.keys, self.values = [], []
         for sets, kv_heads, dim in layers:
             # (channels in whole 16-byte pieces; the rows are written before they are read, so nothing needs clearing)
