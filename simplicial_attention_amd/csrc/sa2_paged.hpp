@@ -892,9 +892,9 @@ __global__ __launch_bounds__(FewCfg<D>::NW * 64) __attribute__((amdgpu_waves_per
 // tile's K along the value chain (a scheduling fence behind every product keeps them there).  Steps that need a mask, two or three of a
 // walk, take the plain form of PagedWave.
 //
-// Bound by instruction issue of two waves per SIMD.  Dense, 128 channels: 2048 tokens of 16 heads over 32768 keys 495 to 533 us by card (532 GFLOP, 1.0 to 1.07 PFLOP/s where a
+// Bound by instruction issue of two waves per SIMD.  Dense, 128 channels: 2048 tokens of 16 heads over 32768 keys 491 to 533 us by card (532 GFLOP, 1.0 to 1.07 PFLOP/s where a
 // large product of the library reaches 1.27), the matrix unit busy 54 % of the time; a step issues 16 products, 62 other vector instructions and 16 exponentials, which with
-// their issue times fill nine tenths of it.  2-simplicial: 4 x 1024 tokens, 8 heads, w1 512, w2 32 424 to 449 us (276 GFLOP, and its logits' 138 again for the second part of
+// their issue times fill nine tenths of it.  2-simplicial: 4 x 1024 tokens, 8 heads, w1 512, w2 32 424 to 453 us (276 GFLOP, and its logits' 138 again for the second part of
 // the operand); its windows are short, so of a wave's 3400 vector instructions 2000 stand in front of and behind the walk.
 // Tried and taken back: the two waves of a SIMD half a step apart by a second barrier (499 -> 581 us).
 template <int D, bool SIMP>
