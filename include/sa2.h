@@ -367,6 +367,64 @@ int64_t sa2_sample_workspace_bytes(int64_t rows, int64_t vocab);     /* -1 witho
 int sa2_sample(const void *logits, int32_t type, int64_t rows, int64_t vocab, int64_t stride, const float *noise, int64_t noise_stride,
                const sa2_sample_params *params, int64_t *tokens, float *logprobs, void *workspace, int64_t workspace_bytes, void *hip_stream);
 
+/* ---- the training step around the attention: norm behind a residual's addition, optimizer ----
+ *
+ * total = round(x + residual), normed = round(total * rsqrt(mean(total^2) + eps) * weight), rows of `dim` channels (1 to 16384); without a residual
+ * (NULL) x itself is normalised and `total` is not written.  Sums are fp32; what is normalised is the rounded sum.  total has the residual's type, which is that of x or
+ * fp32; normed that of x.  x and residual may have any row stride (elements, innermost stride 1) and are aligned to their elements; outputs are
+ * contiguous.  weight NULL: ones.  rstd (fp32 [rows]) is for the backward, or NULL.  The counterpart in the reference is every
+ * `x = attn(x) + x` in front of an RMSNorm (two_simplicial_transformer.py:126-141). */
+typedef struct sa2_norm_problem {
+    int64_t rows;
+    int32_t dim;
+    int32_t x_type, residual_type, weight_type;      /* sa2_element */
+    float   eps;
+} sa2_norm_problem;
+int sa2_add_rms_norm(const sa2_norm_problem *prob, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const void *weight, void *normed,
+                     void *total, float *rstd, void *hip_stream);
+
+/* The same with `normed` as e4m3 values and fp32 scales, one per row (group 0; scales [rows]) or per `group` = 32, 64 or 128 channels
+ * (scales [rows][ceil(dim / group)]): scale = max(amax / 448, 2^-126), value = the nearest e4m3 to y / scale.  A group that holds no number has no number as its scale. */
+int sa2_add_rms_norm_8bit(const sa2_norm_problem *prob, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const void *weight, int32_t group,
+                          void *values, float *scales, void *total, void *hip_stream);
+
+/* Backward of sa2_add_rms_norm from the rows that were normalised (total, or x without a residual: residual_type is their type), rstd, and the gradients of normed and
+ * (NULL: none) of total.  dx (type of x) and dresidual (residual_type) are the same numbers, each written if not NULL; dweight (weight_type) is written,
+ * not added to, if not NULL, and needs the workspace (16-byte aligned, no clearing).  Sums over rows are in a fixed order. */
+int64_t sa2_add_rms_norm_bwd_workspace_bytes(const sa2_norm_problem *prob);     /* -1 if the problem is invalid */
+int sa2_add_rms_norm_bwd(const sa2_norm_problem *prob, const void *total, int64_t total_stride, const void *weight, const float *rstd, const void *dnormed,
+                         int64_t dnormed_stride, const void *dtotal, int64_t dtotal_stride, void *dx, void *dresidual, void *dweight, void *workspace, int64_t workspace_bytes,
+                         void *hip_stream);
+
+/* One step of AdamW (decoupled weight decay, no amsgrad) over `count` contiguous tensors, in place:
+ *   g = grad * *grad_scale     m = beta1 m + (1 - beta1) g     v = beta2 v + (1 - beta2) g^2
+ *   p = (1 - lr weight_decay) p - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * p is the fp32 master where there is one (the parameter is then its rounding), else the parameter.  bits 32: exp_avg and exp_avg_sq are fp32.  bits 8: exp_avg holds
+ * m and exp_avg_sq the root of v, both as e4m3 values times one fp32 scale per 256 consecutive elements (ceil(n / 256) of them), scale = max(amax / 448, 2^-126).
+ * They are rounded up with the probability that keeps the expectation: t = |value| / scale becomes ((bits(t) + (u << 4)) >> 20) - 960 from 2^-6 on and
+ * floor(512 t + u / 65536) below, at most 126, where u is the low (m) or high (root) half of mix(e ^ (mix(mix(step + 0x9e3779b9 (i + 1)) ^ seed) + 0x9e3779b9 (e >> 32))), i the
+ * tensor's place in the list, e the element, all modulo 2^32 and mix the finalizer of MurmurHash3; the root of a v above 0 gets a code of at least 1.
+ * step_at, lr_at, grad_scale: device memory, read by the kernels, or NULL: the number beside (no scaling of gradients).  The reference has no optimizer of its own. */
+typedef struct sa2_adamw_tensor {
+    void *param;
+    const void *grad;               /* the parameter's type */
+    void *exp_avg, *exp_avg_sq;
+    float *exp_avg_scales, *exp_avg_sq_scales;
+    float *master;                  /* or NULL */
+    int64_t n;
+    int32_t type;                   /* sa2_element of param and grad */
+    int32_t bits;                   /* of the states: 32 or 8 */
+} sa2_adamw_tensor;
+typedef struct sa2_adamw_step {
+    double beta1, beta2, eps, weight_decay, lr;
+    int64_t step;                   /* 1 for the first */
+    const int64_t *step_at;
+    const float *lr_at, *grad_scale;
+    uint32_t seed;
+} sa2_adamw_step;
+/* Refused: tensors of the list that share memory they are written in. */
+int sa2_adamw(const sa2_adamw_tensor *tensors, int64_t count, const sa2_adamw_step *step, void *hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,7 +34,8 @@ EXPORTS = ('sa2_version', 'sa2_last_error', 'sa2_supported', 'sa2_saved_t_bytes'
            'sa2_convert', 'sa2_qkv_norm_fwd', 'sa2_qkv_norm_bwd_workspace_bytes', 'sa2_qkv_norm_bwd',
            'sa2_wgrad_workspace_bytes', 'sa2_wgrad',
            'sa2_paged_attn_workspace_bytes', 'sa2_paged_attn', 'sa2_paged_simplicial_attn_workspace_bytes', 'sa2_paged_simplicial_attn',
-           'sa2_paged_append', 'sa2_copy_pages', 'sa2_sample_workspace_bytes', 'sa2_sample')
+           'sa2_paged_append', 'sa2_copy_pages', 'sa2_sample_workspace_bytes', 'sa2_sample',
+           'sa2_add_rms_norm', 'sa2_add_rms_norm_8bit', 'sa2_add_rms_norm_bwd_workspace_bytes', 'sa2_add_rms_norm_bwd', 'sa2_adamw')
 
 
 class Sa2Error(RuntimeError):
@@ -87,6 +88,21 @@ class SampleParams(ctypes.Structure):
         ('temperature_all', ctypes.c_float), ('top_p_all', ctypes.c_float), ('min_p_all', ctypes.c_float), ('top_k_all', ctypes.c_int32)]
 
 
+class NormProblem(ctypes.Structure):
+    _fields_ = [('rows', ctypes.c_int64), ('dim', ctypes.c_int32), ('x_type', ctypes.c_int32), ('residual_type', ctypes.c_int32), ('weight_type', ctypes.c_int32),
+                ('eps', ctypes.c_float)]
+
+
+class AdamwTensor(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ('param', 'grad', 'exp_avg', 'exp_avg_sq', 'exp_avg_scales', 'exp_avg_sq_scales', 'master')] + [
+        ('n', ctypes.c_int64), ('type', ctypes.c_int32), ('bits', ctypes.c_int32)]
+
+
+class AdamwStep(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_double) for name in ('beta1', 'beta2', 'eps', 'weight_decay', 'lr')] + [
+        ('step', ctypes.c_int64), ('step_at', ctypes.c_void_p), ('lr_at', ctypes.c_void_p), ('grad_scale', ctypes.c_void_p), ('seed', ctypes.c_uint32)]
+
+
 _lib = None
 _prof_lib = None
 _torch_ext = None
@@ -96,7 +112,7 @@ _lock = threading.Lock()
 def build(verbose: bool = False) -> str:
     """Compile libsa2.so for gfx950 (always recompiles)."""
     out = None if verbose else subprocess.DEVNULL
-    subprocess.check_call(['make', '-B', '-j4', '-C', _CSRC, 'libsa2.so', 'libsa2_prof.so', '_sa2_torch.so'], stdout=out, stderr=out)
+    subprocess.check_call(['make', '-B', '-j6', '-C', _CSRC, 'libsa2.so', 'libsa2_prof.so', '_sa2_torch.so'], stdout=out, stderr=out)
     return LIB_PATH
 
 
@@ -158,6 +174,17 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.sa2_sample_workspace_bytes.argtypes = [I64, I64]
     lib.sa2_sample.restype = ctypes.c_int
     lib.sa2_sample.argtypes = [V, ctypes.c_int32, I64, I64, I64, V, I64, ctypes.POINTER(SampleParams), V, V, V, I64, V]
+    N = ctypes.POINTER(NormProblem)
+    lib.sa2_add_rms_norm.restype = ctypes.c_int
+    lib.sa2_add_rms_norm.argtypes = [N, V, I64, V, I64, V, V, V, V, V]
+    lib.sa2_add_rms_norm_8bit.restype = ctypes.c_int
+    lib.sa2_add_rms_norm_8bit.argtypes = [N, V, I64, V, I64, V, ctypes.c_int32, V, V, V, V]
+    lib.sa2_add_rms_norm_bwd_workspace_bytes.restype = I64
+    lib.sa2_add_rms_norm_bwd_workspace_bytes.argtypes = [N]
+    lib.sa2_add_rms_norm_bwd.restype = ctypes.c_int
+    lib.sa2_add_rms_norm_bwd.argtypes = [N, V, I64, V, V, V, I64, V, I64, V, V, V, V, I64, V]
+    lib.sa2_adamw.restype = ctypes.c_int
+    lib.sa2_adamw.argtypes = [ctypes.POINTER(AdamwTensor), I64, ctypes.POINTER(AdamwStep), V]
     return lib
 
 

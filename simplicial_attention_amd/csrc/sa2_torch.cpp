@@ -3,41 +3,16 @@
 // for a forward and backward, which is what small calls then cost whatever the kernels do.)
 //
 // Bound to Python as the module _sa2_torch; two_simplicial_attention.py, qkv_norm.py, linear.py, paged.py and sampling.py are its callers.
-#include <torch/extension.h>
-
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/DeviceGuard.h>
-
 #include <array>
 #include <atomic>
 
-#include "sa2.h"
-
-namespace py = pybind11;
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
+#include "sa2_torch.hpp"
 
 namespace {
 
 constexpr int kMostDevices = 64;
 // bytes of saved partials that have died, per device (the budget in Python subtracts them from what it admitted)
 std::array<std::atomic<int64_t>, kMostDevices> g_released{};
-
-void check(int status) {
-    if (status == SA2_OK) return;
-    // the exception class of the package (Sa2Error) is raised by its own check function
-    py::gil_scoped_acquire gil;
-    py::module_::import("simplicial_attention_amd._native").attr("check_failed")(status, std::string(sa2_last_error()));
-}
-
-[[noreturn]] void raise(PyObject *type, const std::string &text) {
-    py::gil_scoped_acquire gil;
-    PyErr_SetString(type, text.c_str());
-    throw py::error_already_set();
-}
-
-void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
 
 sa2_tensor arg(const Tensor &t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
 
@@ -46,15 +21,6 @@ Tensor aligned(const Tensor &t) {
     const bool ok = t.stride(3) == 1 && (t.size(1) == 1 || t.stride(1) <= SA2_MOST_STRIDE_N) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
                     t.stride(2) % 8 == 0;
     return ok ? t : t.clone(at::MemoryFormat::Contiguous);
-}
-
-int element_of(const Tensor &t) {
-    switch (t.scalar_type()) {
-        case at::kBFloat16: return SA2_ELEMENT_BF16;
-        case at::kHalf: return SA2_ELEMENT_F16;
-        case at::kFloat: return SA2_ELEMENT_F32;
-        default: return -1;
-    }
 }
 
 // Several conversions in one launch.
@@ -261,14 +227,6 @@ Geometry geometry_of(const Tensor &q, const Tensor &k1, const Tensor &v1, int64_
     return g;
 }
 
-// a call that autograd has to see: a backward may follow, or an input carries a forward-mode tangent (which the node refuses,
-// also without a graph: the derivative would be lost without a word)
-bool in_autograd(std::initializer_list<const Tensor *> inputs) {
-    for (const Tensor *t : inputs)
-        if ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined()) return true;
-    return false;
-}
-
 Tensor attend(const Tensor &q, const Tensor &k1, const Tensor &k2, const Tensor &v1, const Tensor &v2, const Geometry &g, const py::object &admit) {
     if (!in_autograd({&q, &k1, &k2, &v1, &v2})) return run_forward(q, k1, k2, v1, v2, g, nullptr).result;
     return Attend::apply(q, k1, k2, v1, v2, g, admit);
@@ -440,14 +398,6 @@ MaybeTensors qkv_norm_backward(const MaybeTensors &saved, const std::vector<int6
     return maybe(QKVNorm::run_backward(defined(saved), sizes, douts));
 }
 
-// batched tensors (vmap's and is_grads_batched's), functorch's wrappers, subclasses with a dispatch of their own and
-// forward-mode tangents: a kernel launched on their data pointers would miss what they carry
-bool foreign(const Tensor &t) {
-    static const c10::DispatchKeySet keys({c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-                                           c10::DispatchKey::Python, c10::DispatchKey::Functionalize});
-    return t.key_set().has_any(keys) || t._fw_grad(0).defined();
-}
-
 // ---- linear layer whose weight gradient is this library's kernel (the products with the weight stay torch's)
 struct Linear : public torch::autograd::Function<Linear> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const std::optional<Tensor> &bias) {
@@ -491,13 +441,6 @@ Tensor linear(const Tensor &x, const Tensor &w, const std::optional<Tensor> &bia
 }
 
 // ---- serving: paged caches and sampling (no gradients: a call that autograd would have to see is refused)
-void refuse_autograd(const char *what, std::initializer_list<const Tensor *> inputs) {
-    for (const Tensor *t : inputs)
-        if (in_autograd({t}) || foreign(*t)) raise(PyExc_RuntimeError, std::string(what) + " has no derivative and takes plain tensors: call it under torch.no_grad()");
-}
-
-std::string shape_text(const Tensor &t) { return std::string(py::str(py::cast(t.sizes().vec()))); }
-
 // int32 vectors and tables that the kernels read
 void check_index(const Tensor &t, const Tensor &q, const char *name, int64_t dims, int64_t rows) {
     if (t.scalar_type() != at::kInt) raise(PyExc_TypeError, std::string(name) + " must be int32");
@@ -713,5 +656,6 @@ PYBIND11_MODULE(_sa2_torch, m) {
     m.def("paged_append", &paged_append);
     m.def("copy_pages", &copy_pages);
     m.def("sample_tokens", &sample_tokens);
+    bind_training(m);
     m.def("released_bytes", [](int device) { return device >= 0 && device < kMostDevices ? g_released[device].load() : int64_t(0); });
 }

@@ -1,0 +1,298 @@
+// Host path of the operators of a training step: the norm behind a residual's addition, and the optimizer.
+// Callers: rms_norm.py, adamw.py.
+#include <array>
+
+#include "sa2_torch.hpp"
+
+namespace {
+
+void refuse_foreign(const char *what, std::initializer_list<const Tensor *> inputs) {
+    for (const Tensor *t : inputs)
+        if (t->defined() && foreign(*t)) raise(PyExc_RuntimeError, std::string(what) + " takes plain tensors (no batched, functionalised or forward-mode ones)");
+}
+
+// a backward that is itself recorded: its kernels have no derivative
+void refuse_second(const char *what) {
+    if (at::GradMode::is_enabled()) raise(PyExc_RuntimeError, std::string(what) + " has no second derivative: call its backward without create_graph");
+}
+
+// (..., dim) as rows of dim channels that lie `stride` elements apart, copied if they do not
+Tensor as_matrix(const Tensor &t, int64_t dim) {
+    if (t.dim() == 2 && (t.stride(1) == 1 || dim == 1)) return t;
+    bool rows = t.dim() >= 1 && (t.stride(-1) == 1 || dim == 1);
+    int64_t next = -1;                       // what the stride of the next dimension has to be (-1: any)
+    for (int64_t x = t.dim() - 2; rows && x >= 0; --x) {
+        if (t.size(x) == 1) continue;
+        rows = next < 0 || t.stride(x) == next;
+        next = t.stride(x) * t.size(x);
+    }
+    return rows ? t.view({-1, dim}) : t.contiguous().view({-1, dim});
+}
+
+int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// ---- norm behind a residual's addition
+using MaybeTensor = std::optional<Tensor>;
+
+struct NormCall {
+    Tensor x, residual, weight;              // matrices; residual and weight may be undefined
+    sa2_norm_problem prob{};
+    std::vector<int64_t> shape;
+};
+
+NormCall norm_call(const char *what, const Tensor &x, const MaybeTensor &residual, const MaybeTensor &weight, std::optional<double> eps) {
+    for (const Tensor *t : {&x, residual ? &*residual : nullptr, weight ? &*weight : nullptr}) {
+        if (!t) continue;
+        refuse_foreign(what, {t});
+        if (!t->is_cuda()) raise(PyExc_AssertionError, std::string(what) + " runs on the GPU only");
+        if (element_of(*t) < 0) raise(PyExc_TypeError, std::string(what) + " takes bfloat16, float16 and float32 tensors");
+        if (t->device() != x.device()) raise(PyExc_ValueError, std::string(what) + ": tensors on " + x.device().str() + " and " + t->device().str());
+    }
+    if (x.dim() < 1 || x.size(-1) < 1) raise(PyExc_ValueError, std::string(what) + ": rows without channels: " + shape_text(x));
+    const int64_t dim = x.size(-1);
+    if (residual && residual->sizes() != x.sizes()) raise(PyExc_ValueError, "residual " + shape_text(*residual) + " does not match " + shape_text(x));
+    if (residual && residual->scalar_type() != x.scalar_type() && residual->scalar_type() != at::kFloat)
+        raise(PyExc_TypeError, "the residual has the dtype of x, or float32");
+    if (weight && (weight->dim() != 1 || weight->size(0) != dim)) raise(PyExc_ValueError, "weight " + shape_text(*weight) + " does not match " + std::to_string(dim) + " channels");
+    const double e = eps ? *eps : (double)std::numeric_limits<float>::epsilon();
+    if (!(e >= 0) || std::isinf(e)) raise(PyExc_ValueError, "eps must be finite and not negative");
+    NormCall c;
+    c.shape = x.sizes().vec();
+    c.prob = {dim ? x.numel() / dim : 0, (int32_t)std::min<int64_t>(dim, INT32_MAX), element_of(x), element_of(residual ? *residual : x),
+              weight ? element_of(*weight) : SA2_ELEMENT_F32, (float)e};
+    const c10::DeviceGuard guard(x.device());
+    if (c.prob.rows > 0) {
+        c.x = as_matrix(x, dim);
+        if (residual) c.residual = as_matrix(*residual, dim);
+    }
+    if (weight) c.weight = weight->contiguous();
+    return c;
+}
+
+const void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+struct AddNorm : public torch::autograd::Function<AddNorm> {
+    // normed, and with a residual the sum; saved: the normalised rows, rstd and weight
+    static variable_list run(const NormCall &c, const Tensor &x, const MaybeTensor &residual, variable_list *saved) {
+        const c10::DeviceGuard guard(x.device());
+        const Tensor normed = at::empty(c.shape, x.options());
+        Tensor total, rstd;
+        if (residual) total = at::empty(c.shape, residual->options());
+        if (saved) rstd = at::empty({c.prob.rows}, x.options().dtype(at::kFloat));
+        if (c.prob.rows > 0)
+            check(sa2_add_rms_norm(&c.prob, c.x.data_ptr(), row_stride(c.x), ptr(c.residual), residual ? row_stride(c.residual) : 0, ptr(c.weight), normed.data_ptr(),
+                                   residual ? total.data_ptr() : nullptr, saved ? static_cast<float *>(rstd.data_ptr()) : nullptr, stream_of(x)));
+        if (saved) *saved = {residual ? total : x, rstd, c.weight};
+        variable_list out{normed};
+        if (residual) out.push_back(total);
+        return out;
+    }
+
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const MaybeTensor &residual, const MaybeTensor &weight, std::optional<double> eps) {
+        const NormCall c = norm_call("add_rms_norm", x, residual, weight, eps);
+        variable_list saved;
+        const variable_list out = run(c, x, residual, &saved);
+        ctx->save_for_backward(saved);
+        ctx->saved_data["types"] = c10::List<int64_t>({c.prob.x_type, c.prob.residual_type, c.prob.weight_type, (int64_t)residual.has_value()});
+        ctx->saved_data["eps"] = (double)c.prob.eps;
+        ctx->set_materialize_grads(false);
+        return out;
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list ups) {
+        refuse_second("add_rms_norm");
+        const variable_list s = ctx->get_saved_variables();
+        const auto types = ctx->saved_data["types"].toIntVector();
+        const bool has_residual = types[3] != 0;
+        const Tensor &rows = s[0], &rstd = s[1], &weight = s[2];
+        const Tensor up = ups[0], up_total = has_residual ? ups[1] : Tensor();
+        for (const Tensor *t : {&up, &up_total})
+            if (t->defined()) refuse_foreign("add_rms_norm", {t});
+        const c10::DeviceGuard guard(rows.device());
+        // (edges are counted over the tensors that were given)
+        const bool want_x = ctx->needs_input_grad(0), want_r = has_residual && ctx->needs_input_grad(1), want_w = weight.defined() && ctx->needs_input_grad(has_residual ? 2 : 1);
+        const auto x_type = types[0] == SA2_ELEMENT_F32 ? at::kFloat : types[0] == SA2_ELEMENT_F16 ? at::kHalf : at::kBFloat16;
+        variable_list grads(4);
+        if (!up.defined()) {                  // (the norm's output was not used)
+            if (up_total.defined()) {
+                if (want_x) grads[0] = up_total.to(x_type);
+                if (want_r) grads[1] = up_total;
+            }
+            return grads;
+        }
+        const int64_t dim = rows.size(-1), count = dim ? rows.numel() / dim : 0;
+        if (want_w) grads[2] = at::empty({dim}, weight.options());
+        if (count == 0) {
+            if (want_x) grads[0] = at::empty(rows.sizes(), rows.options().dtype(x_type));
+            if (want_r) grads[1] = at::empty(rows.sizes(), rows.options());
+            if (want_w) grads[2].zero_();
+            return grads;
+        }
+        const sa2_norm_problem prob{count, (int32_t)dim, (int32_t)types[0], (int32_t)types[1], (int32_t)types[2], (float)ctx->saved_data["eps"].toDouble()};
+        const bool same = prob.x_type == prob.residual_type;       // (one tensor is the gradient of both)
+        if (want_x || (want_r && same)) grads[0] = at::empty(rows.sizes(), rows.options().dtype(x_type));
+        if (want_r) grads[1] = same ? grads[0] : at::empty(rows.sizes(), rows.options());
+        const Tensor t = as_matrix(rows, dim), g = as_matrix(up, dim), gt = up_total.defined() ? as_matrix(up_total, dim) : Tensor();
+        Tensor ws;
+        const int64_t bytes = want_w ? sa2_add_rms_norm_bwd_workspace_bytes(&prob) : 0;
+        if (bytes > 0) ws = at::empty({bytes}, rows.options().dtype(at::kByte));
+        check(sa2_add_rms_norm_bwd(&prob, t.data_ptr(), row_stride(t), ptr(weight), static_cast<float *>(rstd.data_ptr()), g.data_ptr(), row_stride(g), ptr(gt),
+                                   gt.defined() ? row_stride(gt) : 0, const_cast<void *>(ptr(grads[0])), want_r && !same ? grads[1].data_ptr() : nullptr,
+                                   const_cast<void *>(ptr(grads[2])), const_cast<void *>(ptr(ws)), bytes, stream_of(rows)));
+        if (!want_x) grads[0] = Tensor();
+        return grads;
+    }
+};
+
+std::tuple<Tensor, Tensor> add_rms_norm(const Tensor &x, const MaybeTensor &residual, const MaybeTensor &weight, std::optional<double> eps) {
+    variable_list out;
+    if (in_autograd({&x, residual ? &*residual : &x, weight ? &*weight : &x})) {
+        out = AddNorm::apply(x, residual, weight, eps);
+    } else {
+        out = AddNorm::run(norm_call("add_rms_norm", x, residual, weight, eps), x, residual, nullptr);
+    }
+    return {out[0], residual ? out[1] : x};
+}
+
+std::tuple<Tensor, Tensor, Tensor> add_rms_norm_8bit(const Tensor &x, const MaybeTensor &residual, const MaybeTensor &weight, std::optional<double> eps, int64_t group) {
+    refuse_autograd("add_rms_norm_8bit", {&x, residual ? &*residual : &x, weight ? &*weight : &x});
+    const NormCall c = norm_call("add_rms_norm_8bit", x, residual, weight, eps);
+    if (group != 0 && group != 32 && group != 64 && group != 128) raise(PyExc_ValueError, "groups of " + std::to_string(group) + " channels: 32, 64, 128, or None for whole rows");
+    const c10::DeviceGuard guard(x.device());
+    auto shape = c.shape;
+    const Tensor values = at::empty(shape, x.options().dtype(at::kFloat8_e4m3fn));
+    shape.back() = group ? (c.prob.dim + group - 1) / group : 1;
+    const Tensor scales = at::empty(shape, x.options().dtype(at::kFloat));
+    Tensor total;
+    if (residual) total = at::empty(c.shape, residual->options());
+    if (c.prob.rows > 0)
+        check(sa2_add_rms_norm_8bit(&c.prob, c.x.data_ptr(), row_stride(c.x), ptr(c.residual), residual ? row_stride(c.residual) : 0, ptr(c.weight), (int32_t)group, values.data_ptr(),
+                                    static_cast<float *>(scales.data_ptr()), residual ? total.data_ptr() : nullptr, stream_of(x)));
+    return {values, scales, residual ? total : x};
+}
+
+// ---- AdamW
+const Tensor &tensor_of(const py::handle &h, const char *name) {
+    if (!THPVariable_Check(h.ptr())) raise(PyExc_TypeError, std::string(name) + " must be tensors");
+    return THPVariable_Unpack(h.ptr());
+}
+
+bool laid_out_alike(const Tensor &a, const Tensor &b) {
+    return a.sizes() == b.sizes() && ((a.is_contiguous() && b.is_contiguous()) || a.strides() == b.strides());
+}
+
+void adamw_step(const py::sequence &params, const py::sequence &grads, const py::sequence &averages, const py::sequence &squares, const std::optional<py::sequence> &masters,
+                const py::object &step, const py::object &lr, double beta1, double beta2, double eps, double weight_decay, const MaybeTensor &grad_scale, int64_t seed) {
+    const size_t count = params.size();
+    if (grads.size() != count || averages.size() != count || squares.size() != count || (masters && masters->size() != count))
+        raise(PyExc_ValueError, "as many gradients, states and masters as parameters are required");
+    std::vector<sa2_adamw_tensor> items;
+    std::vector<Tensor> alive, written;
+    items.reserve(count);
+    written.reserve(4 * count);
+    std::optional<at::Device> device;
+    auto on_device = [&](const Tensor &t) {
+        if (!t.is_cuda()) raise(PyExc_AssertionError, "adamw_step runs on the GPU only");
+        if (!device) device = t.device();
+        if (t.device() != *device) raise(PyExc_ValueError, "adamw_step: tensors on " + device->str() + " and " + t.device().str());
+        refuse_foreign("adamw_step", {&t});
+    };
+    for (size_t i = 0; i < count; ++i) {
+        const Tensor &p = tensor_of(params[i], "parameters");
+        Tensor g = tensor_of(grads[i], "gradients");
+        on_device(p);
+        on_device(g);
+        if (element_of(p) < 0 || g.scalar_type() != p.scalar_type()) raise(PyExc_TypeError, "parameters are bfloat16, float16 or float32, and gradients of the same dtype");
+        if (p.layout() != at::kStrided || g.layout() != at::kStrided || !p.is_non_overlapping_and_dense()) raise(PyExc_ValueError, "parameters and gradients must be dense: " + shape_text(p));
+        if (g.sizes() != p.sizes()) raise(PyExc_ValueError, "gradient " + shape_text(g) + " does not match its parameter's " + shape_text(p));
+        if (!laid_out_alike(p, g)) {
+            const c10::DeviceGuard guard(p.device());
+            const at::NoGradGuard no_grad;
+            g = at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g);
+            alive.push_back(g);
+        }
+        sa2_adamw_tensor t{};
+        t.param = p.data_ptr();
+        t.grad = g.data_ptr();
+        t.n = p.numel();
+        t.type = element_of(p);
+        written.push_back(p);
+        const bool eight = PyTuple_Check(py::object(averages[i]).ptr());
+        if (eight != (bool)PyTuple_Check(py::object(squares[i]).ptr())) raise(PyExc_TypeError, "both states of a parameter are tensors, or (values, scales) pairs");
+        t.bits = eight ? 8 : 32;
+        for (int which = 0; which < 2; ++which) {
+            const py::object state = which ? squares[i] : averages[i];
+            if (eight) {
+                const py::tuple pair = state;
+                if (pair.size() != 2) raise(PyExc_TypeError, "states in 8 bits are (values, scales) pairs");
+                const Tensor &values = tensor_of(pair[0], "states"), &scales = tensor_of(pair[1], "scales");
+                on_device(values);
+                on_device(scales);
+                if (values.scalar_type() != at::kFloat8_e4m3fn || scales.scalar_type() != at::kFloat) raise(PyExc_TypeError, "states in 8 bits are float8_e4m3fn values and float32 scales");
+                if (values.numel() != t.n || !values.is_contiguous() || scales.numel() != (t.n + 255) / 256 || !scales.is_contiguous())
+                    raise(PyExc_ValueError, "states " + shape_text(values) + " with scales " + shape_text(scales) + " do not match a parameter " + shape_text(p) + ": contiguous, one scale for 256 elements");
+                (which ? t.exp_avg_sq : t.exp_avg) = values.data_ptr();
+                (which ? t.exp_avg_sq_scales : t.exp_avg_scales) = static_cast<float *>(scales.data_ptr());
+                written.push_back(values);
+                written.push_back(scales);
+            } else {
+                const Tensor &values = tensor_of(state, "states");
+                on_device(values);
+                if (values.scalar_type() != at::kFloat) raise(PyExc_TypeError, "states are float32 tensors, or (values, scales) pairs in 8 bits");
+                if (!laid_out_alike(p, values)) raise(PyExc_ValueError, "state " + shape_text(values) + " is not laid out as its parameter " + shape_text(p));
+                (which ? t.exp_avg_sq : t.exp_avg) = values.data_ptr();
+                written.push_back(values);
+            }
+        }
+        if (masters && !py::object((*masters)[i]).is_none()) {
+            const Tensor &m = tensor_of((*masters)[i], "masters");
+            on_device(m);
+            if (m.scalar_type() != at::kFloat) raise(PyExc_TypeError, "masters are float32");
+            if (!laid_out_alike(p, m)) raise(PyExc_ValueError, "master " + shape_text(m) + " is not laid out as its parameter " + shape_text(p));
+            t.master = static_cast<float *>(m.data_ptr());
+            written.push_back(m);
+        }
+        items.push_back(t);
+    }
+    sa2_adamw_step s{};
+    s.beta1 = beta1;
+    s.beta2 = beta2;
+    s.eps = eps;
+    s.weight_decay = weight_decay;
+    s.seed = (uint32_t)seed;
+    if (THPVariable_Check(step.ptr())) {
+        const Tensor &t = THPVariable_Unpack(step.ptr());
+        on_device(t);
+        if (t.scalar_type() != at::kLong || t.numel() != 1) raise(PyExc_TypeError, "step is a number, or an int64 tensor of one");
+        s.step_at = static_cast<const int64_t *>(t.data_ptr());
+    } else {
+        s.step = step.cast<int64_t>();
+        if (s.step < 1) raise(PyExc_ValueError, "step counts from 1");
+    }
+    if (THPVariable_Check(lr.ptr())) {
+        const Tensor &t = THPVariable_Unpack(lr.ptr());
+        on_device(t);
+        if (t.scalar_type() != at::kFloat || t.numel() != 1) raise(PyExc_TypeError, "lr is a number, or a float32 tensor of one");
+        s.lr_at = static_cast<const float *>(t.data_ptr());
+    } else {
+        s.lr = lr.cast<double>();
+    }
+    if (grad_scale) {
+        on_device(*grad_scale);
+        if (grad_scale->scalar_type() != at::kFloat || grad_scale->numel() != 1) raise(PyExc_TypeError, "grad_scale is a float32 tensor of one number");
+        s.grad_scale = static_cast<const float *>(grad_scale->data_ptr());
+    }
+    if (items.empty()) return;
+    const c10::DeviceGuard guard(*device);
+    check(sa2_adamw(items.data(), (int64_t)items.size(), &s, c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device->index()).stream()));
+    // (a graph that saved one of these sees that it has changed)
+    for (const Tensor &t : written) t.unsafeGetTensorImpl()->bump_version();
+}
+
+}  // namespace
+
+void bind_training(py::module_ &m) {
+    m.def("add_rms_norm", &add_rms_norm);
+    m.def("add_rms_norm_8bit", &add_rms_norm_8bit);
+    m.def("adamw_step", &adamw_step);
+}

@@ -1,0 +1,41 @@
+"""The residual's addition and the RMSNorm behind it in one pass over the rows, with gradients, and with an output in 8 bits."""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from . import _native
+
+
+def add_rms_norm(x: Tensor, residual: Tensor | None = None, weight: Tensor | None = None, eps: float | None = None) -> tuple[Tensor, Tensor]:
+    """``total = x + residual`` and ``normed = rms_norm(total, weight, eps)`` over the last dimension: ``(normed, total)``, both differentiable.
+
+    What ``x = x + attn(x); y = norm(x)`` of a pre-normed stack computes, to the bit but for the order of the sums: total is rounded to its dtype (the
+    residual's: that of x, or float32 for a residual stream in 32 bits) and normalised as rounded, with float32 sums; normed has the dtype of x.  Without a residual total is x itself.
+    ``weight`` (dim,) may have a dtype of its own; ``eps=None`` is float32's, as in ``torch.nn.RMSNorm`` (which takes float32's for narrower inputs too).  bfloat16, float16 and float32 tensors
+    on the GPU of any strides, rows of up to 16384 channels.
+    """
+    return _native.torch_ext().add_rms_norm(x, residual, weight, eps)
+
+
+def add_rms_norm_8bit(x: Tensor, residual: Tensor | None = None, weight: Tensor | None = None, eps: float | None = None, *,
+                      group: int | None = None) -> tuple[Tensor, Tensor, Tensor]:
+    """:func:`add_rms_norm` with its first output as operands of an 8-bit product: ``(values, scales, total)``, for inference.
+
+    ``values`` are float8_e4m3fn, ``scales`` float32, one per row (..., 1), or with ``group`` 32, 64 or 128 one per so many channels (..., ceil(dim / group)):
+    scale = max(amax / 448, 2**-126) over the row or group, value = the nearest e4m3 to normed / scale (which is not rounded to x's dtype in between).  A group that holds a value
+    that is not a number has no number as its scale.
+    """
+    return _native.torch_ext().add_rms_norm_8bit(x, residual, weight, eps, 0 if group is None else group)
+
+
+def norm_behind(norm, x: Tensor, residual: Tensor | None) -> tuple[Tensor, Tensor]:
+    """``total = x + residual`` (x alone without one) and ``norm(total)`` of an ``nn.RMSNorm`` module: ``(normed, total)``.  Modules and tensors that the kernel does not cover
+    go through torch."""
+    weight = norm.weight if type(norm) is torch.nn.RMSNorm else None
+    if (weight is None or not x.is_cuda or x.shape[-1] > 16384 or norm.normalized_shape != (x.shape[-1],) or torch.is_autocast_enabled() or torch.compiler.is_compiling()
+            or torch.jit.is_tracing() or norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks
+            or weight.dtype != x.dtype or x.dtype not in (torch.bfloat16, torch.float16, torch.float32) or (residual is not None and residual.dtype != x.dtype)):
+        total = x if residual is None else residual + x
+        return norm(total), total
+    return add_rms_norm(x, residual, weight, norm.eps)
