@@ -1,6 +1,7 @@
 """MI355X-native sliding-window 2-simplicial attention (gfx950 HIP kernels behind the
 Python API of lucidrains/simplicial-attention for that one path)."""
 from .adamw import AdamW, adamw_step, state_8bit
+from .cross_entropy import linear_cross_entropy
 from .naive import naive_two_simplicial_attend, nth_order_attend, signed_determinant
 from .paged import OutOfPages, PagedBatch, PagedCache, copy_pages, paged_append, paged_attn, paged_two_simplicial_attn
 from .rms_norm import add_rms_norm, add_rms_norm_8bit
@@ -29,6 +30,7 @@ __all__ = [
     'paged_attn',
     'paged_two_simplicial_attn',
     'sample_tokens',
+    'linear_cross_entropy',
     'add_rms_norm',
     'add_rms_norm_8bit',
     'AdamW',

@@ -35,7 +35,8 @@ EXPORTS = ('sa2_version', 'sa2_last_error', 'sa2_supported', 'sa2_saved_t_bytes'
            'sa2_wgrad_workspace_bytes', 'sa2_wgrad',
            'sa2_paged_attn_workspace_bytes', 'sa2_paged_attn', 'sa2_paged_simplicial_attn_workspace_bytes', 'sa2_paged_simplicial_attn',
            'sa2_paged_append', 'sa2_copy_pages', 'sa2_sample_workspace_bytes', 'sa2_sample',
-           'sa2_add_rms_norm', 'sa2_add_rms_norm_8bit', 'sa2_add_rms_norm_bwd_workspace_bytes', 'sa2_add_rms_norm_bwd', 'sa2_adamw')
+           'sa2_add_rms_norm', 'sa2_add_rms_norm_8bit', 'sa2_add_rms_norm_bwd_workspace_bytes', 'sa2_add_rms_norm_bwd', 'sa2_adamw',
+           'sa2_linear_ce_workspace_bytes', 'sa2_linear_ce', 'sa2_linear_ce_bwd_workspace_bytes', 'sa2_linear_ce_bwd')
 
 
 class Sa2Error(RuntimeError):
@@ -91,6 +92,11 @@ class SampleParams(ctypes.Structure):
 class NormProblem(ctypes.Structure):
     _fields_ = [('rows', ctypes.c_int64), ('dim', ctypes.c_int32), ('x_type', ctypes.c_int32), ('residual_type', ctypes.c_int32), ('weight_type', ctypes.c_int32),
                 ('eps', ctypes.c_float)]
+
+
+class LinearCeProblem(ctypes.Structure):
+    _fields_ = [('rows', ctypes.c_int64), ('dim', ctypes.c_int32), ('vocab', ctypes.c_int32), ('dtype', ctypes.c_int32), ('reduction', ctypes.c_int32),
+                ('ignore_index', ctypes.c_int64)]
 
 
 class AdamwTensor(ctypes.Structure):
@@ -185,6 +191,14 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.sa2_add_rms_norm_bwd.argtypes = [N, V, I64, V, V, V, I64, V, I64, V, V, V, V, I64, V]
     lib.sa2_adamw.restype = ctypes.c_int
     lib.sa2_adamw.argtypes = [ctypes.POINTER(AdamwTensor), I64, ctypes.POINTER(AdamwStep), V]
+    C = ctypes.POINTER(LinearCeProblem)
+    for name in ('sa2_linear_ce_workspace_bytes', 'sa2_linear_ce_bwd_workspace_bytes'):
+        getattr(lib, name).restype = I64
+        getattr(lib, name).argtypes = [C]
+    lib.sa2_linear_ce.restype = ctypes.c_int
+    lib.sa2_linear_ce.argtypes = [C, V, I64, V, I64, V, V, V, V, V, V, I64, V]
+    lib.sa2_linear_ce_bwd.restype = ctypes.c_int
+    lib.sa2_linear_ce_bwd.argtypes = [C, V, I64, V, I64, V, V, V, V, V, V, V, V, I64, V]
     return lib
 
 

@@ -1,5 +1,5 @@
-// Host path of the operators of a training step: the norm behind a residual's addition, and the optimizer.
-// Callers: rms_norm.py, adamw.py.
+// Host path of the operators of a training step: the norm behind a residual's addition, the read-out layer's loss, and the optimizer.
+// Callers: rms_norm.py, cross_entropy.py, adamw.py.
 #include <array>
 
 #include "sa2_torch.hpp"
@@ -171,6 +171,116 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_8bit(const Tensor &x, const Mayb
     return {values, scales, residual ? total : x};
 }
 
+// ---- cross entropy of a read-out layer
+struct LinearCE : public torch::autograd::Function<LinearCE> {
+    // rows of whole 16-byte pieces: others are copied, with channels of zeros behind them
+    static Tensor pieces(const Tensor &t, int64_t dim) {
+        const Tensor m = as_matrix(t, dim);
+        const int64_t more = (8 - dim % 8) % 8;
+        if (more) return at::constant_pad_nd(m, {0, more}).contiguous();
+        const bool ok = reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 == 0 && (m.size(0) <= 1 || (m.stride(0) % 8 == 0 && m.stride(0) >= 0 && m.stride(0) <= SA2_LINEAR_CE_MOST_STRIDE));
+        return ok ? m : m.clone(at::MemoryFormat::Contiguous);
+    }
+
+    struct Call {
+        Tensor hidden, weight, targets;
+        sa2_linear_ce_problem prob{};
+        int64_t dim = 0;
+    };
+
+    static Call checked(const Tensor &hidden, const Tensor &weight, const Tensor &targets, int64_t ignore_index, int64_t reduction) {
+        for (const Tensor *t : {&hidden, &weight, &targets}) {
+            refuse_foreign("linear_cross_entropy", {t});
+            if (!t->is_cuda()) raise(PyExc_AssertionError, "linear_cross_entropy runs on the GPU only");
+            if (t->device() != hidden.device()) raise(PyExc_ValueError, "linear_cross_entropy: tensors on " + hidden.device().str() + " and " + t->device().str());
+        }
+        if ((hidden.scalar_type() != at::kBFloat16 && hidden.scalar_type() != at::kHalf) || weight.scalar_type() != hidden.scalar_type())
+            raise(PyExc_TypeError, "hidden and weight must share one dtype out of bfloat16 and float16");
+        if (targets.scalar_type() != at::kLong && targets.scalar_type() != at::kInt) raise(PyExc_TypeError, "targets must be int64 or int32");
+        if (weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1 || hidden.dim() < 1 || hidden.size(-1) != weight.size(1))
+            raise(PyExc_ValueError, "hidden " + shape_text(hidden) + " does not match weight " + shape_text(weight));
+        if (targets.sizes() != hidden.sizes().slice(0, hidden.dim() - 1)) raise(PyExc_ValueError, "targets " + shape_text(targets) + " do not match hidden " + shape_text(hidden));
+        Call c;
+        c.dim = hidden.size(-1);
+        c.prob = {targets.numel(), (int32_t)std::min<int64_t>((c.dim + 7) / 8 * 8, INT32_MAX), (int32_t)std::min<int64_t>(weight.size(0), INT32_MAX), element_of(hidden),
+                  (int32_t)reduction, ignore_index};
+        const c10::DeviceGuard guard(hidden.device());
+        if (c.prob.rows > 0) {
+            c.hidden = pieces(hidden, c.dim);
+            c.weight = pieces(weight, c.dim);
+            c.targets = targets.to(at::kLong).contiguous();
+        }
+        return c;
+    }
+
+    // the loss; saved: operands, targets, and what the backward needs of the rows
+    static Tensor run(const Call &c, const Tensor &like, variable_list *saved) {
+        const c10::DeviceGuard guard(like.device());
+        const auto f32 = like.options().dtype(at::kFloat);
+        if (c.prob.rows == 0) return c.prob.reduction == 0 ? at::empty(like.sizes(), f32) : at::full({}, c.prob.reduction == 1 ? std::nan("") : 0., f32);
+        const Tensor loss = c.prob.reduction == 0 ? at::empty(like.sizes(), f32) : at::empty({}, f32);
+        const int64_t blocks = (c.prob.rows + 31) / 32;
+        // lse, then the count, then the mask
+        const Tensor kept = at::empty({c.prob.rows + 1 + blocks}, f32);
+        float *const lse = static_cast<float *>(kept.data_ptr());
+        const int64_t bytes = sa2_linear_ce_workspace_bytes(&c.prob);
+        Tensor ws;
+        if (bytes > 0) ws = at::empty({bytes}, like.options().dtype(at::kByte));
+        check(sa2_linear_ce(&c.prob, c.hidden.data_ptr(), row_stride(c.hidden), c.weight.data_ptr(), row_stride(c.weight), static_cast<const int64_t *>(c.targets.data_ptr()),
+                            static_cast<float *>(loss.data_ptr()), lse, lse + c.prob.rows, reinterpret_cast<uint32_t *>(lse + c.prob.rows + 1), const_cast<void *>(ptr(ws)), std::max<int64_t>(bytes, 0),
+                            stream_of(like)));
+        if (saved) *saved = {c.hidden, c.weight, c.targets, kept};
+        return loss;
+    }
+
+    static Tensor forward(AutogradContext *ctx, const Tensor &hidden, const Tensor &weight, const Tensor &targets, int64_t ignore_index, int64_t reduction) {
+        const Call c = checked(hidden, weight, targets, ignore_index, reduction);
+        variable_list saved;
+        const Tensor loss = run(c, targets, &saved);
+        ctx->save_for_backward(saved);
+        ctx->saved_data["hidden"] = c10::List<int64_t>(hidden.sizes().vec());
+        ctx->saved_data["weight"] = c10::List<int64_t>(weight.sizes().vec());
+        ctx->saved_data["problem"] = c10::List<int64_t>({c.prob.rows, c.prob.dim, c.prob.vocab, c.prob.dtype, c.prob.reduction, c.prob.ignore_index});
+        ctx->saved_data["type"] = (int64_t)hidden.scalar_type();
+        return loss;
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list ups) {
+        refuse_second("linear_cross_entropy");
+        refuse_foreign("linear_cross_entropy", {&ups[0]});
+        const auto n = ctx->saved_data["problem"].toIntVector(), h_shape = ctx->saved_data["hidden"].toIntVector(), w_shape = ctx->saved_data["weight"].toIntVector();
+        const sa2_linear_ce_problem prob{n[0], (int32_t)n[1], (int32_t)n[2], (int32_t)n[3], (int32_t)n[4], n[5]};
+        const auto options = ups[0].options().dtype((at::ScalarType)ctx->saved_data["type"].toInt());
+        const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        const c10::DeviceGuard guard(ups[0].device());
+        variable_list grads(5);
+        if (prob.rows == 0) {
+            if (want_h) grads[0] = at::empty(h_shape, options);
+            if (want_w) grads[1] = at::zeros(w_shape, options);
+            return grads;
+        }
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor &hidden = s[0], &weight = s[1], up = ups[0].contiguous();
+        if (want_h) grads[0] = at::empty({prob.rows, prob.dim}, options);
+        if (want_w) grads[1] = at::empty({prob.vocab, prob.dim}, options);
+        const int64_t bytes = sa2_linear_ce_bwd_workspace_bytes(&prob);
+        const Tensor ws = at::empty({std::max<int64_t>(bytes, 0)}, options.dtype(at::kByte));
+        const float *lse = static_cast<const float *>(s[3].data_ptr());
+        check(sa2_linear_ce_bwd(&prob, hidden.data_ptr(), row_stride(hidden), weight.data_ptr(), row_stride(weight), static_cast<const int64_t *>(s[2].data_ptr()), lse, lse + prob.rows,
+                                reinterpret_cast<const uint32_t *>(lse + prob.rows + 1), static_cast<const float *>(up.data_ptr()), const_cast<void *>(ptr(grads[0])),
+                                const_cast<void *>(ptr(grads[1])), ws.data_ptr(), bytes, stream_of(up)));
+        const int64_t dim = w_shape[1];
+        if (want_h) grads[0] = (dim == prob.dim ? grads[0] : grads[0].narrow(1, 0, dim).contiguous()).view(h_shape);
+        if (want_w && dim != prob.dim) grads[1] = grads[1].narrow(1, 0, dim).contiguous();
+        return grads;
+    }
+};
+
+Tensor linear_cross_entropy(const Tensor &hidden, const Tensor &weight, const Tensor &targets, int64_t ignore_index, int64_t reduction) {
+    if (in_autograd({&hidden, &weight})) return LinearCE::apply(hidden, weight, targets, ignore_index, reduction);
+    return LinearCE::run(LinearCE::checked(hidden, weight, targets, ignore_index, reduction), targets, nullptr);
+}
+
 // ---- AdamW
 const Tensor &tensor_of(const py::handle &h, const char *name) {
     if (!THPVariable_Check(h.ptr())) raise(PyExc_TypeError, std::string(name) + " must be tensors");
@@ -294,5 +404,6 @@ void adamw_step(const py::sequence &params, const py::sequence &grads, const py:
 void bind_training(py::module_ &m) {
     m.def("add_rms_norm", &add_rms_norm);
     m.def("add_rms_norm_8bit", &add_rms_norm_8bit);
+    m.def("linear_cross_entropy", &linear_cross_entropy);
     m.def("adamw_step", &adamw_step);
 }
