@@ -87,6 +87,22 @@ __device__ __forceinline__ void ld_some8(int type, const char *p, int count, flo
     else ld_some8<kF32>(p, count, v);
 }
 
+// eight floats as bf16 or fp16
+template <int T>
+__device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (T == kF16) {
+            const f16x2 h = {(_Float16)v[2 * i], (_Float16)v[2 * i + 1]};
+            o[i] = __builtin_bit_cast(uint32_t, h);
+        } else {
+            o[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+        }
+    }
+    return o;
+}
+
 template <int T>
 __device__ __forceinline__ void st_some8(char *p, int count, const float (&v)[8]) {
     if (count >= 8) {
@@ -94,17 +110,7 @@ __device__ __forceinline__ void st_some8(char *p, int count, const float (&v)[8]
             st_any16(p, (u32x4){as_u32(v[0]), as_u32(v[1]), as_u32(v[2]), as_u32(v[3])});
             st_any16(p + 16, (u32x4){as_u32(v[4]), as_u32(v[5]), as_u32(v[6]), as_u32(v[7])});
         } else {
-            u32x4 o;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (T == kF16) {
-                    const f16x2 h = {(_Float16)v[2 * i], (_Float16)v[2 * i + 1]};
-                    o[i] = __builtin_bit_cast(uint32_t, h);
-                } else {
-                    o[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-                }
-            }
-            st_any16(p, o);
+            st_any16(p, pack8<T>(v));
         }
     } else {
 #pragma unroll

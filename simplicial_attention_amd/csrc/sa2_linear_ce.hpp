@@ -44,6 +44,8 @@ constexpr float kCeFar = 4096.f;
 
 template <int T>
 constexpr float ce_scale = T == kF16 ? 1024.f : 1.f;
+template <int T>
+constexpr float ce_log2_scale = T == kF16 ? 10.f : 0.f;
 
 // ---- forward: a tile of logits
 
@@ -102,12 +104,14 @@ __global__ __launch_bounds__(256) void ce_logits_kernel(CeParams p) {
     }
 }
 
-// 32 rows a workgroup: the parts of each merged by 32 threads; the last workgroup adds up the losses in order
-static __global__ __launch_bounds__(1024) void ce_merge_kernel(CeParams p) {
-    __shared__ float2 parts[32][33];
-    __shared__ float2 totals[16];
+// ROWS rows a workgroup, the parts of each merged by G threads; the last workgroup adds up the losses in order
+template <int ROWS, int G>
+__global__ __launch_bounds__(ROWS *G) void ce_merge_kernel(CeParams p) {
+    constexpr int WAVES = ROWS * G / 64;
+    __shared__ float2 parts[G > 1 ? G : 1][G > 1 ? ROWS + 1 : 1];
+    __shared__ float2 totals[WAVES];
     __shared__ uint32_t last;
-    const int c = threadIdx.x & 31, g = threadIdx.x >> 5, row = blockIdx.x * 32 + c;
+    const int c = threadIdx.x % ROWS, g = threadIdx.x / ROWS, row = blockIdx.x * ROWS + c;
     float m = -INFINITY, s = 0.f;
     auto add = [&](float2 x) {
         const float top = fmaxf(m, x.x), ref = top == -INFINITY ? 0.f : top;
@@ -116,41 +120,45 @@ static __global__ __launch_bounds__(1024) void ce_merge_kernel(CeParams p) {
     };
     if (row < p.rows)
 #pragma unroll 4
-        for (int i = g; i < p.n_parts; i += 32) add(p.parts[(int64_t)i * p.rows + row]);
-    parts[g][c] = make_float2(m, s);
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        float loss = 0.f;
-        bool counts = false;
-        if (threadIdx.x < 32) {
-            m = -INFINITY, s = 0.f;
+        for (int i = g; i < p.n_parts; i += G) add(p.parts[(int64_t)i * p.rows + row]);
+    if constexpr (G > 1) {
+        parts[g][c] = make_float2(m, s);
+        __syncthreads();
+        m = -INFINITY, s = 0.f;
+        if (g == 0)
 #pragma unroll 4
-            for (int i = 0; i < 32; ++i) add(parts[i][c]);
-            if (row < p.rows) {
-                const float lse = m + logf(s);
-                const int64_t target = p.targets[row];
-                counts = target != p.ignore;
-                // (a target that is no token: no number comes of it)
-                if (counts) loss = target >= 0 && target < p.vocab ? lse - p.at_target[row] : NAN;
-                p.lse[row] = lse;
-                if (p.reduction == kCeNone) p.loss[row] = loss;
-            }
-        }
-        const uint32_t bits = (uint32_t)__ballot(counts);
-        loss = lanes_sum<32>(loss);
-        if (threadIdx.x == 0) {
-            p.mask[blockIdx.x] = bits;
-            p.sums[2 * blockIdx.x] = loss;
-            p.sums[2 * blockIdx.x + 1] = (float)__popc(bits);
-            __threadfence();
-            last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
-        }
+            for (int i = 0; i < G; ++i) add(parts[i][c]);
+    }
+    float loss = 0.f;
+    bool counts = false;
+    if (g == 0 && row < p.rows) {
+        const float lse = m + logf(s);
+        const int64_t target = p.targets[row];
+        counts = target != p.ignore;
+        // (a target that is no token: no number comes of it)
+        if (counts) loss = target >= 0 && target < p.vocab ? lse - p.at_target[row] : NAN;
+        p.lse[row] = lse;
+        if (p.reduction == kCeNone) p.loss[row] = loss;
+    }
+    const uint64_t bits = __ballot(counts);
+    if (g == 0 && (threadIdx.x & 31) == 0 && row < p.rows) p.mask[row >> 5] = (uint32_t)(bits >> (threadIdx.x & 32));
+    loss = lanes_sum<64>(loss);
+    if ((threadIdx.x & 63) == 0) totals[threadIdx.x >> 6] = make_float2(loss, (float)__popcll(bits));
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float2 sum = totals[0];
+        for (int i = 1; i < WAVES; ++i) sum.x += totals[i].x, sum.y += totals[i].y;
+        p.sums[2 * blockIdx.x] = sum.x;
+        p.sums[2 * blockIdx.x + 1] = sum.y;
+        __threadfence();
+        last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
     }
     __syncthreads();
     if (!last) return;
     __threadfence();
-    float loss = 0.f, count = 0.f;
-    for (int i = threadIdx.x; i < (int)gridDim.x; i += 1024) {
+    loss = 0.f;
+    float count = 0.f;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += ROWS * G) {
         loss += __hip_atomic_load(&p.sums[2 * i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         count += __hip_atomic_load(&p.sums[2 * i + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -160,7 +168,7 @@ static __global__ __launch_bounds__(1024) void ce_merge_kernel(CeParams p) {
     __syncthreads();
     if (threadIdx.x == 0) {
         loss = count = 0.f;
-        for (int i = 0; i < 16; ++i) loss += totals[i].x, count += totals[i].y;
+        for (int i = 0; i < WAVES; ++i) loss += totals[i].x, count += totals[i].y;
         *p.count = count;
         if (p.reduction == kCeMean) *p.loss = loss / count;
         else if (p.reduction == kCeSum) *p.loss = loss;
@@ -201,41 +209,77 @@ __global__ __launch_bounds__(256) void ce_dz_kernel(CeParams p) {
     P::run(p.shape, p.w, p.h, at, nullptr, lds, acc);
     const int lane = threadIdx.x & 63, wave = wave_index(), hf = lane >> 5;
     const int c0 = at.tile_r * P::TILE + 32 * NB * (wave & 1);           // column of the piece
+    // Blocks of 32 rows go through LDS, 16-byte pieces XORed with the row, so that a store writes whole rows of the wave's columns.  (From the registers
+    // it would be 16 bytes of 64 rows: 628 us for 8192 x 16384 of them, where the product without them takes 445.)
+    constexpr int PIECES = 4 * NB;                                       // of a row
+    __syncthreads();                                                     // (the tiles have been read)
+    char *const block = lds + wave * 32 * PIECES * 16;
+    const int in_block = dmap_row(lane & 31);
+    char *const mine_lds = block + in_block * PIECES * 16;
 #pragma unroll
     for (int a = 0; a < NB; ++a) {
-        const int row = at.tile_l * P::TILE + 32 * (NB * (wave >> 1) + a) + dmap_row(lane & 31);
-        if (row >= p.rows) continue;
+        const int row0 = at.tile_l * P::TILE + 32 * (NB * (wave >> 1) + a), row = min(row0 + in_block, p.rows - 1);
         const int64_t target = p.targets[row];
         const bool counts = target != p.ignore;
-        float weight = ce_scale<T>;
+        const float ref = p.lse[row], ref2 = ref * kLog2e - ce_log2_scale<T>;
+        const bool far = fabsf(ref) > kCeFar;
+        // (what only some rows or tiles need is asked of the wave: a tile in the middle takes a multiply-add, an exponential and half a packing per element)
+        if (wave_any(far)) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[a][b][r] = fast_exp2(far ? (acc[a][b][r] - ref) * kLog2e + ce_log2_scale<T> : acc[a][b][r] * kLog2e - ref2);
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[a][b][r] = fast_exp2(acc[a][b][r] * kLog2e - ref2);
+        }
+        const int64_t from = p.first + c0;
+        const int mine = counts && target >= from && target < from + 32 * NB ? (int)(target - from) - 16 * hf : -100;
+        if (wave_any(mine > -100)) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (mine == 32 * b + r) acc[a][b][r] -= ce_scale<T>;
+        }
+        float weight = 1.f;
         if (p.reduction == kCeNone) {
             const float most = *p.most;
-            weight *= most > 0.f ? p.up[row] / most : most;              // (all weights zero, or one that is no number)
+            weight = most > 0.f ? p.up[row] / most : most;               // (all weights zero, or one that is no number)
         }
         if (counts && !(target >= 0 && target < p.vocab)) weight = NAN;
-        const float ref = p.lse[row], ref2 = ref * kLog2e;
-        const bool far = fabsf(ref) > kCeFar;
-        const bool any_far = wave_any(far);
-        const int64_t mine = target - p.first - c0;
-        char *out = p.dz + row * p.dz_row + 2 * (c0 + 16 * hf);
+        if (wave_any(weight != 1.f)) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[a][b][r] *= weight;
+        }
+        const int end = p.vocab - p.first - c0 - 16 * hf;                // columns of this half that are tokens
+        if (wave_any(!counts || end < 32 * NB)) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!counts || 32 * b + r >= end) acc[a][b][r] = 0.f;
+        }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            float x[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int col = 32 * b + 16 * hf + r;
-                float e = acc[a][b][r] * kLog2e - ref2;
-                if (any_far) e = far ? (acc[a][b][r] - ref) * kLog2e : e;
-                e = fast_exp2(e);
-                if (mine == col) e -= 1.f;
-                x[r] = counts && p.first + c0 + col < p.vocab ? e * weight : 0.f;
-            }
             float lo[8], hi[8];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) lo[r] = x[r], hi[r] = x[8 + r];
-            st_some8<T>(out + 64 * b, 8, lo);
-            st_some8<T>(out + 64 * b + 16, 8, hi);
+            for (int r = 0; r < 8; ++r) lo[r] = acc[a][b][r], hi[r] = acc[a][b][8 + r];
+            *reinterpret_cast<u32x4 *>(mine_lds + 16 * ((4 * b + 2 * hf) ^ (in_block & (PIECES - 1)))) = pack8<T>(lo);
+            *reinterpret_cast<u32x4 *>(mine_lds + 16 * ((4 * b + 2 * hf + 1) ^ (in_block & (PIECES - 1)))) = pack8<T>(hi);
         }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < PIECES / 2; ++i) {
+            const int r = 64 / PIECES * i + lane / PIECES, piece = lane % PIECES, at_row = row0 + r;
+            const u32x4 v = ld_lds16(block + r * PIECES * 16 + 16 * (piece ^ (r & (PIECES - 1))));
+            if (at_row < p.rows) st_global16(p.dz + (int64_t)at_row * p.dz_row + 2 * c0 + 16 * piece, v);
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 

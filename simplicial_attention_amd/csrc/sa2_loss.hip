@@ -39,7 +39,7 @@ ProductPlan plan_of(int64_t l, int64_t r, int64_t k, bool shared, bool masked) {
 struct CePlan {
     ProductPlan logits, dz, dh, dw;
     int64_t piece = 0, pieces = 0;
-    int64_t dz_bytes = 0, h_bytes = 0, w_bytes = 0;
+    int64_t dz_row = 0, dz_bytes = 0, h_bytes = 0, w_bytes = 0;
     int64_t parts_bytes = 0;
 };
 
@@ -63,7 +63,9 @@ CePlan plan(const sa2_linear_ce_problem &p) {
     c.dz = plan_of(p.rows, c.piece, p.dim, false, false);
     c.dh = plan_of(p.rows, p.dim, c.piece, true, false);
     c.dw = plan_of(c.piece, p.dim, p.rows, true, true);
-    c.dz_bytes = up_to(p.rows * c.piece * 2, 256);
+    // (rows of a power of two of bytes would all begin in the same channel of the L2)
+    c.dz_row = c.piece * 2 + 256;
+    c.dz_bytes = up_to(p.rows * c.dz_row, 256);
     c.h_bytes = c.pieces > 1 || c.dh.shape.shares > 1 ? up_to((int64_t)c.dh.shape.shares * p.rows * p.dim * 4, 256) : 0;
     c.w_bytes = c.dw.shape.shares > 1 ? up_to((int64_t)c.dw.shape.shares * c.piece * p.dim * 4, 256) : 0;
     return c;
@@ -153,7 +155,9 @@ int sa2_linear_ce(const sa2_linear_ce_problem *p, const void *hidden, int64_t hi
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);
     with_kernel(p->dtype, c.logits.nb, [&](auto t, auto nb) { hipLaunchKernelGGL((ce_logits_kernel<t.value, nb.value>), dim3((unsigned)c.logits.groups()), dim3(256), 0, s, k); });
     if (const int rc = launched("logits")) return rc;
-    hipLaunchKernelGGL(ce_merge_kernel, dim3((unsigned)blocks_of(*p)), dim3(1024), 0, s, k);
+    // few parts: a thread a row
+    if (k.n_parts <= 16) hipLaunchKernelGGL((ce_merge_kernel<256, 1>), dim3((unsigned)((p->rows + 255) / 256)), dim3(256), 0, s, k);
+    else hipLaunchKernelGGL((ce_merge_kernel<32, 32>), dim3((unsigned)blocks_of(*p)), dim3(1024), 0, s, k);
     return launched("cross entropy");
 }
 
@@ -176,7 +180,7 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
     k.up = dloss;
     k.most = reinterpret_cast<float *>(ws);
     k.dz = ws + 256;
-    k.dz_row = c.piece * 2;
+    k.dz_row = c.dz_row;
     float *const h_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes), *const w_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes + c.h_bytes);
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);
     if (p->reduction == kCeNone) hipLaunchKernelGGL(ce_most_kernel, dim3(1), dim3(1024), 0, s, dloss, mask, (int)p->rows, reinterpret_cast<float *>(ws));

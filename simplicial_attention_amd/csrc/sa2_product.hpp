@@ -90,6 +90,11 @@ struct ProductSide {
         const bool ok = k < count && (ROW || (bits >> k & 1));
         load_to_lds16_from(ok ? p : reinterpret_cast<const char *>(kZeroPiece), uniform((int)(lds + 1024 * (wave + 4 * i))));
     }
+    // ... of the step that begins at p, with zeros for k whose bit is clear
+    __device__ __forceinline__ void issue_masked(int i, const char *p, uint32_t lds, int wave, uint32_t bits) const {
+        const bool ok = bits >> (k_of + 16 * (i & 1)) & 1;
+        load_to_lds16_from(ok ? p + off[i] : reinterpret_cast<const char *>(kZeroPiece), uniform((int)(lds + 1024 * (wave + 4 * i))));
+    }
     // 32 indices (block b) x 16 k (half s) of the tile
     __device__ __forceinline__ u32x4 fragment(const char *tile, int s, int b) const {
         if constexpr (ROW) {
@@ -198,7 +203,58 @@ struct Product {
         using Zero = std::integral_constant<int, 0>;
         using One = std::integral_constant<int, 1>;
         read(0, Zero{});
-        for (int t = 0; t < nt; ++t) {
+        int t = 0;
+        // The steps in the middle, in the order they are written: a product takes 32 clocks of the matrix unit, in whose shadow one read of the next
+        // fragments or one direct load is issued; the barrier stands behind the first products of the second half.
+        const int full = !MASKED && rest != 32 && t0 + nt == all ? nt - 1 : nt;      // (tiles that are filled up with zeros are the other loop's)
+        const char *pr = r.base + (int64_t)(t0 + 3) * r.advance, *pl = l.base + (int64_t)(t0 + 3) * l.advance;
+        uint32_t b3 = 0xffffffffu;
+        if constexpr (MASKED) b3 = bits[min(3, nt - 1)];
+        for (; t + 3 < full; ++t) {
+            const char *now = lds + (t % RING) * STAGE, *next = lds + ((t + 1) % RING) * STAGE;
+            const uint32_t to = lds0 + ((t + 3) % RING) * STAGE;
+            constexpr int N = NB * NB, READS = 2 * NB, FIRST = NB == 4 ? 4 : 1;
+            auto read_one = [&](const char *tile, auto half, auto i) {
+                if constexpr (i.value % 2 == 0) fr[half.value][i.value / 2] = r.fragment(tile, half.value, br + i.value / 2);
+                else fl[half.value][i.value / 2] = l.fragment(tile + R::BYTES, half.value, bl + i.value / 2);
+            };
+            auto multiply_one = [&](auto half, auto i) {
+                constexpr int a = i.value / NB, b = i.value % NB;
+                acc[a][b] = mfma_of<T>(fr[half.value][b], fl[half.value][a], acc[a][b]);
+            };
+            auto load_one = [&](auto i) {
+                if constexpr (i.value < R::CHUNKS) {
+                    if constexpr (MASKED) r.issue_masked(i.value, pr, to, wave, b3);
+                    else load_to_lds16(pr, r.off[i.value], uniform((int)(to + 1024 * (wave + 4 * i.value))));
+                } else {
+                    constexpr int j = i.value - R::CHUNKS;
+                    if constexpr (MASKED) l.issue_masked(j, pl, to + R::BYTES, wave, b3);
+                    else load_to_lds16(pl, l.off[j], uniform((int)(to + R::BYTES + 1024 * (wave + 4 * j))));
+                }
+            };
+            static_for<0, N>([&](auto i) {
+                multiply_one(Zero{}, i);
+                if constexpr (i.value < READS) read_one(now, One{}, i);
+                if constexpr (i.value >= N - LOADS) load_one(std::integral_constant<int, i.value - (N - LOADS)>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            pr += r.advance;
+            pl += l.advance;
+            static_for<0, FIRST>([&](auto i) { multiply_one(One{}, i); });
+            __builtin_amdgcn_sched_barrier(0);
+            // step t + 1 is in (two more are under way), and this wave has read all of step t
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+            if constexpr (MASKED) b3 = bits[min(t + 4, nt - 1)];
+            static_for<FIRST, N>([&](auto i) {
+                multiply_one(One{}, i);
+                constexpr int per = NB == 4 ? 1 : 2, at = (i.value - FIRST) * per;
+                static_for<0, per>([&](auto j) {
+                    if constexpr (at + j.value < READS) read_one(next, Zero{}, std::integral_constant<int, at + j.value>{});
+                });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        }
+        for (; t < nt; ++t) {
             read(t, One{});
             if (t + 3 < nt) issue(t + 3);
             multiply(Zero{});
