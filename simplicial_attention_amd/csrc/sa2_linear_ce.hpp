@@ -63,6 +63,7 @@ __global__ __launch_bounds__(256) void ce_logits_kernel(CeParams p) {
 #pragma unroll
     for (int a = 0; a < NB; ++a) {
         const int row = at.tile_l * P::TILE + 32 * (NB * (wave >> 1) + a) + dmap_row(lane & 31);
+        take(acc[a]);
         if (ragged) {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -73,11 +74,13 @@ __global__ __launch_bounds__(256) void ce_logits_kernel(CeParams p) {
         const int64_t target = row < p.rows ? p.targets[row] : -1;
         const int mine = target >= v0 && target < v0 + 32 * NB && target < p.vocab ? (int)(target - v0) : -1;
         if (wave_any(mine >= 0)) {
+            const int here = mine - 16 * hf;
+            float x = 0.f;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (mine == 32 * b + 16 * hf + r) p.at_target[row] = acc[a][b][r];
+                for (int r = 0; r < 16; ++r) x = here == 32 * b + r ? acc[a][b][r] : x;
+            if (mine >= 0 && (mine >> 4 & 1) == hf) p.at_target[row] = x;
         }
         float m = -INFINITY;
 #pragma unroll
@@ -209,20 +212,16 @@ __global__ __launch_bounds__(256) void ce_dz_kernel(CeParams p) {
     P::run(p.shape, p.w, p.h, at, nullptr, lds, acc);
     const int lane = threadIdx.x & 63, wave = wave_index(), hf = lane >> 5;
     const int c0 = at.tile_r * P::TILE + 32 * NB * (wave & 1);           // column of the piece
-    // Blocks of 32 rows go through LDS, 16-byte pieces XORed with the row, so that a store writes whole rows of the wave's columns.  (From the registers
-    // it would be 16 bytes of 64 rows: 628 us for 8192 x 16384 of them, where the product without them takes 445.)
-    constexpr int PIECES = 4 * NB;                                       // of a row
     __syncthreads();                                                     // (the tiles have been read)
-    char *const block = lds + wave * 32 * PIECES * 16;
-    const int in_block = dmap_row(lane & 31);
-    char *const mine_lds = block + in_block * PIECES * 16;
+    const ProductRows<T, NB> rows(lds);
 #pragma unroll
     for (int a = 0; a < NB; ++a) {
-        const int row0 = at.tile_l * P::TILE + 32 * (NB * (wave >> 1) + a), row = min(row0 + in_block, p.rows - 1);
+        const int row0 = at.tile_l * P::TILE + 32 * (NB * (wave >> 1) + a), row = min(row0 + rows.row, p.rows - 1);
         const int64_t target = p.targets[row];
         const bool counts = target != p.ignore;
         const float ref = p.lse[row], ref2 = ref * kLog2e - ce_log2_scale<T>;
         const bool far = fabsf(ref) > kCeFar;
+        take(acc[a]);
         // (what only some rows or tiles need is asked of the wave: a tile in the middle takes a multiply-add, an exponential and half a packing per element)
         if (wave_any(far)) {
 #pragma unroll
@@ -265,103 +264,100 @@ __global__ __launch_bounds__(256) void ce_dz_kernel(CeParams p) {
                     if (!counts || 32 * b + r >= end) acc[a][b][r] = 0.f;
         }
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            float lo[8], hi[8];
-#pragma unroll
-            for (int r = 0; r < 8; ++r) lo[r] = acc[a][b][r], hi[r] = acc[a][b][8 + r];
-            *reinterpret_cast<u32x4 *>(mine_lds + 16 * ((4 * b + 2 * hf) ^ (in_block & (PIECES - 1)))) = pack8<T>(lo);
-            *reinterpret_cast<u32x4 *>(mine_lds + 16 * ((4 * b + 2 * hf + 1) ^ (in_block & (PIECES - 1)))) = pack8<T>(hi);
-        }
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int i = 0; i < PIECES / 2; ++i) {
-            const int r = 64 / PIECES * i + lane / PIECES, piece = lane % PIECES, at_row = row0 + r;
-            const u32x4 v = ld_lds16(block + r * PIECES * 16 + 16 * (piece ^ (r & (PIECES - 1))));
-            if (at_row < p.rows) st_global16(p.dz + (int64_t)at_row * p.dz_row + 2 * c0 + 16 * piece, v);
-        }
-        __builtin_amdgcn_wave_barrier();
+        for (int b = 0; b < NB; ++b) rows.put(b, acc[a][b]);
+        rows.each([&](int r, int col, u32x4 v) {
+            if (row0 + r < p.rows) st_global16(p.dz + (int64_t)(row0 + r) * p.dz_row + 2 * (c0 + col), v);
+        });
     }
 }
 
-// where the results of a product with dz go
+// Where the results of a product with dz go.  DIRECT: rounded, times what they were divided by; else fp32, for ce_combine_kernel.
 struct CeOutput {
-    char *out;                     // [rows][dim] in the operands' type (the sum is complete), or NULL
-    float *parts;                  // [share][rows][dim]
+    char *out;                     // DIRECT: [rows][dim] in the operands' type
+    float *parts;                  // else: [share][rows][dim]
     int rows, add;                 // add: to what is in the parts
     int masked;                    // rows that do not count become zero
 };
 
-template <int T, int NB, typename P>
-__device__ __forceinline__ void ce_store(const CeParams &p, const CeOutput &o, const ProductPlace &at, const f32x16 (&acc)[NB][NB]) {
-    const float factor = o.out ? ce_factor<T>(p) : 1.f;
-    P::each_run(at, acc, [&](int row, int col, const f32x16 &x) {
-        if (row >= o.rows) return;
-        const bool counts = !o.masked || (p.mask[row >> 5] >> (row & 31) & 1);
+template <int T, int NB, bool DIRECT>
+__device__ __forceinline__ void ce_store(const CeParams &p, const CeOutput &o, const ProductPlace &at, char *lds, f32x16 (&acc)[NB][NB]) {
+    const int wave = wave_index();
+    const int c0 = 64 * NB * at.tile_r + 32 * NB * (wave & 1);
+    char *const out = DIRECT ? o.out : reinterpret_cast<char *>(o.parts + (int64_t)at.share * o.rows * p.dim);
+    const float factor = DIRECT ? ce_factor<T>(p) : 1.f;
+    __syncthreads();                              // (the tiles have been read)
+    const ProductRows<DIRECT ? T : kF32, NB> rows(lds);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int d = col + 8 * half;
-            if (d >= p.dim) continue;
-            float *part = o.parts + ((int64_t)at.share * o.rows + row) * p.dim + d;
-            float v[8];
+    for (int a = 0; a < NB; ++a) {
+        const int row0 = 64 * NB * at.tile_l + 32 * (NB * (wave >> 1) + a);
+        take(acc[a]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = x[8 * half + i];
-            if (o.add) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] += part[i];
+        for (int b = 0; b < NB; ++b) rows.put(b, acc[a][b], factor);
+        rows.each([&](int r, int col, u32x4 v) {
+            const int row = row0 + r, d = c0 + col;
+            if (row >= o.rows || d >= p.dim) return;
+            char *to = out + ((int64_t)row * p.dim + d) * (DIRECT ? 2 : 4);
+            if constexpr (DIRECT) {
+                if (o.masked && !(p.mask[row >> 5] >> (row & 31) & 1)) v = (u32x4){0, 0, 0, 0};
+            } else if (o.add) {
+                const float4 x = __builtin_bit_cast(float4, v), y = *reinterpret_cast<const float4 *>(to);
+                v = __builtin_bit_cast(u32x4, make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w));
             }
-            if (o.out) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = counts ? v[i] * factor : 0.f;
-                st_some8<T>(o.out + ((int64_t)row * p.dim + d) * 2, 8, v);
-            } else {
-                st_some8<kF32>(reinterpret_cast<char *>(part), 8, v);
-            }
-        }
-    });
+            st_global16(to, v);
+        });
+    }
 }
 
 // dH of a piece: rows x dim, contracted over the piece's tokens (r side: W read along dim)
-template <int T, int NB>
+template <int T, int NB, bool DIRECT>
 __global__ __launch_bounds__(256) void ce_dh_kernel(CeParams p, CeOutput o) {
     using P = Product<T, NB, false, true, false>;
     __shared__ __attribute__((aligned(16))) char lds[P::LDS];
     const ProductPlace at = product_place(p.shape);
     f32x16 acc[NB][NB];
     P::run(p.shape, p.w, p.h, at, nullptr, lds, acc);
-    ce_store<T, NB, P>(p, o, at, acc);
+    ce_store<T, NB, DIRECT>(p, o, at, lds, acc);
 }
 
 // dW of a piece: tokens x dim, contracted over the rows that count
-template <int T, int NB>
+template <int T, int NB, bool DIRECT>
 __global__ __launch_bounds__(256) void ce_dw_kernel(CeParams p, CeOutput o) {
     using P = Product<T, NB, false, false, true>;
     __shared__ __attribute__((aligned(16))) char lds[P::LDS];
     const ProductPlace at = product_place(p.shape);
     f32x16 acc[NB][NB];
     P::run(p.shape, p.w, p.h, at, p.mask, lds, acc);
-    ce_store<T, NB, P>(p, o, at, acc);
+    ce_store<T, NB, DIRECT>(p, o, at, lds, acc);
 }
 
-// the shares added in order, eight elements a thread
+// the shares added in order, four elements a thread
 template <int T>
 __global__ __launch_bounds__(256) void ce_combine_kernel(CeParams p, CeOutput o, char *out) {
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8, all = (int64_t)o.rows * p.dim;
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = (int64_t)o.rows * p.dim;
     if (at >= all) return;
     const int row = (int)(at / p.dim);
-    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const float *src = o.parts + at;
-#pragma unroll 4
-    for (int x = 0; x < p.shape.shares; ++x, src += all) {
-        float v[8];
-        ld_some8<kF32>(reinterpret_cast<const char *>(src), 8, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] += v[i];
-    }
     const float factor = ce_factor<T>(p);
     const bool counts = !o.masked || (p.mask[row >> 5] >> (row & 31) & 1);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float *src = o.parts + at;
+#pragma unroll 8
+    for (int x = 0; x < p.shape.shares; ++x, src += all) {
+        const float4 v = *reinterpret_cast<const float4 *>(src);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const float v[4] = {s.x * factor, s.y * factor, s.z * factor, s.w * factor};
+    u32x2 w;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = counts ? s[i] * factor : 0.f;
-    st_some8<T>(out + at * 2, 8, s);
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (T == kF16) {
+            const f16x2 h = {(_Float16)v[2 * i], (_Float16)v[2 * i + 1]};
+            w[i] = __builtin_bit_cast(uint32_t, h);
+        } else {
+            w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+        }
+    }
+    if (!counts) w = (u32x2){0, 0};
+    *reinterpret_cast<u32x2 *>(out + at * 2) = w;
 }
 
 }  // namespace sa2

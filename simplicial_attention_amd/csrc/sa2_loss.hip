@@ -23,17 +23,30 @@ struct ProductPlan {
     int64_t groups() const { return (int64_t)shape.tiles_r * shape.tiles_l * shape.shares; }
 };
 
+// Of the tiles and shares whose workgroups fill the chip, those with the least estimated time.  A step of 256 x 256 takes a CU 0.83 us at the power that the
+// matrix units draw (1.25 PFLOP/s over all), a workgroup of 256 x 256 9 us more (first loads, epilogue); two workgroups of 128 x 128 on a CU take 0.52 us a step and 4.5 us,
+// one alone 0.30 us a step.  Shares write and read their fp32 results (4 TB/s, and a launch).  Measured: gradient of 4096 rows of 1024 channels over 50021 tokens 386 us in
+// 256 x 256 with four shares, 467 in 128 x 128 with two; of 1237 rows of 328 channels over 10007 tokens 38 and 24 us.
 ProductPlan plan_of(int64_t l, int64_t r, int64_t k, bool shared, bool masked) {
-    ProductPlan p;
-    auto tiles = [&](int64_t t) { return ((l + t - 1) / t) * ((r + t - 1) / t); };
-    p.nb = tiles(256) >= 192 ? 4 : 2;
-    const int64_t t = 64 * p.nb, steps = (k + 31) / 32, all = tiles(t), target = p.nb == 4 ? 256 : 512;
-    int64_t shares = 1;
-    if (shared && all < target) shares = std::max<int64_t>(1, std::min(target / all, steps / 16));
-    int64_t per = (steps + shares - 1) / shares;
-    if (masked) per = std::min<int64_t>(per, kProductMostSteps);
-    p.shape = {(int)k, (int)((r + t - 1) / t), (int)((l + t - 1) / t), (int)((steps + per - 1) / per), (int)per};
-    return p;
+    ProductPlan best;
+    double least = 0;
+    const int64_t steps = (k + 31) / 32;
+    for (const int nb : {2, 4})
+        for (int64_t shares = 1; shares <= (shared ? 64 : 1) && (shares == 1 || steps / shares >= 4); shares += shares < 8 ? 1 : shares / 4) {
+            const int64_t t = 64 * nb, tiles_l = (l + t - 1) / t, tiles_r = (r + t - 1) / t;
+            int64_t per = (steps + shares - 1) / shares;
+            if (masked) per = std::min<int64_t>(per, kProductMostSteps);
+            const int64_t real = (steps + per - 1) / per, groups = tiles_l * tiles_r * real, slots = nb == 4 ? 256 : 512;
+            const double step = nb == 4 ? 0.83 : groups <= 256 ? 0.30 : 0.52, fixed = nb == 4 ? 9 : 4.5, rounds = (double)groups / (double)slots;
+            double us = (rounds <= 1 ? 1. : rounds + 0.3) * ((double)per * step + fixed);
+            if (real > 1) us += 3 + (double)real * (double)l * (double)r * 8 / 4e6;
+            if (best.shape.shares == 0 || us < least) {
+                least = us;
+                best.nb = nb;
+                best.shape = {(int)k, (int)tiles_r, (int)tiles_l, (int)real, (int)per};
+            }
+        }
+    return best;
 }
 
 struct CePlan {
@@ -203,10 +216,14 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
             k.w = {w.ptr, w.row, p->dim};
             k.h = {k.dz, k.dz_row, (int)p->rows};
             const bool done = i + 1 == c.pieces;
-            const CeOutput o{done && c.dh.shape.shares == 1 ? static_cast<char *>(dhidden) : nullptr, h_parts, (int)p->rows, i > 0, 1};
-            with_kernel(p->dtype, c.dh.nb, [&](auto t, auto nb) { hipLaunchKernelGGL((ce_dh_kernel<t.value, nb.value>), dim3((unsigned)c.dh.groups()), dim3(256), 0, s, k, o); });
-            if (done && c.dh.shape.shares > 1) {
-                const dim3 grid((unsigned)((p->rows * p->dim / 8 + 255) / 256));
+            const CeOutput o{c.h_bytes == 0 ? static_cast<char *>(dhidden) : nullptr, h_parts, (int)p->rows, i > 0, 1};
+            with_kernel(p->dtype, c.dh.nb, [&](auto t, auto nb) { 
+                const dim3 grid((unsigned)c.dh.groups());
+                if (o.out) hipLaunchKernelGGL((ce_dh_kernel<t.value, nb.value, true>), grid, dim3(256), 0, s, k, o);
+                else hipLaunchKernelGGL((ce_dh_kernel<t.value, nb.value, false>), grid, dim3(256), 0, s, k, o);
+            });
+            if (done && c.h_bytes > 0) {
+                const dim3 grid((unsigned)((p->rows * p->dim / 4 + 255) / 256));
                 with_kernel(p->dtype, 2, [&](auto t, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, o, static_cast<char *>(dhidden)); });
             }
         }
@@ -216,9 +233,13 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
             k.h = {k.dz, k.dz_row, (int)up_to(tokens, 8)};          // (tiles of dz end with zeros)
             char *const out = static_cast<char *>(dweight) + first * p->dim * 2;
             const CeOutput o{c.dw.shape.shares == 1 ? out : nullptr, w_parts, (int)tokens, 0, 0};
-            with_kernel(p->dtype, c.dw.nb, [&](auto t, auto nb) { hipLaunchKernelGGL((ce_dw_kernel<t.value, nb.value>), dim3((unsigned)dw.groups()), dim3(256), 0, s, k, o); });
+            with_kernel(p->dtype, c.dw.nb, [&](auto t, auto nb) { 
+                const dim3 grid((unsigned)dw.groups());
+                if (o.out) hipLaunchKernelGGL((ce_dw_kernel<t.value, nb.value, true>), grid, dim3(256), 0, s, k, o);
+                else hipLaunchKernelGGL((ce_dw_kernel<t.value, nb.value, false>), grid, dim3(256), 0, s, k, o);
+            });
             if (c.dw.shape.shares > 1) {
-                const dim3 grid((unsigned)((tokens * p->dim / 8 + 255) / 256));
+                const dim3 grid((unsigned)((tokens * p->dim / 4 + 255) / 256));
                 with_kernel(p->dtype, 2, [&](auto t, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, o, out); });
             }
         }

@@ -79,20 +79,11 @@ struct ProductSide {
         }
     }
 
-    // chunk i of the wave, of step t; `lds`: the tile's place
-    __device__ __forceinline__ void issue(int i, int t, uint32_t lds, int wave) const {
-        load_to_lds16(uniform(base + t * advance), off[i], uniform((int)(lds + 1024 * (wave + 4 * i))));
-    }
-    // the same with zeros for k from `count` on and (not ROW) for k whose bit is clear
-    __device__ __forceinline__ void issue_some(int i, int t, uint32_t lds, int wave, int count, uint32_t bits) const {
-        const int k = ROW ? k_of : k_of + 16 * (i & 1);
-        const char *p = base + t * advance + off[i];
-        const bool ok = k < count && (ROW || (bits >> k & 1));
-        load_to_lds16_from(ok ? p : reinterpret_cast<const char *>(kZeroPiece), uniform((int)(lds + 1024 * (wave + 4 * i))));
-    }
-    // ... of the step that begins at p, with zeros for k whose bit is clear
-    __device__ __forceinline__ void issue_masked(int i, const char *p, uint32_t lds, int wave, uint32_t bits) const {
-        const bool ok = bits >> (k_of + 16 * (i & 1)) & 1;
+    // chunk i of the wave, of the step that begins at p; `lds`: the tile's place
+    __device__ __forceinline__ void issue(int i, const char *p, uint32_t lds, int wave) const { load_to_lds16(p, off[i], uniform((int)(lds + 1024 * (wave + 4 * i)))); }
+    // the same with zeros for k whose bit is clear
+    __device__ __forceinline__ void issue_some(int i, const char *p, uint32_t lds, int wave, uint32_t bits) const {
+        const bool ok = bits >> (ROW ? k_of : k_of + 16 * (i & 1)) & 1;
         load_to_lds16_from(ok ? p + off[i] : reinterpret_cast<const char *>(kZeroPiece), uniform((int)(lds + 1024 * (wave + 4 * i))));
     }
     // 32 indices (block b) x 16 k (half s) of the tile
@@ -148,103 +139,83 @@ struct Product {
         const L l(lo, at.tile_l * TILE, lane, wave);
         const int t0 = at.share * shape.share_steps, all = (shape.k + 31) / 32;
         const int nt = min(shape.share_steps, all - t0);
-        const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
-        uint32_t *bits = reinterpret_cast<uint32_t *>(lds + RING * STAGE);
         if constexpr (MASKED) {
+            uint32_t *bits = reinterpret_cast<uint32_t *>(lds + RING * STAGE);
             for (int i = threadIdx.x; i < nt; i += 256) bits[i] = mask[t0 + i];
             __syncthreads();
         }
-        const int rest = shape.k - 32 * (all - 1);          // k of the last step
-        auto issue = [&](int t) {
-            const uint32_t to = lds0 + (t % RING) * STAGE;
-            if (MASKED || (t0 + t == all - 1 && rest != 32)) {
-                const int count = t0 + t == all - 1 ? rest : 32;
-                uint32_t b = 0xffffffffu;
-                if constexpr (MASKED) b = bits[t];
-#pragma unroll
-                for (int i = 0; i < R::CHUNKS; ++i) r.issue_some(i, t0 + t, to, wave, count, b);
-#pragma unroll
-                for (int i = 0; i < L::CHUNKS; ++i) l.issue_some(i, t0 + t, to + R::BYTES, wave, count, b);
-            } else {
-#pragma unroll
-                for (int i = 0; i < R::CHUNKS; ++i) r.issue(i, t0 + t, to, wave);
-#pragma unroll
-                for (int i = 0; i < L::CHUNKS; ++i) l.issue(i, t0 + t, to + R::BYTES, wave);
-            }
-        };
+        // Steps whose k do not all count: those with a mask, or the last one of k where it is not whole (pieces of eight k: what a piece holds beyond k is zero)
+        const uint32_t last = 0xffffffffu >> (32 * all - shape.k);
+        if (MASKED || (t0 + nt == all && last != 0xffffffffu)) steps<true>(r, l, t0, nt, t0 + nt == all ? last : 0xffffffffu, lds, acc);
+        else steps<false>(r, l, t0, nt, 0xffffffffu, lds, acc);
+    }
+
+    // `last`: bits of the k of the last step that count
+    template <bool SOME>
+    static __device__ __forceinline__ void steps(const R &r, const L &l, int t0, int nt, uint32_t last, char *lds, f32x16 (&acc)[NB][NB]) {
+        const int wave = wave_index();
+        const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
+        [[maybe_unused]] const uint32_t *bits = reinterpret_cast<const uint32_t *>(lds + RING * STAGE);
 #pragma unroll
         for (int a = 0; a < NB; ++a)
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[a][b] = zero16();
         if (nt <= 0) return;
-        issue(0);
-        if (nt > 1) issue(1);
-        if (nt > 2) issue(2);
-        if (nt > 2) wait_loads<2 * LOADS>();
-        else if (nt > 1) wait_loads<LOADS>();
-        else wait_loads<0>();
-        __syncthreads();
-        u32x4 fr[2][NB], fl[2][NB];
-        const int br = NB * (wave & 1), bl = NB * (wave >> 1);
-        auto read = [&](int t, auto s) {
-            const char *tile = lds + (t % RING) * STAGE;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                fr[s.value][b] = r.fragment(tile, s.value, br + b);
-                fl[s.value][b] = l.fragment(tile + R::BYTES, s.value, bl + b);
+        const char *pr = r.base + t0 * r.advance, *pl = l.base + t0 * l.advance;      // of the step that is loaded next
+        uint32_t next_bits = MASKED ? bits[0] : nt == 1 ? last : 0xffffffffu;
+        auto load_one = [&](uint32_t to, auto i) {
+            if constexpr (i.value < R::CHUNKS) {
+                if constexpr (SOME) r.issue_some(i.value, pr, to, wave, next_bits);
+                else r.issue(i.value, pr, to, wave);
+            } else {
+                if constexpr (SOME) l.issue_some(i.value - R::CHUNKS, pl, to + R::BYTES, wave, next_bits);
+                else l.issue(i.value - R::CHUNKS, pl, to + R::BYTES, wave);
             }
         };
-        auto multiply = [&](auto s) {
-#pragma unroll
-            for (int a = 0; a < NB; ++a)
-#pragma unroll
-                for (int b = 0; b < NB; ++b) acc[a][b] = mfma_of<T>(fr[s.value][b], fl[s.value][a], acc[a][b]);
+        // after step t has been issued: the next one, or behind the last step that one again (into a place that nobody reads; so every step is alike)
+        auto go_on = [&](int t) {
+            const bool more = t + 1 < nt;
+            pr += more ? r.advance : 0;
+            pl += more ? l.advance : 0;
+            if constexpr (MASKED) next_bits = bits[min(t + 1, nt - 1)];
+            else if constexpr (SOME) next_bits = t + 1 >= nt - 1 ? last : 0xffffffffu;
         };
+#pragma unroll
+        for (int t = 0; t < 3; ++t) {
+            static_for<0, LOADS>([&](auto i) { load_one(lds0 + t * STAGE, i); });
+            go_on(t);
+        }
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+        u32x4 fr[2][NB], fl[2][NB];
+        const int br = NB * (wave & 1), bl = NB * (wave >> 1);
         using Zero = std::integral_constant<int, 0>;
         using One = std::integral_constant<int, 1>;
-        read(0, Zero{});
-        int t = 0;
-        // The steps in the middle, in the order they are written: a product takes 32 clocks of the matrix unit, in whose shadow one read of the next
-        // fragments or one direct load is issued; the barrier stands behind the first products of the second half.
-        const int full = !MASKED && rest != 32 && t0 + nt == all ? nt - 1 : nt;      // (tiles that are filled up with zeros are the other loop's)
-        const char *pr = r.base + (int64_t)(t0 + 3) * r.advance, *pl = l.base + (int64_t)(t0 + 3) * l.advance;
-        uint32_t b3 = 0xffffffffu;
-        if constexpr (MASKED) b3 = bits[min(3, nt - 1)];
-        for (; t + 3 < full; ++t) {
+        constexpr int N = NB * NB, READS = 2 * NB, FIRST = NB == 4 ? 4 : 1;
+        auto read_one = [&](const char *tile, auto half, auto i) {
+            if constexpr (i.value % 2 == 0) fr[half.value][i.value / 2] = r.fragment(tile, half.value, br + i.value / 2);
+            else fl[half.value][i.value / 2] = l.fragment(tile + R::BYTES, half.value, bl + i.value / 2);
+        };
+        auto multiply_one = [&](auto half, auto i) {
+            constexpr int a = i.value / NB, b = i.value % NB;
+            acc[a][b] = mfma_of<T>(fr[half.value][b], fl[half.value][a], acc[a][b]);
+        };
+        static_for<0, READS>([&](auto i) { read_one(lds, Zero{}, i); });
+        // In the order in which it is written: a product takes 32 clocks of the matrix unit, in whose shadow one read of the next fragments or one direct load is
+        // issued; the barrier stands behind the first products of the second half.
+        for (int t = 0; t < nt; ++t) {
             const char *now = lds + (t % RING) * STAGE, *next = lds + ((t + 1) % RING) * STAGE;
             const uint32_t to = lds0 + ((t + 3) % RING) * STAGE;
-            constexpr int N = NB * NB, READS = 2 * NB, FIRST = NB == 4 ? 4 : 1;
-            auto read_one = [&](const char *tile, auto half, auto i) {
-                if constexpr (i.value % 2 == 0) fr[half.value][i.value / 2] = r.fragment(tile, half.value, br + i.value / 2);
-                else fl[half.value][i.value / 2] = l.fragment(tile + R::BYTES, half.value, bl + i.value / 2);
-            };
-            auto multiply_one = [&](auto half, auto i) {
-                constexpr int a = i.value / NB, b = i.value % NB;
-                acc[a][b] = mfma_of<T>(fr[half.value][b], fl[half.value][a], acc[a][b]);
-            };
-            auto load_one = [&](auto i) {
-                if constexpr (i.value < R::CHUNKS) {
-                    if constexpr (MASKED) r.issue_masked(i.value, pr, to, wave, b3);
-                    else load_to_lds16(pr, r.off[i.value], uniform((int)(to + 1024 * (wave + 4 * i.value))));
-                } else {
-                    constexpr int j = i.value - R::CHUNKS;
-                    if constexpr (MASKED) l.issue_masked(j, pl, to + R::BYTES, wave, b3);
-                    else load_to_lds16(pl, l.off[j], uniform((int)(to + R::BYTES + 1024 * (wave + 4 * j))));
-                }
-            };
             static_for<0, N>([&](auto i) {
                 multiply_one(Zero{}, i);
                 if constexpr (i.value < READS) read_one(now, One{}, i);
-                if constexpr (i.value >= N - LOADS) load_one(std::integral_constant<int, i.value - (N - LOADS)>{});
+                if constexpr (i.value >= N - LOADS) load_one(to, std::integral_constant<int, i.value - (N - LOADS)>{});
                 __builtin_amdgcn_sched_barrier(0);
             });
-            pr += r.advance;
-            pl += l.advance;
             static_for<0, FIRST>([&](auto i) { multiply_one(One{}, i); });
             __builtin_amdgcn_sched_barrier(0);
             // step t + 1 is in (two more are under way), and this wave has read all of step t
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
-            if constexpr (MASKED) b3 = bits[min(t + 4, nt - 1)];
+            go_on(t + 3);
             static_for<FIRST, N>([&](auto i) {
                 multiply_one(One{}, i);
                 constexpr int per = NB == 4 ? 1 : 2, at = (i.value - FIRST) * per;
@@ -254,30 +225,63 @@ struct Product {
                 __builtin_amdgcn_sched_barrier(0);
             });
         }
-        for (; t < nt; ++t) {
-            read(t, One{});
-            if (t + 3 < nt) issue(t + 3);
-            multiply(Zero{});
-            if (t + 1 < nt) {
-                if (t + 3 < nt) wait_loads<2 * LOADS>();
-                else if (t + 2 < nt) wait_loads<LOADS>();
-                else wait_loads<0>();
-                __syncthreads();                            // step t + 1 is in, and step t has been read by all
-                read(t + 1, Zero{});
-            }
-            multiply(One{});
-        }
+        wait_loads<0>();      // (the last loads may still be on their way into LDS)
     }
 
-    // f(l index, first r index of a run of 16, the run) for every run of the lane
+};
+
+// the blocks of a row of tiles, from here on (the compiler would read those of all rows out of the accumulation registers at once, and spill)
+template <int NB>
+__device__ __forceinline__ void take(f32x16 (&acc)[NB]) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) pin_acc(acc[b]);
+}
+
+// Results of a wave on their way to memory: a block of 32 rows goes through LDS, its 16-byte pieces XORed with the row, so that a store writes whole rows of
+// the wave's 32 NB columns.  (From the registers it would be 16 bytes of 64 rows: an epilogue of 8192 x 16384 results of two bytes took 190 us of 628.)
+// TO: kF32, or the type that the results are rounded to.
+template <int TO, int NB>
+struct ProductRows {
+    static constexpr int PIECES = 2 * NB * element_size<TO>;      // of a row
+    static constexpr int BYTES = 4 * 32 * PIECES * 16;            // of the four waves
+    static constexpr int EACH = 16 / element_size<TO>;            // results of a piece
+    char *block, *mine;
+    int row, lane;
+
+    __device__ ProductRows(char *lds) {
+        lane = threadIdx.x & 63;
+        block = lds + wave_index() * 32 * PIECES * 16;
+        row = dmap_row(lane & 31);
+        mine = block + row * PIECES * 16;
+    }
+    static __device__ int place(int row, int piece) { return 16 * (piece ^ (row & (PIECES < 16 ? PIECES - 1 : 15))); }
+    // the lane's run of block b, times `factor`
+    __device__ __forceinline__ void put(int b, const f32x16 &x, float factor = 1.f) const {
+        const int first = PIECES / NB * b + PIECES / NB / 2 * (lane >> 5);
+        if constexpr (TO == kF32) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<float4 *>(mine + place(row, first + q)) = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = x[8 * q + i] * factor;
+                *reinterpret_cast<u32x4 *>(mine + place(row, first + q)) = pack8<TO>(v);
+            }
+        }
+    }
+    // f(row of the block, first column of the wave's, the piece) for every piece that the lane stores
     template <typename F>
-    static __device__ __forceinline__ void each_run(const ProductPlace &at, const f32x16 (&acc)[NB][NB], F &&f) {
-        const int lane = threadIdx.x & 63, wave = wave_index();
+    __device__ __forceinline__ void each(F &&f) const {
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int a = 0; a < NB; ++a)
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-                f(at.tile_l * TILE + 32 * (NB * (wave >> 1) + a) + dmap_row(lane & 31), at.tile_r * TILE + 32 * (NB * (wave & 1) + b) + 16 * (lane >> 5), acc[a][b]);
+        for (int i = 0; i < PIECES / 2; ++i) {
+            const int r = 64 / PIECES * i + lane / PIECES, piece = lane % PIECES;
+            f(r, EACH * piece, ld_lds16(block + r * PIECES * 16 + place(r, piece)));
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 };
 
