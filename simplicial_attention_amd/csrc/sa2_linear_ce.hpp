@@ -29,7 +29,7 @@ struct CeParams {
     uint32_t *ticket;
     int n_parts;
     float *sums;                             // [blocks of 32 rows]: loss and number of rows that count
-    float *loss, *lse, *count;
+    float *loss, *lse, *count;               // count: mean and sum only
     uint32_t *mask;                          // [blocks of 32 rows]: rows that count
     // backward
     const float *up;                         // gradient of the loss: one number, or one per row
@@ -113,52 +113,70 @@ __global__ __launch_bounds__(ROWS *G) void ce_merge_kernel(CeParams p) {
     constexpr int WAVES = ROWS * G / 64;
     __shared__ float2 parts[G > 1 ? G : 1][G > 1 ? ROWS + 1 : 1];
     __shared__ float2 totals[WAVES];
+    __shared__ uint32_t two[WAVES];
     __shared__ uint32_t last;
-    const int c = threadIdx.x % ROWS, g = threadIdx.x / ROWS, row = blockIdx.x * ROWS + c;
+    const int c = threadIdx.x % ROWS, g = threadIdx.x / ROWS;
+    // the row that this thread says something about in the end (with G > 1: the first lane of each 32)
+    const int row = blockIdx.x * ROWS + (G > 1 ? threadIdx.x / 32 : c);
+    const bool says = row < p.rows && (G == 1 || (threadIdx.x & 31) == 0);
+    int64_t target = -1;
+    float at_target = 0.f;
+    if (says) target = p.targets[row], at_target = p.at_target[row];
     float m = -INFINITY, s = 0.f;
     auto add = [&](float2 x) {
         const float top = fmaxf(m, x.x), ref = top == -INFINITY ? 0.f : top;
         s = s * fast_exp2((m - ref) * kLog2e) + x.y * fast_exp2((x.x - ref) * kLog2e);
         m = top;
     };
-    if (row < p.rows)
+    if (blockIdx.x * ROWS + c < p.rows)
 #pragma unroll 4
-        for (int i = g; i < p.n_parts; i += G) add(p.parts[(int64_t)i * p.rows + row]);
+        for (int i = g; i < p.n_parts; i += G) add(p.parts[(int64_t)i * p.rows + blockIdx.x * ROWS + c]);
     if constexpr (G > 1) {
+        static_assert(ROWS == 32 && G == 32, "a row's parts are the 32 lanes of half a wave then");
         parts[g][c] = make_float2(m, s);
         __syncthreads();
-        m = -INFINITY, s = 0.f;
-        if (g == 0)
-#pragma unroll 4
-            for (int i = 0; i < G; ++i) add(parts[i][c]);
+        const float2 x = parts[threadIdx.x & 31][threadIdx.x / 32];
+        m = x.x, s = x.y;
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) add(make_float2(__shfl_xor(m, off, 64), __shfl_xor(s, off, 64)));
     }
     float loss = 0.f;
     bool counts = false;
-    if (g == 0 && row < p.rows) {
+    if (says) {
         const float lse = m + logf(s);
-        const int64_t target = p.targets[row];
         counts = target != p.ignore;
         // (a target that is no token: no number comes of it)
-        if (counts) loss = target >= 0 && target < p.vocab ? lse - p.at_target[row] : NAN;
+        if (counts) loss = target >= 0 && target < p.vocab ? lse - at_target : NAN;
         p.lse[row] = lse;
         if (p.reduction == kCeNone) p.loss[row] = loss;
     }
     const uint64_t bits = __ballot(counts);
-    if (g == 0 && (threadIdx.x & 31) == 0 && row < p.rows) p.mask[row >> 5] = (uint32_t)(bits >> (threadIdx.x & 32));
+    if constexpr (G == 1) {
+        if ((threadIdx.x & 31) == 0 && row < p.rows) p.mask[row >> 5] = (uint32_t)(bits >> (threadIdx.x & 32));
+    }
     loss = lanes_sum<64>(loss);
-    if ((threadIdx.x & 63) == 0) totals[threadIdx.x >> 6] = make_float2(loss, (float)__popcll(bits));
+    if ((threadIdx.x & 63) == 0) totals[threadIdx.x >> 6] = make_float2(loss, (float)__popcll(bits)), two[threadIdx.x >> 6] = (uint32_t)(bits & 1) | (uint32_t)(bits >> 32 & 1) << 1;
     __syncthreads();
     if (threadIdx.x == 0) {
         float2 sum = totals[0];
         for (int i = 1; i < WAVES; ++i) sum.x += totals[i].x, sum.y += totals[i].y;
-        p.sums[2 * blockIdx.x] = sum.x;
-        p.sums[2 * blockIdx.x + 1] = sum.y;
-        __threadfence();
-        last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+        if constexpr (G > 1) {
+            uint32_t word = 0;
+            for (int i = 0; i < WAVES; ++i) word |= two[i] << (2 * i);
+            p.mask[blockIdx.x] = word;
+        }
+        if (p.reduction == kCeNone) {
+            last = 0;                            // (nobody asks for the sums)
+        } else {
+            p.sums[2 * blockIdx.x] = sum.x;
+            p.sums[2 * blockIdx.x + 1] = sum.y;
+            __threadfence();
+            last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+        }
     }
     __syncthreads();
     if (!last) return;
-    __threadfence();
+    // (atomic loads at the device's scope: what the other XCDs have written, past this one's cache)
     loss = 0.f;
     float count = 0.f;
     for (int i = threadIdx.x; i < (int)gridDim.x; i += ROWS * G) {
