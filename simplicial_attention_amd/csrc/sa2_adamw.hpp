@@ -90,16 +90,18 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamParams p) {
     const float gs = p.grad_scale ? *p.grad_scale : 1.f;
     const uint32_t key = mixed_bits(mixed_bits(step + 0x9e3779b9u * (p.index[which] + 1u)) ^ p.seed);
 
-    for (int64_t at = begin + threadIdx.x * 8; at - (int64_t)(threadIdx.x * 8) < end; at += 2048) {
-        const int count = (int)min((int64_t)8, end - at);          // (8-bit states: lanes behind the end go along in the reductions)
-        float g[8], x[8], m[8], v[8], root[8];
+    // (E consecutive elements a thread: four with fp32 states, whose accesses are whole lines of 16 bytes a lane then; eight of 8-bit ones)
+    constexpr int E = EIGHT ? 8 : 4;
+    for (int64_t at = begin + threadIdx.x * E; at - (int64_t)(threadIdx.x * E) < end; at += 256 * E) {
+        const int count = (int)min((int64_t)E, end - at);          // (8-bit states: lanes behind the end go along in the reductions)
+        float g[E], x[E], m[E], v[E], root[E];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = x[i] = m[i] = v[i] = 0.f;
+        for (int i = 0; i < E; ++i) g[i] = x[i] = m[i] = v[i] = 0.f;
         float ms = 0.f, vs = 0.f;
         if (count > 0) {
-            ld_some8<TP>(t.g + at * element_size<TP>, count, g);
-            if (t.master) ld_some8<kF32>(reinterpret_cast<const char *>(t.master + at), count, x);
-            else ld_some8<TP>(t.p + at * element_size<TP>, count, x);
+            ld_some<TP>(t.g + at * element_size<TP>, count, g);
+            if (t.master) ld_some<kF32>(reinterpret_cast<const char *>(t.master + at), count, x);
+            else ld_some<TP>(t.p + at * element_size<TP>, count, x);
             if constexpr (EIGHT) {
                 ms = t.ms[at >> 8];
                 vs = t.vs[at >> 8];
@@ -120,13 +122,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamParams p) {
                 unpack_e4m3(vw[0], v);
                 unpack_e4m3(vw[1], v + 4);
             } else {
-                ld_some8<kF32>(t.m + at * 4, count, m);
-                ld_some8<kF32>(t.v + at * 4, count, v);
+                ld_some<kF32>(t.m + at * 4, count, m);
+                ld_some<kF32>(t.v + at * 4, count, v);
             }
         }
         uint32_t m_most = 0, v_most = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < E; ++i) {
             if (p.grad_scale) g[i] *= gs;
             if constexpr (EIGHT) {
                 m[i] *= ms;
@@ -177,12 +179,12 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamParams p) {
                 }
             }
         } else if (count > 0) {
-            st_some8<kF32>(t.m + at * 4, count, m);
-            st_some8<kF32>(t.v + at * 4, count, v);
+            st_some<kF32>(t.m + at * 4, count, m);
+            st_some<kF32>(t.v + at * 4, count, v);
         }
         if (count > 0) {
-            if (t.master) st_some8<kF32>(reinterpret_cast<char *>(t.master + at), count, x);
-            st_some8<TP>(t.p + at * element_size<TP>, count, x);
+            if (t.master) st_some<kF32>(reinterpret_cast<char *>(t.master + at), count, x);
+            st_some<TP>(t.p + at * element_size<TP>, count, x);
         }
     }
 }

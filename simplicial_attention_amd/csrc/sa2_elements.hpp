@@ -119,6 +119,65 @@ __device__ __forceinline__ void st_some8(char *p, int count, const float (&v)[8]
     }
 }
 
+// the first `count` (1 .. N) of N = 4 or 8 elements
+template <int T, int N>
+__device__ __forceinline__ void ld_some(const char *p, int count, float (&v)[N]) {
+    if constexpr (N == 8) {
+        ld_some8<T>(p, count, v);
+    } else {
+        static_assert(N == 4, "pieces of four or eight");
+        if (count >= 4) {
+            if constexpr (T == kF32) {
+                const u32x4 w = ld_any16(p);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = as_f32(w[i]);
+            } else {
+                const u32x2 w = *reinterpret_cast<const u32x2_any *>(p);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if constexpr (T == kF16) {
+                        const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)w[i]);
+                        v[2 * i] = (float)h[0], v[2 * i + 1] = (float)h[1];
+                    } else {
+                        v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = i < count ? element_f32<T>(p + i * element_size<T>) : 0.f;
+        }
+    }
+}
+template <int T, int N>
+__device__ __forceinline__ void st_some(char *p, int count, const float (&v)[N]) {
+    if constexpr (N == 8) {
+        st_some8<T>(p, count, v);
+    } else {
+        if (count >= 4) {
+            if constexpr (T == kF32) {
+                st_any16(p, (u32x4){as_u32(v[0]), as_u32(v[1]), as_u32(v[2]), as_u32(v[3])});
+            } else {
+                u32x2 w;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if constexpr (T == kF16) {
+                        const f16x2 h = {(_Float16)v[2 * i], (_Float16)v[2 * i + 1]};
+                        w[i] = __builtin_bit_cast(uint32_t, h);
+                    } else {
+                        w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+                    }
+                }
+                *reinterpret_cast<u32x2_any *>(p) = w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < count) put_element<T>(p + i * element_size<T>, v[i]);
+        }
+    }
+}
+
 // four floats in e4m3, round to nearest even (v_cvt_pk_fp8_f32)
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);

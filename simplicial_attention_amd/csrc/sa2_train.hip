@@ -233,9 +233,9 @@ int sa2_adamw(const sa2_adamw_tensor *tensors, int64_t count, const sa2_adamw_st
     for (int type = 0; type < 3; ++type)
         for (int eight = 0; eight < 2; ++eight) {
             if (all[type][eight] == 0) continue;
-            // about eight workgroups per CU, chunks of 2048 to 65536 elements
+            // workgroups enough for a launch of some of the tensors to fill the chip several times over, chunks of 2048 to 16384 elements
             int64_t chunk = 2048;
-            while (chunk < 65536 && all[type][eight] > (double)chunk * 2048) chunk *= 2;
+            while (chunk < 16384 && all[type][eight] > (double)chunk * 16384) chunk *= 2;
             while (all[type][eight] / (double)chunk > (double)kMostGroups / 2) chunk *= 2;
             k.chunk = (int)chunk;
             k.count = 0;
