@@ -86,8 +86,13 @@ class HigherOrderAttention(nn.Module):
     def forward(self, tokens):
         return self.attend_with(tokens, self.attend)
 
-    def attend_with(self, tokens, attend):
-        tokens = self.prenorm(tokens)
+    def behind_norm(self, tokens):
+        """``forward`` of tokens that ``prenorm`` has been applied to."""
+        return self.attend_with(tokens, self.attend, normed=True)
+
+    def attend_with(self, tokens, attend, normed=False):
+        if not normed:
+            tokens = self.prenorm(tokens)
         qkv = apply_linear(self.to_qkv, tokens)
         if qkv.dim() == 3 and self._can_fuse(qkv):
             from .qkv_norm import fused_qkv_norm

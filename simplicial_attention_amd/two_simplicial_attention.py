@@ -180,9 +180,10 @@ class SlidingWindowTwoSimplicialMHA(HigherOrderAttention):
         self.w1, self.w2 = w1, w2
 
     @torch.no_grad()
-    def forward_cached(self, tokens, keys, values, batch):
+    def forward_cached(self, tokens, keys, values, batch, normed=False):
         """``forward`` for new tokens (b, n, dim) behind those in a paged cache: ``keys`` and ``values`` are the layer's two pools each, ``batch`` says
-        where the rows go (:meth:`PagedCache.extend`).  Rows beyond ``batch.counts`` are padding.  Queries, keys and values are rounded to the pools' dtype."""
+        where the rows go (:meth:`PagedCache.extend`).  Rows beyond ``batch.counts`` are padding.  Queries, keys and values are rounded to the pools' dtype.  ``normed``: ``prenorm`` has
+        been applied to the tokens."""
         from .paged import paged_append, paged_two_simplicial_attn
 
         def attend(q, k, v):
@@ -197,4 +198,4 @@ class SlidingWindowTwoSimplicialMHA(HigherOrderAttention):
             out = paged_two_simplicial_attn(q.to(pool.dtype), keys, values, *at, w1=self.w1, w2=self.w2, scale=dim ** -0.5, max_length=batch.max_length)
             return out[..., :v[0].shape[-1]].to(tokens.dtype)
 
-        return self.attend_with(tokens, attend)
+        return self.attend_with(tokens, attend, normed)

@@ -10,12 +10,16 @@ are library calls (``scaled_dot_product_attention``, ``Linear``); every
 """
 from __future__ import annotations
 
+from functools import partial
+
 import torch
 import torch.nn.functional as F
 from torch import nn
 
+from .cross_entropy import linear_cross_entropy
 from .linear import apply_linear
 from .paged import PagedCache, paged_append, paged_attn
+from .rms_norm import norm_behind
 from .sampling import sample_tokens
 from .two_simplicial_attention import SlidingWindowTwoSimplicialMHA
 
@@ -35,8 +39,11 @@ class Attention(nn.Module):
         self.to_out = nn.Linear(heads * dim_head, dim, bias=False)
 
     def forward(self, x):
+        return self.behind_norm(self.prenorm(x))
+
+    def behind_norm(self, x):
+        """``forward`` of rows that ``prenorm`` has been applied to."""
         b, n, _ = x.shape
-        x = self.prenorm(x)
         if torch.jit.is_scripting():      # (a scripted module takes its own submodules only)
             q, kv = self.to_q(x), self.to_kv(x)
         else:
@@ -54,11 +61,12 @@ class Attention(nn.Module):
 
     @torch.no_grad()
     @torch.jit.unused
-    def forward_cached(self, x, keys, values, batch):
+    def forward_cached(self, x, keys, values, batch, normed=False):
         """``forward`` for new tokens (b, n, dim) behind those in a paged cache: the layer's key and value pool (tuples of one), and where the rows go.  Queries, keys and
-        values are rounded to the pools' dtype."""
+        values are rounded to the pools' dtype.  ``normed``: ``prenorm`` has been applied to the rows."""
         b, n, _ = x.shape
-        x = self.prenorm(x)
+        if not normed:
+            x = self.prenorm(x)
         q = self.to_q(x).view(b, n, self.heads, self.dim_head)
         k, v = self.to_kv(x).view(b, n, 2, self.key_value_heads, self.dim_head).unbind(2)
         at = (batch.tables, batch.lengths, batch.counts)
@@ -79,6 +87,19 @@ class _Layers(nn.Sequential):
                 x = apply_linear(layer, x)
         return x
 
+    @torch.jit.unused
+    def behind_norm(self, x):
+        """``forward`` of rows that the norm in front has been applied to."""
+        for layer in self[1:]:
+            x = apply_linear(layer, x)
+        return x
+
+
+def _plain(module):
+    """Nobody sees the calls of this module."""
+    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks or module._compiled_call_impl is not None
+                or 'forward' in module.__dict__)
+
 
 def FeedForward(dim, expansion=4.):
     """RMSNorm -> Linear -> GELU -> Linear (two_simplicial_transformer.py:69-76)."""
@@ -87,10 +108,14 @@ def FeedForward(dim, expansion=4.):
 
 
 class TwoSimplicialTransformer(nn.Module):
+    """``fused`` (not an argument of the reference's): every residual's addition and the norm behind it are one pass over the rows (:func:`add_rms_norm`), with and without a
+    cache.  The same roundings; the norms' sums are in another order."""
+
     def __init__(self, dim, *, depth, heads=8, key_value_heads=4, dim_head=64, ff_expansion=4.,
                  two_simplicial_attn_every=4, attn_kwargs: dict | None = None,
-                 two_simplicial_attn_kwargs: dict | None = None, final_norm=True):
+                 two_simplicial_attn_kwargs: dict | None = None, final_norm=True, fused=False):
         super().__init__()
+        self.fused = fused
         attn_kwargs = {} if attn_kwargs is None else attn_kwargs
         if two_simplicial_attn_kwargs is None:
             two_simplicial_attn_kwargs = dict(w1=512, w2=32, qk_rmsnorm=True)
@@ -106,10 +131,30 @@ class TwoSimplicialTransformer(nn.Module):
         self.norm = nn.RMSNorm(dim) if final_norm else nn.Identity()
 
     def forward(self, x):
+        if not torch.jit.is_scripting():
+            if self._can_fuse():
+                return self._fused(x, [attn.behind_norm for attn, _ in self.layers])
         for attn, ff in self.layers:
             x = x + attn(x)
             x = x + ff(x)
         return self.norm(x)
+
+    @torch.jit.unused
+    def _can_fuse(self):
+        return (self.fused and not torch.jit.is_tracing() and not torch.compiler.is_compiling()
+                and all(_plain(attn) and _plain(ff) and type(ff) is _Layers and type(attn) in (Attention, SlidingWindowTwoSimplicialMHA) for attn, ff in self.layers))
+
+    @torch.jit.unused
+    def _fused(self, x, attend):
+        """The stack with every addition in front of the next norm; ``attend``: the layers' attention of normed rows."""
+        branch = None                        # what has yet to be added to x
+        for (attn, ff), of_normed in zip(self.layers, attend):
+            normed, x = norm_behind(attn.prenorm, x, None) if branch is None else norm_behind(attn.prenorm, branch, x)
+            normed, x = norm_behind(ff[0], of_normed(normed), x)
+            branch = ff.behind_norm(normed)
+        if branch is None:
+            return self.norm(x)
+        return norm_behind(self.norm, branch, x)[0]
 
     def cache(self, pages, page_size=64, dtype=None) -> PagedCache:
         """An empty cache for this stack's layers, on its device (in its dtype, or bfloat16 for float32 weights)."""
@@ -128,6 +173,9 @@ class TwoSimplicialTransformer(nn.Module):
     def forward_cached(self, x, cache, batch):
         """The stack for new tokens (b, n, dim) whose places ``batch = cache.extend(...)`` has made; rows beyond ``batch.counts`` are padding.  Queries, keys and values are
         rounded to the cache's dtype."""
+        if self._can_fuse():
+            return self._fused(x, [partial(attn.forward_cached, keys=keys, values=values, batch=batch, normed=True)
+                                   for (attn, _), keys, values in zip(self.layers, cache.keys, cache.values)])
         for (attn, ff), keys, values in zip(self.layers, cache.keys, cache.values):
             x = x + attn.forward_cached(x, keys, values, batch)
             x = x + ff(x)
@@ -136,11 +184,17 @@ class TwoSimplicialTransformer(nn.Module):
 
 class TwoSimplicialLM(nn.Module):
     """Token + learned position embedding, the stack above, and a linear read-out
-    (train.py:64-135).  ``generate`` answers prompts from a paged cache (the reference recomputes the sequence for every token)."""
+    (train.py:64-135).  ``generate`` answers prompts from a paged cache (the reference recomputes the sequence for every token).
+
+    ``fused`` (not an argument of the reference's): the stack's additions and norms in one pass each, and the loss of bfloat16 and float16 models without logits
+    (:func:`linear_cross_entropy`, which does not round them to that dtype in between)."""
 
     def __init__(self, *, num_tokens, dim, depth, max_seq_len=512, dim_head=64, heads=8,
-                 two_simplicial_attn_every=4, transformer_kwargs: dict | None = None):
+                 two_simplicial_attn_every=4, transformer_kwargs: dict | None = None, fused=False):
         super().__init__()
+        self.fused = fused
+        if fused:
+            transformer_kwargs = {'fused': True, **(transformer_kwargs or {})}
         self.token_emb = nn.Embedding(num_tokens, dim)
         self.pos_emb = nn.Embedding(max_seq_len, dim)
         self.transformer = TwoSimplicialTransformer(dim=dim, depth=depth, dim_head=dim_head, heads=heads,
@@ -154,10 +208,18 @@ class TwoSimplicialLM(nn.Module):
             x, target = x[:, :-1], x[:, 1:]
         positions = torch.arange(x.shape[-1], device=x.device)
         hidden = self.transformer(self.token_emb(x) + self.pos_emb(positions))
+        if target is not None and self._can_fuse(hidden):
+            return linear_cross_entropy(hidden, self.to_logits.weight, target)
         logits = apply_linear(self.to_logits, hidden)
         if target is None:
             return logits
         return F.cross_entropy(logits.flatten(0, 1).float(), target.flatten())
+
+    def _can_fuse(self, hidden):
+        weight = self.to_logits.weight
+        return (self.fused and type(self.to_logits) is nn.Linear and self.to_logits.bias is None and _plain(self.to_logits) and hidden.is_cuda and hidden.device == weight.device
+                and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.dtype == weight.dtype and not torch.is_autocast_enabled() and not torch.jit.is_tracing()
+                and not torch.compiler.is_compiling())
 
     @torch.no_grad()
     def logits_cached(self, x, cache, batch, rows=None):
