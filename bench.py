@@ -332,31 +332,37 @@ def time_raw_workload(name, steps=5, warmup=2):
 def time_train_cfg5(steps=5, warmup=2):
     """benchmark config 5: one training step (forward, loss, backward, Adam) of the byte-level LM: depth 12, dim 512,
     8 heads of 64 (4 key/value heads), every 2nd layer simplicial (w1=512, w2=32), batch 8 x 2048 random bytes; and the
-    share of the six simplicial attention cores (the same Function at the layer's shape, timed alone)."""
+    share of the six simplicial attention cores (the same Function at the layer's shape, timed alone).  Then the same step of the fused
+    model with the package's AdamW (32-bit states and masters)."""
     import torch
-    from simplicial_attention_amd import sliding_two_simplicial_attn
+    from simplicial_attention_amd import AdamW, sliding_two_simplicial_attn
     from simplicial_attention_amd.two_simplicial_transformer import TwoSimplicialLM
     dev = torch.device('cuda:0')
     torch.manual_seed(4)
-    lm = TwoSimplicialLM(num_tokens=256, dim=512, depth=12, max_seq_len=2048, dim_head=64, heads=8,
-                         two_simplicial_attn_every=2, transformer_kwargs=dict(key_value_heads=4)).bfloat16().to(dev)
-    opt = torch.optim.Adam(lm.parameters(), lr=1e-4)
     tokens = torch.randint(0, 256, (8, 2049), device=dev)
 
-    def train_step():
-        opt.zero_grad(set_to_none=True)
-        loss = lm(tokens, return_loss=True)
-        loss.backward()
-        opt.step()
-        return loss
-    for _ in range(max(2, warmup)):
-        train_step()
-    torch.cuda.synchronize()
-    t0 = time.perf_counter()
-    for _ in range(steps):
-        loss = train_step()
-    torch.cuda.synchronize()
-    step_ms = (time.perf_counter() - t0) / steps * 1e3
+    def timed(fused):
+        torch.manual_seed(4)
+        lm = TwoSimplicialLM(num_tokens=256, dim=512, depth=12, max_seq_len=2048, dim_head=64, heads=8,
+                             two_simplicial_attn_every=2, transformer_kwargs=dict(key_value_heads=4), fused=fused).bfloat16().to(dev)
+        opt = AdamW(lm.parameters(), lr=1e-4) if fused else torch.optim.Adam(lm.parameters(), lr=1e-4)
+
+        def train_step():
+            opt.zero_grad(set_to_none=True)
+            loss = lm(tokens, return_loss=True)
+            loss.backward()
+            opt.step()
+            return loss
+        for _ in range(max(2, warmup)):
+            train_step()
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for _ in range(steps):
+            loss = train_step()
+        torch.cuda.synchronize()
+        return (time.perf_counter() - t0) / steps * 1e3, loss.item()
+    step_ms, loss = timed(False)
+    fused_ms, fused_loss = timed(True)
     mk5 = lambda h: (torch.randn(8, 2048, h, 64, device=dev) * 0.125).bfloat16().requires_grad_(True)
     q5, k15, k25, v15, v25 = mk5(8), mk5(4), mk5(4), mk5(4), mk5(4)
     do5 = torch.randn(8, 2048, 8, 64, device=dev).bfloat16()
@@ -373,10 +379,10 @@ def time_train_cfg5(steps=5, warmup=2):
     torch.cuda.synchronize()
     core_ms = (time.perf_counter() - t0) / 10 * 1e3
     res = {'workload': 'cfg5_training_step_depth12_dim512_b8_n2048', 'ms_per_step': round(step_ms, 3),
-           'tokens_per_s': round(8 * 2048 / step_ms * 1e3, 1), 'loss': round(loss.item(), 4),
+           'tokens_per_s': round(8 * 2048 / step_ms * 1e3, 1), 'loss': round(loss, 4),
+           'fused_ms_per_step': round(fused_ms, 3), 'fused_loss': round(fused_loss, 4),
            'simplicial_core_fwd_bwd_ms_per_layer': round(core_ms, 3),
            'simplicial_cores_share_of_step': round(6 * core_ms / step_ms, 3), 'steps': steps}
-    del lm, opt
     torch.cuda.empty_cache()
     return res
 
