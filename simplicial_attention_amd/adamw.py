@@ -58,15 +58,14 @@ class AdamW(torch.optim.Optimizer):
 
     def _state_of(self, param, group):
         state = self.state[param]
-        if not state:
-            state['step'] = 0
-            for name in ('exp_avg', 'exp_avg_sq'):
-                if group['state_bits'] == 8 and param.numel() >= group['min_8bit_size']:
-                    state[name], state[name + '_scales'] = state_8bit(param)
-                else:
-                    state[name] = torch.zeros_like(param, dtype=torch.float32, memory_format=torch.preserve_format)
-            if group['masters'] and param.dtype is not torch.float32:
-                state['master'] = param.detach().to(torch.float32, copy=True, memory_format=torch.preserve_format)
+        state['step'] = 0
+        for name in ('exp_avg', 'exp_avg_sq'):
+            if group['state_bits'] == 8 and param.numel() >= group['min_8bit_size']:
+                state[name], state[name + '_scales'] = state_8bit(param)
+            else:
+                state[name] = torch.zeros_like(param, dtype=torch.float32, memory_format=torch.preserve_format)
+        if group['masters'] and param.dtype is not torch.float32:
+            state['master'] = param.detach().to(torch.float32, copy=True, memory_format=torch.preserve_format)
         return state
 
     @torch.no_grad()
@@ -77,26 +76,35 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for index, group in enumerate(self.param_groups):
-            by_step: dict = {}
+            capturable, by_step = group['capturable'], {}
             for param in group['params']:
-                if param.grad is None:
-                    if group['capturable']:
+                grad = param.grad
+                if grad is None:
+                    if capturable:
                         raise RuntimeError('a group that can be captured needs gradients of all its parameters')
                     continue
-                state = self._state_of(param, group)
-                if not group['capturable']:
+                state = self.state[param] or self._state_of(param, group)
+                if not capturable:
                     state['step'] += 1
-                by_step.setdefault(state['step'], []).append((param, state))
-            if group['capturable'] and by_step:
+                lists = by_step.get(state['step'])
+                if lists is None:
+                    lists = by_step[state['step']] = ([], [], [], [], [])
+                lists[0].append(param)
+                lists[1].append(grad)
+                if 'exp_avg_scales' in state:
+                    lists[2].append((state['exp_avg'], state['exp_avg_scales']))
+                    lists[3].append((state['exp_avg_sq'], state['exp_avg_sq_scales']))
+                else:
+                    lists[2].append(state['exp_avg'])
+                    lists[3].append(state['exp_avg_sq'])
+                lists[4].append(state.get('master'))
+            if capturable and by_step:
                 if 'step_at' not in group:
                     group['step_at'] = torch.zeros(1, dtype=torch.int64, device=group['params'][0].device)
                 group['step_at'] += 1
-            for step, members in by_step.items():
-                pair = lambda state, name: (state[name], state[name + '_scales']) if name + '_scales' in state else state[name]
-                adamw_step([p for p, _ in members], [p.grad for p, _ in members], [pair(s, 'exp_avg') for _, s in members],
-                           [pair(s, 'exp_avg_sq') for _, s in members], masters=[s.get('master') for _, s in members],
-                           step=group['step_at'] if group['capturable'] else step, lr=group['lr'], betas=group['betas'], eps=group['eps'],
-                           weight_decay=group['weight_decay'], grad_scale=grad_scale, seed=group['seed'] + 0x10000 * index)
+            for step, (params, grads, averages, squares, masters) in by_step.items():
+                adamw_step(params, grads, averages, squares, masters=masters, step=group['step_at'] if capturable else step, lr=group['lr'], betas=group['betas'],
+                           eps=group['eps'], weight_decay=group['weight_decay'], grad_scale=grad_scale, seed=group['seed'] + 0x10000 * index)
         return loss
 
     @torch.no_grad()

@@ -281,61 +281,81 @@ Tensor linear_cross_entropy(const Tensor &hidden, const Tensor &weight, const Te
     return LinearCE::run(LinearCE::checked(hidden, weight, targets, ignore_index, reduction), targets, nullptr);
 }
 
-// ---- AdamW
-const Tensor &tensor_of(const py::handle &h, const char *name) {
-    if (!THPVariable_Check(h.ptr())) raise(PyExc_TypeError, std::string(name) + " must be tensors");
-    return THPVariable_Unpack(h.ptr());
+// ---- AdamW (lists of a hundred tensors and more: what is done per tensor is kept small)
+const Tensor &tensor_of(PyObject *x, const char *name) {
+    if (!THPVariable_Check(x)) raise(PyExc_TypeError, std::string(name) + " must be tensors");
+    return THPVariable_Unpack(x);
 }
 
 bool laid_out_alike(const Tensor &a, const Tensor &b) {
     return a.sizes() == b.sizes() && ((a.is_contiguous() && b.is_contiguous()) || a.strides() == b.strides());
 }
 
-void adamw_step(const py::sequence &params, const py::sequence &grads, const py::sequence &averages, const py::sequence &squares, const std::optional<py::sequence> &masters,
+// a list or tuple by its items (borrowed; the sequence lives as long as this)
+struct Items {
+    py::object held;
+    PyObject **at = nullptr;
+    size_t count = 0;
+    explicit Items(const py::handle &x, const char *name) {
+        held = py::reinterpret_steal<py::object>(PySequence_Fast(x.ptr(), name));
+        if (!held) throw py::error_already_set();
+        at = PySequence_Fast_ITEMS(held.ptr());
+        count = (size_t)PySequence_Fast_GET_SIZE(held.ptr());
+    }
+};
+
+void adamw_step(const py::object &params_in, const py::object &grads_in, const py::object &averages_in, const py::object &squares_in, const py::object &masters_in,
                 const py::object &step, const py::object &lr, double beta1, double beta2, double eps, double weight_decay, const MaybeTensor &grad_scale, int64_t seed) {
-    const size_t count = params.size();
-    if (grads.size() != count || averages.size() != count || squares.size() != count || (masters && masters->size() != count))
+    const Items params(params_in, "params must be a sequence of tensors"), grads(grads_in, "grads must be a sequence of tensors"),
+        states[2] = {Items(averages_in, "exp_avgs must be a sequence"), Items(squares_in, "exp_avg_sqs must be a sequence")};
+    std::optional<Items> masters;
+    if (!masters_in.is_none()) masters.emplace(masters_in, "masters must be a sequence");
+    const size_t count = params.count;
+    if (grads.count != count || states[0].count != count || states[1].count != count || (masters && masters->count != count))
         raise(PyExc_ValueError, "as many gradients, states and masters as parameters are required");
     std::vector<sa2_adamw_tensor> items;
-    std::vector<Tensor> alive, written;
+    std::vector<Tensor> alive;
+    std::vector<c10::TensorImpl *> written;
     items.reserve(count);
-    written.reserve(4 * count);
+    written.reserve(6 * count);
+    static const c10::DispatchKeySet others({c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Python,
+                                             c10::DispatchKey::Functionalize});
     std::optional<at::Device> device;
     auto on_device = [&](const Tensor &t) {
         if (!t.is_cuda()) raise(PyExc_AssertionError, "adamw_step runs on the GPU only");
         if (!device) device = t.device();
         if (t.device() != *device) raise(PyExc_ValueError, "adamw_step: tensors on " + device->str() + " and " + t.device().str());
-        refuse_foreign("adamw_step", {&t});
+        if (t.key_set().has_any(others)) refuse_foreign("adamw_step", {&t});
     };
     for (size_t i = 0; i < count; ++i) {
-        const Tensor &p = tensor_of(params[i], "parameters");
-        Tensor g = tensor_of(grads[i], "gradients");
+        const Tensor &p = tensor_of(params.at[i], "parameters"), &given = tensor_of(grads.at[i], "gradients");
         on_device(p);
-        on_device(g);
-        if (element_of(p) < 0 || g.scalar_type() != p.scalar_type()) raise(PyExc_TypeError, "parameters are bfloat16, float16 or float32, and gradients of the same dtype");
-        if (p.layout() != at::kStrided || g.layout() != at::kStrided || !p.is_non_overlapping_and_dense()) raise(PyExc_ValueError, "parameters and gradients must be dense: " + shape_text(p));
-        if (g.sizes() != p.sizes()) raise(PyExc_ValueError, "gradient " + shape_text(g) + " does not match its parameter's " + shape_text(p));
-        if (!laid_out_alike(p, g)) {
-            const c10::DeviceGuard guard(p.device());
-            const at::NoGradGuard no_grad;
-            g = at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g);
-            alive.push_back(g);
-        }
+        on_device(given);
+        if (element_of(p) < 0 || given.scalar_type() != p.scalar_type()) raise(PyExc_TypeError, "parameters are bfloat16, float16 or float32, and gradients of the same dtype");
+        if (p.layout() != at::kStrided || given.layout() != at::kStrided || !p.is_non_overlapping_and_dense())
+            raise(PyExc_ValueError, "parameters and gradients must be dense: " + shape_text(p));
+        if (given.sizes() != p.sizes()) raise(PyExc_ValueError, "gradient " + shape_text(given) + " does not match its parameter's " + shape_text(p));
         sa2_adamw_tensor t{};
         t.param = p.data_ptr();
-        t.grad = g.data_ptr();
+        if (laid_out_alike(p, given)) {
+            t.grad = given.data_ptr();
+        } else {
+            const c10::DeviceGuard guard(p.device());
+            const at::NoGradGuard no_grad;
+            alive.push_back(at::empty_strided(p.sizes(), p.strides(), given.options()).copy_(given));
+            t.grad = alive.back().data_ptr();
+        }
         t.n = p.numel();
         t.type = element_of(p);
-        written.push_back(p);
-        const bool eight = PyTuple_Check(py::object(averages[i]).ptr());
-        if (eight != (bool)PyTuple_Check(py::object(squares[i]).ptr())) raise(PyExc_TypeError, "both states of a parameter are tensors, or (values, scales) pairs");
+        written.push_back(p.unsafeGetTensorImpl());
+        const bool eight = PyTuple_Check(states[0].at[i]);
+        if (eight != (bool)PyTuple_Check(states[1].at[i])) raise(PyExc_TypeError, "both states of a parameter are tensors, or (values, scales) pairs");
         t.bits = eight ? 8 : 32;
         for (int which = 0; which < 2; ++which) {
-            const py::object state = which ? squares[i] : averages[i];
+            PyObject *const state = states[which].at[i];
             if (eight) {
-                const py::tuple pair = state;
-                if (pair.size() != 2) raise(PyExc_TypeError, "states in 8 bits are (values, scales) pairs");
-                const Tensor &values = tensor_of(pair[0], "states"), &scales = tensor_of(pair[1], "scales");
+                if (PyTuple_GET_SIZE(state) != 2) raise(PyExc_TypeError, "states in 8 bits are (values, scales) pairs");
+                const Tensor &values = tensor_of(PyTuple_GET_ITEM(state, 0), "states"), &scales = tensor_of(PyTuple_GET_ITEM(state, 1), "scales");
                 on_device(values);
                 on_device(scales);
                 if (values.scalar_type() != at::kFloat8_e4m3fn || scales.scalar_type() != at::kFloat) raise(PyExc_TypeError, "states in 8 bits are float8_e4m3fn values and float32 scales");
@@ -343,24 +363,24 @@ void adamw_step(const py::sequence &params, const py::sequence &grads, const py:
                     raise(PyExc_ValueError, "states " + shape_text(values) + " with scales " + shape_text(scales) + " do not match a parameter " + shape_text(p) + ": contiguous, one scale for 256 elements");
                 (which ? t.exp_avg_sq : t.exp_avg) = values.data_ptr();
                 (which ? t.exp_avg_sq_scales : t.exp_avg_scales) = static_cast<float *>(scales.data_ptr());
-                written.push_back(values);
-                written.push_back(scales);
+                written.push_back(values.unsafeGetTensorImpl());
+                written.push_back(scales.unsafeGetTensorImpl());
             } else {
                 const Tensor &values = tensor_of(state, "states");
                 on_device(values);
                 if (values.scalar_type() != at::kFloat) raise(PyExc_TypeError, "states are float32 tensors, or (values, scales) pairs in 8 bits");
                 if (!laid_out_alike(p, values)) raise(PyExc_ValueError, "state " + shape_text(values) + " is not laid out as its parameter " + shape_text(p));
                 (which ? t.exp_avg_sq : t.exp_avg) = values.data_ptr();
-                written.push_back(values);
+                written.push_back(values.unsafeGetTensorImpl());
             }
         }
-        if (masters && !py::object((*masters)[i]).is_none()) {
-            const Tensor &m = tensor_of((*masters)[i], "masters");
+        if (masters && masters->at[i] != Py_None) {
+            const Tensor &m = tensor_of(masters->at[i], "masters");
             on_device(m);
             if (m.scalar_type() != at::kFloat) raise(PyExc_TypeError, "masters are float32");
             if (!laid_out_alike(p, m)) raise(PyExc_ValueError, "master " + shape_text(m) + " is not laid out as its parameter " + shape_text(p));
             t.master = static_cast<float *>(m.data_ptr());
-            written.push_back(m);
+            written.push_back(m.unsafeGetTensorImpl());
         }
         items.push_back(t);
     }
@@ -396,7 +416,7 @@ void adamw_step(const py::sequence &params, const py::sequence &grads, const py:
     const c10::DeviceGuard guard(*device);
     check(sa2_adamw(items.data(), (int64_t)items.size(), &s, c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device->index()).stream()));
     // (a graph that saved one of these sees that it has changed)
-    for (const Tensor &t : written) t.unsafeGetTensorImpl()->bump_version();
+    for (c10::TensorImpl *t : written) t->bump_version();
 }
 
 }  // namespace

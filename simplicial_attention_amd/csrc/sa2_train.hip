@@ -175,20 +175,22 @@ int sa2_adamw(const sa2_adamw_tensor *tensors, int64_t count, const sa2_adamw_st
     try {
         // what a step writes: no two of these may share memory (workgroups run in no order)
         std::vector<std::pair<uintptr_t, uintptr_t>> written;
-        written.reserve(4 * count);
+        written.reserve(6 * count);
         for (int64_t i = 0; i < count; ++i) {
             const sa2_adamw_tensor &t = tensors[i];
             if (t.n < 1 || t.n > (int64_t)1 << 40 || t.type < 0 || t.type > 2) continue;      // (refused, or skipped, below)
-            const int64_t state = t.bits == 8 ? t.n : 4 * t.n;
+            const int64_t state = t.bits == 8 ? t.n : 4 * t.n, scales = t.bits == 8 ? (t.n + 255) / 256 * 4 : 0;
             const auto add = [&](const void *at, int64_t bytes) {
-                if (at) written.emplace_back(reinterpret_cast<uintptr_t>(at), reinterpret_cast<uintptr_t>(at) + bytes);
+                if (at && bytes) written.emplace_back(reinterpret_cast<uintptr_t>(at), reinterpret_cast<uintptr_t>(at) + bytes);
             };
             add(t.param, t.n * size_of(t.type));
             add(t.exp_avg, state);
             add(t.exp_avg_sq, state);
+            add(t.exp_avg_scales, scales);
+            add(t.exp_avg_sq_scales, scales);
             add(t.master, 4 * t.n);
         }
-        std::sort(written.begin(), written.end());
+        std::sort(written.begin(), written.end(), [](const auto &a, const auto &b) { return a.first < b.first; });
         for (size_t i = 1; i < written.size(); ++i)
             if (written[i].first < written[i - 1].second) return fail_with(SA2_ERR_BAD_SHAPE, "parameters, masters or states share memory: each may be in the list once");
     } catch (const std::bad_alloc &) {
