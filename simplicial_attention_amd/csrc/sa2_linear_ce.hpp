@@ -49,42 +49,42 @@ constexpr float ce_log2_scale = T == kF16 ? 10.f : 0.f;
 
 // ---- forward: a tile of logits
 
-template <int T, int NB>
-__global__ __launch_bounds__(256) void ce_logits_kernel(CeParams p) {
-    using P = Product<T, NB, true, true, false>;
+template <int T, int NL, int NR>
+__global__ __launch_bounds__(256, NL == 4 ? 1 : 2) void ce_logits_kernel(CeParams p) {
+    using P = Product<T, NL, NR, true, true, false>;
     __shared__ __attribute__((aligned(16))) char lds[P::LDS];
     const ProductPlace at = product_place(p.shape);
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
-    f32x16 acc[NB][NB];
+    f32x16 acc[NL][NR];
     P::run(p.shape, p.w, p.h, at, nullptr, lds, acc);
     const int lane = threadIdx.x & 63, wave = wave_index(), hf = lane >> 5;
-    const int v0 = at.tile_r * P::TILE + 32 * NB * (wave & 1);
-    const bool ragged = v0 + 32 * NB > p.vocab;
+    const int v0 = at.tile_r * P::TILE_R + 32 * NR * (wave & 1);
+    const bool ragged = v0 + 32 * NR > p.vocab;
 #pragma unroll
-    for (int a = 0; a < NB; ++a) {
-        const int row = at.tile_l * P::TILE + 32 * (NB * (wave >> 1) + a) + dmap_row(lane & 31);
+    for (int a = 0; a < NL; ++a) {
+        const int row = at.tile_l * P::TILE_L + 32 * (NL * (wave >> 1) + a) + dmap_row(lane & 31);
         take(acc[a]);
         if (ragged) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NR; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (v0 + 32 * b + 16 * hf + r >= p.vocab) acc[a][b][r] = -INFINITY;
         }
         const int64_t target = row < p.rows ? p.targets[row] : -1;
-        const int mine = target >= v0 && target < v0 + 32 * NB && target < p.vocab ? (int)(target - v0) : -1;
+        const int mine = target >= v0 && target < v0 + 32 * NR && target < p.vocab ? (int)(target - v0) : -1;
         if (wave_any(mine >= 0)) {
             const int here = mine - 16 * hf;
             float x = 0.f;
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NR; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x = here == 32 * b + r ? acc[a][b][r] : x;
             if (mine >= 0 && (mine >> 4 & 1) == hf) p.at_target[row] = x;
         }
         float m = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NR; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[a][b][r]);
         m = fmaxf(m, __shfl_xor(m, 32, 64));
@@ -93,12 +93,12 @@ __global__ __launch_bounds__(256) void ce_logits_kernel(CeParams p) {
         const bool far = fabsf(ref) > kCeFar;            // (a row's own matter: its neighbours' results do not depend on it)
         if (wave_any(far)) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NR; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s += fast_exp2(far ? (acc[a][b][r] - ref) * kLog2e : acc[a][b][r] * kLog2e - ref2);
         } else {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NR; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s += fast_exp2(acc[a][b][r] * kLog2e - ref2);
         }
@@ -221,20 +221,20 @@ __device__ __forceinline__ float ce_factor(const CeParams &p) {
     return *p.up * (1.f / ce_scale<T>);
 }
 
-template <int T, int NB>
-__global__ __launch_bounds__(256) void ce_dz_kernel(CeParams p) {
-    using P = Product<T, NB, true, true, false>;
+template <int T, int NL, int NR>
+__global__ __launch_bounds__(256, NL == 4 ? 1 : 2) void ce_dz_kernel(CeParams p) {
+    using P = Product<T, NL, NR, true, true, false>;
     __shared__ __attribute__((aligned(16))) char lds[P::LDS];
     const ProductPlace at = product_place(p.shape);
-    f32x16 acc[NB][NB];
+    f32x16 acc[NL][NR];
     P::run(p.shape, p.w, p.h, at, nullptr, lds, acc);
     const int lane = threadIdx.x & 63, wave = wave_index(), hf = lane >> 5;
-    const int c0 = at.tile_r * P::TILE + 32 * NB * (wave & 1);           // column of the piece
+    const int c0 = at.tile_r * P::TILE_R + 32 * NR * (wave & 1);           // column of the piece
     __syncthreads();                                                     // (the tiles have been read)
-    const ProductRows<T, NB> rows(lds);
+    const ProductRows<T, NR> rows(lds);
 #pragma unroll
-    for (int a = 0; a < NB; ++a) {
-        const int row0 = at.tile_l * P::TILE + 32 * (NB * (wave >> 1) + a), row = min(row0 + rows.row, p.rows - 1);
+    for (int a = 0; a < NL; ++a) {
+        const int row0 = at.tile_l * P::TILE_L + 32 * (NL * (wave >> 1) + a), row = min(row0 + rows.row, p.rows - 1);
         const int64_t target = p.targets[row];
         const bool counts = target != p.ignore;
         const float ref = p.lse[row], ref2 = ref * kLog2e - ce_log2_scale<T>;
@@ -243,20 +243,20 @@ __global__ __launch_bounds__(256) void ce_dz_kernel(CeParams p) {
         // (what only some rows or tiles need is asked of the wave: a tile in the middle takes a multiply-add, an exponential and half a packing per element)
         if (wave_any(far)) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NR; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[a][b][r] = fast_exp2(far ? (acc[a][b][r] - ref) * kLog2e + ce_log2_scale<T> : acc[a][b][r] * kLog2e - ref2);
         } else {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NR; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[a][b][r] = fast_exp2(acc[a][b][r] * kLog2e - ref2);
         }
         const int64_t from = p.first + c0;
-        const int mine = counts && target >= from && target < from + 32 * NB ? (int)(target - from) - 16 * hf : -100;
+        const int mine = counts && target >= from && target < from + 32 * NR ? (int)(target - from) - 16 * hf : -100;
         if (wave_any(mine > -100)) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NR; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (mine == 32 * b + r) acc[a][b][r] -= ce_scale<T>;
@@ -269,20 +269,20 @@ __global__ __launch_bounds__(256) void ce_dz_kernel(CeParams p) {
         if (counts && !(target >= 0 && target < p.vocab)) weight = NAN;
         if (wave_any(weight != 1.f)) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NR; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[a][b][r] *= weight;
         }
         const int end = p.vocab - p.first - c0 - 16 * hf;                // columns of this half that are tokens
-        if (wave_any(!counts || end < 32 * NB)) {
+        if (wave_any(!counts || end < 32 * NR)) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NR; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (!counts || 32 * b + r >= end) acc[a][b][r] = 0.f;
         }
 #pragma unroll
-        for (int b = 0; b < NB; ++b) rows.put(b, acc[a][b]);
+        for (int b = 0; b < NR; ++b) rows.put(b, acc[a][b]);
         rows.each([&](int r, int col, u32x4 v) {
             if (row0 + r < p.rows) st_global16(p.dz + (int64_t)(row0 + r) * p.dz_row + 2 * (c0 + col), v);
         });
@@ -297,20 +297,20 @@ struct CeOutput {
     int masked;                    // rows that do not count become zero
 };
 
-template <int T, int NB, bool DIRECT>
-__device__ __forceinline__ void ce_store(const CeParams &p, const CeOutput &o, const ProductPlace &at, char *lds, f32x16 (&acc)[NB][NB]) {
+template <int T, int NL, int NR, bool DIRECT>
+__device__ __forceinline__ void ce_store(const CeParams &p, const CeOutput &o, const ProductPlace &at, char *lds, f32x16 (&acc)[NL][NR]) {
     const int wave = wave_index();
-    const int c0 = 64 * NB * at.tile_r + 32 * NB * (wave & 1);
+    const int c0 = 64 * NR * at.tile_r + 32 * NR * (wave & 1);
     char *const out = DIRECT ? o.out : reinterpret_cast<char *>(o.parts + (int64_t)at.share * o.rows * p.dim);
     const float factor = DIRECT ? ce_factor<T>(p) : 1.f;
     __syncthreads();                              // (the tiles have been read)
-    const ProductRows<DIRECT ? T : kF32, NB> rows(lds);
+    const ProductRows<DIRECT ? T : kF32, NR> rows(lds);
 #pragma unroll
-    for (int a = 0; a < NB; ++a) {
-        const int row0 = 64 * NB * at.tile_l + 32 * (NB * (wave >> 1) + a);
+    for (int a = 0; a < NL; ++a) {
+        const int row0 = 64 * NL * at.tile_l + 32 * (NL * (wave >> 1) + a);
         take(acc[a]);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) rows.put(b, acc[a][b], factor);
+        for (int b = 0; b < NR; ++b) rows.put(b, acc[a][b], factor);
         rows.each([&](int r, int col, u32x4 v) {
             const int row = row0 + r, d = c0 + col;
             if (row >= o.rows || d >= p.dim) return;
@@ -327,25 +327,25 @@ __device__ __forceinline__ void ce_store(const CeParams &p, const CeOutput &o, c
 }
 
 // dH of a piece: rows x dim, contracted over the piece's tokens (r side: W read along dim)
-template <int T, int NB, bool DIRECT>
-__global__ __launch_bounds__(256) void ce_dh_kernel(CeParams p, CeOutput o) {
-    using P = Product<T, NB, false, true, false>;
+template <int T, int NL, int NR, bool DIRECT>
+__global__ __launch_bounds__(256, NL == 4 ? 1 : 2) void ce_dh_kernel(CeParams p, CeOutput o) {
+    using P = Product<T, NL, NR, false, true, false>;
     __shared__ __attribute__((aligned(16))) char lds[P::LDS];
     const ProductPlace at = product_place(p.shape);
-    f32x16 acc[NB][NB];
+    f32x16 acc[NL][NR];
     P::run(p.shape, p.w, p.h, at, nullptr, lds, acc);
-    ce_store<T, NB, DIRECT>(p, o, at, lds, acc);
+    ce_store<T, NL, NR, DIRECT>(p, o, at, lds, acc);
 }
 
 // dW of a piece: tokens x dim, contracted over the rows that count
-template <int T, int NB, bool DIRECT>
-__global__ __launch_bounds__(256) void ce_dw_kernel(CeParams p, CeOutput o) {
-    using P = Product<T, NB, false, false, true>;
+template <int T, int NL, int NR, bool DIRECT>
+__global__ __launch_bounds__(256, NL == 4 ? 1 : 2) void ce_dw_kernel(CeParams p, CeOutput o) {
+    using P = Product<T, NL, NR, false, false, true>;
     __shared__ __attribute__((aligned(16))) char lds[P::LDS];
     const ProductPlace at = product_place(p.shape);
-    f32x16 acc[NB][NB];
+    f32x16 acc[NL][NR];
     P::run(p.shape, p.w, p.h, at, p.mask, lds, acc);
-    ce_store<T, NB, DIRECT>(p, o, at, lds, acc);
+    ce_store<T, NL, NR, DIRECT>(p, o, at, lds, acc);
 }
 
 // the shares added in order, four elements a thread

@@ -16,34 +16,48 @@ constexpr int64_t kMostDzBytes = (int64_t)256 << 20;      // of a piece of dz, w
 
 int64_t up_to(int64_t x, int64_t unit) { return (x + unit - 1) / unit * unit; }
 
-// the tile (NB: 64 NB x 64 NB) and the shares of a product of l x r results over k
+// the tile (64 nl x 64 nr) and the shares of a product of l x r results over k
 struct ProductPlan {
-    int nb = 2;
+    int nl = 0, nr = 0;
     ProductShape shape{};
     int64_t groups() const { return (int64_t)shape.tiles_r * shape.tiles_l * shape.shares; }
 };
 
-// Of the tiles and shares whose workgroups fill the chip, those with the least estimated time.  A step of 256 x 256 takes a CU 0.83 us at the power that the
-// matrix units draw (1.25 PFLOP/s over all), a workgroup of 256 x 256 9 us more (first loads, epilogue); two workgroups of 128 x 128 on a CU take 0.52 us a step and 4.5 us,
-// one alone 0.30 us a step.  Shares write and read their fp32 results (4 TB/s, and a launch).  Measured: gradient of 4096 rows of 1024 channels over 50021 tokens 386 us in
-// 256 x 256 with four shares, 467 in 128 x 128 with two; of 1237 rows of 328 channels over 10007 tokens 38 and 24 us.
-ProductPlan plan_of(int64_t l, int64_t r, int64_t k, bool shared, bool masked) {
+// What a workgroup takes, in us: a step with few others on the chip, with one on each CU, with as many as fit (the matrix units' power is shared); and the
+// first loads and the epilogue.  Measured: logits of 8192 x 32000 over 512 channels 301 us in 128 x 256 (256 x 256: 325, 128 x 128: 373), of 300 x 40000 over 4096 144
+// (197, 168); weight's gradient of 25024 x 1024 over 4096 rows 193 us in 256 x 256 (222, 235).
+struct ProductCost {
+    int nl, nr, per_cu;
+    double few, each, most, fixed;
+};
+// (operands of rows of k; where one is read transposed out of LDS 128 x 256 is slower)
+constexpr ProductCost kRowCosts[3] = {{2, 2, 2, 0.28, 0.31, 0.60, 4.2}, {2, 4, 2, 0.45, 0.51, 0.95, 4.5}, {4, 4, 1, 0.65, 0.83, 0.83, 7}};
+constexpr ProductCost kTransposedCosts[3] = {{2, 2, 2, 0.28, 0.31, 0.58, 4.2}, {2, 4, 2, 0.55, 0.65, 1.15, 5}, {4, 4, 1, 0.65, 0.83, 0.83, 7}};
+
+double product_us(const ProductCost &c, int64_t groups, int64_t steps) {
+    const int64_t slots = 256 * c.per_cu, rest = groups % slots;
+    // (where some CUs have two, their time counts)
+    const double step = rest <= 256 ? c.few + (c.each - c.few) * (double)rest / 256 : c.most * (0.85 + 0.15 * (double)(rest - 256) / 256);
+    return (double)(groups / slots) * ((double)steps * c.most + c.fixed) + (rest ? (double)steps * step + c.fixed : 0);
+}
+
+// Of the tiles and shares that there are, those with the least estimated time.  Shares write and read their fp32 results (4 TB/s, and a launch).
+// `gradient`: not of the logits, which are not shared.
+ProductPlan plan_of(int64_t l, int64_t r, int64_t k, bool gradient, bool masked) {
     ProductPlan best;
     double least = 0;
     const int64_t steps = (k + 31) / 32;
-    for (const int nb : {2, 4})
-        for (int64_t shares = 1; shares <= (shared ? 64 : 1) && (shares == 1 || steps / shares >= 4); shares += shares < 8 ? 1 : shares / 4) {
-            const int64_t t = 64 * nb, tiles_l = (l + t - 1) / t, tiles_r = (r + t - 1) / t;
+    for (const ProductCost &c : gradient ? kTransposedCosts : kRowCosts)
+        for (int64_t shares = 1; shares <= (gradient ? 64 : 1) && (shares == 1 || steps / shares >= 4); shares += shares < 8 ? 1 : shares / 4) {
+            const int64_t tiles_l = (l + 64 * c.nl - 1) / (64 * c.nl), tiles_r = (r + 64 * c.nr - 1) / (64 * c.nr);
             int64_t per = (steps + shares - 1) / shares;
             if (masked) per = std::min<int64_t>(per, kProductMostSteps);
-            const int64_t real = (steps + per - 1) / per, groups = tiles_l * tiles_r * real, slots = nb == 4 ? 256 : 512;
-            const double step = nb == 4 ? 0.83 : groups <= 256 ? 0.30 : 0.52, fixed = nb == 4 ? 9 : 4.5, rounds = (double)groups / (double)slots;
-            double us = (rounds <= 1 ? 1. : rounds + 0.3) * ((double)per * step + fixed);
+            const int64_t real = (steps + per - 1) / per, groups = tiles_l * tiles_r * real;
+            double us = product_us(c, groups, per);
             if (real > 1) us += 3 + (double)real * (double)l * (double)r * 8 / 4e6;
-            if (best.shape.shares == 0 || us < least) {
+            if (best.nl == 0 || us < least) {
                 least = us;
-                best.nb = nb;
-                best.shape = {(int)k, (int)tiles_r, (int)tiles_l, (int)real, (int)per};
+                best = {c.nl, c.nr, {(int)k, (int)tiles_r, (int)tiles_l, (int)real, (int)per}};
             }
         }
     return best;
@@ -107,11 +121,13 @@ int64_t blocks_of(const sa2_linear_ce_problem &p) { return (p.rows + 31) / 32; }
 int64_t forward_bytes(const sa2_linear_ce_problem &p, const CePlan &c) { return c.parts_bytes + up_to(p.rows * 4, 256) + up_to(blocks_of(p) * 8, 256) + 256; }
 int64_t backward_bytes(const CePlan &c) { return 256 + c.dz_bytes + c.h_bytes + c.w_bytes; }
 
-// f(integral_constant type, integral_constant NB)
+// f(integral_constant type, integral_constants nl and nr)
 template <typename F>
-void with_kernel(int type, int nb, F &&f) {
+void with_kernel(int type, const ProductPlan &plan, F &&f) {
     using std::integral_constant;
-    auto go = [&](auto t) { nb == 4 ? f(t, integral_constant<int, 4>{}) : f(t, integral_constant<int, 2>{}); };
+    using Two = integral_constant<int, 2>;
+    using Four = integral_constant<int, 4>;
+    auto go = [&](auto t) { plan.nl == 4 ? f(t, Four{}, Four{}) : plan.nr == 4 ? f(t, Two{}, Four{}) : f(t, Two{}, Two{}); };
     if (type == SA2_ELEMENT_F16) go(integral_constant<int, kF16>{});
     else go(integral_constant<int, kBf16>{});
 }
@@ -166,7 +182,7 @@ int sa2_linear_ce(const sa2_linear_ce_problem *p, const void *hidden, int64_t hi
     k.count = count;
     k.mask = mask;
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);
-    with_kernel(p->dtype, c.logits.nb, [&](auto t, auto nb) { hipLaunchKernelGGL((ce_logits_kernel<t.value, nb.value>), dim3((unsigned)c.logits.groups()), dim3(256), 0, s, k); });
+    with_kernel(p->dtype, c.logits, [&](auto t, auto nl, auto nr) { hipLaunchKernelGGL((ce_logits_kernel<t.value, nl.value, nr.value>), dim3((unsigned)c.logits.groups()), dim3(256), 0, s, k); });
     if (const int rc = launched("logits")) return rc;
     // few parts: a thread a row
     if (k.n_parts <= 16) hipLaunchKernelGGL((ce_merge_kernel<256, 1>), dim3((unsigned)((p->rows + 255) / 256)), dim3(256), 0, s, k);
@@ -204,12 +220,12 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
         const ProductOperand w{static_cast<const char *>(weight) + first * weight_stride * 2, weight_stride * 2, (int)tokens};
         // (the last piece may be shorter)
         ProductPlan dz = c.dz, dw = c.dw;
-        dz.shape.tiles_r = (int)((tokens + 64 * dz.nb - 1) / (64 * dz.nb));
-        dw.shape.tiles_l = (int)((tokens + 64 * dw.nb - 1) / (64 * dw.nb));
+        dz.shape.tiles_r = (int)((tokens + 64 * dz.nr - 1) / (64 * dz.nr));
+        dw.shape.tiles_l = (int)((tokens + 64 * dw.nl - 1) / (64 * dw.nl));
         k.shape = dz.shape;
         k.w = w;
         k.h = h;
-        with_kernel(p->dtype, dz.nb, [&](auto t, auto nb) { hipLaunchKernelGGL((ce_dz_kernel<t.value, nb.value>), dim3((unsigned)dz.groups()), dim3(256), 0, s, k); });
+        with_kernel(p->dtype, dz, [&](auto t, auto nl, auto nr) { hipLaunchKernelGGL((ce_dz_kernel<t.value, nl.value, nr.value>), dim3((unsigned)dz.groups()), dim3(256), 0, s, k); });
         if (dhidden) {
             k.shape = c.dh.shape;
             k.shape.k = (int)tokens;
@@ -217,14 +233,14 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
             k.h = {k.dz, k.dz_row, (int)p->rows};
             const bool done = i + 1 == c.pieces;
             const CeOutput o{c.h_bytes == 0 ? static_cast<char *>(dhidden) : nullptr, h_parts, (int)p->rows, i > 0, 1};
-            with_kernel(p->dtype, c.dh.nb, [&](auto t, auto nb) { 
+            with_kernel(p->dtype, c.dh, [&](auto t, auto nl, auto nr) { 
                 const dim3 grid((unsigned)c.dh.groups());
-                if (o.out) hipLaunchKernelGGL((ce_dh_kernel<t.value, nb.value, true>), grid, dim3(256), 0, s, k, o);
-                else hipLaunchKernelGGL((ce_dh_kernel<t.value, nb.value, false>), grid, dim3(256), 0, s, k, o);
+                if (o.out) hipLaunchKernelGGL((ce_dh_kernel<t.value, nl.value, nr.value, true>), grid, dim3(256), 0, s, k, o);
+                else hipLaunchKernelGGL((ce_dh_kernel<t.value, nl.value, nr.value, false>), grid, dim3(256), 0, s, k, o);
             });
             if (done && c.h_bytes > 0) {
                 const dim3 grid((unsigned)((p->rows * p->dim / 4 + 255) / 256));
-                with_kernel(p->dtype, 2, [&](auto t, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, o, static_cast<char *>(dhidden)); });
+                with_kernel(p->dtype, dz, [&](auto t, auto, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, o, static_cast<char *>(dhidden)); });
             }
         }
         if (dweight) {
@@ -233,14 +249,14 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
             k.h = {k.dz, k.dz_row, (int)up_to(tokens, 8)};          // (tiles of dz end with zeros)
             char *const out = static_cast<char *>(dweight) + first * p->dim * 2;
             const CeOutput o{c.dw.shape.shares == 1 ? out : nullptr, w_parts, (int)tokens, 0, 0};
-            with_kernel(p->dtype, c.dw.nb, [&](auto t, auto nb) { 
+            with_kernel(p->dtype, dw, [&](auto t, auto nl, auto nr) { 
                 const dim3 grid((unsigned)dw.groups());
-                if (o.out) hipLaunchKernelGGL((ce_dw_kernel<t.value, nb.value, true>), grid, dim3(256), 0, s, k, o);
-                else hipLaunchKernelGGL((ce_dw_kernel<t.value, nb.value, false>), grid, dim3(256), 0, s, k, o);
+                if (o.out) hipLaunchKernelGGL((ce_dw_kernel<t.value, nl.value, nr.value, true>), grid, dim3(256), 0, s, k, o);
+                else hipLaunchKernelGGL((ce_dw_kernel<t.value, nl.value, nr.value, false>), grid, dim3(256), 0, s, k, o);
             });
             if (c.dw.shape.shares > 1) {
                 const dim3 grid((unsigned)((tokens * p->dim / 4 + 255) / 256));
-                with_kernel(p->dtype, 2, [&](auto t, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, o, out); });
+                with_kernel(p->dtype, dz, [&](auto t, auto, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, o, out); });
             }
         }
         if (const int rc = launched("cross entropy backward")) return rc;

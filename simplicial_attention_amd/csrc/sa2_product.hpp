@@ -1,8 +1,8 @@
 // Tiles of a matrix product for gfx950: out[l][r] = sum over k of L(l, k) R(r, k), bf16 or fp16 operands, fp32 sums, what becomes of them is the caller's.
 //
 // Each operand is in memory as rows of k (ROW: k is the fast index) or as rows along l or r (k is the slow index: read transposed out of
-// LDS).  A workgroup of four waves owns TILE x TILE results, a wave a quarter of them as NB x NB blocks of 32 x 32; k goes by in
-// steps of 32, of which a ring of four is under way (direct-to-LDS loads, three steps ahead), one barrier a step.  The fragments of the next half step
+// LDS).  A workgroup of four waves owns 64 NL x 64 NR results, a wave a quarter of them as NL x NR blocks of 32 x 32; k goes by in
+// steps of 32, of which a ring of three or four is in LDS (direct loads, two or three steps ahead), one barrier a step.  The fragments of the next half step
 // are read while the products of the present one run.
 //
 // Registers: column c of an MFMA result is row dmap_row(c) of the l side, register r of half hf column 16 hf + r of the r side, so a
@@ -126,22 +126,23 @@ __device__ __forceinline__ ProductPlace product_place(const ProductShape &s) {
 
 constexpr int kProductMostSteps = 2048;       // of a share, where k has a mask
 
-template <int T, int NB, bool R_ROW, bool L_ROW, bool MASKED>
+template <int T, int NL, int NR, bool R_ROW, bool L_ROW, bool MASKED>
 struct Product {
-    static constexpr int TILE = 64 * NB;
-    static constexpr int RING = 4;
-    static constexpr int STAGE = 2 * TILE * 64;
+    static constexpr int TILE_L = 64 * NL, TILE_R = 64 * NR;
+    static constexpr int RING = NL != NR ? 3 : 4;            // (two workgroups of 128 x 256 on a CU)
+    static constexpr int AHEAD = RING - 1;                   // steps that the loads run ahead
+    static constexpr int STAGE = (TILE_L + TILE_R) * 64;
     static constexpr int LDS = RING * STAGE + (MASKED ? kProductMostSteps * 4 : 0);
-    using R = ProductSide<R_ROW, TILE>;
-    using L = ProductSide<L_ROW, TILE>;
+    using R = ProductSide<R_ROW, TILE_R>;
+    using L = ProductSide<L_ROW, TILE_L>;
     static constexpr int LOADS = R::CHUNKS + L::CHUNKS;      // of a wave and step
 
-    // acc[l block][r block] of this wave, whose blocks begin at NB (wave & 1) on the r side and NB (wave >> 1) on the l side
+    // acc[l block][r block] of this wave, whose blocks begin at NR (wave & 1) on the r side and NL (wave >> 1) on the l side
     static __device__ __forceinline__ void run(const ProductShape &shape, const ProductOperand &ro, const ProductOperand &lo, const ProductPlace &at, const uint32_t *mask, char *lds,
-                                               f32x16 (&acc)[NB][NB]) {
+                                               f32x16 (&acc)[NL][NR]) {
         const int lane = threadIdx.x & 63, wave = wave_index();
-        const R r(ro, at.tile_r * TILE, lane, wave);
-        const L l(lo, at.tile_l * TILE, lane, wave);
+        const R r(ro, at.tile_r * TILE_R, lane, wave);
+        const L l(lo, at.tile_l * TILE_L, lane, wave);
         const int t0 = at.share * shape.share_steps, all = (shape.k + 31) / 32;
         const int nt = min(shape.share_steps, all - t0);
         if constexpr (MASKED) {
@@ -157,14 +158,14 @@ struct Product {
 
     // `last`: bits of the k of the last step that count
     template <bool SOME>
-    static __device__ __forceinline__ void steps(const R &r, const L &l, int t0, int nt, uint32_t last, char *lds, f32x16 (&acc)[NB][NB]) {
+    static __device__ __forceinline__ void steps(const R &r, const L &l, int t0, int nt, uint32_t last, char *lds, f32x16 (&acc)[NL][NR]) {
         const int wave = wave_index();
         const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
         [[maybe_unused]] const uint32_t *bits = reinterpret_cast<const uint32_t *>(lds + RING * STAGE);
 #pragma unroll
-        for (int a = 0; a < NB; ++a)
+        for (int a = 0; a < NL; ++a)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) acc[a][b] = zero16();
+            for (int b = 0; b < NR; ++b) acc[a][b] = zero16();
         if (nt <= 0) return;
         const char *pr = r.base + t0 * r.advance, *pl = l.base + t0 * l.advance;      // of the step that is loaded next
         uint32_t next_bits = MASKED ? bits[0] : nt == 1 ? last : 0xffffffffu;
@@ -186,22 +187,25 @@ struct Product {
             else if constexpr (SOME) next_bits = t + 1 >= nt - 1 ? last : 0xffffffffu;
         };
 #pragma unroll
-        for (int t = 0; t < 3; ++t) {
+        for (int t = 0; t < AHEAD; ++t) {
             static_for<0, LOADS>([&](auto i) { load_one(lds0 + t * STAGE, i); });
             go_on(t);
         }
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
-        u32x4 fr[2][NB], fl[2][NB];
-        const int br = NB * (wave & 1), bl = NB * (wave >> 1);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((AHEAD - 1) * LOADS) : "memory");
+        u32x4 fr[2][NR], fl[2][NL];
+        const int br = NR * (wave & 1), bl = NL * (wave >> 1);
         using Zero = std::integral_constant<int, 0>;
         using One = std::integral_constant<int, 1>;
-        constexpr int N = NB * NB, READS = 2 * NB, FIRST = NB == 4 ? 4 : 1;
+        constexpr int N = NL * NR, READS = NL + NR, FIRST = N / 4, PER = (READS + N - FIRST - 1) / (N - FIRST);
+        static_assert(NR >= NL && READS <= N && LOADS <= N, "one of each in the shadow of a product");
         auto read_one = [&](const char *tile, auto half, auto i) {
-            if constexpr (i.value % 2 == 0) fr[half.value][i.value / 2] = r.fragment(tile, half.value, br + i.value / 2);
+            // (by turns, as the products take them)
+            if constexpr (i.value >= 2 * NL) fr[half.value][i.value - NL] = r.fragment(tile, half.value, br + i.value - NL);
+            else if constexpr (i.value % 2 == 0) fr[half.value][i.value / 2] = r.fragment(tile, half.value, br + i.value / 2);
             else fl[half.value][i.value / 2] = l.fragment(tile + R::BYTES, half.value, bl + i.value / 2);
         };
         auto multiply_one = [&](auto half, auto i) {
-            constexpr int a = i.value / NB, b = i.value % NB;
+            constexpr int a = i.value / NR, b = i.value % NR;
             acc[a][b] = mfma_of<T>(fr[half.value][b], fl[half.value][a], acc[a][b]);
         };
         static_for<0, READS>([&](auto i) { read_one(lds, Zero{}, i); });
@@ -209,7 +213,7 @@ struct Product {
         // issued; the barrier stands behind the first products of the second half.
         for (int t = 0; t < nt; ++t) {
             const char *now = lds + (t % RING) * STAGE, *next = lds + ((t + 1) % RING) * STAGE;
-            const uint32_t to = lds0 + ((t + 3) % RING) * STAGE;
+            const uint32_t to = lds0 + ((t + AHEAD) % RING) * STAGE;
             static_for<0, N>([&](auto i) {
                 multiply_one(Zero{}, i);
                 if constexpr (i.value < READS) read_one(now, One{}, i);
@@ -218,13 +222,13 @@ struct Product {
             });
             static_for<0, FIRST>([&](auto i) { multiply_one(One{}, i); });
             __builtin_amdgcn_sched_barrier(0);
-            // step t + 1 is in (two more are under way), and this wave has read all of step t
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
-            go_on(t + 3);
+            // step t + 1 is in (those behind it are under way), and this wave has read all of step t
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((AHEAD - 1) * LOADS) : "memory");
+            go_on(t + AHEAD);
             static_for<FIRST, N>([&](auto i) {
                 multiply_one(One{}, i);
-                constexpr int per = NB == 4 ? 1 : 2, at = (i.value - FIRST) * per;
-                static_for<0, per>([&](auto j) {
+                constexpr int at = (i.value - FIRST) * PER;
+                static_for<0, PER>([&](auto j) {
                     if constexpr (at + j.value < READS) read_one(next, Zero{}, std::integral_constant<int, at + j.value>{});
                 });
                 __builtin_amdgcn_sched_barrier(0);
