@@ -429,7 +429,7 @@ int sa2_adamw(const sa2_adamw_tensor *tensors, int64_t count, const sa2_adamw_st
  * targets[i] is ignore_index; loss is per row (reduction 0), their sum over the number of rows that count (1) or their sum (2).  No logits are kept.  hidden is
  * [rows][dim], weight [vocab][dim], both bf16 or fp16 with 16-byte aligned rows (strides in elements, 0 to SA2_LINEAR_CE_MOST_STRIDE); sums are fp32.  A target that is neither a token nor
  * ignore_index makes its row's loss, and what depends on it, NaN.  Without a row that counts the mean is NaN and the gradients are zero.
- * lse [rows], count [1] and mask [ceil(rows / 32)] (bit r: row 32 i + r counts) are kept for the backward.  The reference forms the logits
+ * lse [rows], count [1] (reduction 1 and 2) and mask [ceil(rows / 32)] (bit r: row 32 i + r counts) are kept for the backward.  The reference forms the logits
  * and their fp32 copy (train.py:127-135). */
 #define SA2_LINEAR_CE_MOST_STRIDE (1ll << 23)
 typedef struct sa2_linear_ce_problem {
@@ -437,13 +437,14 @@ typedef struct sa2_linear_ce_problem {
     int32_t dim, vocab;             /* dim: a multiple of 8 up to 65536; vocab up to 2^24 */
     int32_t dtype;                  /* SA2_ELEMENT_BF16 or SA2_ELEMENT_F16 */
     int32_t reduction;              /* 0 none, 1 mean, 2 sum */
+    int32_t channels;               /* of the gradients' rows, 1 to dim: channels of hidden and weight beyond it are zeros that pad their rows; 0: dim */
     int64_t ignore_index;
 } sa2_linear_ce_problem;
 int64_t sa2_linear_ce_workspace_bytes(const sa2_linear_ce_problem *prob);         /* -1 if the problem is invalid */
 int sa2_linear_ce(const sa2_linear_ce_problem *prob, const void *hidden, int64_t hidden_stride, const void *weight, int64_t weight_stride, const int64_t *targets,
                   float *loss, float *lse, float *count, uint32_t *mask, void *workspace, int64_t workspace_bytes, void *hip_stream);
 
-/* Its gradients, contiguous in the operands' type, each written if not NULL, from dloss (device memory: one number, or with reduction 0 one per row).  Rows that do not
+/* Its gradients, contiguous rows of `channels` in the operands' type, each written if not NULL, from dloss (device memory: one number, or with reduction 0 one per row).  Rows that do not
  * count have a gradient of zero and add nothing to the weight's, whatever they hold.  The vocabulary goes by in pieces of at least 256 tokens, of whose logits'
  * gradients the workspace holds 256 MiB or 256 tokens at a time.  Bitwise reproducible (no atomics on results). */
 int64_t sa2_linear_ce_bwd_workspace_bytes(const sa2_linear_ce_problem *prob);     /* -1 if the problem is invalid */

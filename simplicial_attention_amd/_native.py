@@ -96,7 +96,7 @@ class NormProblem(ctypes.Structure):
 
 class LinearCeProblem(ctypes.Structure):
     _fields_ = [('rows', ctypes.c_int64), ('dim', ctypes.c_int32), ('vocab', ctypes.c_int32), ('dtype', ctypes.c_int32), ('reduction', ctypes.c_int32),
-                ('ignore_index', ctypes.c_int64)]
+                ('channels', ctypes.c_int32), ('ignore_index', ctypes.c_int64)]
 
 
 class AdamwTensor(ctypes.Structure):

@@ -21,6 +21,7 @@ struct CeParams {
     ProductShape shape;
     ProductOperand w, h;                     // vocabulary x dim, rows x dim
     int rows, vocab, dim, first, reduction;  // first: token at which the piece begins
+    int channels;                            // of the gradients' rows, at most dim
     const int64_t *targets;
     int64_t ignore;
     // forward
@@ -289,6 +290,22 @@ __global__ __launch_bounds__(256, NL == 4 ? 1 : 2) void ce_dz_kernel(CeParams p)
     }
 }
 
+// N results of two bytes of a row of `channels`, from d on; the others are padding
+template <int N, typename V>
+__device__ __forceinline__ void put_channels(char *out, int row, int d, int channels, const V &v) {
+    char *to = out + ((int64_t)row * channels + d) * 2;
+    typedef V any __attribute__((aligned(2)));
+    if (channels % N == 0) {
+        if (d < channels) *reinterpret_cast<V *>(to) = v;
+    } else if (d + N <= channels) {
+        *reinterpret_cast<any *>(to) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (d + i < channels) *reinterpret_cast<uint16_t *>(to + 2 * i) = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+    }
+}
+
 // Where the results of a product with dz go.  DIRECT: rounded, times what they were divided by; else fp32, for ce_combine_kernel.
 struct CeOutput {
     char *out;                     // DIRECT: [rows][dim] in the operands' type
@@ -314,9 +331,11 @@ __device__ __forceinline__ void ce_store(const CeParams &p, const CeOutput &o, c
         rows.each([&](int r, int col, u32x4 v) {
             const int row = row0 + r, d = c0 + col;
             if (row >= o.rows || d >= p.dim) return;
-            char *to = out + ((int64_t)row * p.dim + d) * (DIRECT ? 2 : 4);
+            [[maybe_unused]] char *to = out + ((int64_t)row * p.dim + d) * 4;
             if constexpr (DIRECT) {
                 if (o.masked && !(p.mask[row >> 5] >> (row & 31) & 1)) v = (u32x4){0, 0, 0, 0};
+                put_channels<8>(out, row, d, p.channels, v);
+                return;
             } else if (o.add) {
                 const float4 x = __builtin_bit_cast(float4, v), y = *reinterpret_cast<const float4 *>(to);
                 v = __builtin_bit_cast(u32x4, make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w));
@@ -353,7 +372,7 @@ template <int T>
 __global__ __launch_bounds__(256) void ce_combine_kernel(CeParams p, CeOutput o, char *out) {
     const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = (int64_t)o.rows * p.dim;
     if (at >= all) return;
-    const int row = (int)(at / p.dim);
+    const int row = (int)(at / p.dim), d = (int)(at - (int64_t)row * p.dim);
     const float factor = ce_factor<T>(p);
     const bool counts = !o.masked || (p.mask[row >> 5] >> (row & 31) & 1);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -375,7 +394,7 @@ __global__ __launch_bounds__(256) void ce_combine_kernel(CeParams p, CeOutput o,
         }
     }
     if (!counts) w = (u32x2){0, 0};
-    *reinterpret_cast<u32x2 *>(out + at * 2) = w;
+    put_channels<4>(out, row, d, p.channels, w);
 }
 
 }  // namespace sa2

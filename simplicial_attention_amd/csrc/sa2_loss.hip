@@ -75,6 +75,7 @@ int check_problem(const sa2_linear_ce_problem *p) {
     if (p->rows < 1 || p->rows > 1 << 24 || p->vocab < 1 || p->vocab > 1 << 24 || p->dim < 8 || p->dim > 65536 || p->dim % 8 != 0)
         return fail_with(SA2_ERR_BAD_SHAPE, "rows=%lld vocab=%d (1 to 2^24) dim=%d (multiples of 8 up to 65536)", (long long)p->rows, p->vocab, p->dim);
     if (p->dtype != SA2_ELEMENT_BF16 && p->dtype != SA2_ELEMENT_F16) return fail_with(SA2_ERR_UNSUPPORTED, "hidden rows and weights of type %d: bf16 and fp16 are covered", p->dtype);
+    if (p->channels < 0 || p->channels > p->dim) return fail_with(SA2_ERR_BAD_SHAPE, "%d channels of %d", p->channels, p->dim);
     if (p->reduction < 0 || p->reduction > 2) return fail_with(SA2_ERR_BAD_SHAPE, "reduction=%d", p->reduction);
     return SA2_OK;
 }
@@ -137,6 +138,7 @@ CeParams params_of(const sa2_linear_ce_problem &p, const int64_t *targets) {
     k.rows = (int)p.rows;
     k.vocab = p.vocab;
     k.dim = p.dim;
+    k.channels = p.channels ? p.channels : p.dim;
     k.reduction = p.reduction;
     k.targets = targets;
     k.ignore = p.ignore_index;
@@ -196,7 +198,9 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
     if (const int rc = check_problem(p)) return rc;
     if (!targets || !lse || !count || !mask || !dloss) return fail_with(SA2_ERR_NULL_POINTER, "targets, lse, count, mask and the loss's gradient are required");
     if (const int rc = check_rows(*p, hidden, hidden_stride, weight, weight_stride)) return rc;
-    if (((reinterpret_cast<uintptr_t>(dhidden) | reinterpret_cast<uintptr_t>(dweight)) & 15) != 0) return fail_with(SA2_ERR_ALIGNMENT, "gradients must be 16-byte aligned");
+    // (rows of other channels than whole pieces are written at any alignment of their elements)
+    const int unit = p->channels % 8 == 0 ? 15 : 1;
+    if (((reinterpret_cast<uintptr_t>(dhidden) | reinterpret_cast<uintptr_t>(dweight)) & unit) != 0) return fail_with(SA2_ERR_ALIGNMENT, "gradients must be 16-byte aligned, or to their elements");
     const CePlan c = plan(*p);
     if (too_large(c)) return fail_with(SA2_ERR_BAD_SHAPE, "rows=%lld vocab=%d dim=%d: too large for a 1-D grid", (long long)p->rows, p->vocab, p->dim);
     if (const int rc = check_workspace(workspace, workspace_bytes, backward_bytes(c))) return rc;
@@ -247,7 +251,7 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
             k.shape = dw.shape;
             k.w = {h.ptr, h.row, p->dim};
             k.h = {k.dz, k.dz_row, (int)up_to(tokens, 8)};          // (tiles of dz end with zeros)
-            char *const out = static_cast<char *>(dweight) + first * p->dim * 2;
+            char *const out = static_cast<char *>(dweight) + first * k.channels * 2;
             const CeOutput o{c.dw.shape.shares == 1 ? out : nullptr, w_parts, (int)tokens, 0, 0};
             with_kernel(p->dtype, dw, [&](auto t, auto nl, auto nr) { 
                 const dim3 grid((unsigned)dw.groups());

@@ -173,13 +173,24 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_8bit(const Tensor &x, const Mayb
 
 // ---- cross entropy of a read-out layer
 struct LinearCE : public torch::autograd::Function<LinearCE> {
-    // rows of whole 16-byte pieces: others are copied, with channels of zeros behind them
-    static Tensor pieces(const Tensor &t, int64_t dim) {
-        const Tensor m = as_matrix(t, dim);
-        const int64_t more = (8 - dim % 8) % 8;
-        if (more) return at::constant_pad_nd(m, {0, more}).contiguous();
-        const bool ok = reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 == 0 && (m.size(0) <= 1 || (m.stride(0) % 8 == 0 && m.stride(0) >= 0 && m.stride(0) <= SA2_LINEAR_CE_MOST_STRIDE));
-        return ok ? m : m.clone(at::MemoryFormat::Contiguous);
+    // Rows of whole 16-byte pieces: others are copied, with channels of zeros behind them, those of both operands in one launch.
+    static void pieces(const Tensor &hidden, const Tensor &weight, int64_t dim, Tensor &h, Tensor &w) {
+        const int64_t padded = (dim + 7) / 8 * 8;
+        sa2_conversion items[2];
+        int count = 0;
+        auto take = [&](const Tensor &t, Tensor &out) {
+            const Tensor m = as_matrix(t, dim);
+            if (dim == padded && reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 == 0 &&
+                (m.size(0) <= 1 || (m.stride(0) % 8 == 0 && m.stride(0) >= 0 && m.stride(0) <= SA2_LINEAR_CE_MOST_STRIDE))) {
+                out = m;
+                return;
+            }
+            out = at::empty({m.size(0), padded}, m.options());
+            items[count++] = {{m.data_ptr(), 0, row_stride(m), 0}, {out.data_ptr(), 0, padded, 0}, element_of(m), element_of(m), (int32_t)dim, (int32_t)padded, 1, (int32_t)m.size(0), 1};
+        };
+        take(hidden, h);
+        take(weight, w);
+        if (count) check(sa2_convert(items, count, stream_of(hidden)));
     }
 
     struct Call {
@@ -203,11 +214,10 @@ struct LinearCE : public torch::autograd::Function<LinearCE> {
         Call c;
         c.dim = hidden.size(-1);
         c.prob = {targets.numel(), (int32_t)std::min<int64_t>((c.dim + 7) / 8 * 8, INT32_MAX), (int32_t)std::min<int64_t>(weight.size(0), INT32_MAX), element_of(hidden),
-                  (int32_t)reduction, ignore_index};
+                  (int32_t)reduction, (int32_t)std::min<int64_t>(c.dim, INT32_MAX), ignore_index};
         const c10::DeviceGuard guard(hidden.device());
         if (c.prob.rows > 0) {
-            c.hidden = pieces(hidden, c.dim);
-            c.weight = pieces(weight, c.dim);
+            pieces(hidden, weight, c.dim, c.hidden, c.weight);
             c.targets = targets.to(at::kLong).contiguous();
         }
         return c;
@@ -240,7 +250,7 @@ struct LinearCE : public torch::autograd::Function<LinearCE> {
         ctx->save_for_backward(saved);
         ctx->saved_data["hidden"] = c10::List<int64_t>(hidden.sizes().vec());
         ctx->saved_data["weight"] = c10::List<int64_t>(weight.sizes().vec());
-        ctx->saved_data["problem"] = c10::List<int64_t>({c.prob.rows, c.prob.dim, c.prob.vocab, c.prob.dtype, c.prob.reduction, c.prob.ignore_index});
+        ctx->saved_data["problem"] = c10::List<int64_t>({c.prob.rows, c.prob.dim, c.prob.vocab, c.prob.dtype, c.prob.reduction, c.prob.channels, c.prob.ignore_index});
         ctx->saved_data["type"] = (int64_t)hidden.scalar_type();
         return loss;
     }
@@ -249,7 +259,7 @@ struct LinearCE : public torch::autograd::Function<LinearCE> {
         refuse_second("linear_cross_entropy");
         refuse_foreign("linear_cross_entropy", {&ups[0]});
         const auto n = ctx->saved_data["problem"].toIntVector(), h_shape = ctx->saved_data["hidden"].toIntVector(), w_shape = ctx->saved_data["weight"].toIntVector();
-        const sa2_linear_ce_problem prob{n[0], (int32_t)n[1], (int32_t)n[2], (int32_t)n[3], (int32_t)n[4], n[5]};
+        const sa2_linear_ce_problem prob{n[0], (int32_t)n[1], (int32_t)n[2], (int32_t)n[3], (int32_t)n[4], (int32_t)n[5], n[6]};
         const auto options = ups[0].options().dtype((at::ScalarType)ctx->saved_data["type"].toInt());
         const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
         const c10::DeviceGuard guard(ups[0].device());
@@ -261,17 +271,14 @@ struct LinearCE : public torch::autograd::Function<LinearCE> {
         }
         const variable_list s = ctx->get_saved_variables();
         const Tensor &hidden = s[0], &weight = s[1], up = ups[0].contiguous();
-        if (want_h) grads[0] = at::empty({prob.rows, prob.dim}, options);
-        if (want_w) grads[1] = at::empty({prob.vocab, prob.dim}, options);
+        if (want_h) grads[0] = at::empty(h_shape, options);
+        if (want_w) grads[1] = at::empty(w_shape, options);
         const int64_t bytes = sa2_linear_ce_bwd_workspace_bytes(&prob);
         const Tensor ws = at::empty({std::max<int64_t>(bytes, 0)}, options.dtype(at::kByte));
         const float *lse = static_cast<const float *>(s[3].data_ptr());
         check(sa2_linear_ce_bwd(&prob, hidden.data_ptr(), row_stride(hidden), weight.data_ptr(), row_stride(weight), static_cast<const int64_t *>(s[2].data_ptr()), lse, lse + prob.rows,
                                 reinterpret_cast<const uint32_t *>(lse + prob.rows + 1), static_cast<const float *>(up.data_ptr()), const_cast<void *>(ptr(grads[0])),
                                 const_cast<void *>(ptr(grads[1])), ws.data_ptr(), bytes, stream_of(up)));
-        const int64_t dim = w_shape[1];
-        if (want_h) grads[0] = (dim == prob.dim ? grads[0] : grads[0].narrow(1, 0, dim).contiguous()).view(h_shape);
-        if (want_w && dim != prob.dim) grads[1] = grads[1].narrow(1, 0, dim).contiguous();
         return grads;
     }
 };

@@ -56,7 +56,8 @@ def ce(**changes):
 
 
 @pytest.mark.parametrize('field,value,code', [('rows', 0, 2), ('rows', (1 << 24) + 1, 2), ('dim', 60, 2), ('dim', 0, 2), ('dim', 65544, 2), ('vocab', 0, 2), ('vocab', (1 << 24) + 1, 2), ('dtype', 2, 3),
-                                              ('reduction', 3, 2), ('reduction', -1, 2)])
+                                              ('reduction', 3, 2), ('reduction', -1, 2),
+                                              ('channels', 65, 2), ('channels', -1, 2)])
 def test_loss_refuses_problems(lib, field, value, code):
     p = ce(**{field: value})
     assert lib.sa2_linear_ce(p, 0x1000, 64, 0x2000, 64, 0x3000, 0x4000, 0x5000, 0x6000, 0x7000, 0x8000, 1 << 30, None) == code and text(lib) != ''
