@@ -372,7 +372,7 @@ int sa2_sample(const void *logits, int32_t type, int64_t rows, int64_t vocab, in
  * total = round(x + residual), normed = round(total * rsqrt(mean(total^2) + eps) * weight), rows of `dim` channels (1 to 16384); without a residual
  * (NULL) x itself is normalised and `total` is not written.  Sums are fp32; what is normalised is the rounded sum.  total has the residual's type, which is that of x or
  * fp32; normed that of x.  x and residual may have any row stride (elements, innermost stride 1) and are aligned to their elements; outputs are
- * contiguous.  weight NULL: ones.  rstd (fp32 [rows]) is for the backward, or NULL.  The counterpart in the reference is every
+ * contiguous and share no memory with the inputs (nor do those of the backward).  weight NULL: ones.  rstd (fp32 [rows]) is for the backward, or NULL.  The counterpart in the reference is every
  * `x = attn(x) + x` in front of an RMSNorm (two_simplicial_transformer.py:126-141). */
 typedef struct sa2_norm_problem {
     int64_t rows;

@@ -62,6 +62,33 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x, float *scratch) {
     return s;
 }
 
+// Eight channels of a row from `at` on, of which the first `skip` are the piece's before (the last piece of a row whose channels are no multiple of eight ends with
+// the row: whole accesses, and what is stored twice is the same); `count` (1 to 8; 0: none) are there from `at` on if the row has fewer than eight.
+struct NormPiece {
+    int at, skip, count;
+    __device__ NormPiece(int index, int dim, bool here) {
+        const int d = index * 8;
+        at = dim >= 8 ? min(d, dim - 8) : d;
+        skip = d - at;
+        count = here && d < dim ? (dim >= 8 ? 8 : dim) : 0;
+    }
+};
+
+// e4m3 of eight values for a store of `count` from the `skip`-th on
+__device__ __forceinline__ void store_e4m3(char *y, const NormPiece &piece, const float (&t)[8], float inv) {
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = t[i] * inv;
+    const uint32_t a = pack_e4m3(q[0], q[1], q[2], q[3]), b = pack_e4m3(q[4], q[5], q[6], q[7]);
+    // (those of the piece before may have another scale)
+    if (piece.skip == 0 && piece.count == 8) *reinterpret_cast<u32x2_any *>(y) = (u32x2){a, b};
+    else
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i >= piece.skip && i < piece.count) y[i] = (char)((i < 4 ? a : b) >> (8 * (i & 3)));
+}
+__device__ __forceinline__ float e4m3_scale(uint32_t most) { return most > 0x7f800000u ? as_f32(most) : fmaxf(as_f32(most) * (float)(1 / 448.), 0x1p-126f); }
+
 template <int TX, int TR, int L, int E, bool EIGHT>
 __global__ __launch_bounds__((NormShape<L, E>::THREADS)) void norm_kernel(NormParams p) {
     using S = NormShape<L, E>;
@@ -74,80 +101,59 @@ __global__ __launch_bounds__((NormShape<L, E>::THREADS)) void norm_kernel(NormPa
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int d = (e * L + l) * 8, count = here ? p.dim - d : 0;
+        const NormPiece piece(e * L + l, p.dim, here);
 #pragma unroll
         for (int i = 0; i < 8; ++i) t[e][i] = 0.f;
-        if (count > 0) {
-            ld_some8<TX>(x + (int64_t)d * element_size<TX>, count, t[e]);
+        if (piece.count > 0) {
+            ld_some8<TX>(x + (int64_t)piece.at * element_size<TX>, piece.count, t[e]);
             if (p.r) {
                 float add[8];
-                ld_some8<TR>(r + (int64_t)d * element_size<TR>, count, add);
+                ld_some8<TR>(r + (int64_t)piece.at * element_size<TR>, piece.count, add);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) t[e][i] = rounded<TR>(t[e][i] + add[i]);
-                st_some8<TR>(p.t + (row * p.dim + d) * element_size<TR>, count, t[e]);
+                st_some8<TR>(p.t + (row * p.dim + piece.at) * element_size<TR>, piece.count, t[e]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += t[e][i] * t[e][i];
+        for (int i = 0; i < 8; ++i) sum += i >= piece.skip ? t[e][i] * t[e][i] : 0.f;
     }
     const float rstd = rsqrtf(row_sum<L>(sum, scratch) / (float)p.dim + p.eps);
     if (p.rstd && here && l == 0) p.rstd[row] = rstd;
     uint32_t most = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int d = (e * L + l) * 8, count = here ? p.dim - d : 0;
+        const NormPiece piece(e * L + l, p.dim, here);
         float w[8];
-        if (count > 0 && p.w) ld_some8(p.w_type, p.w + (int64_t)d * (p.w_type == kF32 ? 4 : 2), count, w);
+        if (piece.count > 0 && p.w) ld_some8(p.w_type, p.w + (int64_t)piece.at * (p.w_type == kF32 ? 4 : 2), piece.count, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[e][i] = count > 0 ? (p.w ? t[e][i] * rstd * w[i] : t[e][i] * rstd) : 0.f;
+        for (int i = 0; i < 8; ++i) t[e][i] = piece.count > 0 ? (p.w ? t[e][i] * rstd * w[i] : t[e][i] * rstd) : 0.f;
         if constexpr (EIGHT) {
             uint32_t m = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (i < count) m = max(m, magnitude(t[e][i]));
+                if (i >= piece.skip && i < piece.count) m = max(m, magnitude(t[e][i]));
             if (p.group_lanes) {
                 // (groups are aligned lanes of one piece index)
                 for (int off = p.group_lanes / 2; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, 64));
-                const float scale = fmaxf(as_f32(m) * (float)(1 / 448.), 0x1p-126f), some = as_u32(as_f32(m)) > 0x7f800000u ? as_f32(m) : scale;
-                if (count > 0) {
-                    if (l % p.group_lanes == 0) p.scales[row * p.groups + (e * L + l) / p.group_lanes] = some;
-                    const float inv = 1.f / some;
-                    float q[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) q[i] = t[e][i] * inv;
-                    const uint32_t a = pack_e4m3(q[0], q[1], q[2], q[3]), b = pack_e4m3(q[4], q[5], q[6], q[7]);
-                    char *y = p.y + row * p.dim + d;
-                    if (count >= 8) *reinterpret_cast<u32x2_any *>(y) = (u32x2){a, b};
-                    else
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (i < count) y[i] = (char)((i < 4 ? a : b) >> (8 * (i & 3)));
+                const float scale = e4m3_scale(m);
+                if (piece.count > 0) {
+                    if (l % p.group_lanes == 0) p.scales[row * p.groups + (e * L + l) / p.group_lanes] = scale;
+                    store_e4m3(p.y + row * p.dim + piece.at, piece, t[e], 1.f / scale);
                 }
             }
             most = max(most, m);
         } else {
-            if (count > 0) st_some8<TX>(p.y + (row * p.dim + d) * element_size<TX>, count, t[e]);
+            if (piece.count > 0) st_some8<TX>(p.y + (row * p.dim + piece.at) * element_size<TX>, piece.count, t[e]);
         }
     }
     if constexpr (EIGHT) {
         if (p.group_lanes) return;
-        most = row_max<L>(most, scratch);
-        const float scale = most > 0x7f800000u ? as_f32(most) : fmaxf(as_f32(most) * (float)(1 / 448.), 0x1p-126f), inv = 1.f / scale;
+        const float scale = e4m3_scale(row_max<L>(most, scratch)), inv = 1.f / scale;
         if (here && l == 0) p.scales[row] = scale;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int d = (e * L + l) * 8, count = here ? p.dim - d : 0;
-            if (count <= 0) continue;
-            float q[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = t[e][i] * inv;
-            const uint32_t a = pack_e4m3(q[0], q[1], q[2], q[3]), b = pack_e4m3(q[4], q[5], q[6], q[7]);
-            char *y = p.y + row * p.dim + d;
-            if (count >= 8) *reinterpret_cast<u32x2_any *>(y) = (u32x2){a, b};
-            else
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < count) y[i] = (char)((i < 4 ? a : b) >> (8 * (i & 3)));
+            const NormPiece piece(e * L + l, p.dim, here);
+            if (piece.count > 0) store_e4m3(p.y + row * p.dim + piece.at, piece, t[e], inv);
         }
     }
 }
@@ -171,36 +177,36 @@ __global__ __launch_bounds__((NormShape<L, E>::THREADS)) void norm_bwd_kernel(No
         float t[E][8], g[E][8], inner = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int d = (e * L + l) * 8, count = here ? p.dim - d : 0;
+            const NormPiece piece(e * L + l, p.dim, here);
 #pragma unroll
             for (int i = 0; i < 8; ++i) t[e][i] = g[e][i] = 0.f;
-            if (count <= 0) continue;
+            if (piece.count <= 0) continue;
             float w[8];
-            ld_some8<TR>(p.x + row * p.x_row + (int64_t)d * element_size<TR>, count, t[e]);
-            ld_some8<TX>(p.dy + row * p.dy_row + (int64_t)d * element_size<TX>, count, g[e]);
-            if (p.w) ld_some8(p.w_type, p.w + (int64_t)d * (p.w_type == kF32 ? 4 : 2), count, w);
+            ld_some8<TR>(p.x + row * p.x_row + (int64_t)piece.at * element_size<TR>, piece.count, t[e]);
+            ld_some8<TX>(p.dy + row * p.dy_row + (int64_t)piece.at * element_size<TX>, piece.count, g[e]);
+            if (p.w) ld_some8(p.w_type, p.w + (int64_t)piece.at * (p.w_type == kF32 ? 4 : 2), piece.count, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 t[e][i] *= rstd;
                 dw[e][i] += g[e][i] * t[e][i];
                 if (p.w) g[e][i] *= w[i];
-                inner += g[e][i] * t[e][i];
+                inner += i >= piece.skip ? g[e][i] * t[e][i] : 0.f;
             }
         }
         inner = row_sum<L>(inner, scratch) / (float)p.dim;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int d = (e * L + l) * 8, count = here ? p.dim - d : 0;
-            if (count <= 0) continue;
+            const NormPiece piece(e * L + l, p.dim, here);
+            if (piece.count <= 0) continue;
             float up[8];
-            if (p.dt) ld_some8<TR>(p.dt + row * p.dt_row + (int64_t)d * element_size<TR>, count, up);
+            if (p.dt) ld_some8<TR>(p.dt + row * p.dt_row + (int64_t)piece.at * element_size<TR>, piece.count, up);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 g[e][i] = rstd * (g[e][i] - t[e][i] * inner);
                 if (p.dt) g[e][i] += up[i];
             }
-            if (p.dx) st_some8<TX>(p.dx + (row * p.dim + d) * element_size<TX>, count, g[e]);
-            if (p.dr) st_some8<TR>(p.dr + (row * p.dim + d) * element_size<TR>, count, g[e]);
+            if (p.dx) st_some8<TX>(p.dx + (row * p.dim + piece.at) * element_size<TX>, piece.count, g[e]);
+            if (p.dr) st_some8<TR>(p.dr + (row * p.dim + piece.at) * element_size<TR>, piece.count, g[e]);
         }
     }
     if (!p.dw_parts) return;
@@ -209,20 +215,27 @@ __global__ __launch_bounds__((NormShape<L, E>::THREADS)) void norm_bwd_kernel(No
         for (int s = 0; s < S::ROWS; ++s) {
             if (threadIdx.x / L == s)
 #pragma unroll
-                for (int e = 0; e < E; ++e)
+                for (int e = 0; e < E; ++e) {
+                    const NormPiece piece(e * L + l, p.dim, true);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int at = (e * L + l) * 8 + i;
-                        sums[at] = s ? sums[at] + dw[e][i] : dw[e][i];
-                    }
+                    for (int i = 0; i < 8; ++i)
+                        if (i >= piece.skip && i < piece.count) sums[piece.at + i] = s ? sums[piece.at + i] + dw[e][i] : dw[e][i];
+                }
             __syncthreads();
         }
         for (int d = threadIdx.x; d < p.dim; d += S::THREADS) p.dw_parts[(int64_t)blockIdx.x * p.dim + d] = sums[d];
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int d = (e * L + l) * 8, count = p.dim - d;
-            if (count > 0) st_some8<kF32>(reinterpret_cast<char *>(p.dw_parts + (int64_t)blockIdx.x * p.dim + d), count, dw[e]);
+            const NormPiece piece(e * L + l, p.dim, true);
+            float *to = p.dw_parts + (int64_t)blockIdx.x * p.dim + piece.at;
+            if (piece.count == 8 && piece.skip == 0) {
+                st_some8<kF32>(reinterpret_cast<char *>(to), 8, dw[e]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i >= piece.skip && i < piece.count) to[i] = dw[e][i];
+            }
         }
     }
 }

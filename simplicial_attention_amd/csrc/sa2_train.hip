@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "sa2.h"
@@ -58,6 +59,13 @@ int bwd_groups(int64_t rows, int dim) {
 
 bool element_aligned(const void *p, int type) { return (reinterpret_cast<uintptr_t>(p) & (size_of(type) - 1)) == 0; }
 
+// a contiguous output that begins inside rows of an input, or these inside it.  (Rows that lie apart may have an output between them: of these the first counts.)
+bool shared(const void *out, int64_t out_bytes, const void *in, int64_t rows, int64_t row_bytes, int64_t stride_bytes) {
+    if (!out || !in) return false;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(in);
+    return a < b + (stride_bytes == row_bytes ? rows * row_bytes : row_bytes) && b < a + out_bytes;
+}
+
 int check_norm(const sa2_norm_problem *p) {
     if (!p) return fail_with(SA2_ERR_NULL_POINTER, "the problem is required");
     if (p->rows < 1 || p->dim < 1) return fail_with(SA2_ERR_BAD_SHAPE, "rows=%lld dim=%d", (long long)p->rows, p->dim);
@@ -78,6 +86,10 @@ int forward(const sa2_norm_problem *p, const void *x, int64_t x_stride, const vo
         !element_aligned(total, p->residual_type))
         return fail_with(SA2_ERR_ALIGNMENT, "tensors must be aligned to their elements");
     if (group != 0 && group != 32 && group != 64 && group != 128) return fail_with(SA2_ERR_UNSUPPORTED, "groups of %d channels: 32, 64, 128 or 0 for the row", group);
+    const int64_t x_row = (int64_t)p->dim * size_of(p->x_type), r_row = (int64_t)p->dim * size_of(p->residual_type), y_row = eight ? p->dim : x_row;
+    for (const auto &[out, row] : {std::pair<const void *, int64_t>(y, y_row), std::pair<const void *, int64_t>(total, r_row)})
+        if (shared(out, p->rows * row, x, p->rows, x_row, x_stride * size_of(p->x_type)) || shared(out, p->rows * row, residual, p->rows, r_row, residual_stride * size_of(p->residual_type)))
+            return fail_with(SA2_ERR_BAD_SHAPE, "outputs share memory with x or the residual");
     NormParams k{};
     k.x = static_cast<const char *>(x);
     k.r = static_cast<const char *>(residual);
@@ -136,6 +148,11 @@ int sa2_add_rms_norm_bwd(const sa2_norm_problem *p, const void *total, int64_t t
     if (dweight && (!workspace || workspace_bytes < (int64_t)groups * p->dim * 4))
         return fail_with(SA2_ERR_BAD_SHAPE, "workspace of %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0), (long long)groups * p->dim * 4);
     if (dweight && (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return fail_with(SA2_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
+    const int64_t x_row = (int64_t)p->dim * size_of(p->x_type), r_row = (int64_t)p->dim * size_of(p->residual_type);
+    for (const auto &[out, row] : {std::pair<const void *, int64_t>(dx, x_row), std::pair<const void *, int64_t>(dresidual, r_row)})
+        if (shared(out, p->rows * row, total, p->rows, r_row, total_stride * size_of(p->residual_type)) ||
+            shared(out, p->rows * row, dnormed, p->rows, x_row, dnormed_stride * size_of(p->x_type)) || shared(out, p->rows * row, dtotal, p->rows, r_row, dtotal_stride * size_of(p->residual_type)))
+            return fail_with(SA2_ERR_BAD_SHAPE, "gradients that are written share memory with what is read");
     NormParams k{};
     k.x = static_cast<const char *>(total);
     k.w = static_cast<const char *>(weight);

@@ -51,6 +51,17 @@ def test_norm_refuses_pointers_and_groups(lib):
     assert lib.sa2_add_rms_norm_bwd_workspace_bytes(norm(rows=1 << 20)) == lib.sa2_add_rms_norm_bwd_workspace_bytes(norm(rows=1 << 22))
 
 
+def test_norm_refuses_outputs_within_its_inputs(lib):
+    # (a row's last piece may be read by two lanes, so nothing may be written over it)
+    p = norm()                         # 4 rows of 128 bytes
+    call = lambda x=0x1000, xs=64, r=0x2000, rs=64, y=0x3000, t=0x4000: lib.sa2_add_rms_norm(p, x, xs, r, rs, None, y, t, None, None)
+    assert call(y=0x1000) == 2 and 'share memory' in text(lib)
+    assert call(t=0x2000) == 2 and call(t=0x11fe) == 2 and call(y=0x0e02) == 2 and call(x=0x1000, xs=128, y=0x107e) == 2 and call(rs=0, r=0x3002) == 2
+    assert lib.sa2_add_rms_norm_8bit(p, 0x1000, 64, None, 0, None, 0, 0x11ff, 0x5000, None, None) == 2
+    back = lambda dx=0x5000, dr=None, dt=0x4000: lib.sa2_add_rms_norm_bwd(p, 0x1000, 64, None, 0x2000, 0x3000, 64, dt, 64, dx, dr, None, None, 0, None)
+    assert back(dx=0x1000) == 2 and back(dx=0x3000) == 2 and back(dr=0x4000) == 2 and back(dx=None, dr=0x3180) == 2
+
+
 def ce(**changes):
     return _native.LinearCeProblem(**{**dict(rows=100, dim=64, vocab=300, dtype=0, reduction=1, ignore_index=-100), **changes})
 
