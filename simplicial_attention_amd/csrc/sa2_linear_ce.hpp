@@ -34,7 +34,7 @@ struct CeParams {
     uint32_t *mask;                          // [blocks of 32 rows]: rows that count
     // backward
     const float *up;                         // gradient of the loss: one number, or one per row
-    const float *most;                       // largest |up| of a row that counts (reduction none)
+    const float *most;                       // largest finite |up| of a row that counts (reduction none)
     char *dz;                                // [rows][piece]
     int64_t dz_row;                          // bytes
 };
@@ -199,12 +199,12 @@ __global__ __launch_bounds__(ROWS *G) void ce_merge_kernel(CeParams p) {
 
 // ---- backward
 
-// the largest |up| of a row that counts
+// the largest finite |up| of a row that counts
 static __global__ __launch_bounds__(1024) void ce_most_kernel(const float *up, const uint32_t *mask, int rows, float *most) {
     __shared__ uint32_t tops[16];
     uint32_t m = 0;
     for (int i = threadIdx.x; i < rows; i += 1024)
-        if (mask[i >> 5] >> (i & 31) & 1) m = max(m, magnitude(up[i]));
+        if (const uint32_t x = magnitude(up[i]); x < 0x7f800000u && (mask[i >> 5] >> (i & 31) & 1)) m = max(m, x);
     m = lanes_max<64>(m);
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
     __syncthreads();
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(256, NL == 4 ? 1 : 2) void ce_dz_kernel(CeParams p)
         float weight = 1.f;
         if (p.reduction == kCeNone) {
             const float most = *p.most;
-            weight = most > 0.f ? p.up[row] / most : most;               // (all weights zero, or one that is no number)
+            weight = most > 0.f ? p.up[row] / most : p.up[row];          // (an infinite weight, or one that is no number, is its own row's matter)
         }
         if (counts && !(target >= 0 && target < p.vocab)) weight = NAN;
         if (wave_any(weight != 1.f)) {
@@ -367,34 +367,35 @@ __global__ __launch_bounds__(256, NL == 4 ? 1 : 2) void ce_dw_kernel(CeParams p,
     ce_store<T, NL, NR, DIRECT>(p, o, at, lds, acc);
 }
 
-// the shares added in order, four elements a thread
+// the shares added in order, four elements a thread and turn
 template <int T>
 __global__ __launch_bounds__(256) void ce_combine_kernel(CeParams p, CeOutput o, char *out) {
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = (int64_t)o.rows * p.dim;
-    if (at >= all) return;
-    const int row = (int)(at / p.dim), d = (int)(at - (int64_t)row * p.dim);
+    const int64_t all = (int64_t)o.rows * p.dim;
     const float factor = ce_factor<T>(p);
-    const bool counts = !o.masked || (p.mask[row >> 5] >> (row & 31) & 1);
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float *src = o.parts + at;
+    for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; at < all; at += (int64_t)gridDim.x * 1024) {
+        const int row = (int)(at / p.dim), d = (int)(at - (int64_t)row * p.dim);
+        const bool counts = !o.masked || (p.mask[row >> 5] >> (row & 31) & 1);
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float *src = o.parts + at;
 #pragma unroll 8
-    for (int x = 0; x < p.shape.shares; ++x, src += all) {
-        const float4 v = *reinterpret_cast<const float4 *>(src);
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-    }
-    const float v[4] = {s.x * factor, s.y * factor, s.z * factor, s.w * factor};
-    u32x2 w;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if constexpr (T == kF16) {
-            const f16x2 h = {(_Float16)v[2 * i], (_Float16)v[2 * i + 1]};
-            w[i] = __builtin_bit_cast(uint32_t, h);
-        } else {
-            w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+        for (int x = 0; x < p.shape.shares; ++x, src += all) {
+            const float4 v = *reinterpret_cast<const float4 *>(src);
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
         }
+        const float v[4] = {s.x * factor, s.y * factor, s.z * factor, s.w * factor};
+        u32x2 w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (T == kF16) {
+                const f16x2 h = {(_Float16)v[2 * i], (_Float16)v[2 * i + 1]};
+                w[i] = __builtin_bit_cast(uint32_t, h);
+            } else {
+                w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+            }
+        }
+        if (!counts) w = (u32x2){0, 0};
+        put_channels<4>(out, row, d, p.channels, w);
     }
-    if (!counts) w = (u32x2){0, 0};
-    put_channels<4>(out, row, d, p.channels, w);
 }
 
 }  // namespace sa2

@@ -99,8 +99,9 @@ CePlan plan(const sa2_linear_ce_problem &p) {
     return c;
 }
 
-bool too_large(const CePlan &c) {
-    return c.logits.groups() > kMostGroups || c.dz.groups() > kMostGroups || c.dh.groups() > kMostGroups || c.dw.groups() > kMostGroups;
+int check_size(const sa2_linear_ce_problem &p, const CePlan &c) {
+    if (c.logits.groups() <= kMostGroups && c.dz.groups() <= kMostGroups && c.dh.groups() <= kMostGroups && c.dw.groups() <= kMostGroups) return SA2_OK;
+    return fail_with(SA2_ERR_BAD_SHAPE, "rows=%lld vocab=%d dim=%d: too large for a 1-D grid", (long long)p.rows, p.vocab, p.dim);
 }
 
 int check_rows(const sa2_linear_ce_problem &p, const void *hidden, int64_t hidden_stride, const void *weight, int64_t weight_stride) {
@@ -133,6 +134,9 @@ void with_kernel(int type, const ProductPlan &plan, F &&f) {
     else go(integral_constant<int, kBf16>{});
 }
 
+// (2^34 results and more take several turns: a launch has at most 2^32 threads)
+unsigned combine_groups(int64_t results) { return (unsigned)std::min<int64_t>((results + 1023) / 1024, kMostGroups); }
+
 CeParams params_of(const sa2_linear_ce_problem &p, const int64_t *targets) {
     CeParams k{};
     k.rows = (int)p.rows;
@@ -152,13 +156,13 @@ extern "C" {
 int64_t sa2_linear_ce_workspace_bytes(const sa2_linear_ce_problem *p) {
     if (check_problem(p)) return -1;
     const CePlan c = plan(*p);
-    return too_large(c) ? -1 : forward_bytes(*p, c);
+    return check_size(*p, c) ? -1 : forward_bytes(*p, c);
 }
 
 int64_t sa2_linear_ce_bwd_workspace_bytes(const sa2_linear_ce_problem *p) {
     if (check_problem(p)) return -1;
     const CePlan c = plan(*p);
-    return too_large(c) ? -1 : backward_bytes(c);
+    return check_size(*p, c) ? -1 : backward_bytes(c);
 }
 
 int sa2_linear_ce(const sa2_linear_ce_problem *p, const void *hidden, int64_t hidden_stride, const void *weight, int64_t weight_stride, const int64_t *targets, float *loss,
@@ -167,7 +171,7 @@ int sa2_linear_ce(const sa2_linear_ce_problem *p, const void *hidden, int64_t hi
     if (!targets || !loss || !lse || !count || !mask) return fail_with(SA2_ERR_NULL_POINTER, "targets, loss, lse, count and mask are required");
     if (const int rc = check_rows(*p, hidden, hidden_stride, weight, weight_stride)) return rc;
     const CePlan c = plan(*p);
-    if (too_large(c)) return fail_with(SA2_ERR_BAD_SHAPE, "rows=%lld vocab=%d dim=%d: too large for a 1-D grid", (long long)p->rows, p->vocab, p->dim);
+    if (const int rc = check_size(*p, c)) return rc;
     if (const int rc = check_workspace(workspace, workspace_bytes, forward_bytes(*p, c))) return rc;
     CeParams k = params_of(*p, targets);
     k.shape = c.logits.shape;
@@ -202,7 +206,7 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
     const int unit = p->channels % 8 == 0 ? 15 : 1;
     if (((reinterpret_cast<uintptr_t>(dhidden) | reinterpret_cast<uintptr_t>(dweight)) & unit) != 0) return fail_with(SA2_ERR_ALIGNMENT, "gradients must be 16-byte aligned, or to their elements");
     const CePlan c = plan(*p);
-    if (too_large(c)) return fail_with(SA2_ERR_BAD_SHAPE, "rows=%lld vocab=%d dim=%d: too large for a 1-D grid", (long long)p->rows, p->vocab, p->dim);
+    if (const int rc = check_size(*p, c)) return rc;
     if (const int rc = check_workspace(workspace, workspace_bytes, backward_bytes(c))) return rc;
     if (!dhidden && !dweight) return SA2_OK;
     CeParams k = params_of(*p, targets);
@@ -243,7 +247,7 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
                 else hipLaunchKernelGGL((ce_dh_kernel<t.value, nl.value, nr.value, false>), grid, dim3(256), 0, s, k, o);
             });
             if (done && c.h_bytes > 0) {
-                const dim3 grid((unsigned)((p->rows * p->dim / 4 + 255) / 256));
+                const dim3 grid(combine_groups(p->rows * p->dim));
                 with_kernel(p->dtype, dz, [&](auto t, auto, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, o, static_cast<char *>(dhidden)); });
             }
         }
@@ -259,7 +263,7 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
                 else hipLaunchKernelGGL((ce_dw_kernel<t.value, nl.value, nr.value, false>), grid, dim3(256), 0, s, k, o);
             });
             if (c.dw.shape.shares > 1) {
-                const dim3 grid((unsigned)((tokens * p->dim / 4 + 255) / 256));
+                const dim3 grid(combine_groups(tokens * p->dim));
                 with_kernel(p->dtype, dz, [&](auto t, auto, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, o, out); });
             }
         }

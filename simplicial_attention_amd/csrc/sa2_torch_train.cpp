@@ -217,6 +217,8 @@ struct LinearCE : public torch::autograd::Function<LinearCE> {
                   (int32_t)reduction, (int32_t)std::min<int64_t>(c.dim, INT32_MAX), ignore_index};
         const c10::DeviceGuard guard(hidden.device());
         if (c.prob.rows > 0) {
+            // (before anything is copied, or narrowed)
+            if (sa2_linear_ce_workspace_bytes(&c.prob) < 0) check(SA2_ERR_BAD_SHAPE);
             pieces(hidden, weight, c.dim, c.hidden, c.weight);
             c.targets = targets.to(at::kLong).contiguous();
         }

@@ -140,6 +140,30 @@ def test_targets_that_are_no_tokens_are_loud():
         assert bool(dh[17].isnan().all()) and int(dh.isnan().any(1).sum()) == 1 and bool(dw.isnan().any())
 
 
+def test_weights_of_the_losses_that_are_not_numbers_stay_with_their_rows():
+    from simplicial_attention_amd import linear_cross_entropy
+    for dtype in (torch.bfloat16, torch.float16):
+        hidden, weight, targets = inputs(70, 64, 300, dtype)
+        targets[0], targets[1] = 5, -100
+        up = torch.linspace(.5, 1, 70, device='cuda')
+        # (the largest counts, so that the rows are scaled alike with and without the first ones)
+        targets[-1] = 7
+        hidden.requires_grad_()
+        loss = linear_cross_entropy(hidden, weight, targets, reduction='none')
+        want = torch.autograd.grad(loss, hidden, up, retain_graph=True)[0]
+        for bad in (float('nan'), float('inf'), -float('inf')):
+            for rows in ([0], [0, 1]):
+                given = up.clone()
+                given[rows] = bad
+                got = torch.autograd.grad(loss, hidden, given, retain_graph=True)[0]
+                assert not got[0].isfinite().any() and not got[1].any() and torch.equal(got[2:], want[2:])
+        # weights of zero and one that is no number
+        given = torch.zeros_like(up)
+        given[0] = float('nan')
+        got = torch.autograd.grad(loss, hidden, given, retain_graph=True)[0]
+        assert got[0].isnan().all() and not got[1:].any()
+
+
 def test_logits_without_bound():
     hidden, weight, targets = inputs(70, 64, 500, torch.bfloat16)
     for scale in (30., 1e4, 1e15):                          # probabilities of 0 and 1
@@ -268,6 +292,16 @@ def test_refusals():
             linear_cross_entropy(*bad)
     with pytest.raises(ValueError):
         linear_cross_entropy(h, w, t, reduction='max')
+    # (more rows than the count holds, in no memory; nothing is copied in front of the refusal)
+    from simplicial_attention_amd._native import Sa2Error
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for rows in (2 ** 24 + 1, 2 ** 32 + 4):
+        with pytest.raises(Sa2Error, match='rows='):
+            linear_cross_entropy(h[0, :3].expand(rows, 3), w[:, :3], t[0].expand(rows))
+    with pytest.raises(Sa2Error, match='too large'):
+        linear_cross_entropy(h[0].expand(2 ** 24, 64), w[0].expand(2 ** 24, 64), t[0].expand(2 ** 24))
+    assert torch.cuda.max_memory_allocated() - before < 2 ** 24
     leaf = h.clone().requires_grad_()
     loss = linear_cross_entropy(leaf, w, t)
     with pytest.raises(RuntimeError, match='second derivative'):
