@@ -40,7 +40,7 @@ class AdamW(torch.optim.Optimizer):
     count their own steps.
 
     ``capturable``: the step count of each group is on the GPU, and ``lr`` may be a float32 tensor there, so that a recorded :meth:`step` can be replayed; all parameters of a group
-    need gradients then, in every step.
+    need gradients then, in every step, and the first one is not recorded (a replay would make the states anew).  The parameters of a group are on one GPU.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits: int = 32, masters: bool = True, min_8bit_size: int = 4096,
@@ -75,15 +75,22 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        recording = torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
         for index, group in enumerate(self.param_groups):
             capturable, by_step = group['capturable'], {}
+            if recording and not capturable:
+                raise RuntimeError('a step that is recorded needs capturable=True: every replay would be the same step')
             for param in group['params']:
                 grad = param.grad
                 if grad is None:
                     if capturable:
                         raise RuntimeError('a group that can be captured needs gradients of all its parameters')
                     continue
-                state = self.state[param] or self._state_of(param, group)
+                state = self.state[param]
+                if not state:
+                    if recording:
+                        raise RuntimeError('the first step of a parameter cannot be recorded: a replay would make its states anew')
+                    state = self._state_of(param, group)
                 if not capturable:
                     state['step'] += 1
                 lists = by_step.get(state['step'])
@@ -109,6 +116,8 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
+        if not all('state_bits' in group for group in state_dict['param_groups']):
+            raise ValueError('these are the states of another optimizer')
         super().load_state_dict(state_dict)
         # (torch casts states to their parameter's dtype: these have dtypes of their own)
         saved = [index for group in state_dict['param_groups'] for index in group['params']]

@@ -111,6 +111,8 @@ class TwoSimplicialTransformer(nn.Module):
     """``fused`` (not an argument of the reference's): every residual's addition and the norm behind it are one pass over the rows (:func:`add_rms_norm`), with and without a
     cache.  The same roundings; the norms' sums are in another order."""
 
+    fused = False                            # (stacks that were pickled without it)
+
     def __init__(self, dim, *, depth, heads=8, key_value_heads=4, dim_head=64, ff_expansion=4.,
                  two_simplicial_attn_every=4, attn_kwargs: dict | None = None,
                  two_simplicial_attn_kwargs: dict | None = None, final_norm=True, fused=False):
@@ -188,6 +190,8 @@ class TwoSimplicialLM(nn.Module):
 
     ``fused`` (not an argument of the reference's): the stack's additions and norms in one pass each, and the loss of bfloat16 and float16 models without logits
     (:func:`linear_cross_entropy`, which does not round them to that dtype in between)."""
+
+    fused = False
 
     def __init__(self, *, num_tokens, dim, depth, max_seq_len=512, dim_head=64, heads=8,
                  two_simplicial_attn_every=4, transformer_kwargs: dict | None = None, fused=False):

@@ -148,3 +148,35 @@ def test_optimizer_checks_its_arguments():
     AdamW([p]).step()                       # (no gradients: nothing to do)
     with pytest.raises(RuntimeError):
         AdamW([p], capturable=True).step()
+
+
+def test_optimizer_refuses_what_a_replay_would_get_wrong(monkeypatch):
+    from simplicial_attention_amd import AdamW
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    monkeypatch.setattr(torch.cuda, 'is_initialized', lambda: True)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    with pytest.raises(RuntimeError, match='capturable'):
+        AdamW([p]).step()
+    with pytest.raises(RuntimeError, match='first step'):
+        AdamW([p], capturable=True).step()
+
+
+def test_optimizer_refuses_states_of_another():
+    from simplicial_attention_amd import AdamW
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    other = torch.optim.AdamW([p])
+    other.step()
+    with pytest.raises(ValueError, match='another optimizer'):
+        AdamW([p]).load_state_dict(other.state_dict())
+
+
+def test_stacks_without_the_option_still_run():
+    """Models pickled before there was one have no such attribute."""
+    from simplicial_attention_amd.two_simplicial_transformer import TwoSimplicialTransformer
+    stack = TwoSimplicialTransformer(16, depth=1, heads=1, key_value_heads=1, dim_head=16, two_simplicial_attn_every=2)
+    x = torch.randn(1, 4, 16)
+    want = stack(x)
+    del stack.__dict__['fused']
+    assert not stack.fused and torch.equal(stack(x), want)
