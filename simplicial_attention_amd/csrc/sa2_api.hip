@@ -843,7 +843,6 @@ int sa2_convert(const sa2_conversion *items, int32_t count, void *hip_stream) {
         t.N = c.seq_len;
         t.H = c.heads;
         t.pieces = (int64_t)c.batch * c.seq_len * c.heads * ((c.dst_dim + 7) / 8);
-        t.src_vec = vec(c.src, c.src_type);
         t.dst_vec = vec(c.dst, c.dst_type);
         most = t.pieces > most ? t.pieces : most;
     }

@@ -3,8 +3,8 @@
 //
 // HBM-bound (each element is read once and written once); what it replaces is a cast, a zero fill and a copy per tensor, one
 // launch each, which at small sizes cost more than the attention kernels (2 sequences of 2999 rows, 6 + 4 * 2 heads of 96 fp16
-// channels: 190 us in 29 launches, 20 us in four of these).  A thread moves eight consecutive destination channels; the source
-// and the destination are accessed 16 bytes at a time where their rows allow it.
+// channels: 190 us in 29 launches, 20 us in four of these).  A thread moves eight consecutive destination channels; the source 16 bytes at a time at any
+// alignment, the destination where its rows allow it.
 #pragma once
 
 #include "sa2_common.hpp"
@@ -19,7 +19,7 @@ struct ConvertTensor {
     int src_dim, dst_dim;                      // channels beyond src_dim become zero
     int N, H;
     int64_t pieces;                            // B * N * H * ceil(dst_dim / 8)
-    bool src_vec, dst_vec;                     // 16-byte accesses are aligned
+    bool dst_vec;                              // 16-byte stores are aligned
 };
 
 constexpr int kConvertMost = 6;
@@ -38,6 +38,9 @@ __device__ __forceinline__ void convert_store1(char *p, int type, int64_t at, fl
     else reinterpret_cast<__bf16 *>(p)[at] = (__bf16)v;
 }
 
+typedef u32x4 convert_piece __attribute__((aligned(2)));
+__device__ __forceinline__ u32x4 convert_load16(const char *p) { return *reinterpret_cast<const convert_piece *>(p); }
+
 static __global__ __launch_bounds__(256) void convert_kernel(ConvertParams p) {
     const ConvertTensor &t = p.t[blockIdx.y];
     typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -51,13 +54,17 @@ static __global__ __launch_bounds__(256) void convert_kernel(ConvertParams p) {
         const int64_t b = bn / t.N;
         const int64_t s = b * t.ssb + n * t.ssn + h * t.ssh + d, o = b * t.dsb + n * t.dsn + h * t.dsh + d;
         float v[8];
-        if (t.src_vec && d + 8 <= t.src_dim) {
+        // (at any alignment of the elements)
+        if (d + 8 <= t.src_dim) {
             if (t.src_type == 2) {
-                const float4 a = *reinterpret_cast<const float4 *>(t.src + s * 4), c = *reinterpret_cast<const float4 *>(t.src + s * 4 + 16);
-                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-                v[4] = c.x; v[5] = c.y; v[6] = c.z; v[7] = c.w;
+                const u32x4 a = convert_load16(t.src + s * 4), c = convert_load16(t.src + s * 4 + 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = as_f32(a[e]);
+                    v[4 + e] = as_f32(c[e]);
+                }
             } else {
-                const u32x4 a = ld_global16(t.src + s * 2);
+                const u32x4 a = convert_load16(t.src + s * 2);
                 if (t.src_type == 1) {
                     const f16x8 f = __builtin_bit_cast(f16x8, a);
 #pragma unroll
