@@ -5,6 +5,11 @@
 // steps of 32, of which a ring of three or four is in LDS (direct loads, two or three steps ahead), one barrier a step.  The fragments of the next half step
 // are read while the products of the present one run.
 //
+// Bound by the matrix unit and the power that it draws: 8192 x 16384 results over 2048 (256 x 256 tiles) run at 1.1 to 1.27 PFLOP/s with the unit busy 60 to 68 % of the clocks at 1.7 GHz,
+// and neither a ring of five, nor another place of the barrier, nor loads two workgroups deep changes the time by more than 2 %.  Launches of fewer
+// workgroups than CUs take 0.24 to 0.31 us a step of 128 x 128; fragments read a whole step ahead and loads eight steps ahead leave that as it is.  Rows that
+// are not 64 bytes apart have their lines fetched twice (256 x 256: 11595 x 7910 over 2032 478 us, over 2048 387).
+//
 // Registers: column c of an MFMA result is row dmap_row(c) of the l side, register r of half hf column 16 hf + r of the r side, so a
 // lane holds runs of 16 consecutive results of one row.
 #pragma once
