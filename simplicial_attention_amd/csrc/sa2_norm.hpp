@@ -6,11 +6,11 @@
 // What is normalised is the rounded sum, the one that the next layer adds to.  A row is held by L lanes (part of a wave, a wave, or a
 // workgroup) in registers between its two uses, so every tensor crosses the memory bus once; bound by bytes.  A lane's pieces of eight channels are next to its
 // neighbours', so that a load or store of a wave is 1 KiB in a run; the last piece of a row that ends inside one overlaps the piece in front instead of
-// going element by element (65752 x 255 in bf16, forward and backward: 151 -> 68 us).  The weight's gradient is summed in registers over the rows that a workgroup
-// takes, then over the workgroups in a fixed order.
+// going element by element (65752 x 255 in bf16, forward and backward: 151 -> 66 us).  The weight's gradient is summed in registers over the rows that a lane
+// takes, over the lanes of a wave, its workgroup's waves and then the workgroups, in a fixed order (rows one after another through LDS: 65536 x 32 38 us, now 16).
 //
-// Measured (bf16, a copy runs at 4.9 TB/s): 16384 x 512 forward 13.3 us (5.0 TB/s), backward 16.9 and 3.8 for the weight's; 8192 x 4096 in e4m3 by groups of 128 42 us; a token of 512
-// channels 2.2 us.  What is left: the backward's second launch, and rows of 33 to 64 and under 24 channels, whose lanes are half idle.
+// Measured (bf16, a copy runs at 4.9 TB/s): 16384 x 512 forward 13.3 us (5.0 TB/s), backward 15.8 and 3.4 for the weight's; 8192 x 4096 in e4m3 by groups of 128 42 us; a token of 512
+// channels 2.2 us.  What is left: the backward's second launch (3 to 5 us).
 #pragma once
 
 #include "sa2_elements.hpp"
@@ -168,8 +168,9 @@ __global__ __launch_bounds__((NormShape<L, E>::THREADS)) void norm_kernel(NormPa
 template <int TX, int TR, int L, int E>
 __global__ __launch_bounds__((NormShape<L, E>::THREADS)) void norm_bwd_kernel(NormParams p) {
     using S = NormShape<L, E>;
-    __shared__ float scratch[S::THREADS / 64];
-    __shared__ float sums[S::ROWS > 1 ? S::MOST : 1];
+    constexpr int WAVES = S::THREADS / 64;
+    __shared__ float scratch[WAVES];
+    __shared__ __attribute__((aligned(16))) float sums[S::ROWS > 1 ? WAVES : 1][S::ROWS > 1 ? S::MOST : 4];
     const int l = threadIdx.x % L;
     float dw[E][8];
 #pragma unroll
@@ -216,20 +217,35 @@ __global__ __launch_bounds__((NormShape<L, E>::THREADS)) void norm_bwd_kernel(No
         }
     }
     if (!p.dw_parts) return;
-    // the rows of a workgroup one after another
     if constexpr (S::ROWS > 1) {
-        for (int s = 0; s < S::ROWS; ++s) {
-            if (threadIdx.x / L == s)
+        // the rows of a wave in its lanes, then the waves
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const NormPiece piece(e * L + l, p.dim, true);
+        for (int off = L; off < 64; off *= 2)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dw[e][i] += __shfl_xor(dw[e][i], off, 64);
+        float *const mine = sums[threadIdx.x / 64];
+        if ((threadIdx.x & 63) < L)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const NormPiece piece(e * L + l, p.dim, true);
+                if (piece.count == 8 && piece.skip == 0) {
+                    *reinterpret_cast<float4 *>(mine + piece.at) = make_float4(dw[e][0], dw[e][1], dw[e][2], dw[e][3]);
+                    *reinterpret_cast<float4 *>(mine + piece.at + 4) = make_float4(dw[e][4], dw[e][5], dw[e][6], dw[e][7]);
+                } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (i >= piece.skip && i < piece.count) sums[piece.at + i] = s ? sums[piece.at + i] + dw[e][i] : dw[e][i];
+                        if (i >= piece.skip && i < piece.count) mine[piece.at + i] = dw[e][i];
                 }
-            __syncthreads();
+            }
+        __syncthreads();
+        for (int d = threadIdx.x; d < p.dim; d += S::THREADS) {
+            float s = sums[0][d];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) s += sums[w][d];
+            p.dw_parts[(int64_t)blockIdx.x * p.dim + d] = s;
         }
-        for (int d = threadIdx.x; d < p.dim; d += S::THREADS) p.dw_parts[(int64_t)blockIdx.x * p.dim + d] = sums[d];
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) {

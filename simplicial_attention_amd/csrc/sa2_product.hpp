@@ -7,7 +7,8 @@
 //
 // Bound by the matrix unit and the power that it draws: 8192 x 16384 results over 2048 (256 x 256 tiles) run at 1.1 to 1.27 PFLOP/s with the unit busy 60 to 68 % of the clocks at 1.7 GHz,
 // and neither a ring of five, nor another place of the barrier, nor loads two workgroups deep changes the time by more than 2 %.  Launches of fewer
-// workgroups than CUs take 0.24 to 0.31 us a step of 128 x 128; fragments read a whole step ahead and loads eight steps ahead leave that as it is.  Rows that
+// workgroups than CUs take 0.24 to 0.31 us a step of 128 x 128, which is the rate at which one CU gets rows that are not in its L2 (40 to 67 bytes a ns, from memory 20 to 40, however far ahead
+// the loads run: fragments read a whole step ahead and loads eight steps ahead leave it as it is).  Rows that
 // are not 64 bytes apart have their lines fetched twice (256 x 256: 11595 x 7910 over 2032 478 us, over 2048 387).
 //
 // Registers: column c of an MFMA result is row dmap_row(c) of the l side, register r of half hf column 16 hf + r of the r side, so a
