@@ -103,6 +103,22 @@ __device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
     return o;
 }
 
+// four
+template <int T>
+__device__ __forceinline__ u32x2 pack4(const float (&v)[4]) {
+    u32x2 w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (T == kF16) {
+            const f16x2 h = {(_Float16)v[2 * i], (_Float16)v[2 * i + 1]};
+            w[i] = __builtin_bit_cast(uint32_t, h);
+        } else {
+            w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+        }
+    }
+    return w;
+}
+
 template <int T>
 __device__ __forceinline__ void st_some8(char *p, int count, const float (&v)[8]) {
     if (count >= 8) {
@@ -158,17 +174,7 @@ __device__ __forceinline__ void st_some(char *p, int count, const float (&v)[N])
             if constexpr (T == kF32) {
                 st_any16(p, (u32x4){as_u32(v[0]), as_u32(v[1]), as_u32(v[2]), as_u32(v[3])});
             } else {
-                u32x2 w;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if constexpr (T == kF16) {
-                        const f16x2 h = {(_Float16)v[2 * i], (_Float16)v[2 * i + 1]};
-                        w[i] = __builtin_bit_cast(uint32_t, h);
-                    } else {
-                        w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-                    }
-                }
-                *reinterpret_cast<u32x2_any *>(p) = w;
+                *reinterpret_cast<u32x2_any *>(p) = pack4<T>(v);
             }
         } else {
 #pragma unroll

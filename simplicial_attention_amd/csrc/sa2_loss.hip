@@ -19,6 +19,7 @@ int64_t up_to(int64_t x, int64_t unit) { return (x + unit - 1) / unit * unit; }
 // the tile (64 nl x 64 nr) and the shares of a product of l x r results over k
 struct ProductPlan {
     int nl = 0, nr = 0;
+    double us = 0;
     ProductShape shape{};
     int64_t groups() const { return (int64_t)shape.tiles_r * shape.tiles_l * shape.shares; }
 };
@@ -42,22 +43,22 @@ double product_us(const ProductCost &c, int64_t groups, int64_t steps) {
 }
 
 // Of the tiles and shares that there are, those with the least estimated time.  Shares write and read their fp32 results (4 TB/s, and a launch).
-// `gradient`: not of the logits, which are not shared.
-ProductPlan plan_of(int64_t l, int64_t r, int64_t k, bool gradient, bool masked) {
+// `gradient`: not of the logits, of which a launch more makes what they are wanted for.
+ProductPlan plan_of(int64_t l, int64_t r, int64_t k, bool gradient, bool masked, int64_t most_shares = 64) {
     ProductPlan best;
     double least = 0;
     const int64_t steps = (k + 31) / 32;
     for (const ProductCost &c : gradient ? kTransposedCosts : kRowCosts)
-        for (int64_t shares = 1; shares <= (gradient ? 64 : 1) && (shares == 1 || steps / shares >= 4); shares += shares < 8 ? 1 : shares / 4) {
+        for (int64_t shares = 1; shares <= most_shares && (shares == 1 || steps / shares >= 4); shares += shares < 8 ? 1 : shares / 4) {
             const int64_t tiles_l = (l + 64 * c.nl - 1) / (64 * c.nl), tiles_r = (r + 64 * c.nr - 1) / (64 * c.nr);
             int64_t per = (steps + shares - 1) / shares;
             if (masked) per = std::min<int64_t>(per, kProductMostSteps);
             const int64_t real = (steps + per - 1) / per, groups = tiles_l * tiles_r * real;
             double us = product_us(c, groups, per);
-            if (real > 1) us += 3 + (double)real * (double)l * (double)r * 8 / 4e6;
+            if (real > 1) us += (gradient ? 3 : 5) + (double)real * (double)l * (double)r * 8 / 4e6;
             if (best.nl == 0 || us < least) {
                 least = us;
-                best = {c.nl, c.nr, {(int)k, (int)tiles_r, (int)tiles_l, (int)real, (int)per}};
+                best = {c.nl, c.nr, us, {(int)k, (int)tiles_r, (int)tiles_l, (int)real, (int)per}};
             }
         }
     return best;
@@ -66,8 +67,8 @@ ProductPlan plan_of(int64_t l, int64_t r, int64_t k, bool gradient, bool masked)
 struct CePlan {
     ProductPlan logits, dz, dh, dw;
     int64_t piece = 0, pieces = 0;
-    int64_t dz_row = 0, dz_bytes = 0, h_bytes = 0, w_bytes = 0;
-    int64_t parts_bytes = 0;
+    int64_t dz_row = 0, dz_bytes = 0, h_bytes = 0, w_bytes = 0, z_bytes = 0;
+    int64_t parts = 0, parts_bytes = 0, logits_bytes = 0;           // parts: of a row's maximum and sum
 };
 
 int check_problem(const sa2_linear_ce_problem *p) {
@@ -80,17 +81,30 @@ int check_problem(const sa2_linear_ce_problem *p) {
     return SA2_OK;
 }
 
+// the shares of the logits of `tokens` tokens
+int64_t shares_bytes(const ProductPlan &p, int64_t rows, int64_t tokens) { return p.shape.shares > 1 ? up_to(p.shape.shares * rows * up_to(tokens, 8) * 4, 256) : 0; }
+
 CePlan plan(const sa2_linear_ce_problem &p) {
     CePlan c;
-    c.logits = plan_of(p.rows, p.vocab, p.dim, false, false);
-    c.parts_bytes = up_to((int64_t)c.logits.shape.tiles_r * 2 * p.rows * 8, 256);
     const int64_t most = std::max<int64_t>(256, kMostDzBytes / (2 * p.rows) / 256 * 256);
     c.pieces = (p.vocab + most - 1) / most;
     c.piece = up_to((p.vocab + c.pieces - 1) / c.pieces, 256);
     c.pieces = (p.vocab + c.piece - 1) / c.piece;
-    c.dz = plan_of(p.rows, c.piece, p.dim, false, false);
     c.dh = plan_of(p.rows, p.dim, c.piece, true, false);
     c.dw = plan_of(c.piece, p.dim, p.rows, true, true);
+    c.logits = plan_of(p.rows, p.vocab, p.dim, false, false, 1);
+    c.dz = plan_of(p.rows, c.piece, p.dim, false, false, 1);
+    // Few tiles of logits over many channels leave most of the chip without work: shares of them take two launches more, which cost a training call of less than 70 us
+    // of kernels 5 us of the host's time (6 rows of 832 channels over 2900 tokens: 69 us, 75 in shares; 172 of 3816 over 745: 98 and 74, 5 of 3992 over 1148: 86 and 77,
+    // 106 of 1992 over 8439: 96 and 80).
+    if (p.rows * p.vocab <= 1 << 24 && c.logits.us + c.dz.us + c.dh.us + c.dw.us > 70) {
+        c.logits = plan_of(p.rows, p.vocab, p.dim, false, false);
+        c.dz = plan_of(p.rows, c.piece, p.dim, false, false);
+    }
+    c.parts = c.logits.shape.shares > 1 ? (p.vocab + kCeColumns - 1) / kCeColumns : 2 * c.logits.shape.tiles_r;
+    c.parts_bytes = up_to(c.parts * p.rows * 8, 256);
+    c.logits_bytes = shares_bytes(c.logits, p.rows, p.vocab);
+    c.z_bytes = shares_bytes(c.dz, p.rows, c.piece);
     // (rows of a power of two of bytes would all begin in the same channel of the L2)
     c.dz_row = c.piece * 2 + 256;
     c.dz_bytes = up_to(p.rows * c.dz_row, 256);
@@ -120,8 +134,8 @@ int check_workspace(const void *workspace, int64_t given, int64_t needed) {
 }
 
 int64_t blocks_of(const sa2_linear_ce_problem &p) { return (p.rows + 31) / 32; }
-int64_t forward_bytes(const sa2_linear_ce_problem &p, const CePlan &c) { return c.parts_bytes + up_to(p.rows * 4, 256) + up_to(blocks_of(p) * 8, 256) + 256; }
-int64_t backward_bytes(const CePlan &c) { return 256 + c.dz_bytes + c.h_bytes + c.w_bytes; }
+int64_t forward_bytes(const sa2_linear_ce_problem &p, const CePlan &c) { return c.logits_bytes + c.parts_bytes + up_to(p.rows * 4, 256) + up_to(blocks_of(p) * 8, 256) + 256; }
+int64_t backward_bytes(const CePlan &c) { return 256 + c.dz_bytes + c.h_bytes + c.w_bytes + c.z_bytes; }
 
 // f(integral_constant type, integral_constants nl and nr)
 template <typename F>
@@ -132,6 +146,18 @@ void with_kernel(int type, const ProductPlan &plan, F &&f) {
     auto go = [&](auto t) { plan.nl == 4 ? f(t, Four{}, Four{}) : plan.nr == 4 ? f(t, Two{}, Four{}) : f(t, Two{}, Two{}); };
     if (type == SA2_ELEMENT_F16) go(integral_constant<int, kF16>{});
     else go(integral_constant<int, kBf16>{});
+}
+
+// the logits of `tokens` tokens in shares, and what is made of their sums
+template <bool DZ>
+void shared_logits(int type, const ProductPlan &plan, CeParams k, float *shares, int64_t tokens, hipStream_t s) {
+    k.dim = (int)up_to(tokens, 8);
+    const CeOutput o{nullptr, shares, k.rows, 0, 0};
+    const int chunks = (k.dim + kCeColumns - 1) / kCeColumns;
+    with_kernel(type, plan, [&](auto t, auto nl, auto nr) {
+        hipLaunchKernelGGL((ce_shares_kernel<t.value, nl.value, nr.value>), dim3((unsigned)plan.groups()), dim3(256), 0, s, k, o);
+        hipLaunchKernelGGL((ce_shared_logits_kernel<t.value, DZ>), dim3((unsigned)(((int64_t)k.rows * chunks + 3) / 4)), dim3(256), 0, s, k, o, chunks);
+    });
 }
 
 // (2^34 results and more take several turns: a launch has at most 2^32 threads)
@@ -177,18 +203,20 @@ int sa2_linear_ce(const sa2_linear_ce_problem *p, const void *hidden, int64_t hi
     k.shape = c.logits.shape;
     k.w = {static_cast<const char *>(weight), weight_stride * 2, p->vocab};
     k.h = {static_cast<const char *>(hidden), hidden_stride * 2, (int)p->rows};
-    char *ws = static_cast<char *>(workspace);
+    float *const shares = static_cast<float *>(workspace);
+    char *ws = static_cast<char *>(workspace) + c.logits_bytes;
     k.parts = reinterpret_cast<float2 *>(ws);
     k.at_target = reinterpret_cast<float *>(ws + c.parts_bytes);
     k.sums = reinterpret_cast<float *>(ws + c.parts_bytes + up_to(p->rows * 4, 256));
-    k.ticket = reinterpret_cast<uint32_t *>(ws + forward_bytes(*p, c) - 256);
-    k.n_parts = 2 * c.logits.shape.tiles_r;
+    k.ticket = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + forward_bytes(*p, c) - 256);
+    k.n_parts = (int)c.parts;
     k.loss = loss;
     k.lse = lse;
     k.count = count;
     k.mask = mask;
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);
-    with_kernel(p->dtype, c.logits, [&](auto t, auto nl, auto nr) { hipLaunchKernelGGL((ce_logits_kernel<t.value, nl.value, nr.value>), dim3((unsigned)c.logits.groups()), dim3(256), 0, s, k); });
+    if (c.logits.shape.shares > 1) shared_logits<false>(p->dtype, c.logits, k, shares, p->vocab, s);
+    else with_kernel(p->dtype, c.logits, [&](auto t, auto nl, auto nr) { hipLaunchKernelGGL((ce_logits_kernel<t.value, nl.value, nr.value>), dim3((unsigned)c.logits.groups()), dim3(256), 0, s, k); });
     if (const int rc = launched("logits")) return rc;
     // few parts: a thread a row
     if (k.n_parts <= 16) hipLaunchKernelGGL((ce_merge_kernel<256, 1>), dim3((unsigned)((p->rows + 255) / 256)), dim3(256), 0, s, k);
@@ -218,7 +246,8 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
     k.most = reinterpret_cast<float *>(ws);
     k.dz = ws + 256;
     k.dz_row = c.dz_row;
-    float *const h_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes), *const w_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes + c.h_bytes);
+    float *const h_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes), *const w_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes + c.h_bytes),
+          *const z_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes + c.h_bytes + c.w_bytes);
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);
     if (p->reduction == kCeNone) hipLaunchKernelGGL(ce_most_kernel, dim3(1), dim3(1024), 0, s, dloss, mask, (int)p->rows, reinterpret_cast<float *>(ws));
     const ProductOperand h{static_cast<const char *>(hidden), hidden_stride * 2, (int)p->rows};
@@ -233,7 +262,8 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
         k.shape = dz.shape;
         k.w = w;
         k.h = h;
-        with_kernel(p->dtype, dz, [&](auto t, auto nl, auto nr) { hipLaunchKernelGGL((ce_dz_kernel<t.value, nl.value, nr.value>), dim3((unsigned)dz.groups()), dim3(256), 0, s, k); });
+        if (dz.shape.shares > 1) shared_logits<true>(p->dtype, dz, k, z_parts, tokens, s);
+        else with_kernel(p->dtype, dz, [&](auto t, auto nl, auto nr) { hipLaunchKernelGGL((ce_dz_kernel<t.value, nl.value, nr.value>), dim3((unsigned)dz.groups()), dim3(256), 0, s, k); });
         if (dhidden) {
             k.shape = c.dh.shape;
             k.shape.k = (int)tokens;

@@ -90,6 +90,47 @@ def test_loss_and_gradients(rows, dim, vocab, dtype, reduction):
     check(hidden, weight, targets, reduction, up, run(hidden, weight, targets, reduction, up))
 
 
+# few tiles of logits over many channels, which are computed in shares
+FEW = [(1, 4096, 900), (5, 3992, 1148), (33, 4088, 2049), (40, 3993, 777), (172, 3816, 745), (6, 3160, 5506), (129, 4096, 129)]
+
+
+@pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=['bf16', 'fp16'])
+@pytest.mark.parametrize('rows,dim,vocab', FEW)
+def test_few_tiles_over_many_channels(rows, dim, vocab, dtype, reduction):
+    hidden, weight, targets = inputs(rows, dim, vocab, dtype)
+    up = up_of(reduction, rows)
+    got = run(hidden, weight, targets, reduction, up)
+    check(hidden, weight, targets, reduction, up, got)
+    for a, b in zip(got, run(hidden, weight, targets, reduction, up)):
+        assert torch.equal(a, b)
+
+
+def test_few_tiles_with_rows_that_do_not_count():
+    hidden, weight, targets = inputs(60, 4096, 700, torch.bfloat16)
+    targets[3], targets[4], targets[59] = -100, 699, 0
+    up = up_of('none', 60)
+    want = run(hidden, weight, targets, 'none', up)
+    dirty = hidden.clone()
+    dirty[targets == -100] = float('nan')
+    dirty[3] = float('inf')
+    for a, b in zip(run(dirty, weight, targets, 'none', torch.where(targets == -100, float('nan'), up)), want):
+        assert torch.equal(a, b)
+    for bad in (700, 703, 1 << 40, -1):
+        other = targets.clone()
+        other[4] = bad
+        loss, dh, dw = run(hidden, weight, other, 'none', up)
+        keep = torch.arange(60, device='cuda') != 4
+        assert bool(loss[4].isnan()) and bool(dh[4].isnan().all()) and bool(dw.isnan().all())
+        assert torch.equal(loss[keep], want[0][keep]) and torch.equal(dh[keep], want[1][keep])
+    # logits far beyond what their exponentials hold: the largest alone is left
+    big = (hidden.float() * 2 ** 60).to(torch.bfloat16)
+    z = big.double() @ weight.double().t()
+    top = z.argmax(1)
+    loss, dh, dw = run(big, weight, torch.where(targets == -100, -100, top), 'sum', up_of('sum', 0))
+    assert float(loss) == 0 and not dh.any() and not dw.any()
+
+
 def test_pieces_of_the_vocabulary():
     """16384 rows over 17000 tokens: three pieces, the last one ragged"""
     hidden, weight, targets = inputs(16384, 16, 17000, torch.bfloat16)
