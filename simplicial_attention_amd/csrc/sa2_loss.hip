@@ -114,7 +114,7 @@ CePlan plan(const sa2_linear_ce_problem &p) {
 }
 
 int check_size(const sa2_linear_ce_problem &p, const CePlan &c) {
-    if (c.logits.groups() <= kMostGroups && c.dz.groups() <= kMostGroups && c.dh.groups() <= kMostGroups && c.dw.groups() <= kMostGroups) return SA2_OK;
+    if (c.logits.groups() <= kMostGroups && c.dz.groups() <= kMostGroups && c.dh.groups() + 7 + c.dw.groups() <= kMostGroups) return SA2_OK;
     return fail_with(SA2_ERR_BAD_SHAPE, "rows=%lld vocab=%d dim=%d: too large for a 1-D grid", (long long)p.rows, p.vocab, p.dim);
 }
 
@@ -160,8 +160,8 @@ void shared_logits(int type, const ProductPlan &plan, CeParams k, float *shares,
     });
 }
 
-// (2^34 results and more take several turns: a launch has at most 2^32 threads)
-unsigned combine_groups(int64_t results) { return (unsigned)std::min<int64_t>((results + 1023) / 1024, kMostGroups); }
+// (2^33 results and more take several turns: a launch has at most 2^32 threads)
+unsigned combine_groups(int64_t results) { return (unsigned)std::min<int64_t>((results + 1023) / 1024, kMostGroups / 2); }
 
 CeParams params_of(const sa2_linear_ce_problem &p, const int64_t *targets) {
     CeParams k{};
@@ -264,38 +264,52 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
         k.h = h;
         if (dz.shape.shares > 1) shared_logits<true>(p->dtype, dz, k, z_parts, tokens, s);
         else with_kernel(p->dtype, dz, [&](auto t, auto nl, auto nr) { hipLaunchKernelGGL((ce_dz_kernel<t.value, nl.value, nr.value>), dim3((unsigned)dz.groups()), dim3(256), 0, s, k); });
+        CeParams kh = k, kw = k;
+        CeOutput oh{}, ow{};
+        CeSum sums[2];
+        int count = 0;
         if (dhidden) {
-            k.shape = c.dh.shape;
-            k.shape.k = (int)tokens;
-            k.w = {w.ptr, w.row, p->dim};
-            k.h = {k.dz, k.dz_row, (int)p->rows};
-            const bool done = i + 1 == c.pieces;
-            const CeOutput o{c.h_bytes == 0 ? static_cast<char *>(dhidden) : nullptr, h_parts, (int)p->rows, i > 0, 1};
-            with_kernel(p->dtype, c.dh, [&](auto t, auto nl, auto nr) { 
-                const dim3 grid((unsigned)c.dh.groups());
-                if (o.out) hipLaunchKernelGGL((ce_dh_kernel<t.value, nl.value, nr.value, true>), grid, dim3(256), 0, s, k, o);
-                else hipLaunchKernelGGL((ce_dh_kernel<t.value, nl.value, nr.value, false>), grid, dim3(256), 0, s, k, o);
-            });
-            if (done && c.h_bytes > 0) {
-                const dim3 grid(combine_groups(p->rows * p->dim));
-                with_kernel(p->dtype, dz, [&](auto t, auto, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, o, static_cast<char *>(dhidden)); });
-            }
+            kh.shape = c.dh.shape;
+            kh.shape.k = (int)tokens;
+            kh.w = {w.ptr, w.row, p->dim};
+            kh.h = {k.dz, k.dz_row, (int)p->rows};
+            oh = {c.h_bytes == 0 ? static_cast<char *>(dhidden) : nullptr, h_parts, (int)p->rows, i > 0, 1};
+            if (c.h_bytes > 0 && i + 1 == c.pieces) sums[count++] = {oh, static_cast<char *>(dhidden), c.dh.shape.shares, p->dim};
         }
         if (dweight) {
-            k.shape = dw.shape;
-            k.w = {h.ptr, h.row, p->dim};
-            k.h = {k.dz, k.dz_row, (int)up_to(tokens, 8)};          // (tiles of dz end with zeros)
+            kw.shape = dw.shape;
+            kw.w = {h.ptr, h.row, p->dim};
+            kw.h = {k.dz, k.dz_row, (int)up_to(tokens, 8)};          // (tiles of dz end with zeros)
             char *const out = static_cast<char *>(dweight) + first * k.channels * 2;
-            const CeOutput o{c.dw.shape.shares == 1 ? out : nullptr, w_parts, (int)tokens, 0, 0};
-            with_kernel(p->dtype, dw, [&](auto t, auto nl, auto nr) { 
-                const dim3 grid((unsigned)dw.groups());
-                if (o.out) hipLaunchKernelGGL((ce_dw_kernel<t.value, nl.value, nr.value, true>), grid, dim3(256), 0, s, k, o);
-                else hipLaunchKernelGGL((ce_dw_kernel<t.value, nl.value, nr.value, false>), grid, dim3(256), 0, s, k, o);
+            ow = {c.dw.shape.shares == 1 ? out : nullptr, w_parts, (int)tokens, 0, 0};
+            if (!ow.out) sums[count++] = {ow, out, dw.shape.shares, p->dim};
+        }
+        if (dhidden && dweight && c.dh.nr == 2 && dw.nr == 2) {
+            const dim3 grid((unsigned)(up_to(c.dh.groups(), 8) + dw.groups()));
+            with_kernel(p->dtype, dz, [&](auto t, auto, auto) {
+                const auto go = [&](auto h_direct, auto w_direct) {
+                    hipLaunchKernelGGL((ce_gradients_kernel<t.value, h_direct.value, w_direct.value>), grid, dim3(256), 0, s, kh, oh, kw, ow, (int)c.dh.groups());
+                };
+                if (oh.out) ow.out ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+                else ow.out ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
             });
-            if (c.dw.shape.shares > 1) {
-                const dim3 grid(combine_groups(tokens * p->dim));
-                with_kernel(p->dtype, dz, [&](auto t, auto, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, o, out); });
-            }
+        } else {
+            if (dhidden)
+                with_kernel(p->dtype, c.dh, [&](auto t, auto nl, auto nr) {
+                    const dim3 grid((unsigned)c.dh.groups());
+                    if (oh.out) hipLaunchKernelGGL((ce_dh_kernel<t.value, nl.value, nr.value, true>), grid, dim3(256), 0, s, kh, oh);
+                    else hipLaunchKernelGGL((ce_dh_kernel<t.value, nl.value, nr.value, false>), grid, dim3(256), 0, s, kh, oh);
+                });
+            if (dweight)
+                with_kernel(p->dtype, dw, [&](auto t, auto nl, auto nr) {
+                    const dim3 grid((unsigned)dw.groups());
+                    if (ow.out) hipLaunchKernelGGL((ce_dw_kernel<t.value, nl.value, nr.value, true>), grid, dim3(256), 0, s, kw, ow);
+                    else hipLaunchKernelGGL((ce_dw_kernel<t.value, nl.value, nr.value, false>), grid, dim3(256), 0, s, kw, ow);
+                });
+        }
+        if (count > 0) {
+            const int64_t most = std::max((int64_t)sums[0].o.rows, count > 1 ? (int64_t)sums[1].o.rows : 0) * p->dim;
+            with_kernel(p->dtype, dz, [&](auto t, auto, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, dim3(combine_groups(most), (unsigned)count), dim3(256), 0, s, k, sums[0], sums[count - 1]); });
         }
         if (const int rc = launched("cross entropy backward")) return rc;
     }

@@ -121,8 +121,8 @@ __device__ __forceinline__ int xcd_run(int wg, int total) {
     return x * each + min(x, total % 8) + wg / 8;
 }
 // Consecutive workgroups of an XCD take eight l tiles by as many r tiles as there are, l first: what they read at a time fits its L2.
-__device__ __forceinline__ ProductPlace product_place(const ProductShape &s) {
-    const int item = xcd_run(blockIdx.x, gridDim.x);
+__device__ __forceinline__ ProductPlace product_place(const ProductShape &s, int wg, int total) {
+    const int item = xcd_run(wg, total);
     const int per_share = s.tiles_r * s.tiles_l, share = uniform(item / per_share), at = item - share * per_share;
     const int group = uniform(at / (8 * s.tiles_r)), rest = at - group * 8 * s.tiles_r;
     const int wide = min(8, s.tiles_l - 8 * group);
