@@ -6,7 +6,7 @@
 // The forward keeps, of every tile of logits, a maximum and a sum per row; they are merged to lse.  The backward goes over the vocabulary in pieces: logits of a piece
 // are formed again, become dz in the operands' type, and are multiplied both ways.  Four products of 2 N V D operations for the three that a
 // gradient needs, and N x (a piece) of memory.  Bound by the matrix unit; with few channels by the exponentials of the two epilogues.
-// 8192 rows of 2048 channels over 131072 tokens: 15.0 ms (logits 3.9, dz 4.2, dH 3.6, dW 3.4), 1.17 PFLOP/s; over 32000 of 512 channels 1.3 ms.  The smallest (60 rows, 256 tokens): 27 us in five
+// 8192 rows of 2048 channels over 131072 tokens: 15.0 ms (logits 3.9, dz 4.2, dH 3.6, dW 3.4), 1.17 PFLOP/s; over 32000 of 512 channels 1.3 ms.  The smallest (60 rows, 256 tokens): 22 us in four
 // launches.
 //
 // dz is rounded to the operands' type for its products.  To use that type's range well it is divided by the largest weight G of a row's loss
