@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256, 2) void ce_gradients_kernel(CeParams h, CeOutp
     }
 }
 
-// the shares added in order, four elements a thread and turn
+// the shares added in order, four elements a thread (blockIdx.y: of dH or dW; z: beyond 2^32 threads)
 struct CeSum {
     CeOutput o;
     char *out;
@@ -465,25 +465,27 @@ struct CeSum {
 };
 template <int T>
 __global__ __launch_bounds__(256) void ce_combine_kernel(CeParams p, CeSum a, CeSum b) {
-    const CeSum &c = blockIdx.y ? b : a;
-    const CeOutput &o = c.o;
-    const int64_t all = (int64_t)o.rows * c.dim;
+    // (by value: pointers out of a chosen struct would be accessed as if they could be LDS)
+    const bool second = blockIdx.y != 0;
+    const float *const parts = second ? b.o.parts : a.o.parts;
+    char *const out = second ? b.out : a.out;
+    const int rows = second ? b.o.rows : a.o.rows, masked = second ? b.o.masked : a.o.masked, shares = second ? b.shares : a.shares, dim = a.dim;
+    const int64_t at = (((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 256 + threadIdx.x) * 4, all = (int64_t)rows * dim;
+    if (at >= all) return;
+    const int row = (int)(at / dim), d = (int)(at - (int64_t)row * dim);
     const float factor = ce_factor<T>(p);
-    for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; at < all; at += (int64_t)gridDim.x * 1024) {
-        const int row = (int)(at / c.dim), d = (int)(at - (int64_t)row * c.dim);
-        const bool counts = !o.masked || (p.mask[row >> 5] >> (row & 31) & 1);
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float *src = o.parts + at;
+    const bool counts = !masked || (p.mask[row >> 5] >> (row & 31) & 1);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float *src = parts + at;
 #pragma unroll 8
-        for (int x = 0; x < c.shares; ++x, src += all) {
-            const float4 v = *reinterpret_cast<const float4 *>(src);
-            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-        }
-        const float v[4] = {s.x * factor, s.y * factor, s.z * factor, s.w * factor};
-        u32x2 w = pack4<T>(v);
-        if (!counts) w = (u32x2){0, 0};
-        put_channels<4>(c.out, row, d, p.channels, w);
+    for (int x = 0; x < shares; ++x, src += all) {
+        const float4 v = *reinterpret_cast<const float4 *>(src);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
+    const float v[4] = {s.x * factor, s.y * factor, s.z * factor, s.w * factor};
+    u32x2 w = pack4<T>(v);
+    if (!counts) w = (u32x2){0, 0};
+    put_channels<4>(out, row, d, p.channels, w);
 }
 
 }  // namespace sa2

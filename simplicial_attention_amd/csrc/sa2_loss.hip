@@ -160,8 +160,11 @@ void shared_logits(int type, const ProductPlan &plan, CeParams k, float *shares,
     });
 }
 
-// (2^33 results and more take several turns: a launch has at most 2^32 threads)
-unsigned combine_groups(int64_t results) { return (unsigned)std::min<int64_t>((results + 1023) / 1024, kMostGroups / 2); }
+// (2^33 results and more: a launch has at most 2^32 threads in one dimension)
+dim3 combine_grid(int64_t results, int outputs) {
+    const int64_t groups = (results + 1023) / 1024, x = std::min<int64_t>(groups, kMostGroups / 2);
+    return dim3((unsigned)x, (unsigned)outputs, (unsigned)((groups + x - 1) / x));
+}
 
 CeParams params_of(const sa2_linear_ce_problem &p, const int64_t *targets) {
     CeParams k{};
@@ -268,6 +271,10 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
         CeOutput oh{}, ow{};
         CeSum sums[2];
         int count = 0;
+        const auto combine = [&](const CeSum &a, const CeSum &b, int outputs) {
+            const dim3 grid = combine_grid((int64_t)std::max(a.o.rows, b.o.rows) * p->dim, outputs);
+            with_kernel(p->dtype, dz, [&](auto t, auto, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, grid, dim3(256), 0, s, k, a, b); });
+        };
         if (dhidden) {
             kh.shape = c.dh.shape;
             kh.shape.k = (int)tokens;
@@ -293,23 +300,25 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
                 if (oh.out) ow.out ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
                 else ow.out ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
             });
+            if (count > 0) combine(sums[0], sums[count - 1], count);
         } else {
-            if (dhidden)
+            // (shares are added up while the caches hold them: 300 rows of 4096 channels over 40000 tokens 9.1 us, behind both products 13.3)
+            if (dhidden) {
                 with_kernel(p->dtype, c.dh, [&](auto t, auto nl, auto nr) {
                     const dim3 grid((unsigned)c.dh.groups());
                     if (oh.out) hipLaunchKernelGGL((ce_dh_kernel<t.value, nl.value, nr.value, true>), grid, dim3(256), 0, s, kh, oh);
                     else hipLaunchKernelGGL((ce_dh_kernel<t.value, nl.value, nr.value, false>), grid, dim3(256), 0, s, kh, oh);
                 });
-            if (dweight)
+                if (count > 0 && sums[0].out == dhidden) combine(sums[0], sums[0], 1);
+            }
+            if (dweight) {
                 with_kernel(p->dtype, dw, [&](auto t, auto nl, auto nr) {
                     const dim3 grid((unsigned)dw.groups());
                     if (ow.out) hipLaunchKernelGGL((ce_dw_kernel<t.value, nl.value, nr.value, true>), grid, dim3(256), 0, s, kw, ow);
                     else hipLaunchKernelGGL((ce_dw_kernel<t.value, nl.value, nr.value, false>), grid, dim3(256), 0, s, kw, ow);
                 });
-        }
-        if (count > 0) {
-            const int64_t most = std::max((int64_t)sums[0].o.rows, count > 1 ? (int64_t)sums[1].o.rows : 0) * p->dim;
-            with_kernel(p->dtype, dz, [&](auto t, auto, auto) { hipLaunchKernelGGL(ce_combine_kernel<t.value>, dim3(combine_groups(most), (unsigned)count), dim3(256), 0, s, k, sums[0], sums[count - 1]); });
+                if (!ow.out) combine(sums[count - 1], sums[count - 1], 1);
+            }
         }
         if (const int rc = launched("cross entropy backward")) return rc;
     }
