@@ -5,6 +5,8 @@
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "sa2.h"
 
@@ -56,6 +58,16 @@ bool foreign(const Tensor &t) {
     static const c10::DispatchKeySet keys({c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
                                            c10::DispatchKey::Python, c10::DispatchKey::Functionalize});
     return t.key_set().has_any(keys) || t._fw_grad(0).defined();
+}
+
+// Recorders (torch.jit.trace, make_fx, fake tensors) see torch's operators alone: they would keep the allocation of a result without the kernel that fills it, and a
+// replay would return what was in memory.
+void refuse_recorder(const char *what) {
+    using c10::impl::TorchDispatchModeKey;
+    bool recorded = torch::jit::tracer::isTracing();
+    for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+        recorded = recorded || c10::impl::TorchDispatchModeTLS::get_mode(mode).has_value();
+    if (recorded) raise(PyExc_RuntimeError, std::string(what) + " cannot be traced: a recorder does not see its kernels");
 }
 
 void refuse_autograd(const char *what, std::initializer_list<const Tensor *> inputs) {

@@ -13,6 +13,7 @@ void refuse_foreign(const char *what, std::initializer_list<const Tensor *> inpu
 
 // a backward that is itself recorded: its kernels have no derivative
 void refuse_second(const char *what) {
+    refuse_recorder(what);
     if (at::GradMode::is_enabled()) raise(PyExc_RuntimeError, std::string(what) + " has no second derivative: call its backward without create_graph");
 }
 
@@ -41,6 +42,7 @@ struct NormCall {
 };
 
 NormCall norm_call(const char *what, const Tensor &x, const MaybeTensor &residual, const MaybeTensor &weight, std::optional<double> eps) {
+    refuse_recorder(what);
     for (const Tensor *t : {&x, residual ? &*residual : nullptr, weight ? &*weight : nullptr}) {
         if (!t) continue;
         refuse_foreign(what, {t});
@@ -155,6 +157,7 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor &x, const MaybeTensor &resi
 }
 
 std::tuple<Tensor, Tensor, Tensor> add_rms_norm_8bit(const Tensor &x, const MaybeTensor &residual, const MaybeTensor &weight, std::optional<double> eps, int64_t group) {
+    refuse_recorder("add_rms_norm_8bit");
     refuse_autograd("add_rms_norm_8bit", {&x, residual ? &*residual : &x, weight ? &*weight : &x});
     const NormCall c = norm_call("add_rms_norm_8bit", x, residual, weight, eps);
     if (group != 0 && group != 32 && group != 64 && group != 128) raise(PyExc_ValueError, "groups of " + std::to_string(group) + " channels: 32, 64, 128, or None for whole rows");
@@ -203,6 +206,7 @@ struct LinearCE : public torch::autograd::Function<LinearCE> {
     };
 
     static Call checked(const Tensor &hidden, const Tensor &weight, const Tensor &targets, int64_t ignore_index, int64_t reduction) {
+        refuse_recorder("linear_cross_entropy");
         for (const Tensor *t : {&hidden, &weight, &targets}) {
             refuse_foreign("linear_cross_entropy", {t});
             if (!t->is_cuda()) raise(PyExc_AssertionError, "linear_cross_entropy runs on the GPU only");
@@ -318,6 +322,7 @@ struct Items {
 
 void adamw_step(const py::object &params_in, const py::object &grads_in, const py::object &averages_in, const py::object &squares_in, const py::object &masters_in,
                 const py::object &step, const py::object &lr, double beta1, double beta2, double eps, double weight_decay, const MaybeTensor &grad_scale, int64_t seed) {
+    refuse_recorder("adamw_step");
     const Items params(params_in, "params must be a sequence of tensors"), grads(grads_in, "grads must be a sequence of tensors"),
         states[2] = {Items(averages_in, "exp_avgs must be a sequence"), Items(squares_in, "exp_avg_sqs must be a sequence")};
     std::optional<Items> masters;

@@ -13,7 +13,7 @@ def add_rms_norm(x: Tensor, residual: Tensor | None = None, weight: Tensor | Non
     What ``x = x + attn(x); y = norm(x)`` of a pre-normed stack computes, to the bit but for the order of the sums: total is rounded to its dtype (the
     residual's: that of x, or float32 for a residual stream in 32 bits) and normalised as rounded, with float32 sums; normed has the dtype of x.  Without a residual total is x itself.
     ``weight`` (dim,) may have a dtype of its own; ``eps=None`` is float32's, as in ``torch.nn.RMSNorm`` (which takes float32's for narrower inputs too).  bfloat16, float16 and float32 tensors
-    on the GPU of any strides, rows of up to 16384 channels.
+    on the GPU of any strides, rows of up to 16384 channels.  Recorders (``torch.jit.trace``, ``make_fx``) are refused: they do not see the kernel.
     """
     return _native.torch_ext().add_rms_norm(x, residual, weight, eps)
 
