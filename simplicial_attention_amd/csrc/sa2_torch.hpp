@@ -71,6 +71,7 @@ void refuse_recorder(const char *what) {
 }
 
 void refuse_autograd(const char *what, std::initializer_list<const Tensor *> inputs) {
+    refuse_recorder(what);
     for (const Tensor *t : inputs)
         if (in_autograd({t}) || foreign(*t)) raise(PyExc_RuntimeError, std::string(what) + " has no derivative and takes plain tensors: call it under torch.no_grad()");
 }

@@ -157,7 +157,6 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor &x, const MaybeTensor &resi
 }
 
 std::tuple<Tensor, Tensor, Tensor> add_rms_norm_8bit(const Tensor &x, const MaybeTensor &residual, const MaybeTensor &weight, std::optional<double> eps, int64_t group) {
-    refuse_recorder("add_rms_norm_8bit");
     refuse_autograd("add_rms_norm_8bit", {&x, residual ? &*residual : &x, weight ? &*weight : &x});
     const NormCall c = norm_call("add_rms_norm_8bit", x, residual, weight, eps);
     if (group != 0 && group != 32 && group != 64 && group != 128) raise(PyExc_ValueError, "groups of " + std::to_string(group) + " channels: 32, 64, 128, or None for whole rows");
