@@ -9,17 +9,31 @@ from torch.nn.modules import module as _module
 from . import _native
 
 
-# what a call of a linear layer goes through, as torch has it
-_FORWARD, _CALL, _CALL_IMPL, _LINEAR = nn.Linear.forward, nn.Linear.__call__, nn.Linear._call_impl, F.linear
+# what a call of a module goes through, as torch has it
+_CALL, _CALL_IMPL = nn.Module.__call__, nn.Module._call_impl
+_FORWARD, _LINEAR = nn.Linear.forward, F.linear
+
+
+def modes():
+    """Someone sees torch's operators or functions (the kernels of this package are none)."""
+    return torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack()
+
+
+def all_watched():
+    """Someone sees the calls of all modules, or has changed what they are."""
+    return bool(nn.Module.__call__ is not _CALL or nn.Module._call_impl is not _CALL_IMPL or _module._global_forward_hooks or _module._global_forward_pre_hooks
+                or _module._global_backward_hooks or _module._global_backward_pre_hooks)
+
+
+def watched(module):
+    """Someone else sees the calls of this module, or has changed what it is."""
+    return bool(module._compiled_call_impl is not None or module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+                or 'forward' in module.__dict__)
 
 
 def _watched(layer):
-    """Someone else sees the calls of this layer, or has changed what it is."""
-    if nn.Linear.forward is not _FORWARD or nn.Linear.__call__ is not _CALL or nn.Linear._call_impl is not _CALL_IMPL or F.linear is not _LINEAR:
-        return True
-    return bool(layer._compiled_call_impl is not None or layer._forward_hooks or layer._forward_pre_hooks or layer._backward_hooks or layer._backward_pre_hooks
-                or _module._global_forward_hooks or _module._global_forward_pre_hooks or _module._global_backward_hooks
-                or _module._global_backward_pre_hooks or 'forward' in layer.__dict__)
+    return (nn.Linear.forward is not _FORWARD or nn.Linear.__call__ is not _CALL or nn.Linear._call_impl is not _CALL_IMPL or F.linear is not _LINEAR
+            or watched(layer) or all_watched())
 
 
 def _faster(rows, out_features, in_features):
@@ -40,6 +54,6 @@ def apply_linear(layer, x):
             or x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16 or (bias is not None and bias.dtype is not torch.bfloat16)
             or x.device != weight.device or x.dim() < 2 or x.shape[-1] != weight.shape[1]
             or not _faster(x.numel() // x.shape[-1] if x.shape[-1] else 0, *weight.shape)
-            or torch.is_autocast_enabled() or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack() or _watched(layer)):
+            or torch.is_autocast_enabled() or modes() or _watched(layer)):
         return layer(x)
     return _native.torch_ext().linear(x, weight, bias)

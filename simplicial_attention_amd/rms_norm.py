@@ -2,9 +2,11 @@
 from __future__ import annotations
 
 import torch
-from torch import Tensor
+import torch.nn.functional as F
+from torch import Tensor, nn
 
 from . import _native
+from .linear import all_watched, modes, watched
 
 
 def add_rms_norm(x: Tensor, residual: Tensor | None = None, weight: Tensor | None = None, eps: float | None = None) -> tuple[Tensor, Tensor]:
@@ -29,13 +31,22 @@ def add_rms_norm_8bit(x: Tensor, residual: Tensor | None = None, weight: Tensor 
     return _native.torch_ext().add_rms_norm_8bit(x, residual, weight, eps, 0 if group is None else group)
 
 
+_FORWARD, _RMS_NORM = nn.RMSNorm.forward, F.rms_norm
+
+
+def _covered(norm):
+    """What this module computes is the kernel's to compute, and nobody sees its calls."""
+    return (type(norm) is nn.RMSNorm and norm.weight is not None and nn.RMSNorm.forward is _FORWARD and nn.RMSNorm.__call__ is nn.Module.__call__ and F.rms_norm is _RMS_NORM
+            and not (modes() or all_watched() or watched(norm)))
+
+
 def norm_behind(norm, x: Tensor, residual: Tensor | None) -> tuple[Tensor, Tensor]:
-    """``total = x + residual`` (x alone without one) and ``norm(total)`` of an ``nn.RMSNorm`` module: ``(normed, total)``.  Modules and tensors that the kernel does not cover
-    go through torch."""
-    weight = norm.weight if type(norm) is torch.nn.RMSNorm else None
-    if (weight is None or not x.is_cuda or x.shape[-1] > 16384 or norm.normalized_shape != (x.shape[-1],) or torch.is_autocast_enabled() or torch.compiler.is_compiling()
-            or torch.jit.is_tracing() or norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks
-            or weight.dtype != x.dtype or x.dtype not in (torch.bfloat16, torch.float16, torch.float32) or (residual is not None and residual.dtype != x.dtype)):
+    """``total = x + residual`` (x alone without one) and ``norm(total)`` of an ``nn.RMSNorm`` module: ``(normed, total)``.  Modules and tensors that the kernel does not cover, and modules
+    whose calls someone sees (hooks, tracers, modes), go through torch."""
+    # (torch.fx hands over proxies: the type comes first)
+    if (not isinstance(x, Tensor) or not _covered(norm) or not x.is_cuda or x.shape[-1] > 16384 or norm.normalized_shape != (x.shape[-1],)
+            or torch.is_autocast_enabled() or torch.compiler.is_compiling() or torch.jit.is_tracing()
+            or norm.weight.dtype != x.dtype or x.dtype not in (torch.bfloat16, torch.float16, torch.float32) or (residual is not None and residual.dtype != x.dtype)):
         total = x if residual is None else residual + x
         return norm(total), total
-    return add_rms_norm(x, residual, weight, norm.eps)
+    return add_rms_norm(x, residual, norm.weight, norm.eps)

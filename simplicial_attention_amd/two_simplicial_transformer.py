@@ -17,7 +17,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .cross_entropy import linear_cross_entropy
-from .linear import apply_linear
+from .linear import _watched, all_watched, apply_linear, modes, watched
 from .paged import PagedCache, paged_append, paged_attn
 from .rms_norm import norm_behind
 from .sampling import sample_tokens
@@ -95,21 +95,21 @@ class _Layers(nn.Sequential):
         return x
 
 
-def _plain(module):
-    """Nobody sees the calls of this module."""
-    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks or module._compiled_call_impl is not None
-                or 'forward' in module.__dict__)
-
-
 def FeedForward(dim, expansion=4.):
     """RMSNorm -> Linear -> GELU -> Linear (two_simplicial_transformer.py:69-76)."""
     inner = int(dim * expansion)
     return _Layers(nn.RMSNorm(dim), nn.Linear(dim, inner), nn.GELU(), nn.Linear(inner, dim))
 
 
+_CROSS_ENTROPY = F.cross_entropy
+# the forward of the modules whose calls a fused stack leaves out, as they are here
+_FORWARDS = {module: module.forward for module in (Attention, SlidingWindowTwoSimplicialMHA, _Layers)}
+
+
 class TwoSimplicialTransformer(nn.Module):
     """``fused`` (not an argument of the reference's): every residual's addition and the norm behind it are one pass over the rows (:func:`add_rms_norm`), with and without a
-    cache.  The same roundings; the norms' sums are in another order."""
+    cache.  The same roundings; the norms' sums are in another order.  Where someone sees the calls of modules or operators (hooks, tracers, modes) or has replaced a ``forward``, and
+    under autocast, they are separate calls."""
 
     fused = False                            # (stacks that were pickled without it)
 
@@ -134,7 +134,7 @@ class TwoSimplicialTransformer(nn.Module):
 
     def forward(self, x):
         if not torch.jit.is_scripting():
-            if self._can_fuse():
+            if self._can_fuse(x):
                 return self._fused(x, [attn.behind_norm for attn, _ in self.layers])
         for attn, ff in self.layers:
             x = x + attn(x)
@@ -142,9 +142,11 @@ class TwoSimplicialTransformer(nn.Module):
         return self.norm(x)
 
     @torch.jit.unused
-    def _can_fuse(self):
-        return (self.fused and not torch.jit.is_tracing() and not torch.compiler.is_compiling()
-                and all(_plain(attn) and _plain(ff) and type(ff) is _Layers and type(attn) in (Attention, SlidingWindowTwoSimplicialMHA) for attn, ff in self.layers))
+    def _can_fuse(self, x):
+        # (torch.fx hands over proxies)
+        return (self.fused and isinstance(x, torch.Tensor) and not torch.jit.is_tracing() and not torch.compiler.is_compiling() and not modes() and not all_watched()
+                and all(type(ff) is _Layers and type(attn) in _FORWARDS and not watched(attn) and not watched(ff) for attn, ff in self.layers)
+                and all(module.forward is forward and module.__call__ is nn.Module.__call__ for module, forward in _FORWARDS.items()))
 
     @torch.jit.unused
     def _fused(self, x, attend):
@@ -175,7 +177,7 @@ class TwoSimplicialTransformer(nn.Module):
     def forward_cached(self, x, cache, batch):
         """The stack for new tokens (b, n, dim) whose places ``batch = cache.extend(...)`` has made; rows beyond ``batch.counts`` are padding.  Queries, keys and values are
         rounded to the cache's dtype."""
-        if self._can_fuse():
+        if self._can_fuse(x):
             return self._fused(x, [partial(attn.forward_cached, keys=keys, values=values, batch=batch, normed=True)
                                    for (attn, _), keys, values in zip(self.layers, cache.keys, cache.values)])
         for (attn, ff), keys, values in zip(self.layers, cache.keys, cache.values):
@@ -189,7 +191,7 @@ class TwoSimplicialLM(nn.Module):
     (train.py:64-135).  ``generate`` answers prompts from a paged cache (the reference recomputes the sequence for every token).
 
     ``fused`` (not an argument of the reference's): the stack's additions and norms in one pass each, and the loss of bfloat16 and float16 models without logits
-    (:func:`linear_cross_entropy`, which does not round them to that dtype in between)."""
+    (:func:`linear_cross_entropy`, which does not round them to that dtype in between).  Under autocast, and where someone sees the calls of modules or operators, they are separate calls."""
 
     fused = False
 
@@ -221,7 +223,8 @@ class TwoSimplicialLM(nn.Module):
 
     def _can_fuse(self, hidden):
         weight = self.to_logits.weight
-        return (self.fused and type(self.to_logits) is nn.Linear and self.to_logits.bias is None and _plain(self.to_logits) and hidden.is_cuda and hidden.device == weight.device
+        return (self.fused and isinstance(hidden, torch.Tensor) and type(self.to_logits) is nn.Linear and self.to_logits.bias is None and not _watched(self.to_logits)
+                and F.cross_entropy is _CROSS_ENTROPY and not modes() and hidden.is_cuda and hidden.device == weight.device
                 and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.dtype == weight.dtype and not torch.is_autocast_enabled() and not torch.jit.is_tracing()
                 and not torch.compiler.is_compiling())
 

@@ -1,0 +1,109 @@
+"""A fused stack whose modules' calls, or operators, someone watches or has replaced runs as the separate calls."""
+import pytest
+import torch
+import torch.nn.functional as F
+from torch import nn
+from torch.overrides import TorchFunctionMode
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from simplicial_attention_amd.two_simplicial_transformer import Attention, TwoSimplicialLM, TwoSimplicialTransformer
+
+DEVICES = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+
+
+def stack(fused, device='cpu', dtype=torch.float32):
+    torch.manual_seed(0)
+    return TwoSimplicialTransformer(64, depth=3, heads=2, key_value_heads=2, dim_head=32, two_simplicial_attn_every=4, fused=fused).to(device, dtype)
+
+
+def language_model(fused, device):
+    torch.manual_seed(0)
+    return TwoSimplicialLM(num_tokens=50, dim=64, depth=2, heads=2, dim_head=32, two_simplicial_attn_every=4, transformer_kwargs=dict(key_value_heads=2), fused=fused).to(device, torch.bfloat16)
+
+
+def rows(device='cpu'):
+    return torch.randn(2, 9, 64, generator=torch.Generator().manual_seed(1)).to(device)
+
+
+def close(a, b):
+    # (norms that are not replaced add up 64 squares in another order: some last places of 2^-24 in each of seven norms; what is replaced is larger by a factor)
+    return torch.equal(a, b) if not a.is_cuda else float(((a - b).norm() / a.norm()).detach()) < 2. ** -18
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_global_hooks_see_every_module(device):
+    x, seen = rows(device), []
+    for fused in (False, True):
+        modules = []
+        handle = nn.modules.module.register_module_forward_hook(lambda module, *_: modules.append(type(module).__name__))
+        try:
+            out = stack(fused, device)(x)
+        finally:
+            handle.remove()
+        seen.append((modules, out))
+    assert seen[0][0] == seen[1][0] and torch.equal(seen[0][1], seen[1][1])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('mode', [TorchDispatchMode, TorchFunctionMode])
+def test_modes_see_every_operator(device, mode):
+    class Seen(mode):
+        def __init__(self):
+            super().__init__()
+            self.calls = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.calls.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            self.calls.append(getattr(func, '__name__', str(func)))
+            return func(*args, **(kwargs or {}))
+    tokens = torch.arange(16, device=device).view(2, 8)
+    seen = []
+    for fused in (False, True):
+        lm = language_model(fused, device)
+        with Seen() as calls:
+            loss = lm(tokens, return_loss=True)
+        seen.append((calls.calls, loss.detach()))
+    assert seen[0][0] == seen[1][0] and torch.equal(seen[0][1], seen[1][1])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('which', ['prenorm', 'ff_norm', 'norm', 'attn', 'ff'])
+def test_replaced_forwards_are_called(device, which):
+    x, outs = rows(device), []
+    for fused in (False, True):
+        t = stack(fused, device)
+        attn, ff = t.layers[1]
+        module = {'prenorm': attn.prenorm, 'ff_norm': ff[0], 'norm': t.norm, 'attn': attn, 'ff': ff}[which]
+        module.forward = lambda x: 3 * x
+        outs.append(t(x))
+    assert close(*outs)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_replaced_classes_and_functions_are_called(device, monkeypatch):
+    x = rows(device)
+    separate, fused = stack(False, device), stack(True, device)
+    for owner, name, other in ((nn.RMSNorm, 'forward', lambda self, x: 2 * x), (Attention, 'forward', lambda self, x: x.sin()), (F, 'rms_norm', lambda x, *_: 4 * x),
+                               (nn.RMSNorm, '__call__', lambda self, x: 5 * x), (Attention, '__call__', lambda self, x: x.cos())):
+        with monkeypatch.context() as patch:
+            patch.setattr(owner, name, other)
+            assert torch.equal(fused(x), separate(x)), name
+
+
+def test_symbolic_traces_of_a_fused_stack():
+    x, t = rows(), stack(True)
+    assert torch.equal(torch.fx.symbolic_trace(t)(x), t(x))
+
+
+@pytest.mark.gpu
+def test_compiled_norms_are_called():
+    x, outs = rows('cuda'), []
+    for fused in (False, True):
+        t, calls = stack(fused, 'cuda'), []
+        t.norm._compiled_call_impl = lambda x: calls.append(1) or 2 * x
+        outs.append(t(x))
+        assert calls == [1]
+    assert close(*outs)
