@@ -71,6 +71,16 @@ NormCall norm_call(const char *what, const Tensor &x, const MaybeTensor &residua
     return c;
 }
 
+// whether the call of a module's norm is one that add_rms_norm does not refuse (functorch's tensors, tangents, subclasses and more rows than a launch takes go through torch)
+bool norm_covers(const Tensor &x, const MaybeTensor &residual, const Tensor &weight) {
+    for (const Tensor *t : {&x, residual ? &*residual : &x, &weight})
+        if (foreign(*t) || t->layout() != at::kStrided || !t->is_cuda() || element_of(*t) < 0 || t->device() != x.device()) return false;
+    if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > INT32_MAX || (residual && residual->sizes() != x.sizes()) || weight.dim() != 1 || weight.size(0) != x.size(-1)) return false;
+    const int type = element_of(x), wide = element_of(residual ? *residual : x);
+    const sa2_norm_problem prob{std::max<int64_t>(x.numel() / x.size(-1), 1), (int32_t)x.size(-1), type, wide, element_of(weight), 0};
+    return sa2_add_rms_norm_bwd_workspace_bytes(&prob) >= 0;
+}
+
 const void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 struct AddNorm : public torch::autograd::Function<AddNorm> {
@@ -296,6 +306,14 @@ Tensor linear_cross_entropy(const Tensor &hidden, const Tensor &weight, const Te
     return LinearCE::run(LinearCE::checked(hidden, weight, targets, ignore_index, reduction), targets, nullptr);
 }
 
+// whether the call of a model's loss is one that linear_cross_entropy does not refuse, the memory of its logits aside
+bool loss_covers(const Tensor &hidden, const Tensor &weight, const Tensor &targets) {
+    for (const Tensor *t : {&hidden, &weight, &targets})
+        if (foreign(*t) || t->layout() != at::kStrided || !t->is_cuda() || t->device() != hidden.device()) return false;
+    return weight.dim() == 2 && weight.size(0) >= 1 && weight.size(0) <= 1 << 24 && weight.size(1) >= 1 && weight.size(1) <= 65536 && targets.numel() <= 1 << 24 &&
+           (targets.scalar_type() == at::kLong || targets.scalar_type() == at::kInt);
+}
+
 // ---- AdamW (lists of a hundred tensors and more: what is done per tensor is kept small)
 const Tensor &tensor_of(PyObject *x, const char *name) {
     if (!THPVariable_Check(x)) raise(PyExc_TypeError, std::string(name) + " must be tensors");
@@ -440,6 +458,8 @@ void adamw_step(const py::object &params_in, const py::object &grads_in, const p
 void bind_training(py::module_ &m) {
     m.def("add_rms_norm", &add_rms_norm);
     m.def("add_rms_norm_8bit", &add_rms_norm_8bit);
+    m.def("norm_covers", &norm_covers);
+    m.def("loss_covers", &loss_covers);
     m.def("linear_cross_entropy", &linear_cross_entropy);
     m.def("adamw_step", &adamw_step);
 }

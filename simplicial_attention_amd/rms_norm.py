@@ -32,11 +32,12 @@ def add_rms_norm_8bit(x: Tensor, residual: Tensor | None = None, weight: Tensor 
 
 
 _FORWARD, _RMS_NORM = nn.RMSNorm.forward, F.rms_norm
+_PLAIN = (Tensor, nn.Parameter)
 
 
 def _covered(norm):
     """What this module computes is the kernel's to compute, and nobody sees its calls."""
-    return (type(norm) is nn.RMSNorm and norm.weight is not None and nn.RMSNorm.forward is _FORWARD and nn.RMSNorm.__call__ is nn.Module.__call__ and F.rms_norm is _RMS_NORM
+    return (type(norm) is nn.RMSNorm and type(norm.weight) in _PLAIN and nn.RMSNorm.forward is _FORWARD and nn.RMSNorm.__call__ is nn.Module.__call__ and F.rms_norm is _RMS_NORM
             and not (modes() or all_watched() or watched(norm)))
 
 
@@ -44,9 +45,10 @@ def norm_behind(norm, x: Tensor, residual: Tensor | None) -> tuple[Tensor, Tenso
     """``total = x + residual`` (x alone without one) and ``norm(total)`` of an ``nn.RMSNorm`` module: ``(normed, total)``.  Modules and tensors that the kernel does not cover, and modules
     whose calls someone sees (hooks, tracers, modes), go through torch."""
     # (torch.fx hands over proxies: the type comes first)
-    if (not isinstance(x, Tensor) or not _covered(norm) or not x.is_cuda or x.shape[-1] > 16384 or norm.normalized_shape != (x.shape[-1],)
+    if (type(x) not in _PLAIN or not _covered(norm) or not x.is_cuda or norm.normalized_shape != (x.shape[-1],)
             or torch.is_autocast_enabled() or torch.compiler.is_compiling() or torch.jit.is_tracing()
-            or norm.weight.dtype != x.dtype or x.dtype not in (torch.bfloat16, torch.float16, torch.float32) or (residual is not None and residual.dtype != x.dtype)):
+            or norm.weight.dtype != x.dtype or (residual is not None and (type(residual) not in _PLAIN or residual.dtype != x.dtype))
+            or not _native.torch_ext().norm_covers(x, residual, norm.weight)):
         total = x if residual is None else residual + x
         return norm(total), total
     return add_rms_norm(x, residual, norm.weight, norm.eps)

@@ -16,6 +16,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from . import _native
 from .cross_entropy import linear_cross_entropy
 from .linear import _watched, all_watched, apply_linear, modes, watched
 from .paged import PagedCache, paged_append, paged_attn
@@ -109,7 +110,8 @@ _FORWARDS = {module: module.forward for module in (Attention, SlidingWindowTwoSi
 class TwoSimplicialTransformer(nn.Module):
     """``fused`` (not an argument of the reference's): every residual's addition and the norm behind it are one pass over the rows (:func:`add_rms_norm`), with and without a
     cache.  The same roundings; the norms' sums are in another order.  Where someone sees the calls of modules or operators (hooks, tracers, modes) or has replaced a ``forward``, and
-    under autocast, they are separate calls."""
+    under autocast, they are separate calls, as for tensors that the kernel does not cover.  Its backward refuses second
+    derivatives and batched gradients."""
 
     fused = False                            # (stacks that were pickled without it)
 
@@ -191,7 +193,9 @@ class TwoSimplicialLM(nn.Module):
     (train.py:64-135).  ``generate`` answers prompts from a paged cache (the reference recomputes the sequence for every token).
 
     ``fused`` (not an argument of the reference's): the stack's additions and norms in one pass each, and the loss of bfloat16 and float16 models without logits
-    (:func:`linear_cross_entropy`, which does not round them to that dtype in between).  Under autocast, and where someone sees the calls of modules or operators, they are separate calls."""
+    (:func:`linear_cross_entropy`, which does not round them to that dtype in between).  Under autocast, where someone sees the calls of modules or operators, and of
+    tensors that the kernels do not cover (transforms of ``torch.func``, tangents, subclasses), they are separate calls.  Second derivatives and batched gradients
+    (``create_graph=True``, ``is_grads_batched=True``) are refused by the kernels' backward passes."""
 
     fused = False
 
@@ -214,19 +218,19 @@ class TwoSimplicialLM(nn.Module):
             x, target = x[:, :-1], x[:, 1:]
         positions = torch.arange(x.shape[-1], device=x.device)
         hidden = self.transformer(self.token_emb(x) + self.pos_emb(positions))
-        if target is not None and self._can_fuse(hidden):
+        if target is not None and self._can_fuse(hidden, target):
             return linear_cross_entropy(hidden, self.to_logits.weight, target)
         logits = apply_linear(self.to_logits, hidden)
         if target is None:
             return logits
         return F.cross_entropy(logits.flatten(0, 1).float(), target.flatten())
 
-    def _can_fuse(self, hidden):
+    def _can_fuse(self, hidden, target):
         weight = self.to_logits.weight
-        return (self.fused and isinstance(hidden, torch.Tensor) and type(self.to_logits) is nn.Linear and self.to_logits.bias is None and not _watched(self.to_logits)
-                and F.cross_entropy is _CROSS_ENTROPY and not modes() and hidden.is_cuda and hidden.device == weight.device
+        return (self.fused and type(self.to_logits) is nn.Linear and all(type(t) in (torch.Tensor, nn.Parameter) for t in (hidden, target, weight))
+                and self.to_logits.bias is None and not _watched(self.to_logits) and F.cross_entropy is _CROSS_ENTROPY and not modes() and hidden.is_cuda
                 and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.dtype == weight.dtype and not torch.is_autocast_enabled() and not torch.jit.is_tracing()
-                and not torch.compiler.is_compiling())
+                and not torch.compiler.is_compiling() and _native.torch_ext().loss_covers(hidden, weight, target))
 
     @torch.no_grad()
     def logits_cached(self, x, cache, batch, rows=None):
