@@ -40,7 +40,8 @@ class AdamW(torch.optim.Optimizer):
     count their own steps.
 
     ``capturable``: the step count of each group is on the GPU, and ``lr`` may be a float32 tensor there, so that a recorded :meth:`step` can be replayed; all parameters of a group
-    need gradients then, in every step, and the first one is not recorded (a replay would make the states anew).  The parameters of a group are on one GPU.
+    need gradients then, in every step, and the first one is not recorded (a replay would make the states anew).  The parameters of a group are on one GPU.  The option may be
+    changed between steps (``group['capturable'] = True`` behind a checkpoint that was saved without it): the count goes on where it was, which has to be one for all parameters.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits: int = 32, masters: bool = True, min_8bit_size: int = 4096,
@@ -80,6 +81,12 @@ class AdamW(torch.optim.Optimizer):
             capturable, by_step = group['capturable'], {}
             if recording and not capturable:
                 raise RuntimeError('a step that is recorded needs capturable=True: every replay would be the same step')
+            if not capturable and 'step_at' in group:
+                # (the option has been taken back: the parameters count on from there)
+                count = int(group.pop('step_at'))
+                for param in group['params']:
+                    if self.state.get(param):
+                        self.state[param]['step'] = count
             for param in group['params']:
                 grad = param.grad
                 if grad is None:
@@ -90,6 +97,8 @@ class AdamW(torch.optim.Optimizer):
                 if not state:
                     if recording:
                         raise RuntimeError('the first step of a parameter cannot be recorded: a replay would make its states anew')
+                    if capturable and 'step_at' in group:
+                        raise RuntimeError('a group that can be captured has one count of steps: parameters that come later need a group of their own')
                     state = self._state_of(param, group)
                 if not capturable:
                     state['step'] += 1
@@ -107,7 +116,11 @@ class AdamW(torch.optim.Optimizer):
                 lists[4].append(state.get('master'))
             if capturable and by_step:
                 if 'step_at' not in group:
-                    group['step_at'] = torch.zeros(1, dtype=torch.int64, device=group['params'][0].device)
+                    if recording:
+                        raise RuntimeError('the first step of a group that can be captured cannot be recorded: a replay would begin its count anew')
+                    if len(by_step) > 1:
+                        raise RuntimeError('a group that can be captured has one count of steps: its parameters have made different numbers of them')
+                    group['step_at'] = torch.full((1,), next(iter(by_step)), dtype=torch.int64, device=group['params'][0].device)
                 group['step_at'] += 1
             for step, (params, grads, averages, squares, masters) in by_step.items():
                 adamw_step(params, grads, averages, squares, masters=masters, step=group['step_at'] if capturable else step, lr=group['lr'], betas=group['betas'],
