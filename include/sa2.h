@@ -424,6 +424,8 @@ typedef struct sa2_adamw_step {
 } sa2_adamw_step;
 /* Refused: tensors of the list that share memory they are written in. */
 int sa2_adamw(const sa2_adamw_tensor *tensors, int64_t count, const sa2_adamw_step *step, void *hip_stream);
+/* Its checks alone, for steps that take several calls: nothing is launched. */
+int sa2_adamw_check(const sa2_adamw_tensor *tensors, int64_t count, const sa2_adamw_step *step);
 
 /* Softmax cross entropy of a read-out layer: with z = hidden weight^T, lse_i = log sum over the vocabulary of exp z_iv, the loss of row i is lse_i - z[i][targets[i]], 0 where
  * targets[i] is ignore_index; loss is per row (reduction 0), their sum over the number of rows that count (1) or their sum (2).  No logits are kept.  hidden is

@@ -35,7 +35,7 @@ EXPORTS = ('sa2_version', 'sa2_last_error', 'sa2_supported', 'sa2_saved_t_bytes'
            'sa2_wgrad_workspace_bytes', 'sa2_wgrad',
            'sa2_paged_attn_workspace_bytes', 'sa2_paged_attn', 'sa2_paged_simplicial_attn_workspace_bytes', 'sa2_paged_simplicial_attn',
            'sa2_paged_append', 'sa2_copy_pages', 'sa2_sample_workspace_bytes', 'sa2_sample',
-           'sa2_add_rms_norm', 'sa2_add_rms_norm_8bit', 'sa2_add_rms_norm_bwd_workspace_bytes', 'sa2_add_rms_norm_bwd', 'sa2_adamw',
+           'sa2_add_rms_norm', 'sa2_add_rms_norm_8bit', 'sa2_add_rms_norm_bwd_workspace_bytes', 'sa2_add_rms_norm_bwd', 'sa2_adamw', 'sa2_adamw_check',
            'sa2_linear_ce_workspace_bytes', 'sa2_linear_ce', 'sa2_linear_ce_bwd_workspace_bytes', 'sa2_linear_ce_bwd')
 
 
@@ -191,6 +191,8 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.sa2_add_rms_norm_bwd.argtypes = [N, V, I64, V, V, V, I64, V, I64, V, V, V, V, I64, V]
     lib.sa2_adamw.restype = ctypes.c_int
     lib.sa2_adamw.argtypes = [ctypes.POINTER(AdamwTensor), I64, ctypes.POINTER(AdamwStep), V]
+    lib.sa2_adamw_check.restype = ctypes.c_int
+    lib.sa2_adamw_check.argtypes = [ctypes.POINTER(AdamwTensor), I64, ctypes.POINTER(AdamwStep)]
     C = ctypes.POINTER(LinearCeProblem)
     for name in ('sa2_linear_ce_workspace_bytes', 'sa2_linear_ce_bwd_workspace_bytes'):
         getattr(lib, name).restype = I64

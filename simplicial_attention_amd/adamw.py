@@ -22,8 +22,13 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     ``step`` counts from 1, this step included.  ``step`` (int64) and ``lr`` (float32) may be tensors of one number on the GPU, which a recorded and
     replayed call reads anew; ``grad_scale`` is one that gradients are multiplied by (a clipping coefficient).  Parameters that share memory, or one that is given twice, are refused.
     """
+    _call(params, grads, exp_avgs, exp_avg_sqs, masters, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, grad_scale=grad_scale, seed=seed)
+
+
+def _call(params, grads, exp_avgs, exp_avg_sqs, masters, *, step, lr, betas, eps, weight_decay, grad_scale, seed, launch=True):
+    # (without a launch: the checks alone)
     _native.torch_ext().adamw_step(params, grads, exp_avgs, exp_avg_sqs, masters, step, lr, float(betas[0]), float(betas[1]), float(eps), float(weight_decay), grad_scale,
-                                   int(seed) & 0xffffffff)
+                                   int(seed) & 0xffffffff, launch)
 
 
 def state_8bit(param: Tensor) -> tuple[Tensor, Tensor]:
@@ -77,55 +82,86 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         recording = torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
-        for index, group in enumerate(self.param_groups):
-            capturable, by_step = group['capturable'], {}
-            if recording and not capturable:
-                raise RuntimeError('a step that is recorded needs capturable=True: every replay would be the same step')
-            if not capturable and 'step_at' in group:
-                # (the option has been taken back: the parameters count on from there)
-                count = int(group.pop('step_at'))
-                for param in group['params']:
-                    if self.state.get(param):
-                        self.state[param]['step'] = count
-            for param in group['params']:
-                grad = param.grad
-                if grad is None:
-                    if capturable:
-                        raise RuntimeError('a group that can be captured needs gradients of all its parameters')
-                    continue
-                state = self.state[param]
-                if not state:
-                    if recording:
-                        raise RuntimeError('the first step of a parameter cannot be recorded: a replay would make its states anew')
-                    if capturable and 'step_at' in group:
-                        raise RuntimeError('a group that can be captured has one count of steps: parameters that come later need a group of their own')
-                    state = self._state_of(param, group)
-                if not capturable:
-                    state['step'] += 1
-                lists = by_step.get(state['step'])
-                if lists is None:
-                    lists = by_step[state['step']] = ([], [], [], [], [])
-                lists[0].append(param)
-                lists[1].append(grad)
-                if 'exp_avg_scales' in state:
-                    lists[2].append((state['exp_avg'], state['exp_avg_scales']))
-                    lists[3].append((state['exp_avg_sq'], state['exp_avg_sq_scales']))
+        # (all groups are looked at before the first is changed: a step that is refused leaves the optimizer as it was)
+        calls, made, begun = [], {}, []
+        try:
+            for index, group in enumerate(self.param_groups):
+                for count, lists in self._lists(group, recording, made, begun).items():
+                    calls.append((group, count, lists, dict(lr=group['lr'], betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'], grad_scale=grad_scale,
+                                                            seed=group['seed'] + 0x10000 * index)))
+            if len(calls) > 1:                     # (one call is refused as a whole)
+                for group, count, (_, *lists), more in calls:
+                    _call(*lists, step=group['step_at'] if group['capturable'] else count + 1, launch=False, **more)
+            for group, count, (states, *lists), more in calls:
+                if group['capturable']:
+                    group['step_at'] += 1
+                    try:
+                        _call(*lists, step=group['step_at'], **more)
+                    except BaseException:
+                        group['step_at'] -= 1
+                        raise
                 else:
-                    lists[2].append(state['exp_avg'])
-                    lists[3].append(state['exp_avg_sq'])
-                lists[4].append(state.get('master'))
-            if capturable and by_step:
-                if 'step_at' not in group:
-                    if recording:
-                        raise RuntimeError('the first step of a group that can be captured cannot be recorded: a replay would begin its count anew')
-                    if len(by_step) > 1:
-                        raise RuntimeError('a group that can be captured has one count of steps: its parameters have made different numbers of them')
-                    group['step_at'] = torch.full((1,), next(iter(by_step)), dtype=torch.int64, device=group['params'][0].device)
-                group['step_at'] += 1
-            for step, (params, grads, averages, squares, masters) in by_step.items():
-                adamw_step(params, grads, averages, squares, masters=masters, step=group['step_at'] if capturable else step, lr=group['lr'], betas=group['betas'],
-                           eps=group['eps'], weight_decay=group['weight_decay'], grad_scale=grad_scale, seed=group['seed'] + 0x10000 * index)
+                    _call(*lists, step=count + 1, **more)
+                    for state in states:
+                        state['step'] = count + 1
+                for param in lists[0] if made else ():
+                    made.pop(param, None)
+                begun = [other for other in begun if other is not group]
+        except BaseException:
+            for param in made:
+                del self.state[param]
+            for group in begun:
+                del group['step_at']
+            raise
         return loss
+
+    def _lists(self, group, recording, made, begun):
+        """What a step of a group works on, by the steps that its parameters have made: lists of states, parameters, gradients, both averages, masters.  New states go to ``made``, a
+        group whose count moves to the GPU to ``begun``."""
+        capturable, by_count = group['capturable'], {}
+        if recording and not capturable:
+            raise RuntimeError('a step that is recorded needs capturable=True: every replay would be the same step')
+        if not capturable and 'step_at' in group:
+            # (the option has been taken back: the parameters count on from there)
+            count = int(group.pop('step_at'))
+            for param in group['params']:
+                if self.state.get(param):
+                    self.state[param]['step'] = count
+        for param in group['params']:
+            grad = param.grad
+            if grad is None:
+                if capturable:
+                    raise RuntimeError('a group that can be captured needs gradients of all its parameters')
+                continue
+            state = self.state.get(param)
+            if not state:
+                if recording:
+                    raise RuntimeError('the first step of a parameter cannot be recorded: a replay would make its states anew')
+                if capturable and 'step_at' in group:
+                    raise RuntimeError('a group that can be captured has one count of steps: parameters that come later need a group of their own')
+                made[param] = True
+                state = self._state_of(param, group)
+            lists = by_count.get(state['step'])
+            if lists is None:
+                lists = by_count[state['step']] = ([], [], [], [], [], [])
+            lists[0].append(state)
+            lists[1].append(param)
+            lists[2].append(grad)
+            if 'exp_avg_scales' in state:
+                lists[3].append((state['exp_avg'], state['exp_avg_scales']))
+                lists[4].append((state['exp_avg_sq'], state['exp_avg_sq_scales']))
+            else:
+                lists[3].append(state['exp_avg'])
+                lists[4].append(state['exp_avg_sq'])
+            lists[5].append(state.get('master'))
+        if capturable and by_count and 'step_at' not in group:
+            if recording:
+                raise RuntimeError('the first step of a group that can be captured cannot be recorded: a replay would begin its count anew')
+            if len(by_count) > 1:
+                raise RuntimeError('a group that can be captured has one count of steps: its parameters have made different numbers of them')
+            begun.append(group)
+            group['step_at'] = torch.full((1,), next(iter(by_count)), dtype=torch.int64, device=group['params'][0].device)
+        return by_count
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):

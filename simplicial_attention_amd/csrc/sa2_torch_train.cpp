@@ -338,7 +338,7 @@ struct Items {
 };
 
 void adamw_step(const py::object &params_in, const py::object &grads_in, const py::object &averages_in, const py::object &squares_in, const py::object &masters_in,
-                const py::object &step, const py::object &lr, double beta1, double beta2, double eps, double weight_decay, const MaybeTensor &grad_scale, int64_t seed) {
+                const py::object &step, const py::object &lr, double beta1, double beta2, double eps, double weight_decay, const MaybeTensor &grad_scale, int64_t seed, bool launch) {
     refuse_recorder("adamw_step");
     const Items params(params_in, "params must be a sequence of tensors"), grads(grads_in, "grads must be a sequence of tensors"),
         states[2] = {Items(averages_in, "exp_avgs must be a sequence"), Items(squares_in, "exp_avg_sqs must be a sequence")};
@@ -371,7 +371,7 @@ void adamw_step(const py::object &params_in, const py::object &grads_in, const p
         if (given.sizes() != p.sizes()) raise(PyExc_ValueError, "gradient " + shape_text(given) + " does not match its parameter's " + shape_text(p));
         sa2_adamw_tensor t{};
         t.param = p.data_ptr();
-        if (laid_out_alike(p, given)) {
+        if (!launch || laid_out_alike(p, given)) {
             t.grad = given.data_ptr();
         } else {
             const c10::DeviceGuard guard(p.device());
@@ -447,6 +447,7 @@ void adamw_step(const py::object &params_in, const py::object &grads_in, const p
         s.grad_scale = static_cast<const float *>(grad_scale->data_ptr());
     }
     if (items.empty()) return;
+    if (!launch) return check(sa2_adamw_check(items.data(), (int64_t)items.size(), &s));
     const c10::DeviceGuard guard(*device);
     check(sa2_adamw(items.data(), (int64_t)items.size(), &s, c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device->index()).stream()));
     // (a graph that saved one of these sees that it has changed)

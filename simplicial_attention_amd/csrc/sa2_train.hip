@@ -118,6 +118,55 @@ int forward(const sa2_norm_problem *p, const void *x, int64_t x_stride, const vo
     return launched("norm");
 }
 
+// the call's checks; `all`: elements of each kind of launch (type, states in 8 bits)
+int check_adamw(const sa2_adamw_tensor *tensors, int64_t count, const sa2_adamw_step *step, double (&all)[3][2]) {
+    if (!step || (count > 0 && !tensors)) return fail_with(SA2_ERR_NULL_POINTER, "tensors and step are required");
+    if (count < 0 || count > 0x7fffffff) return fail_with(SA2_ERR_BAD_SHAPE, "%lld tensors", (long long)count);
+    if (!(step->beta1 >= 0 && step->beta1 < 1) || !(step->beta2 >= 0 && step->beta2 < 1) || !(step->eps >= 0) || !std::isfinite(step->eps) || !std::isfinite(step->lr) ||
+        !(step->lr >= 0) || !(step->weight_decay >= 0) || !std::isfinite(step->weight_decay))
+        return fail_with(SA2_ERR_BAD_SHAPE, "lr=%g betas=%g, %g eps=%g weight_decay=%g", step->lr, step->beta1, step->beta2, step->eps, step->weight_decay);
+    if (!step->step_at && step->step < 1) return fail_with(SA2_ERR_BAD_SHAPE, "step=%lld, the first is 1", (long long)step->step);
+    try {
+        // what a step writes: no two of these may share memory (workgroups run in no order)
+        std::vector<std::pair<uintptr_t, uintptr_t>> written;
+        written.reserve(6 * count);
+        for (int64_t i = 0; i < count; ++i) {
+            const sa2_adamw_tensor &t = tensors[i];
+            if (t.n < 1 || t.n > (int64_t)1 << 40 || t.type < 0 || t.type > 2) continue;      // (refused, or skipped, below)
+            const int64_t state = t.bits == 8 ? t.n : 4 * t.n, scales = t.bits == 8 ? (t.n + 255) / 256 * 4 : 0;
+            const auto add = [&](const void *at, int64_t bytes) {
+                if (at && bytes) written.emplace_back(reinterpret_cast<uintptr_t>(at), reinterpret_cast<uintptr_t>(at) + bytes);
+            };
+            add(t.param, t.n * size_of(t.type));
+            add(t.exp_avg, state);
+            add(t.exp_avg_sq, state);
+            add(t.exp_avg_scales, scales);
+            add(t.exp_avg_sq_scales, scales);
+            add(t.master, 4 * t.n);
+        }
+        std::sort(written.begin(), written.end(), [](const auto &a, const auto &b) { return a.first < b.first; });
+        for (size_t i = 1; i < written.size(); ++i)
+            if (written[i].first < written[i - 1].second) return fail_with(SA2_ERR_BAD_SHAPE, "parameters, masters or states share memory: each may be in the list once");
+    } catch (const std::bad_alloc &) {
+        return fail_with(SA2_ERR_BAD_SHAPE, "no memory for %lld tensors", (long long)count);
+    }
+    for (int64_t i = 0; i < count; ++i) {
+        const sa2_adamw_tensor &t = tensors[i];
+        if (t.n < 0) return fail_with(SA2_ERR_BAD_SHAPE, "tensor %lld of %lld elements", (long long)i, (long long)t.n);
+        if (t.type < 0 || t.type > 2 || (t.bits != 32 && t.bits != 8)) return fail_with(SA2_ERR_UNSUPPORTED, "tensor %lld: type %d, states of %d bits", (long long)i, t.type, t.bits);
+        if (t.n == 0) continue;
+        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (t.bits == 8 && (!t.exp_avg_scales || !t.exp_avg_sq_scales)))
+            return fail_with(SA2_ERR_NULL_POINTER, "tensor %lld: parameter, gradient, states and, of 8-bit ones, scales are required", (long long)i);
+        const int state = t.bits == 8 ? 0 : 3;
+        if (!element_aligned(t.param, t.type) || !element_aligned(t.grad, t.type) || ((reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq)) & state) != 0 ||
+            !element_aligned(t.master, 2) || !element_aligned(t.exp_avg_scales, 2) || !element_aligned(t.exp_avg_sq_scales, 2))
+            return fail_with(SA2_ERR_ALIGNMENT, "tensor %lld: tensors must be aligned to their elements", (long long)i);
+        if (t.n > (int64_t)1 << 40) return fail_with(SA2_ERR_BAD_SHAPE, "tensor %lld of %lld elements", (long long)i, (long long)t.n);
+        all[t.type][t.bits == 8] += (double)t.n;
+    }
+    return SA2_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -181,52 +230,14 @@ int sa2_add_rms_norm_bwd(const sa2_norm_problem *p, const void *total, int64_t t
     return launched("norm weight gradient");
 }
 
+int sa2_adamw_check(const sa2_adamw_tensor *tensors, int64_t count, const sa2_adamw_step *step) {
+    double all[3][2] = {};
+    return check_adamw(tensors, count, step, all);
+}
+
 int sa2_adamw(const sa2_adamw_tensor *tensors, int64_t count, const sa2_adamw_step *step, void *hip_stream) {
-    if (!step || (count > 0 && !tensors)) return fail_with(SA2_ERR_NULL_POINTER, "tensors and step are required");
-    if (count < 0 || count > 0x7fffffff) return fail_with(SA2_ERR_BAD_SHAPE, "%lld tensors", (long long)count);
-    if (!(step->beta1 >= 0 && step->beta1 < 1) || !(step->beta2 >= 0 && step->beta2 < 1) || !(step->eps >= 0) || !std::isfinite(step->eps) || !std::isfinite(step->lr) ||
-        !(step->lr >= 0) || !(step->weight_decay >= 0) || !std::isfinite(step->weight_decay))
-        return fail_with(SA2_ERR_BAD_SHAPE, "lr=%g betas=%g, %g eps=%g weight_decay=%g", step->lr, step->beta1, step->beta2, step->eps, step->weight_decay);
-    if (!step->step_at && step->step < 1) return fail_with(SA2_ERR_BAD_SHAPE, "step=%lld, the first is 1", (long long)step->step);
-    double all[3][2] = {};                    // elements of each kind of launch
-    try {
-        // what a step writes: no two of these may share memory (workgroups run in no order)
-        std::vector<std::pair<uintptr_t, uintptr_t>> written;
-        written.reserve(6 * count);
-        for (int64_t i = 0; i < count; ++i) {
-            const sa2_adamw_tensor &t = tensors[i];
-            if (t.n < 1 || t.n > (int64_t)1 << 40 || t.type < 0 || t.type > 2) continue;      // (refused, or skipped, below)
-            const int64_t state = t.bits == 8 ? t.n : 4 * t.n, scales = t.bits == 8 ? (t.n + 255) / 256 * 4 : 0;
-            const auto add = [&](const void *at, int64_t bytes) {
-                if (at && bytes) written.emplace_back(reinterpret_cast<uintptr_t>(at), reinterpret_cast<uintptr_t>(at) + bytes);
-            };
-            add(t.param, t.n * size_of(t.type));
-            add(t.exp_avg, state);
-            add(t.exp_avg_sq, state);
-            add(t.exp_avg_scales, scales);
-            add(t.exp_avg_sq_scales, scales);
-            add(t.master, 4 * t.n);
-        }
-        std::sort(written.begin(), written.end(), [](const auto &a, const auto &b) { return a.first < b.first; });
-        for (size_t i = 1; i < written.size(); ++i)
-            if (written[i].first < written[i - 1].second) return fail_with(SA2_ERR_BAD_SHAPE, "parameters, masters or states share memory: each may be in the list once");
-    } catch (const std::bad_alloc &) {
-        return fail_with(SA2_ERR_BAD_SHAPE, "no memory for %lld tensors", (long long)count);
-    }
-    for (int64_t i = 0; i < count; ++i) {
-        const sa2_adamw_tensor &t = tensors[i];
-        if (t.n < 0) return fail_with(SA2_ERR_BAD_SHAPE, "tensor %lld of %lld elements", (long long)i, (long long)t.n);
-        if (t.type < 0 || t.type > 2 || (t.bits != 32 && t.bits != 8)) return fail_with(SA2_ERR_UNSUPPORTED, "tensor %lld: type %d, states of %d bits", (long long)i, t.type, t.bits);
-        if (t.n == 0) continue;
-        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (t.bits == 8 && (!t.exp_avg_scales || !t.exp_avg_sq_scales)))
-            return fail_with(SA2_ERR_NULL_POINTER, "tensor %lld: parameter, gradient, states and, of 8-bit ones, scales are required", (long long)i);
-        const int state = t.bits == 8 ? 0 : 3;
-        if (!element_aligned(t.param, t.type) || !element_aligned(t.grad, t.type) || ((reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq)) & state) != 0 ||
-            !element_aligned(t.master, 2) || !element_aligned(t.exp_avg_scales, 2) || !element_aligned(t.exp_avg_sq_scales, 2))
-            return fail_with(SA2_ERR_ALIGNMENT, "tensor %lld: tensors must be aligned to their elements", (long long)i);
-        if (t.n > (int64_t)1 << 40) return fail_with(SA2_ERR_BAD_SHAPE, "tensor %lld of %lld elements", (long long)i, (long long)t.n);
-        all[t.type][t.bits == 8] += (double)t.n;
-    }
+    double all[3][2] = {};
+    if (const int rc = check_adamw(tensors, count, step, all)) return rc;
     AdamParams k{};
     k.seed = step->seed;
     k.step = (uint32_t)step->step;
