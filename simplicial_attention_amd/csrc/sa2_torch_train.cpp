@@ -447,6 +447,10 @@ void adamw_step(const py::object &params_in, const py::object &grads_in, const p
         s.grad_scale = static_cast<const float *>(grad_scale->data_ptr());
     }
     if (items.empty()) return;
+    // (a tensor made in inference mode has no version to count)
+    if (!c10::InferenceMode::is_enabled())
+        for (c10::TensorImpl *t : written)
+            if (t->is_inference()) raise(PyExc_RuntimeError, "adamw_step: a tensor made in inference mode is updated outside it");
     if (!launch) return check(sa2_adamw_check(items.data(), (int64_t)items.size(), &s));
     const c10::DeviceGuard guard(*device);
     check(sa2_adamw(items.data(), (int64_t)items.size(), &s, c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device->index()).stream()));
