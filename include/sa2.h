@@ -448,7 +448,8 @@ int sa2_linear_ce(const sa2_linear_ce_problem *prob, const void *hidden, int64_t
 
 /* Its gradients, contiguous rows of `channels` in the operands' type, each written if not NULL, from dloss (device memory: one number, or with reduction 0 one per row).  Rows that do not
  * count have a gradient of zero and add nothing to the weight's, whatever they hold.  The vocabulary goes by in pieces of at least 256 tokens, of whose logits'
- * gradients the workspace holds 256 MiB or 256 tokens at a time.  Bitwise reproducible (no atomics on results). */
+ * gradients the workspace holds 256 MiB or 256 tokens at a time (fp16 with reduction 0: with the rows' weights and without, half as many tokens or 256 each).  A row of dhidden does not depend on what
+ * other rows weigh; of dweight, fp16 with reduction 0 leaves each row's part off by up to 2^-35 of the largest weight times the row.  Bitwise reproducible (no atomics on results). */
 int64_t sa2_linear_ce_bwd_workspace_bytes(const sa2_linear_ce_problem *prob);     /* -1 if the problem is invalid */
 int sa2_linear_ce_bwd(const sa2_linear_ce_problem *prob, const void *hidden, int64_t hidden_stride, const void *weight, int64_t weight_stride, const int64_t *targets,
                       const float *lse, const float *count, const uint32_t *mask, const float *dloss, void *dhidden, void *dweight, void *workspace, int64_t workspace_bytes,

@@ -10,7 +10,9 @@
 // launches.
 //
 // dz is rounded to the operands' type for its products.  To use that type's range well it is divided by the largest weight G of a row's loss
-// (mean and sum: the one weight of all) and in fp16 multiplied by 1024, which the products' results are multiplied by again in 32 bits.
+// (mean and sum: the one weight of all) and in fp16 multiplied by 1024, which the products' results are multiplied by again in 32 bits.  Where every row has a weight
+// of its own (reduction none), that would leave rows of small weights the least steps of fp16 (over 32000 tokens dH of a row at a millionth of G was off by 9 %): there dH is made from a second
+// dz without weights, and the rows of the result are multiplied by theirs.  dW adds rows up, and what it loses of one (2^-35 G of each dz) is small beside G.
 #pragma once
 
 #include "sa2_product.hpp"
@@ -37,7 +39,8 @@ struct CeParams {
     // backward
     const float *up;                         // gradient of the loss: one number, or one per row
     const float *most;                       // largest finite |up| of a row that counts (reduction none)
-    char *dz;                                // [rows][piece]
+    char *dz;                                // [rows][piece], or NULL
+    char *dz_rows;                           // the same without the rows' weights, for dH (reduction none in fp16), or NULL
     int64_t dz_row;                          // bytes
 };
 
@@ -224,7 +227,13 @@ __device__ __forceinline__ float ce_factor(const CeParams &p) {
     return *p.up * (1.f / ce_scale<T>);
 }
 
-template <int T, int NL, int NR>
+template <int T>
+__device__ __forceinline__ float ce_row_factor(const CeParams &p, int row) {
+    return p.up[row] * (1.f / ce_scale<T>);
+}
+
+// TWO: dz_rows too
+template <int T, int NL, int NR, bool TWO>
 __global__ __launch_bounds__(256, NL == 4 ? 1 : 2) void ce_dz_kernel(CeParams p) {
     using P = Product<T, NL, NR, true, true, false>;
     __shared__ __attribute__((aligned(16))) char lds[P::LDS];
@@ -264,31 +273,38 @@ __global__ __launch_bounds__(256, NL == 4 ? 1 : 2) void ce_dz_kernel(CeParams p)
                 for (int r = 0; r < 16; ++r)
                     if (mine == 32 * b + r) acc[a][b][r] -= ce_scale<T>;
         }
-        float weight = 1.f;
-        if (p.reduction == kCeNone) {
-            const float most = *p.most;
-            weight = most > 0.f ? p.up[row] / most : p.up[row];          // (an infinite weight, or one that is no number, is its own row's matter)
+        const float valid = counts && !(target >= 0 && target < p.vocab) ? NAN : 1.f;
+        const auto store = [&](char *dz, float by) {
+            if (wave_any(by != 1.f)) {
+#pragma unroll
+                for (int b = 0; b < NR; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[a][b][r] *= by;
+            }
+            int end = p.vocab - p.first - c0 - 16 * hf, first_row = row0;   // columns of this half that are tokens
+            asm("" : "+v"(end), "+s"(first_row));                           // (else the compiler keeps masks of all columns, and addresses for the next store, and spills them)
+            if (wave_any(!counts || end < 32 * NR)) {
+#pragma unroll
+                for (int b = 0; b < NR; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (!counts || 32 * b + r >= end) acc[a][b][r] = 0.f;
+            }
+#pragma unroll
+            for (int b = 0; b < NR; ++b) rows.put(b, acc[a][b]);
+            rows.each([&](int r, int col, u32x4 v) {
+                if (first_row + r < p.rows) st_global16(dz + (int64_t)(first_row + r) * p.dz_row + 2 * (c0 + col), v);
+            });
+        };
+        if constexpr (TWO) store(p.dz_rows, valid);
+        if (!TWO || p.dz) {
+            float weight = TWO ? 1.f : valid;
+            if (p.reduction == kCeNone) {
+                const float most = *p.most;
+                weight *= most > 0.f ? p.up[row] / most : p.up[row];          // (an infinite weight, or one that is no number, is its own row's matter)
+            }
+            store(p.dz, weight);
         }
-        if (counts && !(target >= 0 && target < p.vocab)) weight = NAN;
-        if (wave_any(weight != 1.f)) {
-#pragma unroll
-            for (int b = 0; b < NR; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[a][b][r] *= weight;
-        }
-        const int end = p.vocab - p.first - c0 - 16 * hf;                // columns of this half that are tokens
-        if (wave_any(!counts || end < 32 * NR)) {
-#pragma unroll
-            for (int b = 0; b < NR; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!counts || 32 * b + r >= end) acc[a][b][r] = 0.f;
-        }
-#pragma unroll
-        for (int b = 0; b < NR; ++b) rows.put(b, acc[a][b]);
-        rows.each([&](int r, int col, u32x4 v) {
-            if (row0 + r < p.rows) st_global16(p.dz + (int64_t)(row0 + r) * p.dz_row + 2 * (c0 + col), v);
-        });
     }
 }
 
@@ -314,6 +330,7 @@ struct CeOutput {
     float *parts;                  // else: [share][rows][dim]
     int rows, add;                 // add: to what is in the parts
     int masked;                    // rows that do not count become zero
+    int by_row;                    // rows of a dz without weights: each is multiplied by its own
 };
 
 template <int T, int NL, int NR, bool DIRECT>
@@ -328,8 +345,12 @@ __device__ __forceinline__ void ce_store(const CeParams &p, const CeOutput &o, c
     for (int a = 0; a < NL; ++a) {
         const int row0 = 64 * NL * at.tile_l + 32 * (NL * (wave >> 1) + a);
         take(acc[a]);
+        float by = factor;
+        if constexpr (DIRECT && T == kF16) {
+            if (o.by_row) by = ce_row_factor<T>(p, min(row0 + rows.row, o.rows - 1));
+        }
 #pragma unroll
-        for (int b = 0; b < NR; ++b) rows.put(b, acc[a][b], factor);
+        for (int b = 0; b < NR; ++b) rows.put(b, acc[a][b], by);
         rows.each([&](int r, int col, u32x4 v) {
             const int row = row0 + r, d = c0 + col;
             if (row >= o.rows || d >= p.dim) return;
@@ -398,18 +419,22 @@ __global__ __launch_bounds__(256) void ce_shared_logits_kernel(CeParams p, CeOut
         if (c >= p.dim) return;
         const bool counts = target != p.ignore;
         const float lse = p.lse[row];
-        float weight = 1.f;
+        const float valid = counts && !(target >= 0 && target < p.vocab) ? NAN : 1.f;
+        float weight = valid;
         if (p.reduction == kCeNone) {
             const float most = *p.most;
-            weight = most > 0.f ? p.up[row] / most : p.up[row];
+            weight *= most > 0.f ? p.up[row] / most : p.up[row];
         }
-        if (counts && !(target >= 0 && target < p.vocab)) weight = NAN;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            z[i] = (fast_exp2((z[i] - lse) * kLog2e + ce_log2_scale<T>) - (i == mine ? ce_scale<T> : 0.f)) * weight;
-            if (!counts || i >= end) z[i] = 0.f;
-        }
-        *reinterpret_cast<u32x2 *>(p.dz + (int64_t)row * p.dz_row + 2 * c) = pack4<T>(z);
+        for (int i = 0; i < 4; ++i) z[i] = fast_exp2((z[i] - lse) * kLog2e + ce_log2_scale<T>) - (i == mine ? ce_scale<T> : 0.f);
+        const auto store = [&](char *dz, float by) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = !counts || i >= end ? 0.f : z[i] * by;
+            *reinterpret_cast<u32x2 *>(dz + (int64_t)row * p.dz_row + 2 * c) = pack4<T>(v);
+        };
+        if (T == kF16 && p.dz_rows) store(p.dz_rows, valid);
+        if (p.dz) store(p.dz, weight);
     }
 }
 
@@ -469,11 +494,11 @@ __global__ __launch_bounds__(256) void ce_combine_kernel(CeParams p, CeSum a, Ce
     const bool second = blockIdx.y != 0;
     const float *const parts = second ? b.o.parts : a.o.parts;
     char *const out = second ? b.out : a.out;
-    const int rows = second ? b.o.rows : a.o.rows, masked = second ? b.o.masked : a.o.masked, shares = second ? b.shares : a.shares, dim = a.dim;
+    const int rows = second ? b.o.rows : a.o.rows, masked = second ? b.o.masked : a.o.masked, by_row = second ? b.o.by_row : a.o.by_row, shares = second ? b.shares : a.shares, dim = a.dim;
     const int64_t at = (((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 256 + threadIdx.x) * 4, all = (int64_t)rows * dim;
     if (at >= all) return;
     const int row = (int)(at / dim), d = (int)(at - (int64_t)row * dim);
-    const float factor = ce_factor<T>(p);
+    const float factor = by_row ? ce_row_factor<T>(p, row) : ce_factor<T>(p);
     const bool counts = !masked || (p.mask[row >> 5] >> (row & 31) & 1);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     const float *src = parts + at;

@@ -67,7 +67,7 @@ ProductPlan plan_of(int64_t l, int64_t r, int64_t k, bool gradient, bool masked,
 struct CePlan {
     ProductPlan logits, dz, dh, dw;
     int64_t piece = 0, pieces = 0;
-    int64_t dz_row = 0, dz_bytes = 0, h_bytes = 0, w_bytes = 0, z_bytes = 0;
+    int64_t dz_row = 0, dz_bytes = 0, rows_bytes = 0, h_bytes = 0, w_bytes = 0, z_bytes = 0;
     int64_t parts = 0, parts_bytes = 0, logits_bytes = 0;           // parts: of a row's maximum and sum
 };
 
@@ -86,7 +86,8 @@ int64_t shares_bytes(const ProductPlan &p, int64_t rows, int64_t tokens) { retur
 
 CePlan plan(const sa2_linear_ce_problem &p) {
     CePlan c;
-    const int64_t most = std::max<int64_t>(256, kMostDzBytes / (2 * p.rows) / 256 * 256);
+    const bool two = p.dtype == SA2_ELEMENT_F16 && p.reduction == kCeNone;              // dz with and without the rows' weights
+    const int64_t most = std::max<int64_t>(256, kMostDzBytes / (two ? 4 : 2) / p.rows / 256 * 256);
     c.pieces = (p.vocab + most - 1) / most;
     c.piece = up_to((p.vocab + c.pieces - 1) / c.pieces, 256);
     c.pieces = (p.vocab + c.piece - 1) / c.piece;
@@ -108,6 +109,7 @@ CePlan plan(const sa2_linear_ce_problem &p) {
     // (rows of a power of two of bytes would all begin in the same channel of the L2)
     c.dz_row = c.piece * 2 + 256;
     c.dz_bytes = up_to(p.rows * c.dz_row, 256);
+    c.rows_bytes = two ? c.dz_bytes : 0;
     c.h_bytes = c.pieces > 1 || c.dh.shape.shares > 1 ? up_to((int64_t)c.dh.shape.shares * p.rows * p.dim * 4, 256) : 0;
     c.w_bytes = c.dw.shape.shares > 1 ? up_to((int64_t)c.dw.shape.shares * c.piece * p.dim * 4, 256) : 0;
     return c;
@@ -135,7 +137,7 @@ int check_workspace(const void *workspace, int64_t given, int64_t needed) {
 
 int64_t blocks_of(const sa2_linear_ce_problem &p) { return (p.rows + 31) / 32; }
 int64_t forward_bytes(const sa2_linear_ce_problem &p, const CePlan &c) { return c.logits_bytes + c.parts_bytes + up_to(p.rows * 4, 256) + up_to(blocks_of(p) * 8, 256) + 256; }
-int64_t backward_bytes(const CePlan &c) { return 256 + c.dz_bytes + c.h_bytes + c.w_bytes + c.z_bytes; }
+int64_t backward_bytes(const CePlan &c) { return 256 + c.dz_bytes + c.rows_bytes + c.h_bytes + c.w_bytes + c.z_bytes; }
 
 // f(integral_constant type, integral_constants nl and nr)
 template <typename F>
@@ -152,7 +154,7 @@ void with_kernel(int type, const ProductPlan &plan, F &&f) {
 template <bool DZ>
 void shared_logits(int type, const ProductPlan &plan, CeParams k, float *shares, int64_t tokens, hipStream_t s) {
     k.dim = (int)up_to(tokens, 8);
-    const CeOutput o{nullptr, shares, k.rows, 0, 0};
+    const CeOutput o{nullptr, shares, k.rows, 0, 0, 0};
     const int chunks = (k.dim + kCeColumns - 1) / kCeColumns;
     with_kernel(type, plan, [&](auto t, auto nl, auto nr) {
         hipLaunchKernelGGL((ce_shares_kernel<t.value, nl.value, nr.value>), dim3((unsigned)plan.groups()), dim3(256), 0, s, k, o);
@@ -247,10 +249,10 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
     k.mask = const_cast<uint32_t *>(mask);
     k.up = dloss;
     k.most = reinterpret_cast<float *>(ws);
-    k.dz = ws + 256;
+    k.dz = dweight || c.rows_bytes == 0 ? ws + 256 : nullptr;
+    k.dz_rows = dhidden && c.rows_bytes > 0 ? ws + 256 + c.dz_bytes : nullptr;
     k.dz_row = c.dz_row;
-    float *const h_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes), *const w_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes + c.h_bytes),
-          *const z_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes + c.h_bytes + c.w_bytes);
+    float *const h_parts = reinterpret_cast<float *>(ws + 256 + c.dz_bytes + c.rows_bytes), *const w_parts = h_parts + c.h_bytes / 4, *const z_parts = w_parts + c.w_bytes / 4;
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);
     if (p->reduction == kCeNone) hipLaunchKernelGGL(ce_most_kernel, dim3(1), dim3(1024), 0, s, dloss, mask, (int)p->rows, reinterpret_cast<float *>(ws));
     const ProductOperand h{static_cast<const char *>(hidden), hidden_stride * 2, (int)p->rows};
@@ -266,7 +268,11 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
         k.w = w;
         k.h = h;
         if (dz.shape.shares > 1) shared_logits<true>(p->dtype, dz, k, z_parts, tokens, s);
-        else with_kernel(p->dtype, dz, [&](auto t, auto nl, auto nr) { hipLaunchKernelGGL((ce_dz_kernel<t.value, nl.value, nr.value>), dim3((unsigned)dz.groups()), dim3(256), 0, s, k); });
+        else with_kernel(p->dtype, dz, [&](auto t, auto nl, auto nr) {
+            const auto go = [&](auto two) { hipLaunchKernelGGL((ce_dz_kernel<t.value, nl.value, nr.value, two.value>), dim3((unsigned)dz.groups()), dim3(256), 0, s, k); };
+            if constexpr (t.value == kF16) k.dz_rows ? go(std::true_type{}) : go(std::false_type{});
+            else go(std::false_type{});
+        });
         CeParams kh = k, kw = k;
         CeOutput oh{}, ow{};
         CeSum sums[2];
@@ -279,8 +285,8 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
             kh.shape = c.dh.shape;
             kh.shape.k = (int)tokens;
             kh.w = {w.ptr, w.row, p->dim};
-            kh.h = {k.dz, k.dz_row, (int)p->rows};
-            oh = {c.h_bytes == 0 ? static_cast<char *>(dhidden) : nullptr, h_parts, (int)p->rows, i > 0, 1};
+            kh.h = {k.dz_rows ? k.dz_rows : k.dz, k.dz_row, (int)p->rows};
+            oh = {c.h_bytes == 0 ? static_cast<char *>(dhidden) : nullptr, h_parts, (int)p->rows, i > 0, 1, k.dz_rows != nullptr};
             if (c.h_bytes > 0 && i + 1 == c.pieces) sums[count++] = {oh, static_cast<char *>(dhidden), c.dh.shape.shares, p->dim};
         }
         if (dweight) {
@@ -288,7 +294,7 @@ int sa2_linear_ce_bwd(const sa2_linear_ce_problem *p, const void *hidden, int64_
             kw.w = {h.ptr, h.row, p->dim};
             kw.h = {k.dz, k.dz_row, (int)up_to(tokens, 8)};          // (tiles of dz end with zeros)
             char *const out = static_cast<char *>(dweight) + first * k.channels * 2;
-            ow = {c.dw.shape.shares == 1 ? out : nullptr, w_parts, (int)tokens, 0, 0};
+            ow = {c.dw.shape.shares == 1 ? out : nullptr, w_parts, (int)tokens, 0, 0, 0};
             if (!ow.out) sums[count++] = {ow, out, dw.shape.shares, p->dim};
         }
         if (dhidden && dweight && c.dh.nr == 2 && dw.nr == 2) {
