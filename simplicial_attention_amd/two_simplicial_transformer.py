@@ -91,7 +91,8 @@ class _Layers(nn.Sequential):
     @torch.jit.unused
     def behind_norm(self, x):
         """``forward`` of rows that the norm in front has been applied to."""
-        for layer in self[1:]:
+        # (a slice of the layers would be a module made anew: 10 us a call)
+        for layer in list(self)[1:]:
             x = apply_linear(layer, x)
         return x
 

@@ -107,3 +107,10 @@ def test_compiled_norms_are_called():
         outs.append(t(x))
         assert calls == [1]
     assert close(*outs)
+
+
+def test_a_fused_stack_makes_no_modules(monkeypatch):
+    x, t = rows(), stack(True)
+    want = stack(False)(x)
+    monkeypatch.setattr(nn.Module, '__init__', lambda *_: pytest.fail('a module is made'))
+    assert torch.equal(t(x), want)
