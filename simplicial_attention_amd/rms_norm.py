@@ -45,8 +45,8 @@ def norm_behind(norm, x: Tensor, residual: Tensor | None) -> tuple[Tensor, Tenso
     """``total = x + residual`` (x alone without one) and ``norm(total)`` of an ``nn.RMSNorm`` module: ``(normed, total)``.  Modules and tensors that the kernel does not cover, and modules
     whose calls someone sees (hooks, tracers, modes), go through torch."""
     # (torch.fx hands over proxies: the type comes first)
-    if (type(x) not in _PLAIN or not _covered(norm) or not x.is_cuda or norm.normalized_shape != (x.shape[-1],)
-            or torch.is_autocast_enabled() or torch.compiler.is_compiling() or torch.jit.is_tracing()
+    if (torch.compiler.is_compiling() or torch.jit.is_tracing() or type(x) not in _PLAIN or not _covered(norm) or not x.is_cuda or norm.normalized_shape != (x.shape[-1],)
+            or torch.is_autocast_enabled()
             or norm.weight.dtype != x.dtype or (residual is not None and (type(residual) not in _PLAIN or residual.dtype != x.dtype))
             or not _native.torch_ext().norm_covers(x, residual, norm.weight)):
         total = x if residual is None else residual + x

@@ -147,7 +147,7 @@ class TwoSimplicialTransformer(nn.Module):
     @torch.jit.unused
     def _can_fuse(self, x):
         # (torch.fx hands over proxies)
-        return (self.fused and isinstance(x, torch.Tensor) and not torch.jit.is_tracing() and not torch.compiler.is_compiling() and not modes() and not all_watched()
+        return (self.fused and not torch.compiler.is_compiling() and not torch.jit.is_tracing() and isinstance(x, torch.Tensor) and not modes() and not all_watched()
                 and all(type(ff) is _Layers and type(attn) in _FORWARDS and not watched(attn) and not watched(ff) for attn, ff in self.layers)
                 and all(module.forward is forward and module.__call__ is nn.Module.__call__ for module, forward in _FORWARDS.items()))
 
@@ -228,10 +228,11 @@ class TwoSimplicialLM(nn.Module):
 
     def _can_fuse(self, hidden, target):
         weight = self.to_logits.weight
-        return (self.fused and type(self.to_logits) is nn.Linear and all(type(t) in (torch.Tensor, nn.Parameter) for t in (hidden, target, weight))
-                and self.to_logits.bias is None and not _watched(self.to_logits) and F.cross_entropy is _CROSS_ENTROPY and not modes() and hidden.is_cuda
-                and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.dtype == weight.dtype and not torch.is_autocast_enabled() and not torch.jit.is_tracing()
-                and not torch.compiler.is_compiling() and _native.torch_ext().loss_covers(hidden, weight, target))
+        # (torch.compile follows what stands in front)
+        return (self.fused and not torch.compiler.is_compiling() and not torch.jit.is_tracing() and type(self.to_logits) is nn.Linear
+                and all(type(t) in (torch.Tensor, nn.Parameter) for t in (hidden, target, weight)) and self.to_logits.bias is None and not _watched(self.to_logits) and F.cross_entropy is _CROSS_ENTROPY and not modes() and hidden.is_cuda
+                and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.dtype == weight.dtype and not torch.is_autocast_enabled()
+                and _native.torch_ext().loss_covers(hidden, weight, target))
 
     @torch.no_grad()
     def logits_cached(self, x, cache, batch, rows=None):

@@ -114,3 +114,13 @@ def test_a_fused_stack_makes_no_modules(monkeypatch):
     want = stack(False)(x)
     monkeypatch.setattr(nn.Module, '__init__', lambda *_: pytest.fail('a module is made'))
     assert torch.equal(t(x), want)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_compiled_fused_models_are_one_graph(device):
+    """(with torch's own run of the graph: the separate calls)"""
+    tokens = torch.arange(16, device=device).view(2, 8)
+    fused, separate = language_model(True, device), language_model(False, device)
+    compiled = torch.compile(fused, backend='eager', fullgraph=True)
+    assert torch.equal(compiled(tokens, return_loss=True), separate(tokens, return_loss=True))
+    assert torch.equal(torch.compile(fused.transformer, backend='eager', fullgraph=True)(rows(device).bfloat16()), separate.transformer(rows(device).bfloat16()))
