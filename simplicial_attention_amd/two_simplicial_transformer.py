@@ -227,12 +227,12 @@ class TwoSimplicialLM(nn.Module):
         return F.cross_entropy(logits.flatten(0, 1).float(), target.flatten())
 
     def _can_fuse(self, hidden, target):
-        weight = self.to_logits.weight
+        layer = self.to_logits
         # (torch.compile follows what stands in front)
-        return (self.fused and not torch.compiler.is_compiling() and not torch.jit.is_tracing() and type(self.to_logits) is nn.Linear
-                and all(type(t) in (torch.Tensor, nn.Parameter) for t in (hidden, target, weight)) and self.to_logits.bias is None and not _watched(self.to_logits) and F.cross_entropy is _CROSS_ENTROPY and not modes() and hidden.is_cuda
-                and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.dtype == weight.dtype and not torch.is_autocast_enabled()
-                and _native.torch_ext().loss_covers(hidden, weight, target))
+        return (self.fused and not torch.compiler.is_compiling() and not torch.jit.is_tracing() and type(layer) is nn.Linear
+                and all(type(t) in (torch.Tensor, nn.Parameter) for t in (hidden, target, layer.weight)) and layer.bias is None and not _watched(layer)
+                and F.cross_entropy is _CROSS_ENTROPY and not modes() and hidden.is_cuda and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.dtype == layer.weight.dtype
+                and not torch.is_autocast_enabled() and _native.torch_ext().loss_covers(hidden, layer.weight, target))
 
     @torch.no_grad()
     def logits_cached(self, x, cache, batch, rows=None):

@@ -124,3 +124,11 @@ def test_compiled_fused_models_are_one_graph(device):
     compiled = torch.compile(fused, backend='eager', fullgraph=True)
     assert torch.equal(compiled(tokens, return_loss=True), separate(tokens, return_loss=True))
     assert torch.equal(torch.compile(fused.transformer, backend='eager', fullgraph=True)(rows(device).bfloat16()), separate.transformer(rows(device).bfloat16()))
+
+
+@pytest.mark.parametrize('fused', [False, True])
+def test_a_read_out_of_another_kind_has_a_loss(fused):
+    lm, tokens = language_model(fused, 'cpu'), torch.arange(16).view(2, 8)
+    want = lm(tokens, return_loss=True)
+    lm.to_logits = nn.Sequential(lm.to_logits)
+    assert torch.equal(lm(tokens, return_loss=True), want)
