@@ -41,7 +41,8 @@ class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` on :func:`adamw_step` (no amsgrad, no maximize).
 
     ``state_bits``: 32, or 8 for parameters of at least ``min_8bit_size`` elements (the states of smaller ones cost nothing and stay in 32).  ``masters``: bfloat16 and float16 parameters are
-    the roundings of float32 copies that the optimizer keeps, so that steps smaller than half a place of theirs are not lost.  Parameters without a gradient are left out of a step and
+    the roundings of float32 copies that the optimizer keeps, so that steps smaller than half a place of theirs are not lost; a parameter that is set from outside between steps has to be
+    set in ``state[param]['master']`` too, or the next step takes it back.  Parameters without a gradient are left out of a step and
     count their own steps.
 
     ``capturable``: the step count of each group is on the GPU, and ``lr`` may be a float32 tensor there, so that a recorded :meth:`step` can be replayed; all parameters of a group
