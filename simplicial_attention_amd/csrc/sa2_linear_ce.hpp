@@ -6,13 +6,13 @@
 // The forward keeps, of every tile of logits, a maximum and a sum per row; they are merged to lse.  The backward goes over the vocabulary in pieces: logits of a piece
 // are formed again, become dz in the operands' type, and are multiplied both ways.  Four products of 2 N V D operations for the three that a
 // gradient needs, and N x (a piece) of memory.  Bound by the matrix unit; with few channels by the exponentials of the two epilogues.
-// 8192 rows of 2048 channels over 131072 tokens: 15.0 ms (logits 3.9, dz 4.2, dH 3.6, dW 3.4), 1.17 PFLOP/s; over 32000 of 512 channels 1.3 ms.  The smallest (60 rows, 256 tokens): 22 us in four
+// 8192 rows of 2048 channels over 131072 tokens: 14.8 to 15.1 ms by card (logits 3.8, dz 4.1, dH 3.6, dW 3.3), 1.19 PFLOP/s; over 32000 of 512 channels 1.24 to 1.3 ms.  The smallest (60 rows, 256 tokens): 22 us in four
 // launches.
 //
 // dz is rounded to the operands' type for its products.  To use that type's range well it is divided by the largest weight G of a row's loss
 // (mean and sum: the one weight of all) and in fp16 multiplied by 1024, which the products' results are multiplied by again in 32 bits.  Where every row has a weight
 // of its own (reduction none), that would leave rows of small weights the least steps of fp16 (over 32000 tokens dH of a row at a millionth of G was off by 9 %): there dH is made from a second
-// dz without weights, and the rows of the result are multiplied by theirs.  dW adds rows up, and what it loses of one (2^-35 G of each dz) is small beside G.
+// dz without weights (1237 rows of 328 channels over 10007 tokens: ce_dz_kernel 26.4 -> 30.6 us), and the rows of the result are multiplied by theirs.  dW adds rows up, and what it loses of one (2^-35 G of each dz) is small beside G.
 #pragma once
 
 #include "sa2_product.hpp"
