@@ -5,6 +5,7 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
 from torch.nn.modules import module as _module
+from torch.utils._device import DeviceContext
 
 from . import _native
 
@@ -17,6 +18,11 @@ _FORWARD, _LINEAR = nn.Linear.forward, F.linear
 def modes():
     """Someone sees torch's operators or functions (the kernels of this package are none)."""
     return torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack()
+
+
+def modes_but_devices():
+    """The same, but for a default device (``torch.set_default_device``, ``with torch.device(...)``), which is a mode that changes the calls of factories alone."""
+    return torch._C._len_torch_dispatch_stack() or any(type(torch._C._get_function_stack_at(i)) is not DeviceContext for i in range(torch._C._len_torch_function_stack()))
 
 
 def all_watched():

@@ -6,7 +6,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import _native
-from .linear import all_watched, modes, watched
+from .linear import all_watched, modes_but_devices, watched
 
 
 def add_rms_norm(x: Tensor, residual: Tensor | None = None, weight: Tensor | None = None, eps: float | None = None) -> tuple[Tensor, Tensor]:
@@ -38,7 +38,7 @@ _PLAIN = (Tensor, nn.Parameter)
 def _covered(norm):
     """What this module computes is the kernel's to compute, and nobody sees its calls."""
     return (type(norm) is nn.RMSNorm and type(norm.weight) in _PLAIN and nn.RMSNorm.forward is _FORWARD and nn.RMSNorm.__call__ is nn.Module.__call__ and F.rms_norm is _RMS_NORM
-            and not (modes() or all_watched() or watched(norm)))
+            and not (modes_but_devices() or all_watched() or watched(norm)))
 
 
 def norm_behind(norm, x: Tensor, residual: Tensor | None) -> tuple[Tensor, Tensor]:

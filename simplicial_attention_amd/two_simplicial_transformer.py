@@ -18,7 +18,7 @@ from torch import nn
 
 from . import _native
 from .cross_entropy import linear_cross_entropy
-from .linear import _watched, all_watched, apply_linear, modes, watched
+from .linear import _watched, all_watched, apply_linear, modes_but_devices, watched
 from .paged import PagedCache, paged_append, paged_attn
 from .rms_norm import norm_behind
 from .sampling import sample_tokens
@@ -147,7 +147,7 @@ class TwoSimplicialTransformer(nn.Module):
     @torch.jit.unused
     def _can_fuse(self, x):
         # (torch.fx hands over proxies)
-        return (self.fused and not torch.compiler.is_compiling() and not torch.jit.is_tracing() and isinstance(x, torch.Tensor) and not modes() and not all_watched()
+        return (self.fused and not torch.compiler.is_compiling() and not torch.jit.is_tracing() and isinstance(x, torch.Tensor) and not modes_but_devices() and not all_watched()
                 and all(type(ff) is _Layers and type(attn) in _FORWARDS and not watched(attn) and not watched(ff) for attn, ff in self.layers)
                 and all(module.forward is forward and module.__call__ is nn.Module.__call__ for module, forward in _FORWARDS.items()))
 
@@ -231,7 +231,7 @@ class TwoSimplicialLM(nn.Module):
         # (torch.compile follows what stands in front)
         return (self.fused and not torch.compiler.is_compiling() and not torch.jit.is_tracing() and type(layer) is nn.Linear
                 and all(type(t) in (torch.Tensor, nn.Parameter) for t in (hidden, target, layer.weight)) and layer.bias is None and not _watched(layer)
-                and F.cross_entropy is _CROSS_ENTROPY and not modes() and hidden.is_cuda and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.dtype == layer.weight.dtype
+                and F.cross_entropy is _CROSS_ENTROPY and not modes_but_devices() and hidden.is_cuda and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.dtype == layer.weight.dtype
                 and not torch.is_autocast_enabled() and _native.torch_ext().loss_covers(hidden, layer.weight, target))
 
     @torch.no_grad()

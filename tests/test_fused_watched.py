@@ -132,3 +132,28 @@ def test_a_read_out_of_another_kind_has_a_loss(fused):
     want = lm(tokens, return_loss=True)
     lm.to_logits = nn.Sequential(lm.to_logits)
     assert torch.equal(lm(tokens, return_loss=True), want)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_a_default_device_is_nobody_who_watches(device, monkeypatch):
+    from simplicial_attention_amd import two_simplicial_transformer as module
+    behind, fused, separate = [], stack(True, device), stack(False, device)
+    x = rows(device)
+    want = fused(x)
+    monkeypatch.setattr(module, 'norm_behind', lambda *args, whole=module.norm_behind: behind.append(1) or whole(*args))
+    with torch.device(device):
+        assert torch.equal(fused(x), want)
+        separate(x)
+    assert len(behind) == 7
+
+
+@pytest.mark.gpu
+def test_a_default_device_leaves_the_kernels(monkeypatch):
+    from simplicial_attention_amd import rms_norm
+    from simplicial_attention_amd import two_simplicial_transformer as module
+    called = []
+    monkeypatch.setattr(rms_norm, 'add_rms_norm', lambda *args, kernel=rms_norm.add_rms_norm: called.append('norm') or kernel(*args))
+    monkeypatch.setattr(module, 'linear_cross_entropy', lambda *args, kernel=module.linear_cross_entropy: called.append('loss') or kernel(*args))
+    with torch.device('cuda'):
+        language_model(True, 'cuda')(torch.arange(16, device='cuda').view(2, 8), return_loss=True)
+    assert called == ['norm'] * 5 + ['loss']
