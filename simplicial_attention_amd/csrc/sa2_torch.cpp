@@ -161,6 +161,7 @@ struct Attend : public torch::autograd::Function<Attend> {
     }
 
     static variable_list run_backward(const variable_list &s, const std::vector<int64_t> &n, double scale, const Tensor &given) {
+        refuse_modes("sliding-window 2-simplicial attention");
         const Tensor &q = s[0], &k1 = s[1], &k2 = s[2], &v1 = s[3], &v2 = s[4], &out = s[5], &lse = s[6], &residual = s[7], &t_save = s[8], &m_save = s[9];
         Geometry g;
         g.batch = n[0]; g.seq = n[1]; g.heads = n[2]; g.kv_heads = n[3]; g.dim_qk = n[4]; g.dim_v = n[5]; g.dim = n[6]; g.w1 = n[7]; g.w2 = n[8];
@@ -235,6 +236,7 @@ Tensor attend(const Tensor &q, const Tensor &k1, const Tensor &k2, const Tensor 
 // shapes, types and windows of the Function and the wrapper; `pads`: other head dimensions and types than the kernels' are welcome
 Geometry checked(const Tensor &q, const Tensor &k1, const Tensor &k2, const Tensor &v1, const Tensor &v2, int64_t w1, int64_t w2,
                  std::optional<double> scale, bool pads) {
+    refuse_modes("sliding-window 2-simplicial attention");
     const Tensor *all[5] = {&q, &k1, &k2, &v1, &v2};
     for (const Tensor *t : all)
         if (!t->is_cuda()) raise(PyExc_AssertionError, "sliding-window 2-simplicial attention runs on the GPU only");
@@ -313,6 +315,7 @@ struct QKVNorm : public torch::autograd::Function<QKVNorm> {
     // (saved == nullptr: no backward follows)
     static variable_list run(Saved *saved, const Tensor &qkv_in, const std::array<const Weight *, 5> &w, int64_t heads, int64_t kv_heads,
                              int64_t dim, double eps) {
+        refuse_modes("the norms of queries, keys and values");
         const int64_t batch = qkv_in.size(0), seq = qkv_in.size(1);
         const Tensor qkv = qkv_in.stride(2) == 1 && qkv_in.stride(0) == seq * qkv_in.stride(1) ? qkv_in : qkv_in.contiguous();
         const c10::DeviceGuard guard(qkv.device());
@@ -343,6 +346,7 @@ struct QKVNorm : public torch::autograd::Function<QKVNorm> {
     }
 
     static variable_list run_backward(const variable_list &s, const std::vector<int64_t> &n, variable_list douts) {
+        refuse_modes("the norms of queries, keys and values");
         const Tensor &qkv = s[0], &rstd = s[1];
         const int64_t batch = n[0], seq = n[1], heads = n[2], kv_heads = n[3], dim = n[4];
         const c10::DeviceGuard guard(qkv.device());
@@ -420,6 +424,7 @@ struct Linear : public torch::autograd::Function<Linear> {
     }
 
     static Tensor weight_gradient(const Tensor &dy, const Tensor &x) {
+        refuse_modes("a linear layer's weight gradient");
         const c10::DeviceGuard guard(x.device());
         auto rows = [](const Tensor &t) {
             const bool ok = t.stride(1) == 1 && t.stride(0) >= t.size(1) && t.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;

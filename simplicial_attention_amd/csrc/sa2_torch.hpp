@@ -61,14 +61,14 @@ bool foreign(const Tensor &t) {
 }
 
 // Recorders (torch.jit.trace, make_fx, fake tensors) see torch's operators alone: they would keep the allocation of a result without the kernel that fills it, and a
-// replay would return what was in memory.
-void refuse_recorder(const char *what) {
+// replay would return what was in memory.  (torch.jit.trace sees Python Functions too, by which the calls go that it may record: those refuse the others.)
+void refuse_modes(const char *what, bool recorded = false) {
     using c10::impl::TorchDispatchModeKey;
-    bool recorded = torch::jit::tracer::isTracing();
     for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
         recorded = recorded || c10::impl::TorchDispatchModeTLS::get_mode(mode).has_value();
     if (recorded) raise(PyExc_RuntimeError, std::string(what) + " cannot be traced: a recorder does not see its kernels");
 }
+void refuse_recorder(const char *what) { refuse_modes(what, torch::jit::tracer::isTracing()); }
 
 void refuse_autograd(const char *what, std::initializer_list<const Tensor *> inputs) {
     refuse_recorder(what);
